@@ -585,7 +585,7 @@ def _run(args):
         torch.cuda.synchronize()
 
     from stylemesh_amd.runtime.engine import trunk_stream
-    main_stream = trunk_stream(dev)     # the step's trunk on a high-priority stream (the side streams keep normal priority)
+    main_stream = trunk_stream(dev)     # the step's trunk on a stream of its own
     if main_stream is not None:
         torch.cuda.set_stream(main_stream)
     timer = None if args.no_conv_timer else ops.KernelTimer()

@@ -48,7 +48,6 @@ SWITCHES = {
                                "the view's own chunks only; 0 = one update"),
     "STYLEMESH_OVERLAP_MIN_PIXELS": ("400000", "tuning", "pixels over the active levels from which side streams pay (c2's 87 k do not)"),
     "STYLEMESH_SIDE_CUS": ("0", "experiment", "confine the side streams to N compute units (profiles/r03/side_stream_cu_subset_sweep_c3.txt: no gain)"),
-    "STYLEMESH_MAIN_PRIORITY": ("high", "tuning", "trunk on a high-priority HIP stream (+2-4 %); normal = the caller's stream"),
     "STYLEMESH_STEP_PROGRAM": ("1", "mode", "small steps recorded once and replayed with one library call; 0 = always eager; "
                                "verify = record every step and compare it with the program"),
     "STYLEMESH_CONTENT_GRAPH": ("1", "tuning", "content-target VGG pass of a view replayed as one captured hipGraph; 0 = eager launches"),

@@ -76,15 +76,14 @@ class EngineConfig:
 
 
 def trunk_stream(device):
-    """A HIGH-priority HIP stream for the step's trunk (convs, pools, sampling, scatter, the closing update). The
-    engine's side streams - style branches with thousands of microseconds of slack, the early half of the split update -
-    are created at normal priority, so the hardware queues dispatch the trunk's workgroups first and the side work fills
-    what is left: measured +2-4 % on the c3 step (165.8 against 159.6-162.4 views/s, same box, alternating runs).
-    ``MiniTrainer.fit`` and ``bench.py`` make it the current stream (STYLEMESH_MAIN_PRIORITY=normal: keep the caller's)."""
-    if os.environ.get("STYLEMESH_MAIN_PRIORITY", "high") != "high" or not torch.cuda.is_available():
+    """The HIP stream of the step's trunk (convs, pools, sampling, scatter, the closing update), apart from the engine's
+    side streams. Every stream of the process has the DEFAULT priority: work on streams of different priorities has hung
+    MI355X cards for good (a high-priority trunk was worth 2-4 % of the c3 step). ``MiniTrainer.fit`` and ``bench.py``
+    make it the current stream."""
+    if not torch.cuda.is_available():
         return None
     torch.cuda.synchronize(device)
-    return torch.cuda.Stream(device=device, priority=-1)
+    return torch.cuda.Stream(device=device)
 
 
 class TextureArena:
@@ -303,7 +302,7 @@ class StepEngine:
 
     def _new_side_stream(self):
         """Side streams carry work with slack (style branches joined many kernels later, the early half of the update), at
-        normal priority - the trunk's stream is the high-priority one (``trunk_stream``)."""
+        the default priority, as the trunk (``trunk_stream``)."""
         n_cus = int(os.environ.get("STYLEMESH_SIDE_CUS", "0"))
         if n_cus > 0:   # a queue confined to n_cus compute units (n_cus / 8 of every XCD): see sm_stream_create_cu_subset
             import ctypes
@@ -503,10 +502,10 @@ class StepEngine:
         st = self._prep_stream
         if urgent:
             # The view is needed by the very NEXT step (index_repeat 1): its read-back must arrive while the current step
-            # still runs, or the GPU idles while the host enqueues the next one. On a stream of the trunk's priority the
-            # preparation's small kernels are dispatched beside the step's instead of behind them.
+            # still runs, or the GPU idles while the host enqueues the next one: a stream that holds no earlier view's
+            # preparation.
             if getattr(self, "_prep_stream_hi", None) is None:
-                self._prep_stream_hi = torch.cuda.Stream(device=self.device, priority=-1)
+                self._prep_stream_hi = torch.cuda.Stream(device=self.device)
             st = self._prep_stream_hi
             if getattr(self, "_prep_last", None) is not None:
                 st.wait_event(self._prep_last)       # (the two preparation streams share scratch)

@@ -154,7 +154,7 @@ class MiniTrainer:
         caller_stream = None
         if self.device != "cpu" and torch.cuda.is_available():
             from .runtime.engine import trunk_stream
-            st = trunk_stream(self.device)       # high-priority stream for the step's trunk (side work fills the rest)
+            st = trunk_stream(self.device)       # the step's trunk on a stream of its own (side work fills the rest)
             if st is not None:
                 caller_stream = torch.cuda.current_stream()
                 torch.cuda.set_stream(st)
