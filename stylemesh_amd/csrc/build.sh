@@ -6,6 +6,7 @@ OUT=../libstylemesh_hip.so
 FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -munsafe-fp-atomics -fPIC -Wall -Wno-unused-function"
 mkdir -p ../../build
 objs=()
+pids=()
 for f in conv texture gram prep comm eval raster scatter_plan exchange replay; do
   o=../../build/$f.o
   stale=0
@@ -13,10 +14,12 @@ for f in conv texture gram prep comm eval raster scatter_plan exchange replay; d
     if [ ! -f "$o" ] || [ "$dep" -nt "$o" ]; then stale=1; fi
   done
   if [ $stale = 1 ]; then
+    rm -f "$o"
     /opt/rocm/bin/hipcc $FLAGS "$@" -c $f.hip -o $o &
+    pids+=($!)
   fi
   objs+=("$o")
 done
-wait
+for p in "${pids[@]:-}"; do [ -z "$p" ] || wait "$p"; done   # (a failed compile ends the build here)
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -o $OUT "${objs[@]}" -L/opt/rocm/lib -lrccl
 echo "built $(realpath $OUT)"

@@ -72,6 +72,18 @@ __device__ __forceinline__ void side_store(T v, T* p) {
 #endif
 }
 
+// Zero fill as a kernel: a memset node of a captured graph has given wrong results on replays after the first.
+__global__ __launch_bounds__(256) static void zero_fill_kernel(float* __restrict__ dst, size_t n) {
+    const size_t stride = (size_t)gridDim.x * 256;
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += stride) dst[i] = 0.f;
+}
+inline hipError_t zero_fill(float* dst, size_t n, hipStream_t s) {
+    if (n == 0) return hipSuccess;
+    const size_t blocks = (n + 1023) / 1024;
+    hipLaunchKernelGGL(zero_fill_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, s, dst, n);
+    return hipGetLastError();
+}
+
 __host__ __device__ inline int round_up(int x, int m) { return (x + m - 1) / m * m; }
 __host__ __device__ inline int row_stride(int W) { return round_up(W + 1, 4); }
 __host__ __device__ inline int plane_size(int H, int W) { return round_up((H + 2) * row_stride(W), 64); }

@@ -577,8 +577,8 @@ static int gram_masked_split_impl(const float* feat, const float* mask0, const f
     hipStream_t s = (hipStream_t)stream;
     if (zero_fill) {   // the position ranges add into the slab
         const size_t cc = (size_t)C * C;
-        hipError_t e = hipMemsetAsync(S0, 0, cc * sizeof(float), s);
-        if (e == hipSuccess && mask1) e = hipMemsetAsync(S1, 0, cc * sizeof(float), s);
+        hipError_t e = sm::zero_fill(S0, cc, s);
+        if (e == hipSuccess && mask1) e = sm::zero_fill(S1, cc, s);
         if (e != hipSuccess) return (int)e;
     }
     const sm_gram_problem q{feat, mask0, mask1, S0, S1, amax_feat, C, H, W};

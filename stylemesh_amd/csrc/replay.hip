@@ -84,8 +84,7 @@ int sm_copy_floats(float* dst, const float* src, size_t n, void* stream) {
 }
 
 int sm_zero_floats(float* dst, size_t n, void* stream) {
-    if (n == 0) return 0;
-    return (int)hipMemsetAsync(dst, 0, n * sizeof(float), (hipStream_t)stream);
+    return (int)sm::zero_fill(dst, n, (hipStream_t)stream);
 }
 
 int sm_call_id(const char* name) {
