@@ -3,7 +3,8 @@
 set -euo pipefail
 cd "$(dirname "$0")"
 OUT=../libstylemesh_hip.so
-FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -munsafe-fp-atomics -fPIC -Wall -Wno-unused-function"
+# packed fp32 instructions stay off: hipcc forms them by itself and some have given wrong results now and then
+FLAGS="--offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++17 -munsafe-fp-atomics -fPIC -Wall -Wno-unused-function"
 mkdir -p ../../build
 objs=()
 pids=()
