@@ -443,8 +443,8 @@ __global__ __launch_bounds__(256) void adam_kernel(float* __restrict__ p, float*
                 float x = pv[u][j];
                 if (ADAM) {
                     const float gr = fmaf(gv[u][j], grad_scale, segs.reg[k] * x);  // data term (+ mean over ranks) + reg
-                    mv[u][j] = mv[u][j] + (gr - mv[u][j]) * one_minus_beta1;       // exp_avg.lerp_(grad, 1 - beta1)
-                    vv[u][j] = vv[u][j] * beta2 + (gr * gr) * one_minus_beta2;     // exp_avg_sq.mul_(b2).addcmul_(g, g, 1-b2)
+                    mv[u][j] = fmaf(gr - mv[u][j], one_minus_beta1, mv[u][j]);          // exp_avg.lerp_(grad, 1 - beta1)
+                    vv[u][j] = fmaf(gr * gr, one_minus_beta2, vv[u][j] * beta2);        // exp_avg_sq.mul_(b2).addcmul_(g, g, 1-b2)
                     const float denom = sqrtf(vv[u][j]) * inv_sqrt_bc2 + eps;
                     x = x - lr_over_bc1 * (mv[u][j] / denom);
                 }
@@ -575,8 +575,8 @@ __global__ __launch_bounds__(256) void adam_sparse_kernel(float* __restrict__ p,
             for (int j = 0; j < 4; ++j) {
                 float x = pv[u][j];
                 const float gr = fmaf(gv[u][j], grad_scale, reg * x);          // data term (+ mean over ranks) + reg
-                mv[u][j] = mv[u][j] + (gr - mv[u][j]) * one_minus_beta1;       // exp_avg.lerp_(grad, 1 - beta1)
-                vv[u][j] = vv[u][j] * beta2 + (gr * gr) * one_minus_beta2;     // exp_avg_sq.mul_(b2).addcmul_(g, g, 1-b2)
+                mv[u][j] = fmaf(gr - mv[u][j], one_minus_beta1, mv[u][j]);          // exp_avg.lerp_(grad, 1 - beta1)
+                vv[u][j] = fmaf(gr * gr, one_minus_beta2, vv[u][j] * beta2);        // exp_avg_sq.mul_(b2).addcmul_(g, g, 1-b2)
                 const float denom = sqrtf(vv[u][j]) * inv_sqrt_bc2 + eps;
                 x = x - lr_over_bc1 * (mv[u][j] / denom);
                 x = fminf(hi, fmaxf(x, lo));
