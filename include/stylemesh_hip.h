@@ -725,6 +725,48 @@ int sm_mip_downsample(const float* src, float* dst, int C, int Hs, int Ws, void*
 int sm_tex_sample_mip(const float* const* levels, const int* level_w, const int* level_h, int n_levels,
                       const float* uv, int H, int W, float* out, float* lod_out, void* stream);
 
+/* ---- F8: 8-bit floating point with a scale per block of 128 (csrc/fp8.hip) --------------------------------
+ * A matrix in this format: codes [R][pitch] bytes (pitch = C rounded up to 128; the codes behind column C are 0), e4m3
+ * (largest magnitude 448, no infinity) or e5m2 (57344), and one scale per block of 128 columns - of one row ("rows") or of 128
+ * rows ("tiles"). Scales are bytes s (the block's values are codes * 2^(s - 127); 255 = NaN) stored [ceil(KB / 4)][S][4] with
+ * KB = ceil(C / 128), S = R (rows) or ceil(R / 128) (tiles): the byte of (row, block kb) at [kb / 4][row][kb % 4], bytes behind
+ * block KB - 1 = 127. The product also takes fp32 scales of any value, stored [KB][S] floats. */
+#define SM_TYPE_F32 0
+#define SM_TYPE_BF16 1
+#define SM_TYPE_F16 2
+#define SM_FP8_E4M3 0
+#define SM_FP8_E5M2 1
+/* x [rows][cols] (x_type, row stride x_stride elements, aligned to its elements) -> q / q_scale: the matrix in 8 bits, and / or
+ * qt / qt_scale: its transpose [cols][rows rounded up to 128] with the blocks along the rows (either pair may be NULL); tiles:
+ * one scale per 128 x 128 tile instead of per row and block. x is read once. A block's scale is the smallest power of two
+ * 2^e, e in [-127, 127], with max |x| <= 448 2^e (e5m2: 57344 2^e), 1 for a block of zeros; the codes are x 2^-e rounded to
+ * nearest even. NaN and infinities do not take part in the maximum; NaN becomes NaN, an infinity NaN (e4m3) / infinity (e5m2).
+ * q, qt: 16-byte aligned. */
+int sm_fp8_quantize(const void* x, int x_type, int rows, int cols, size_t x_stride, int fmt, int tiles, void* q, void* q_scale,
+                    void* qt, void* qt_scale, void* stream);
+/* out[M][N] (out_type, row stride out_stride elements) = A B^T, or out += A B^T (accumulate), A [M][K] with scales per row and
+ * block, B [N][K] (e4m3) per row and block or per tile (b_tiles); fp32 accumulate, one rounding to out_type. scale_f32: both
+ * scale arrays are floats. a, b: 16-byte aligned, pitches multiples of 16 and at least K rounded up to 128. ws:
+ * sm_fp8_matmul_ws_bytes(M, N, K) bytes (0: may be NULL) of scratch of this call's own. K = 0: zeros / out as it is. */
+size_t sm_fp8_matmul_ws_bytes(int M, int N, int K);
+int sm_fp8_matmul(const void* a, const void* a_scale, int a_fmt, size_t a_pitch, const void* b, const void* b_scale, int b_tiles,
+                  size_t b_pitch, int scale_f32, int M, int N, int K, void* out, int out_type, size_t out_stride, int accumulate,
+                  void* ws, size_t ws_bytes, void* stream);
+
+/* ---- G1: the global norm of many gradient tensors, and clipping by it (csrc/gradnorm.hip) -------------------
+ * What Trainer(gradient_clip_val=...) of the reference's pytorch_lightning does between backward and the optimizer step
+ * (torch.nn.utils.clip_grad_norm_). grads / out / numel / types (SM_TYPE_*) / out_types: HOST arrays of n entries, read during
+ * the call; the tensors are dense, aligned to their elements. norm = sqrt(sum of all squares) (sums in 64 bits) or, inf_norm,
+ * the largest magnitude; *norm_out (device) receives it as fp32. sm_grad_clip: out[i] = grads[i] * min(1, max_norm / (norm +
+ * 1e-6)) rounded once to out_types[i]; out[i] may be grads[i] (then of the same type). A norm that is not finite gives the
+ * coefficient that formula gives (infinity: 0, NaN: NaN). ws: sm_grad_norm_ws_bytes(n) bytes, 8-byte aligned, of this call's
+ * own. Deterministic: the same bits for the same tensors. */
+size_t sm_grad_norm_ws_bytes(int n_tensors);
+int sm_grad_norm(const void* const* grads, const size_t* numel, const int* types, int n, int inf_norm, void* ws, size_t ws_bytes,
+                 float* norm_out, void* stream);
+int sm_grad_clip(const void* const* grads, void* const* out, const size_t* numel, const int* types, const int* out_types, int n,
+                 int inf_norm, double max_norm, void* ws, size_t ws_bytes, float* norm_out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

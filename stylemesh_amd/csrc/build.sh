@@ -8,7 +8,7 @@ FLAGS="--offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O
 mkdir -p ../../build
 objs=()
 pids=()
-for f in conv texture gram prep comm eval raster scatter_plan exchange replay; do
+for f in conv texture gram prep comm eval raster scatter_plan exchange replay fp8 gradnorm; do
   o=../../build/$f.o
   stale=0
   for dep in "$f.hip" *.h ../../include/stylemesh_hip.h; do

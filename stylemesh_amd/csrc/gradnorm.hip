@@ -1,0 +1,281 @@
+// G1: the global norm over a list of gradient tensors and clipping by it (include/stylemesh_hip.h section G1): what
+// pytorch_lightning's Trainer(gradient_clip_val=...) asks of torch.nn.utils.clip_grad_norm_ between backward and the
+// optimizer step.
+//
+//   norm = sqrt(sum over all tensors of g^2)  or  max |g|        coef = min(1, max_norm / (norm + 1e-6))        out = g coef
+//
+// Two kernels per 120 tensors: per-block partial sums, then the scaling pass, whose every block adds the same partial sums in
+// the same order (a few KB from L2) instead of waiting for a third launch. No atomics: the norm has the same bits every time.
+// Sums are held in 64 bits: squares of fp32 gradients over- and underflow fp32 (|g| > 1.8e19, < 1e-23) where the norm
+// does not, and the 64-bit multiply-add runs at the fp32 rate on this chip - both kernels are bound by HBM.
+#include <cmath>
+
+#include "common.h"
+
+namespace sm {
+
+typedef unsigned g_u32x4 __attribute__((ext_vector_type(4)));
+typedef g_u32x4 g_u32x4_u __attribute__((aligned(2)));      // gradient views start at any element
+typedef unsigned g_u32x2 __attribute__((ext_vector_type(2)));
+typedef g_u32x2 g_u32x2_u __attribute__((aligned(2)));
+
+constexpr int GN_TENSORS = 120;      // per launch: the table travels in the kernel arguments (no device copy to keep alive)
+constexpr int GN_PARTIALS = 1024;    // at most this many partial sums per call and launch
+
+struct GradTable {
+    const void* in[GN_TENSORS];
+    void* out[GN_TENSORS];
+    unsigned long long n[GN_TENSORS];
+    int first[GN_TENSORS + 1];       // first chunk of each tensor
+    uint8_t type[GN_TENSORS];        // SM_TYPE_* of in, of out << 4
+    int count;
+    int chunk_log2;                  // elements per chunk
+};
+
+__device__ __forceinline__ double gn_combine(double a, double b, bool inf) {
+    if (!inf) return a + b;
+    return (b > a || b != b) ? b : a;      // a NaN stays
+}
+__device__ __forceinline__ double gn_take(double acc, float v, bool inf) {
+    if (!inf) return fma((double)v, (double)v, acc);
+    const float a = fabsf(v);
+    return gn_combine(acc, (double)a, true);
+}
+__device__ __forceinline__ double gn_block(double v, bool inf) {
+    __shared__ double red[4];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = gn_combine(v, __shfl_xor(v, o, 64), inf);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return gn_combine(gn_combine(red[0], red[1], inf), gn_combine(red[2], red[3], inf), inf);
+}
+__device__ __forceinline__ float gn_up(unsigned h, int type) {
+    return type == SM_TYPE_BF16 ? __builtin_bit_cast(float, h << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)h);
+}
+__device__ __forceinline__ unsigned gn_down(float f, int type) {
+    if (type == SM_TYPE_F16) return __builtin_bit_cast(uint16_t, (_Float16)f);
+    const unsigned u = __builtin_bit_cast(unsigned, f);
+    return (u & 0x7fffffffu) > 0x7f800000u ? ((u >> 16) | 0x40u) : (u + 0x7fffu + ((u >> 16) & 1u)) >> 16;
+}
+// elements i ... i + 7 of a tensor as fp32
+__device__ __forceinline__ void gn_load8(const void* p, size_t i, int type, float* v) {
+    if (type == SM_TYPE_F32) {
+        const g_u32x4_u* q = reinterpret_cast<const g_u32x4_u*>(static_cast<const float*>(p) + i);
+        const g_u32x4 a = q[0], b = q[1];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            v[j] = __builtin_bit_cast(float, (unsigned)a[j]);
+            v[4 + j] = __builtin_bit_cast(float, (unsigned)b[j]);
+        }
+    } else {
+        const g_u32x4 a = *reinterpret_cast<const g_u32x4_u*>(static_cast<const uint16_t*>(p) + i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            v[2 * j] = gn_up(a[j] & 0xffffu, type);
+            v[2 * j + 1] = gn_up(a[j] >> 16, type);
+        }
+    }
+}
+__device__ __forceinline__ float gn_load1(const void* p, size_t i, int type) {
+    return type == SM_TYPE_F32 ? static_cast<const float*>(p)[i] : gn_up(static_cast<const uint16_t*>(p)[i], type);
+}
+__device__ __forceinline__ int gn_tensor_of(const GradTable& t, int chunk) {
+    int lo = 0, hi = t.count;              // last tensor with first <= chunk (an empty tensor has no chunk)
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (t.first[mid] <= chunk) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+
+__global__ __launch_bounds__(256) void grad_norm_partial_kernel(GradTable t, int inf, double* __restrict__ partial) {
+    double acc = 0.0;
+    for (int c = blockIdx.x; c < t.first[t.count]; c += gridDim.x) {
+        const int k = gn_tensor_of(t, c);
+        const size_t begin = (size_t)(c - t.first[k]) << t.chunk_log2;
+        const size_t end = min((size_t)t.n[k], begin + ((size_t)1 << t.chunk_log2));
+        const int type = t.type[k] & 15;
+        size_t i = begin + threadIdx.x * 8;
+        for (; i + 8 <= end; i += 2048) {
+            float v[8];
+            gn_load8(t.in[k], i, type, v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) acc = gn_take(acc, v[j], inf != 0);
+        }
+        for (; i < end; ++i) acc = gn_take(acc, gn_load1(t.in[k], i, type), inf != 0);     // (only the thread the end falls to)
+    }
+    acc = gn_block(acc, inf != 0);
+    if (threadIdx.x == 0) partial[blockIdx.x] = acc;
+}
+
+__device__ __forceinline__ double gn_total(const double* partial, int n, bool inf) {
+    double acc = 0.0;
+    for (int i = threadIdx.x; i < n; i += 256) acc = gn_combine(acc, partial[i], inf);
+    acc = gn_block(acc, inf);
+    return inf ? acc : sqrt(acc);
+}
+
+__global__ __launch_bounds__(256) void grad_norm_final_kernel(const double* __restrict__ partial, int n, int inf, float* norm_out) {
+    const double norm = gn_total(partial, n, inf != 0);
+    if (threadIdx.x == 0) *norm_out = (float)norm;
+}
+
+__global__ __launch_bounds__(256) void grad_clip_kernel(GradTable t, const double* __restrict__ partial, int n_partial, int inf,
+                                                        double max_norm, int in_place, float* norm_out) {
+    const double norm = gn_total(partial, n_partial, inf != 0);
+    if (norm_out != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
+    const double q = max_norm / (norm + 1e-6);
+    const float coef = q > 1.0 ? 1.f : (float)q;          // a NaN norm stays NaN, as in the arithmetic it stands for
+    if (in_place && coef == 1.f) return;                   // x 1 in place is what is there
+    const int total = t.first[t.count];
+    for (int c = blockIdx.x; c < total; c += gridDim.x) {
+        const int k = gn_tensor_of(t, c);
+        const size_t begin = (size_t)(c - t.first[k]) << t.chunk_log2;
+        const size_t end = min((size_t)t.n[k], begin + ((size_t)1 << t.chunk_log2));
+        const int type = t.type[k] & 15, otype = t.type[k] >> 4;
+        size_t i = begin + threadIdx.x * 8;
+        for (; i + 8 <= end; i += 2048) {
+            float v[8];
+            gn_load8(t.in[k], i, type, v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] *= coef;
+            if (otype == SM_TYPE_F32) {
+                g_u32x4_u* o = reinterpret_cast<g_u32x4_u*>(static_cast<float*>(t.out[k]) + i);
+                g_u32x4 a, b;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    a[j] = __builtin_bit_cast(unsigned, v[j]);
+                    b[j] = __builtin_bit_cast(unsigned, v[4 + j]);
+                }
+                o[0] = a;
+                o[1] = b;
+            } else {
+                g_u32x4 a;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) a[j] = gn_down(v[2 * j], otype) | (gn_down(v[2 * j + 1], otype) << 16);
+                *reinterpret_cast<g_u32x4_u*>(static_cast<uint16_t*>(t.out[k]) + i) = a;
+            }
+        }
+        for (; i < end; ++i) {
+            const float x = gn_load1(t.in[k], i, type) * coef;
+            if (otype == SM_TYPE_F32) static_cast<float*>(t.out[k])[i] = x;
+            else static_cast<uint16_t*>(t.out[k])[i] = (uint16_t)gn_down(x, otype);
+        }
+    }
+}
+
+}  // namespace sm
+
+namespace {
+
+// chunks of 4096 elements (two rounds of a block's 8-element loads), or as many more as keep a launch's chunks within an int
+int chunk_log2_of(unsigned long long total) {
+    int l = 12;
+    while ((total >> l) > (1ull << 28)) ++l;
+    return l;
+}
+
+// table of tensors [first, first + count) of a call; returns its chunks
+int fill_table(sm::GradTable& t, const void* const* in, void* const* out, const size_t* numel, const int* types, const int* out_types,
+               int first, int count, int chunk_log2) {
+    t.count = count;
+    t.chunk_log2 = chunk_log2;
+    t.first[0] = 0;
+    for (int i = 0; i < count; ++i) {
+        t.in[i] = in[first + i];
+        t.out[i] = out == nullptr ? nullptr : out[first + i];
+        t.n[i] = numel[first + i];
+        const int ty = types[first + i], oty = out_types == nullptr ? ty : out_types[first + i];
+        t.type[i] = (uint8_t)(ty | (oty << 4));
+        t.first[i + 1] = t.first[i] + (int)((numel[first + i] + ((size_t)1 << chunk_log2) - 1) >> chunk_log2);
+    }
+    return t.first[count];
+}
+
+int check_list(const void* const* in, const size_t* numel, const int* types, int n, unsigned long long* total) {
+    *total = 0;
+    if (n < 0 || (n > 0 && (in == nullptr || numel == nullptr || types == nullptr))) return (int)hipErrorInvalidValue;
+    for (int i = 0; i < n; ++i) {
+        if (types[i] < 0 || types[i] > SM_TYPE_F16 || (numel[i] > 0 && in[i] == nullptr)) return (int)hipErrorInvalidValue;
+        *total += numel[i];
+    }
+    return *total >> 40 ? (int)hipErrorInvalidValue : 0;
+}
+
+// partial sums of every launch of the call into ws; *n_partial = their number
+int launch_partials(const void* const* grads, const size_t* numel, const int* types, int n, int inf, int chunk_log2, double* ws,
+                    size_t ws_doubles, int* n_partial, hipStream_t s) {
+    *n_partial = 0;
+    for (int f = 0; f < n; f += sm::GN_TENSORS) {
+        sm::GradTable t;
+        const int chunks = fill_table(t, grads, nullptr, numel, types, nullptr, f, n - f < sm::GN_TENSORS ? n - f : sm::GN_TENSORS, chunk_log2);
+        if (chunks == 0) continue;
+        const int blocks = chunks < sm::GN_PARTIALS ? chunks : sm::GN_PARTIALS;
+        if ((size_t)(*n_partial + blocks) > ws_doubles) return (int)hipErrorInvalidValue;
+        hipLaunchKernelGGL(sm::grad_norm_partial_kernel, dim3((unsigned)blocks), dim3(256), 0, s, t, inf, ws + *n_partial);
+        SM_LAUNCH_CHECK();
+        *n_partial += blocks;
+    }
+    return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t sm_grad_norm_ws_bytes(int n_tensors) {
+    const int launches = n_tensors <= 0 ? 1 : (n_tensors + sm::GN_TENSORS - 1) / sm::GN_TENSORS;
+    return (size_t)launches * sm::GN_PARTIALS * sizeof(double);
+}
+
+int sm_grad_norm(const void* const* grads, const size_t* numel, const int* types, int n, int inf_norm, void* ws, size_t ws_bytes,
+                 float* norm_out, void* stream) {
+    unsigned long long total;
+    if (const int e = check_list(grads, numel, types, n, &total)) return e;
+    if (norm_out == nullptr || ws == nullptr) return (int)hipErrorInvalidValue;
+    hipStream_t s = (hipStream_t)stream;
+    int n_partial = 0;
+    if (const int e = launch_partials(grads, numel, types, n, inf_norm, chunk_log2_of(total), (double*)ws, ws_bytes / sizeof(double), &n_partial, s))
+        return e;
+    hipLaunchKernelGGL(sm::grad_norm_final_kernel, dim3(1), dim3(256), 0, s, (const double*)ws, n_partial, inf_norm, norm_out);
+    SM_LAUNCH_CHECK();
+    return 0;
+}
+
+int sm_grad_clip(const void* const* grads, void* const* out, const size_t* numel, const int* types, const int* out_types, int n,
+                 int inf_norm, double max_norm, void* ws, size_t ws_bytes, float* norm_out, void* stream) {
+    unsigned long long total;
+    if (const int e = check_list(grads, numel, types, n, &total)) return e;
+    if (norm_out == nullptr || ws == nullptr || !(max_norm >= 0.0) || (n > 0 && (out == nullptr || out_types == nullptr)))
+        return (int)hipErrorInvalidValue;
+    int in_place = 1;
+    for (int i = 0; i < n; ++i) {
+        if (out_types[i] < 0 || out_types[i] > SM_TYPE_F16 || (numel[i] > 0 && out[i] == nullptr)) return (int)hipErrorInvalidValue;
+        if (numel[i] == 0) continue;
+        if (out[i] != grads[i]) in_place = 0;
+        else if (out_types[i] != types[i]) return (int)hipErrorInvalidValue;
+    }
+    hipStream_t s = (hipStream_t)stream;
+    const int cl = chunk_log2_of(total);
+    int n_partial = 0;
+    if (const int e = launch_partials(grads, numel, types, n, inf_norm, cl, (double*)ws, ws_bytes / sizeof(double), &n_partial, s)) return e;
+    bool told = false;
+    for (int f = 0; f < n; f += sm::GN_TENSORS) {
+        sm::GradTable t;
+        const int chunks = fill_table(t, grads, out, numel, types, out_types, f, n - f < sm::GN_TENSORS ? n - f : sm::GN_TENSORS, cl);
+        if (chunks == 0) continue;
+        const int blocks = chunks < 2048 ? chunks : 2048;
+        hipLaunchKernelGGL(sm::grad_clip_kernel, dim3((unsigned)blocks), dim3(256), 0, s, t, (const double*)ws, n_partial, inf_norm,
+                           max_norm, in_place, told ? nullptr : norm_out);
+        SM_LAUNCH_CHECK();
+        told = true;
+    }
+    if (!told) {      // no element at all: the norm is 0
+        hipLaunchKernelGGL(sm::grad_norm_final_kernel, dim3(1), dim3(256), 0, s, (const double*)ws, 0, inf_norm, norm_out);
+        SM_LAUNCH_CHECK();
+    }
+    return 0;
+}
+
+}  // extern "C"

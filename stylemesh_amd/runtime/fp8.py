@@ -1,0 +1,278 @@
+"""Matrices in 8-bit floating point with one scale per block of 128, their products and a layer's forward / backward pass
+over them (``sm_fp8_*``; csrc/fp8.hip). The rung below the library's fp16x2 arithmetic for products that tolerate 8 bits:
+feature maps against filters, activations against a resident weight, and the gradient products of a training step.
+
+Every call is asynchronous on torch's current stream, allocates its results (and, for a product that splits its depth, its
+scratch) from torch's allocator and synchronises nothing. There is no autograd node: ``linear_fp8_fwd`` /
+``linear_fp8_bwd`` are the two halves of a step, as the sampler's and the losses' are (``ops.tex_sample_fwd`` / ``_bwd``).
+"""
+from __future__ import annotations
+
+import torch
+
+from . import hip, ops
+from .hip import ptr
+
+BLOCK = 128
+FORMATS = {"e4m3": torch.float8_e4m3fn, "e5m2": torch.float8_e5m2}
+_FMT_ID = {torch.float8_e4m3fn: 0, torch.float8_e5m2: 1}                      # SM_FP8_*
+_TYPE_ID = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}           # SM_TYPE_*
+_MAX_DIM = 65535 * 128       # rows / columns of a matrix (the quantiser's grid)
+
+
+def _blocks(n: int) -> int:
+    return -(-n // BLOCK)
+
+
+def _check_device(*tensors):
+    """Launches go to the CURRENT device's current stream: tensors of another device (or of the host) are refused."""
+    cur = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError("device tensors only (there is no CPU form)")
+        if cur is None:
+            cur = torch.cuda.current_device()
+        if t.device.index != cur:
+            raise ValueError(f"a tensor lives on {t.device}, the current device is cuda:{cur}")
+
+
+class Fp8Matrix:
+    """[rows, cols] as 8-bit codes and block scales: value = code * scale of its block.
+
+    ``data``: float8_e4m3fn / float8_e5m2 [rows, cols rounded up to 128], contiguous; the codes behind column ``cols`` must be
+    ZERO (the product runs over whole blocks; ``from_parts`` pads). ``block``: "rows" - a scale per row and 128 columns - or
+    "tiles" - per 128 x 128 tile. ``scale``: uint8 power-of-two scales [ceil(KB / 4), S, 4], byte s = 2^(s - 127), the byte of
+    (row, block kb) at [kb / 4, row, kb % 4], KB = ceil(cols / 128), S = rows or ceil(rows / 128) - or float32 scales [KB, S].
+    The tensors are used as they are, no copy is taken."""
+
+    __slots__ = ("data", "scale", "cols", "block")
+
+    def __init__(self, data: torch.Tensor, scale: torch.Tensor, cols: int, block: str = "rows"):
+        if block not in ("rows", "tiles"):
+            raise ValueError(f"block={block!r}: 'rows' or 'tiles'")
+        if data.dtype not in _FMT_ID:
+            raise ValueError(f"codes of type {data.dtype}: float8_e4m3fn or float8_e5m2")
+        if data.dim() != 2 or not data.is_contiguous() or cols < 0 or data.shape[1] != _blocks(cols) * BLOCK:
+            raise ValueError(f"codes must be contiguous [rows, {_blocks(max(cols, 0)) * BLOCK}] for {cols} columns, got "
+                             f"{tuple(data.shape)}, strides {data.stride()}")
+        if data.data_ptr() % 16:
+            raise ValueError("codes must start on a 16-byte boundary")
+        kb, s = _blocks(cols), data.shape[0] if block == "rows" else _blocks(data.shape[0])
+        want = {torch.uint8: (-(-kb // 4), s, 4), torch.float32: (kb, s)}.get(scale.dtype)
+        if want is None or tuple(scale.shape) != want or not scale.is_contiguous():
+            raise ValueError(f"scales must be contiguous uint8 {(-(-kb // 4), s, 4)} or float32 {(kb, s)}, got {scale.dtype} "
+                             f"{tuple(scale.shape)}")
+        if scale.device != data.device:
+            raise ValueError(f"codes on {data.device}, scales on {scale.device}")
+        self.data, self.scale, self.cols, self.block = data, scale, int(cols), block
+
+    @property
+    def rows(self) -> int:
+        return self.data.shape[0]
+
+    @property
+    def shape(self):
+        return (self.data.shape[0], self.cols)
+
+    @property
+    def device(self):
+        return self.data.device
+
+    @classmethod
+    def from_parts(cls, codes: torch.Tensor, scale: torch.Tensor, block: str = "rows") -> "Fp8Matrix":
+        """From codes [rows, cols] of any strides and scales [S, KB] as checkpoints hold them - int32 / uint8 exponent
+        bytes (2^(s - 127)) or float32 - in this class's layout (copies: once per weight, not per call)."""
+        if codes.dim() != 2:
+            raise ValueError(f"codes must be a matrix, got {tuple(codes.shape)}")
+        rows, cols = codes.shape
+        kb, s = _blocks(cols), rows if block == "rows" else _blocks(rows)
+        if tuple(scale.shape) != (s, kb):
+            raise ValueError(f"scales must be {(s, kb)} for {block} of {(rows, cols)}, got {tuple(scale.shape)}")
+        data = torch.zeros(rows, kb * BLOCK, dtype=torch.uint8, device=codes.device)
+        data[:, :cols] = codes.contiguous().view(torch.uint8)
+        if scale.dtype == torch.float32:
+            packed = scale.t().contiguous()
+        elif scale.dtype in (torch.uint8, torch.int32):
+            packed = pack_scale_bytes(scale)
+        else:
+            raise ValueError(f"scales of type {scale.dtype}: float32, or exponent bytes as uint8 / int32")
+        return cls(data.view(codes.dtype), packed, cols, block)
+
+    def scales(self) -> torch.Tensor:
+        """The scales as float32 [S, KB]."""
+        if self.scale.dtype == torch.float32:
+            return self.scale.t()
+        e = self.scale.permute(1, 0, 2).reshape(self.scale.shape[1], -1)[:, :_blocks(self.cols)].int()
+        # 2^(e - 127) from the bits; byte 0 is 2^-127 (a subnormal fp32), 255 is NaN
+        bits = torch.where(e == 255, 0x7fc00000, torch.where(e == 0, 0x00400000, e << 23))
+        return bits.view(torch.float32)
+
+    def dequantize(self) -> torch.Tensor:
+        """float32 [rows, cols] (torch operations: for reports and tests)."""
+        s = self.scales().repeat_interleave(BLOCK, dim=1)
+        if self.block == "tiles":
+            s = s.repeat_interleave(BLOCK, dim=0)[:self.rows]
+        return (self.data.float() * s)[:, :self.cols]
+
+    def transposed(self) -> "Fp8Matrix":
+        """The transpose of a ``tiles`` matrix - its tiles are the transpose's tiles, the codes are the same (a copy: once per
+        weight update; ``fp8_quantize_both(w, block="tiles")`` makes both from the weight in one pass). Row scales have no
+        such transpose: ``ValueError``."""
+        if self.block != "tiles":
+            raise ValueError("only a matrix with tile scales can be transposed as it is (row blocks become column blocks)")
+        rows, cols = self.shape
+        data = torch.zeros(cols, _blocks(rows) * BLOCK, dtype=torch.uint8, device=self.device)
+        data[:, :rows] = self.data.view(torch.uint8)[:, :cols].t()
+        if self.scale.dtype == torch.float32:
+            scale = self.scale.t().contiguous()
+        else:
+            e = self.scale.permute(1, 0, 2).reshape(self.scale.shape[1], -1)[:, :_blocks(cols)]
+            scale = pack_scale_bytes(e.t())
+        return Fp8Matrix(data.view(self.data.dtype), scale, rows, "tiles")
+
+
+def pack_scale_bytes(e: torch.Tensor) -> torch.Tensor:
+    """Exponent bytes [S, KB] -> the stored form [ceil(KB / 4), S, 4] (uint8, padded with 127 = 1.0)."""
+    e = torch.nn.functional.pad(e.to(torch.uint8), (0, -e.shape[1] % 4), value=127)
+    return e.view(e.shape[0], -1, 4).permute(1, 0, 2).contiguous()
+
+
+def _matrix_arg(x, what):
+    if not torch.is_tensor(x) or x.dim() != 2 or x.dtype not in _TYPE_ID:
+        raise ValueError(f"{what} must be a float32 / bfloat16 / float16 matrix, got "
+                         f"{(x.dtype, tuple(x.shape)) if torch.is_tensor(x) else type(x)}")
+    # (the stride of a dimension of one element means nothing)
+    if (x.shape[1] > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
+        raise ValueError(f"{what} must have unit column stride and rows that do not overlap, got strides {x.stride()} for "
+                         f"{tuple(x.shape)}; pass .contiguous(), or transpose=True for a transposed matrix")
+    if max(x.shape) > _MAX_DIM:
+        raise ValueError(f"{what}: {tuple(x.shape)} has a dimension above {_MAX_DIM}")
+    _check_device(x)
+    return x
+
+
+def _empty(rows, cols, fmt, block, device):
+    kb, s = _blocks(cols), rows if block == "rows" else _blocks(rows)
+    return (torch.empty(rows, kb * BLOCK, dtype=FORMATS[fmt], device=device),
+            torch.empty(-(-kb // 4), s, 4, dtype=torch.uint8, device=device))
+
+
+def _quantize(x, block, fmt, plain, transpose):
+    x = _matrix_arg(x, "x")
+    if fmt not in FORMATS:
+        raise ValueError(f"fmt={fmt!r}: 'e4m3' or 'e5m2'")
+    if block not in ("rows", "tiles"):
+        raise ValueError(f"block={block!r}: 'rows' or 'tiles'")
+    rows, cols = x.shape
+    q, qs = _empty(rows, cols, fmt, block, x.device) if plain else (None, None)
+    qt, qts = _empty(cols, rows, fmt, block, x.device) if transpose else (None, None)
+    stride = x.stride(0) if rows > 1 else max(cols, 1)
+    if rows and cols:
+        hip.check(ops.lib.sm_fp8_quantize(x.data_ptr(), _TYPE_ID[x.dtype], rows, cols, stride, _FMT_ID[FORMATS[fmt]],
+                                          int(block == "tiles"), ptr(q), ptr(qs), ptr(qt), ptr(qts), hip.stream()),
+                  "sm_fp8_quantize")
+    return (Fp8Matrix(q, qs, cols, block) if plain else None, Fp8Matrix(qt, qts, rows, block) if transpose else None)
+
+
+def fp8_quantize(x: torch.Tensor, block: str = "rows", fmt: str = "e4m3", transpose: bool = False) -> Fp8Matrix:
+    """``x`` [rows, cols] (float32 / bfloat16 / float16, unit column stride, any row stride) - or, with ``transpose``, its
+    transpose - as an ``Fp8Matrix`` with power-of-two scales: per block the smallest power of two that brings the largest
+    finite magnitude into the format's range; x / scale is exact, the code is it rounded to nearest even. NaN stays NaN, an
+    infinity becomes NaN (e4m3 has none) or infinity (e5m2); neither touches its neighbours' scale."""
+    n, t = _quantize(x, block, fmt, not transpose, transpose)
+    return t if transpose else n
+
+
+def fp8_quantize_both(x: torch.Tensor, block: str = "rows", fmt: str = "e4m3"):
+    """(``fp8_quantize(x)``, ``fp8_quantize(x, transpose=True)``) from one read of ``x``: what a training step needs of its
+    activations and output gradients (rows) and of its weights (tiles)."""
+    return _quantize(x, block, fmt, True, True)
+
+
+def matmul_fp8(a: Fp8Matrix, b: Fp8Matrix, out: torch.Tensor | None = None, out_dtype=None, accumulate: bool = False) -> torch.Tensor:
+    """[M, N] = A B^T for A [M, K] (``rows`` scales, e4m3 or e5m2) and B [N, K] (e4m3, ``rows`` or ``tiles`` scales), both with
+    power-of-two or both with float32 scales; fp32 accumulate, one rounding to ``out_dtype`` (float32 / bfloat16 / float16;
+    default bfloat16). ``out``: result of that type and shape, unit column stride; ``accumulate``: added to it (in fp32, then
+    rounded once)."""
+    if not isinstance(a, Fp8Matrix) or not isinstance(b, Fp8Matrix):
+        raise ValueError("matmul_fp8 takes two Fp8Matrix operands")
+    if a.block != "rows":
+        raise ValueError("the first operand needs row scales")
+    if b.data.dtype != torch.float8_e4m3fn:
+        raise ValueError("the second operand must be e4m3")
+    if a.cols != b.cols:
+        raise ValueError(f"inner dimensions differ: {a.shape} x {b.shape}^T")
+    if a.scale.dtype != b.scale.dtype:
+        raise ValueError(f"one operand has {a.scale.dtype} scales, the other {b.scale.dtype}")
+    M, N, K = a.rows, b.rows, a.cols
+    if max(M, N) > _MAX_DIM:
+        raise ValueError(f"a dimension above {_MAX_DIM}")
+    _check_device(a.data, b.data, out)
+    if out is None:
+        if accumulate:
+            raise ValueError("accumulate needs out")
+        out = torch.empty(M, N, dtype=out_dtype or torch.bfloat16, device=a.device)
+        if out.dtype not in _TYPE_ID:
+            raise ValueError(f"out_dtype={out_dtype}: float32, bfloat16 or float16")
+    else:
+        _matrix_arg(out, "out")
+        if tuple(out.shape) != (M, N) or (out_dtype is not None and out.dtype != out_dtype):
+            raise ValueError(f"out is {out.dtype} {tuple(out.shape)}, the product {out_dtype or out.dtype} {(M, N)}")
+    if M == 0 or N == 0:
+        return out
+    need = ops.lib.sm_fp8_matmul_ws_bytes(M, N, K)
+    # (scratch of this call's own: two captured graphs, or two streams, never share slabs)
+    ws = torch.empty(need, dtype=torch.uint8, device=a.device) if need else None
+    hip.check(ops.lib.sm_fp8_matmul(a.data.data_ptr(), a.scale.data_ptr(), _FMT_ID[a.data.dtype], a.data.shape[1],
+                                    b.data.data_ptr(), b.scale.data_ptr(), int(b.block == "tiles"), b.data.shape[1],
+                                    int(a.scale.dtype == torch.float32), M, N, K, out.data_ptr(), _TYPE_ID[out.dtype],
+                                    out.stride(0) if M > 1 else N, int(accumulate), ptr(ws), need, hip.stream()), "sm_fp8_matmul")
+    return out
+
+
+def _weight_arg(w, what="weight"):
+    if not isinstance(w, Fp8Matrix) or w.data.dtype != torch.float8_e4m3fn or w.scale.dtype != torch.uint8:
+        raise ValueError(f"{what} must be an e4m3 Fp8Matrix with power-of-two scales")
+    return w
+
+
+def linear_fp8_fwd(x: torch.Tensor, weight: Fp8Matrix, out_dtype=None, keep_transposed: bool = False):
+    """y [M, N] = q(x) weight^T for x [M, K] and a resident weight [N, K] (``fp8_quantize(w, block="tiles")``), in ``out_dtype``
+    (default: x's). ``keep_transposed``: returns (y, q(x^T)), the second for ``linear_fp8_bwd``'s weight gradient - quantised
+    from the same read of x."""
+    _weight_arg(weight)
+    _matrix_arg(x, "x")
+    if x.shape[1] != weight.cols:
+        raise ValueError(f"x has {x.shape[1]} columns, the weight {weight.cols}")
+    n, t = _quantize(x, "rows", "e4m3", True, keep_transposed)
+    y = matmul_fp8(n, weight, out_dtype=out_dtype or x.dtype)
+    return (y, t) if keep_transposed else y
+
+
+def linear_fp8_bwd(dy: torch.Tensor, x_t: Fp8Matrix | None, weight_t: Fp8Matrix | None, fmt: str = "e4m3", dx_dtype=None,
+                   dw: torch.Tensor | None = None, accumulate: bool = False):
+    """(dx, dw) of ``linear_fp8_fwd``'s layer: dx [M, K] = q(dy) weight (in ``dx_dtype``, default dy's) from
+    ``weight_t`` = the weight's transpose [K, N] (``weight.transposed()`` / ``fp8_quantize_both(w, block="tiles")[1]``), and
+    dw [N, K] = q(dy^T) q(x^T)^T in float32 from ``x_t`` = [K, M] (``keep_transposed``). ``fmt``: format of the gradient's
+    codes. ``dw`` / ``accumulate``: write into, or add to, an existing float32 gradient. Either of ``x_t`` / ``weight_t`` may be
+    None: that gradient is not computed and None is returned in its place."""
+    _matrix_arg(dy, "dy")
+    M, N = dy.shape
+    if x_t is None and weight_t is None:
+        raise ValueError("nothing to compute: both x_t and weight_t are None")
+    if weight_t is not None and _weight_arg(weight_t, "weight_t").cols != N:
+        raise ValueError(f"dy has {N} columns, weight_t {weight_t.cols}")
+    if x_t is not None:
+        if _weight_arg(x_t, "x_t").cols != M:
+            raise ValueError(f"dy has {M} rows, x_t {x_t.cols} columns")
+        if dw is not None and dw.dtype != torch.float32:
+            raise ValueError(f"dw must be float32, got {dw.dtype}")
+    elif dw is not None:
+        raise ValueError("dw given, but no x_t to compute it from")
+    n, t = _quantize(dy, "rows", fmt, weight_t is not None, x_t is not None)
+    dx = matmul_fp8(n, weight_t, out_dtype=dx_dtype or dy.dtype) if weight_t is not None else None
+    if x_t is not None:
+        dw = matmul_fp8(t, x_t, out=dw, out_dtype=torch.float32, accumulate=accumulate)
+    return dx, dw

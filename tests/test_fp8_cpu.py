@@ -1,0 +1,101 @@
+"""What the 8-bit block-scaled operators refuse (no launch: runs without a GPU)."""
+import pytest
+import torch
+
+import fp8_ref as R
+from stylemesh_amd.runtime import fp8, hip
+
+E4, E5 = torch.float8_e4m3fn, torch.float8_e5m2
+
+
+def mat(rows, cols, block="rows", dtype=E4, scale="e8m0"):
+    kb, s = -(-cols // 128), rows if block == "rows" else -(-rows // 128)
+    sc = torch.full((-(-kb // 4), s, 4), 127, dtype=torch.uint8) if scale == "e8m0" else torch.ones(kb, s)
+    return fp8.Fp8Matrix(torch.zeros(rows, kb * 128, dtype=torch.uint8).view(dtype), sc, cols, block)
+
+
+def test_matrix_refusals():
+    d, s = torch.zeros(4, 256, dtype=torch.uint8).view(E4), torch.full((1, 4, 4), 127, dtype=torch.uint8)
+    assert fp8.Fp8Matrix(d, s, 200).shape == (4, 200)
+    bad = [lambda: fp8.Fp8Matrix(d, s, 300), lambda: fp8.Fp8Matrix(d, s, 100), lambda: fp8.Fp8Matrix(d, s, -1),
+           lambda: fp8.Fp8Matrix(d, s, 200, "columns"), lambda: fp8.Fp8Matrix(d.view(torch.uint8), s, 200),
+           lambda: fp8.Fp8Matrix(d, s[:, :3], 200), lambda: fp8.Fp8Matrix(d, s, 200, "tiles"), lambda: fp8.Fp8Matrix(d, s.int(), 200),
+           lambda: fp8.Fp8Matrix(d, torch.ones(4, 2), 200), lambda: fp8.Fp8Matrix(d[:, :128], s, 100), lambda: fp8.Fp8Matrix(d[0], s, 200),
+           lambda: fp8.Fp8Matrix(torch.zeros(4 * 256 + 1, dtype=torch.uint8)[1:].view(4, 256).view(E4), s, 200),
+           lambda: fp8.Fp8Matrix.from_parts(d, torch.ones(4, 3)), lambda: fp8.Fp8Matrix.from_parts(d[0], torch.ones(4, 2)),
+           lambda: fp8.Fp8Matrix.from_parts(d, torch.ones(4, 2).double()), lambda: mat(4, 200).transposed()]
+    for f in bad:
+        with pytest.raises(ValueError):
+            f()
+
+
+def test_quantize_refusals():
+    x = torch.zeros(4, 8)
+    for f in (lambda: fp8.fp8_quantize(x), lambda: fp8.fp8_quantize(x, fmt="e3m4"), lambda: fp8.fp8_quantize(x, block="cols"),
+              lambda: fp8.fp8_quantize(x.double()), lambda: fp8.fp8_quantize(x[0]), lambda: fp8.fp8_quantize(x.t()),
+              lambda: fp8.fp8_quantize(x[:, ::2]), lambda: fp8.fp8_quantize(x[:1].expand(4, 8)), lambda: fp8.fp8_quantize_both(x.int()),
+              lambda: fp8.fp8_quantize(None), lambda: fp8.fp8_quantize(torch.zeros(1, 1).expand(1, 65535 * 128 + 1))):
+        with pytest.raises(ValueError):
+            f()
+
+
+def test_product_refusals():
+    a, b = mat(4, 200), mat(6, 200)
+    x, out = torch.zeros(4, 200), torch.zeros(4, 6)
+    for f in (lambda: fp8.matmul_fp8(a, b), lambda: fp8.matmul_fp8(a, mat(6, 201)), lambda: fp8.matmul_fp8(mat(4, 200, "tiles"), b),
+              lambda: fp8.matmul_fp8(a, mat(6, 200, dtype=E5)), lambda: fp8.matmul_fp8(a, mat(6, 200, scale="f32")),
+              lambda: fp8.matmul_fp8(a, out), lambda: fp8.matmul_fp8(a, b, accumulate=True), lambda: fp8.matmul_fp8(a, b, out=out),
+              lambda: fp8.linear_fp8_fwd(x, a), lambda: fp8.linear_fp8_fwd(x, mat(6, 300)), lambda: fp8.linear_fp8_fwd(x, x),
+              lambda: fp8.linear_fp8_fwd(x, mat(6, 200, scale="f32")), lambda: fp8.linear_fp8_bwd(x, None, None),
+              lambda: fp8.linear_fp8_bwd(x, mat(8, 4), mat(8, 200, "tiles"), dw=torch.zeros(200, 8).half()),
+              lambda: fp8.linear_fp8_bwd(x, None, mat(8, 200, "tiles"), dw=torch.zeros(200, 8))):
+        with pytest.raises(ValueError):
+            f()
+
+
+def test_c_entry_refusals():
+    """Bad arguments come back as an error code before anything is launched."""
+    lib = hip.lib
+    q = lambda *a: lib.sm_fp8_quantize(*a)
+    buf = torch.zeros(1 << 16, dtype=torch.uint8)
+    p = buf.data_ptr() + (-buf.data_ptr()) % 16
+    assert q(p, 0, 4, 8, 8, 0, 0, None, None, None, None, None) != 0
+    assert q(p, 0, 4, 8, 8, 0, 0, p, None, None, None, None) != 0
+    assert q(p, 3, 4, 8, 8, 0, 0, p, p, None, None, None) != 0
+    assert q(p, 0, 4, 8, 8, 2, 0, p, p, None, None, None) != 0
+    assert q(p, 0, 4, 8, 7, 0, 0, p, p, None, None, None) != 0
+    assert q(p, 0, -1, 8, 8, 0, 0, p, p, None, None, None) != 0
+    assert q(None, 0, 4, 8, 8, 0, 0, p, p, None, None, None) != 0
+    assert q(p, 0, 0, 8, 8, 0, 0, p, p, None, None, None) == 0
+    ok = [p, p, 0, 256, p, p, 0, 256, 0, 4, 6, 200, p, 0, 6, 0, None, 0, None]
+    m = lambda **k: lib.sm_fp8_matmul(*[k.get(f"a{i}", v) for i, v in enumerate(ok)])
+    for bad in (dict(a0=None), dict(a1=None), dict(a2=2), dict(a3=128), dict(a3=250), dict(a0=p + 1), dict(a4=None), dict(a7=100), dict(a9=-1),
+                dict(a12=None), dict(a13=3), dict(a14=5)):
+        assert m(**bad) != 0, bad
+    assert m(a9=0) == 0 and m(a10=0) == 0
+    # a product that splits its depth needs its scratch
+    need = lib.sm_fp8_matmul_ws_bytes(1, 16, 1 << 20)
+    if need:
+        assert m(a9=1, a10=16, a11=1 << 20, a3=1 << 20, a7=1 << 20, a14=16, a16=p, a17=need - 1) != 0
+    assert lib.sm_fp8_matmul_ws_bytes(0, 5, 5) == 0 and lib.sm_fp8_matmul_ws_bytes(5, -1, 5) == 0
+
+
+def test_reference_rounding_is_the_types_own():
+    """The oracle's grid against torch's casts, over all codes and midpoints."""
+    for fmt, dt in fp8.FORMATS.items():
+        v = torch.arange(256, dtype=torch.uint8).view(dt).float()
+        v = v[torch.isfinite(v)]
+        v = torch.cat([v, (v[1:] + v[:-1]) / 2]).double()
+        assert torch.equal(R.round_to(v, fmt), v.float().to(dt).double())
+    assert R.exponent(448.0, "e4m3") == 0 and R.exponent(448.1, "e4m3") == 1 and R.exponent(224.0, "e4m3") == -1 and R.exponent(0.0, "e4m3") == 0
+
+
+def test_scale_bytes_round_trip():
+    e = torch.randint(0, 256, (5, 7), dtype=torch.int32)
+    m = fp8.Fp8Matrix.from_parts(torch.zeros(5, 800, dtype=torch.uint8).view(E4), e)
+    assert tuple(m.scale.shape) == (2, 5, 4) and int(m.scale[1, 2, 1]) == int(e[2, 5]) and int(m.scale[1, 2, 3]) == 127
+    want = torch.pow(torch.tensor(2.0, dtype=torch.float64), e.double() - 127)
+    got = m.scales().double()
+    assert torch.equal(got[e < 255], want[e < 255]) and torch.isnan(got[e == 255]).all()
+    t = fp8.Fp8Matrix.from_parts(torch.zeros(300, 700, dtype=torch.uint8).view(E4), e[:3, :6], "tiles").transposed()
+    assert t.shape == (700, 300) and torch.equal(t.scales()[e[:3, :6].t() < 255], want[:3, :6].t()[e[:3, :6].t() < 255].float())

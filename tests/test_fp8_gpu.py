@@ -1,0 +1,414 @@
+"""8-bit block-scaled matrices (runtime/fp8.py) against their definition in 64 bits (fp8_ref.py)."""
+import math
+
+import pytest
+import torch
+
+import fp8_ref as R
+from gpu_util import require_gpu
+
+pytestmark = pytest.mark.gpu
+DT = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+
+
+def _fp8():
+    require_gpu()
+    from stylemesh_amd.runtime import fp8
+    return fp8
+
+
+def _rand(rows, cols, seed, dtype=torch.float32, spread=4.0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(rows, cols, generator=g) * torch.exp(spread * torch.randn(rows, 1, generator=g))
+    return x.clamp(-6e4, 6e4).to(dtype)
+
+
+def _check_matrix(q, x, block, fmt):
+    """codes, scale bytes and padding of ``q`` are exactly the definition's"""
+    vals, exps = R.quantize(x, block, fmt)
+    got = q.data.float().double().cpu()
+    assert tuple(got.shape) == tuple(vals.shape)
+    torch.testing.assert_close(got, vals, rtol=0, atol=0, equal_nan=True)
+    kb = exps.shape[1]
+    want = torch.full((-(-kb // 4), exps.shape[0], 4), 127, dtype=torch.uint8)
+    for j in range(kb):
+        want[j // 4, :, j % 4] = (exps[:, j] + 127).to(torch.uint8)
+    assert torch.equal(q.scale.cpu(), want)
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 128), (1, 129), (3, 127), (128, 128), (129, 640), (257, 385), (16, 4096), (1000, 5)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("fmt", ["e4m3", "e5m2"])
+def test_quantize_is_the_definition(rows, cols, dtype, fmt):
+    fp8 = _fp8()
+    x = _rand(rows, cols, rows * 7 + cols, DT[dtype])
+    xd = x.cuda()
+    for block in ("rows", "tiles"):
+        _check_matrix(fp8.fp8_quantize(xd, block, fmt), x, block, fmt)
+        _check_matrix(fp8.fp8_quantize(xd, block, fmt, transpose=True), x.t(), block, fmt)
+        n, t = fp8.fp8_quantize_both(xd, block, fmt)
+        _check_matrix(n, x, block, fmt)
+        _check_matrix(t, x.t(), block, fmt)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "e5m2"])
+@pytest.mark.parametrize("block", ["rows", "tiles"])
+def test_quantize_extreme_values(fmt, block):
+    """Zeros, subnormals, the largest floats, values at the rounding borders and exactly at the format's limit, NaN and
+    infinities (which must leave their block's scale alone)."""
+    fp8 = _fp8()
+    big, tiny = torch.finfo(torch.float32).max, 2.0 ** -149
+    rows = [[0.0, -0.0, 0.0], [tiny, -tiny, 3 * tiny], [big, -big, 1.0], [448.0, 447.9999, 1.0], [448.0001, 1.0, -2.0],
+            [57344.0, 57345.0, 3.0], [1.0, 1.0625, 1.1875], [float("nan"), 2.0, 3.0], [float("inf"), 5.0, -0.25],
+            [float("-inf"), float("nan"), 0.0], [2.0 ** -126, 2.0 ** -127, 2.0 ** -140], [2.0 ** 119, 2.0 ** 127 * 1.75, 1e30]]
+    x = torch.zeros(128 * len(rows), 200)
+    for i, r in enumerate(rows):
+        x[128 * i, :3] = torch.tensor(r)
+        x[128 * i + 5, 150:153] = torch.tensor(r)
+    _check_matrix(fp8.fp8_quantize(x.cuda(), block, fmt), x, block, fmt)
+    _check_matrix(fp8.fp8_quantize(x.cuda(), block, fmt, transpose=True), x.t(), block, fmt)
+
+
+def test_quantize_every_rounding_border():
+    """All codes' values and the midpoints between neighbours, shifted by one fp32 step either way."""
+    fp8 = _fp8()
+    for fmt, dt in fp8.FORMATS.items():
+        v = torch.arange(256, dtype=torch.uint8).view(dt).float()
+        v = v[torch.isfinite(v)].sort().values
+        mid = (v[1:] + v[:-1]) / 2
+        pts = torch.cat([v, mid, torch.nextafter(mid, mid + 1), torch.nextafter(mid, mid - 1)])
+        x = torch.zeros(pts.numel(), 130)
+        x[:, 0], x[:, 1] = pts, R.LIMIT[fmt]
+        _check_matrix(fp8.fp8_quantize(x.cuda(), "rows", fmt), x, "rows", fmt)
+
+
+def test_quantize_strided_offset_and_empty():
+    fp8 = _fp8()
+    base = _rand(50, 401, 5).cuda()
+    for dt in DT.values():
+        b = base.to(dt)
+        for view in (b[:, 3:300], b[7:, 1:130], b[::3, 5:], b[4:5, 2:9]):
+            _check_matrix(fp8.fp8_quantize(view), view.cpu(), "rows", "e4m3")
+            _check_matrix(fp8.fp8_quantize(view, transpose=True), view.cpu().t(), "rows", "e4m3")
+    for shape in ((0, 5), (5, 0), (0, 0)):
+        q = fp8.fp8_quantize(torch.zeros(*shape, device="cuda"))
+        assert q.shape == shape and q.data.shape[0] == shape[0]
+        t = fp8.fp8_quantize(torch.zeros(*shape, device="cuda"), transpose=True)
+        assert t.shape == shape[::-1]
+
+
+def _operands(fp8, M, N, K, block, fmt, scale, seed=0):
+    a, b = _rand(M, K, seed + 1, spread=1.0), _rand(N, K, seed + 2, spread=1.0)
+    qa, qb = fp8.fp8_quantize(a.cuda(), "rows", fmt), fp8.fp8_quantize(b.cuda(), block)
+    if scale == "f32":
+        g = torch.Generator().manual_seed(seed)
+        f = lambda q: fp8.Fp8Matrix(q.data, (q.scales() * (1 + torch.rand(q.scales().shape, generator=g).cuda())).t().contiguous(),
+                                    q.cols, q.block)
+        qa, qb = f(qa), f(qb)
+    return qa, qb, _value(qa), _value(qb)
+
+
+def _value(q):
+    """what an Fp8Matrix stands for in 64 bits (its scales are checked against the definition elsewhere)"""
+    s = q.scales().double().cpu().repeat_interleave(128, dim=1)
+    if q.block == "tiles":
+        s = s.repeat_interleave(128, dim=0)[:q.rows]
+    return (q.data.float().double().cpu() * s)[:, :q.cols]
+
+
+SHAPES = [(1, 1, 1), (1, 16, 128), (1, 4096, 512), (2, 130, 257), (5, 33, 1000), (16, 48, 640), (17, 1, 129), (31, 300, 2304), (64, 64, 128),
+          (65, 129, 131), (127, 255, 385), (128, 128, 1024), (200, 513, 1100), (300, 64, 5000), (257, 1025, 513), (1000, 260, 256), (1, 7, 20000),
+          (40, 24, 9000), (700, 700, 130)]
+
+
+@pytest.mark.parametrize("M,N,K", SHAPES)
+@pytest.mark.parametrize("block", ["rows", "tiles"])
+@pytest.mark.parametrize("scale", ["e8m0", "f32"])
+def test_matmul(M, N, K, block, scale):
+    fp8 = _fp8()
+    for fmt in ("e4m3", "e5m2"):
+        a, b, av, bv = _operands(fp8, M, N, K, block, fmt, scale)
+        ref = av @ bv.t()
+        for dt in (torch.float32, torch.bfloat16):
+            out = fp8.matmul_fp8(a, b, out_dtype=dt)
+            assert out.dtype == dt
+            bound = R.matmul_bound(av, bv, dt, ref)
+            assert ((out.double().cpu() - ref).abs() <= bound).all()
+
+
+def test_matmul_is_exact_on_integers():
+    """Small integers: every product and partial sum is exact in fp32, so the result is too - for every shape rule."""
+    fp8 = _fp8()
+    g = torch.Generator().manual_seed(3)
+    for M, N, K in SHAPES + [(512, 512, 2048), (2048, 2048, 256), (4096, 300, 384), (260, 4100, 640)]:
+        a = torch.randint(-8, 9, (M, K), generator=g).float()
+        b = torch.randint(-8, 9, (N, K), generator=g).float()
+        ref = (a.cuda().double() @ b.cuda().double().t())
+        for block in ("rows", "tiles"):
+            out = fp8.matmul_fp8(fp8.fp8_quantize(a.cuda()), fp8.fp8_quantize(b.cuda(), block), out_dtype=torch.float32)
+            assert torch.equal(out.double(), ref), (M, N, K, block)
+            out16 = fp8.matmul_fp8(fp8.fp8_quantize(a.cuda()), fp8.fp8_quantize(b.cuda(), block), out_dtype=torch.float16)
+            assert torch.equal(out16, ref.float().half()), (M, N, K, block)
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 40, 300), (19, 130, 700), (300, 200, 257), (5, 3, 20000)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_matmul_into_strided_out_and_accumulate(M, N, K, dtype):
+    fp8 = _fp8()
+    g = torch.Generator().manual_seed(4)
+    a = torch.randint(-3, 4, (M, K), generator=g).float()
+    b = torch.randint(-1, 2, (N, K), generator=g).float()
+    qa, qb = fp8.fp8_quantize(a.cuda()), fp8.fp8_quantize(b.cuda(), "tiles")
+    big = torch.full((M + 2, N + 9), 7.0, device="cuda", dtype=DT[dtype])
+    out = big[1:M + 1, 3:N + 3]
+    fp8.matmul_fp8(qa, qb, out=out)
+    ref = a.double() @ b.double().t()
+    assert torch.equal(out.cpu(), ref.to(DT[dtype]))
+    first = out.clone().double().cpu()
+    fp8.matmul_fp8(qa, qb, out=out, accumulate=True)
+    assert torch.equal(out.cpu(), (first + ref).to(DT[dtype]))      # |sums| < 2^24: exact in fp32, rounded once
+    border = big.clone()
+    border[1:M + 1, 3:N + 3] = 7.0
+    assert (border == 7.0).all()
+
+
+def test_matmul_empty_dimensions():
+    fp8 = _fp8()
+    z = lambda m, k, block="rows": fp8.fp8_quantize(torch.zeros(m, k, device="cuda"), block)
+    assert fp8.matmul_fp8(z(0, 5), z(3, 5)).shape == (0, 3)
+    assert fp8.matmul_fp8(z(3, 5), z(0, 5, "tiles")).shape == (3, 0)
+    out = torch.full((3, 4), 2.0, device="cuda")
+    assert torch.equal(fp8.matmul_fp8(z(3, 0), z(4, 0), out=out, accumulate=True), torch.full((3, 4), 2.0, device="cuda"))
+    assert torch.equal(fp8.matmul_fp8(z(3, 0), z(4, 0), out=out), torch.zeros(3, 4, device="cuda"))
+
+
+def test_matmul_nan_and_inf_stay_in_their_row():
+    fp8 = _fp8()
+    for M in (4, 300):
+        a, b = _rand(M, 500, 1, spread=0.5), _rand(70, 500, 2, spread=0.5)
+        a[2, 130] = float("nan")
+        b[5, 3] = float("nan")
+        qa, qb = fp8.fp8_quantize(a.cuda()), fp8.fp8_quantize(b.cuda())
+        out = fp8.matmul_fp8(qa, qb, out_dtype=torch.float32).cpu()
+        bad = torch.zeros(M, 70, dtype=torch.bool)
+        bad[2], bad[:, 5] = True, True
+        assert torch.equal(torch.isnan(out), bad)
+        a[2, 130] = float("inf")
+        out = fp8.matmul_fp8(fp8.fp8_quantize(a.cuda(), fmt="e5m2"), fp8.fp8_quantize(b.cuda()), out_dtype=torch.float32).cpu()
+        assert torch.isfinite(out[[0, 1, 3]][:, [0, 4, 6]]).all() and not torch.isfinite(out[2]).any()
+
+
+def test_matmul_scale_bytes_over_the_whole_range():
+    """Scales far from 1 on both sides, 2^-127 (byte 0) among them, and the NaN byte 255."""
+    fp8 = _fp8()
+    for M in (3, 200):
+        K, N = 512, 20
+        codes = torch.ones(M, K).to(torch.float8_e4m3fn).cuda()
+        wcodes = torch.ones(N, K).to(torch.float8_e4m3fn).cuda()
+        sa = torch.full((M, 4), 127, dtype=torch.int32)
+        sa[0], sa[1, 0], sa[2] = 0, 255, torch.tensor([254, 200, 100, 1])
+        sb = torch.full((N, 4), 127, dtype=torch.int32)
+        sb[3] = 60
+        a = fp8.Fp8Matrix.from_parts(codes, sa.cuda())
+        b = fp8.Fp8Matrix.from_parts(wcodes, sb.cuda())
+        out = fp8.matmul_fp8(a, b, out_dtype=torch.float32).double().cpu()
+        two = torch.tensor(2.0, dtype=torch.float64)
+        ref = 128 * (torch.pow(two, sa.double() - 127) @ torch.pow(two, sb.double() - 127).t())
+        ref[1] = float("nan")
+        ref[2, :3] = float("inf") if ref[2, 0] > torch.finfo(torch.float32).max else ref[2, 0]
+        ref = ref.float().double()
+        ok = ~torch.isnan(ref)
+        assert torch.isnan(out[1]).all()
+        # a result below the normal range may be flushed: 2^-126 absolutely; else one rounding
+        fin = ok & torch.isfinite(ref)
+        assert ((out - ref).abs()[fin] <= 2.0 ** -23 * ref.abs()[fin] + 2.0 ** -126).all()
+        assert torch.equal(torch.isinf(out)[ok], torch.isinf(ref)[ok])
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 64, 128), (1, 4100, 1000), (3, 130, 257), (16, 500, 2304), (37, 257, 515), (300, 140, 640)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_linear_forward(M, N, K, dtype):
+    fp8 = _fp8()
+    x, w = _rand(M, K, 11, DT[dtype], spread=1.0), _rand(N, K, 12, spread=1.0) * 0.05
+    w8 = fp8.fp8_quantize(w.cuda(), "tiles")
+    y = fp8.linear_fp8_fwd(x.cuda(), w8)
+    xv, wv = R.requantized(x), R.requantized(w, "tiles")
+    ref = xv @ wv.t()
+    assert y.dtype == DT[dtype]
+    assert ((y.double().cpu() - ref).abs() <= R.matmul_bound(xv, wv, DT[dtype], ref)).all()
+    y2, xt = fp8.linear_fp8_fwd(x.cuda(), w8, out_dtype=torch.float32, keep_transposed=True)
+    assert ((y2.double().cpu() - ref).abs() <= R.matmul_bound(xv, wv, torch.float32, ref)).all()
+    _check_matrix(xt, x.t(), "rows", "e4m3")
+
+
+def test_linear_forward_rows_are_independent():
+    """A row's result does not depend on what else is in the batch, NaN included, at every batch size around the rules' borders."""
+    fp8 = _fp8()
+    x, w = _rand(70, 700, 21, torch.bfloat16, spread=0.5).cuda(), _rand(200, 700, 22, spread=0.5).cuda()
+    w8 = fp8.fp8_quantize(w, "tiles")
+    xv, wv = R.requantized(x.cpu()), R.requantized(w.cpu(), "tiles")
+    ref = xv @ wv.t()
+    bound = R.matmul_bound(xv, wv, torch.bfloat16, ref)
+    for m in (1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 70):
+        y = fp8.linear_fp8_fwd(x[:m], w8)
+        assert ((y.double().cpu() - ref[:m]).abs() <= bound[:m]).all(), m
+        xn = x[:m].clone()
+        xn[m // 2, 5] = float("nan")
+        yn = fp8.linear_fp8_fwd(xn, w8)
+        assert torch.isnan(yn[m // 2]).all()
+        keep = [i for i in range(m) if i != m // 2]
+        assert torch.equal(yn[keep], y[keep])
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 64, 128), (130, 70, 257), (300, 140, 640), (515, 33, 100)])
+@pytest.mark.parametrize("fmt", ["e4m3", "e5m2"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_linear_backward(M, N, K, fmt, dtype):
+    fp8 = _fp8()
+    x, w, dy = _rand(M, K, 31, DT[dtype], spread=1.0), _rand(N, K, 32, spread=1.0) * 0.05, _rand(M, N, 33, DT[dtype], spread=1.0) * 1e-3
+    w8, w8t = fp8.fp8_quantize_both(w.cuda(), "tiles")
+    _, xt = fp8.linear_fp8_fwd(x.cuda(), w8, keep_transposed=True)
+    dx, dw = fp8.linear_fp8_bwd(dy.cuda(), xt, w8t, fmt=fmt)
+    gv, gtv = R.requantized(dy, "rows", fmt), R.requantized(dy.t(), "rows", fmt)
+    wv, xtv = R.requantized(w, "tiles"), R.requantized(x.t())
+    ref = gv @ wv
+    assert dx.dtype == DT[dtype] and ((dx.double().cpu() - ref).abs() <= R.matmul_bound(gv, wv.t(), DT[dtype], ref)).all()
+    ref = gtv @ xtv.t()
+    assert dw.dtype == torch.float32 and ((dw.double().cpu() - ref).abs() <= R.matmul_bound(gtv, xtv, torch.float32, ref)).all()
+    # the stored weight's own transpose gives the same bits; a missing operand leaves its gradient out
+    dx2, none = fp8.linear_fp8_bwd(dy.cuda(), None, w8.transposed(), fmt=fmt)
+    assert none is None and torch.equal(dx2, dx)
+    acc = dw.clone()
+    none, dw2 = fp8.linear_fp8_bwd(dy.cuda(), xt, None, fmt=fmt, dw=acc, accumulate=True)
+    assert none is None and dw2 is acc and torch.equal(acc, dw + dw)
+
+
+def test_linear_gradients_against_differences():
+    """On values the format holds exactly the layer is linear, so finite differences ARE the gradients: integers, exact in
+    fp32 throughout, compared without a tolerance."""
+    fp8 = _fp8()
+    g = torch.Generator().manual_seed(9)
+    M, N, K = 150, 70, 200
+    ints = lambda *s, lim=4: torch.randint(-lim, lim + 1, s, generator=g).float().cuda()
+    x, w, dy = ints(M, K), ints(N, K), ints(M, N, lim=2)
+    f = lambda xx, ww: (dy.double() * fp8.linear_fp8_fwd(xx, fp8.fp8_quantize(ww, "tiles")).double()).sum()
+    _, xt = fp8.linear_fp8_fwd(x, fp8.fp8_quantize(w, "tiles"), keep_transposed=True)
+    dx, dw = fp8.linear_fp8_bwd(dy, xt, fp8.fp8_quantize(w, "tiles", transpose=True))
+    for _ in range(4):
+        d = ints(M, K, lim=2)
+        assert float(f(x + d, w) - f(x, w)) == float((dx.double() * d.double()).sum())
+        d = ints(N, K, lim=2)
+        assert float(f(x, w + d) - f(x, w)) == float((dw.double() * d.double()).sum())
+
+
+def test_from_parts_transposed_and_dequantize():
+    fp8 = _fp8()
+    w = _rand(300, 257, 41, spread=1.0)
+    q, qt = fp8.fp8_quantize_both(w.cuda(), "tiles")
+    t = q.transposed()
+    assert torch.equal(t.data.view(torch.uint8), qt.data.view(torch.uint8)) and torch.equal(t.scale, qt.scale) and t.shape == (257, 300)
+    assert torch.equal(q.dequantize().double().cpu(), R.requantized(w, "tiles"))
+    vals, exps = R.quantize(w, "rows", "e4m3")
+    p = fp8.Fp8Matrix.from_parts(vals[:, :257].to(torch.float8_e4m3fn).cuda(), (exps + 127).int().cuda())
+    n = fp8.fp8_quantize(w.cuda())
+    assert torch.equal(p.data.view(torch.uint8), n.data.view(torch.uint8)) and torch.equal(p.scale, n.scale)
+    f = fp8.Fp8Matrix.from_parts(q.data[:, :257], q.scales(), "tiles")       # fp32 scales
+    assert torch.equal(f.dequantize(), q.dequantize()) and torch.equal(f.transposed().dequantize(), q.dequantize().t())
+
+
+def test_offsets_beyond_32_bits():
+    """Codes, inputs and results larger than 2^32 bytes / 2^31 elements: the last rows are right."""
+    fp8 = _fp8()
+    K, M = 65536, 70000                                   # 4.6 G codes, 9.2 GB of bf16
+    x = torch.zeros(M, K, dtype=torch.bfloat16, device="cuda")
+    g = torch.Generator().manual_seed(5)
+    tail = torch.randint(-4, 5, (3, K), generator=g).float()
+    x[-3:] = tail.cuda().bfloat16()
+    q = fp8.fp8_quantize(x)
+    assert torch.equal(q.data[-3:].float().cpu(), R.quantize(tail, "rows", "e4m3")[0].float())
+    t = fp8.fp8_quantize(x, transpose=True)
+    assert t.shape == (K, M)
+    del x
+    assert torch.equal(t.data[-200:, M - 3:M].float().cpu() * t.scales()[-200:, -1:].cpu(), tail[:, -200:].t())
+    del t
+    w = torch.randint(-2, 3, (24, K), generator=g).float()
+    w8 = fp8.fp8_quantize(w.cuda(), "tiles")
+    out = fp8.matmul_fp8(q, w8, out_dtype=torch.float32)
+    assert torch.equal(out[-3:].cpu().double(), tail.double() @ w.double().t()) and not out[:-3].any()
+    del out
+    # as the second operand (a long list of weight rows against one activation row)
+    a8 = fp8.fp8_quantize(w[:1].cuda())
+    out = fp8.matmul_fp8(a8, fp8.Fp8Matrix(q.data, q.scale, K, "rows"), out_dtype=torch.float32)
+    assert torch.equal(out[0, -3:].cpu().double(), tail.double() @ w[0].double()) and not out[0, :-3].any()
+    del q, out
+    ones = lambda n: fp8.fp8_quantize(torch.ones(n, 128, device="cuda"))
+    out = fp8.matmul_fp8(ones(60000), ones(40000), out_dtype=torch.bfloat16)      # 2.4 G results
+    assert bool((out[-1] == 128).all()) and bool((out[30000] == 128).all())
+
+
+def test_runs_on_the_current_stream_and_in_a_graph():
+    """Two captured graphs of split products (scratch of their own) replayed on two streams, against the eager results."""
+    fp8 = _fp8()
+    g = torch.Generator().manual_seed(6)
+    mk = lambda *s: torch.randint(-4, 5, s, generator=g).float().cuda()
+    xs = [mk(5, 20000), mk(5, 20000)]
+    w8 = fp8.fp8_quantize(mk(64, 20000), "tiles")
+    dy = mk(5, 64)
+    def step(x):
+        y, xt = fp8.linear_fp8_fwd(x, w8, out_dtype=torch.float32, keep_transposed=True)
+        return (y,) + fp8.linear_fp8_bwd(dy, xt, wt)
+    wt = w8.transposed()
+    want = [step(x) for x in xs]
+    side = [torch.cuda.Stream(), torch.cuda.Stream()]
+    graphs, outs = [], []
+    for x, st in zip(xs, side):
+        st.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(st):
+            step(x)
+        st.synchronize()
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr, stream=st):
+            outs.append(step(x))
+        graphs.append(gr)
+    for round_ in range(4):
+        for o in outs:
+            for t in o:
+                t.zero_()
+        torch.cuda.synchronize()
+        for gr, st in zip(graphs, side):
+            with torch.cuda.stream(st):
+                gr.replay()
+        eager = step(xs[round_ % 2])
+        torch.cuda.synchronize()
+        for o, w in zip(outs, want):
+            assert all(torch.equal(a, b) for a, b in zip(o, w))
+        assert all(torch.equal(a, b) for a, b in zip(eager, want[round_ % 2]))
+
+
+def test_training_step_of_a_layer():
+    """Quantise, product, gradient products, norm and clip, update - in the order a training step runs them - against the
+    same step in 64 bits."""
+    fp8 = _fp8()
+    from stylemesh_amd.runtime.gradclip import GradClip
+    M, N, K, lr, max_norm = 200, 96, 300, 0.5, 0.25
+    x, w, target = _rand(M, K, 51, spread=0.3), _rand(N, K, 52, spread=0.3) * 0.05, _rand(M, N, 53, spread=0.1)
+    wd, xd, td = w.cuda(), x.cuda(), target.cuda()
+    dw = torch.empty(N, K, device="cuda")
+    plan = GradClip([dw])
+    w64 = w.double()
+    for step in range(3):
+        w8, w8t = fp8.fp8_quantize_both(wd, "tiles")
+        y, xt = fp8.linear_fp8_fwd(xd, w8, keep_transposed=True)
+        dy = (y - td) * (2.0 / y.numel())
+        _, _ = fp8.linear_fp8_bwd(dy, xt, w8t, dw=dw)
+        raw = dw.clone()
+        norm = plan.clip(max_norm)
+        # the 64-bit step from the same weights and the same output gradient (whose codes a last bit could tip)
+        ref = R.requantized(dy.cpu().t()) @ R.requantized(x.t()).t()
+        bound = R.matmul_bound(R.requantized(dy.cpu().t()), R.requantized(x.t()), torch.float32, ref)
+        assert ((raw.double().cpu() - ref).abs() <= bound).all()
+        rn = float(raw.double().norm())
+        assert abs(float(norm) - rn) <= 2.0 ** -23 * rn
+        coef = min(1.0, max_norm / (rn + 1e-6))
+        assert ((dw.double() - raw.double() * coef).abs() <= 2.0 ** -22 * raw.double().abs() + 1e-44).all()
+        wd -= lr * dw
