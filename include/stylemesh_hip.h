@@ -753,6 +753,14 @@ int sm_fp8_matmul(const void* a, const void* a_scale, int a_fmt, size_t a_pitch,
                   size_t b_pitch, int scale_f32, int M, int N, int K, void* out, int out_type, size_t out_stride, int accumulate,
                   void* ws, size_t ws_bytes, void* stream);
 
+/* A layer's forward pass: out[M][N] = q(x) W^T, x [M][K] (x_type, row stride x_stride), q = sm_fp8_quantize with row scales in
+ * e4m3, W [N][K] e4m3 with power-of-two scales (resident). Up to 16 rows one launch (x is quantised inside the product), above
+ * sm_fp8_quantize into ws + sm_fp8_matmul. ws: sm_fp8_linear_ws_bytes(M, N, K) bytes (0: may be NULL), 16-byte aligned, of this
+ * call's own. */
+size_t sm_fp8_linear_ws_bytes(int M, int N, int K);
+int sm_fp8_linear(const void* x, int x_type, size_t x_stride, const void* w, const void* w_scale, int w_tiles, size_t w_pitch, int M,
+                  int N, int K, void* out, int out_type, size_t out_stride, void* ws, size_t ws_bytes, void* stream);
+
 /* ---- G1: the global norm of many gradient tensors, and clipping by it (csrc/gradnorm.hip) -------------------
  * What Trainer(gradient_clip_val=...) of the reference's pytorch_lightning does between backward and the optimizer step
  * (torch.nn.utils.clip_grad_norm_). grads / out / numel / types (SM_TYPE_*) / out_types: HOST arrays of n entries, read during

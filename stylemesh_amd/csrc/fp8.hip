@@ -10,6 +10,7 @@
 // cores apply the scales themselves: v_mfma_scale_f32_16x16x128_f8f6f4 takes a block of 128 per instruction and one scale
 // byte per operand row, so a scaled block costs no vector instruction. fp32 scales (any value) take the same kernels with
 // the block's partial sum multiplied in on the vector unit.
+#include <algorithm>
 #include <type_traits>
 
 #include "common.h"
@@ -34,26 +35,28 @@ __device__ __forceinline__ unsigned f32_to_bf16(float f) {
 __device__ __forceinline__ float f16_to_f32(unsigned h) { return (float)__builtin_bit_cast(_Float16, (uint16_t)h); }
 __device__ __forceinline__ unsigned f32_to_f16(float f) { return __builtin_bit_cast(uint16_t, (_Float16)f); }
 
+// 16 bytes of fp32 / bf16 / fp16 -> 4 / 8 floats
+template <int T>
+__device__ __forceinline__ void unpack(u32x4 a, float* v) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if constexpr (T == SM_TYPE_F32) v[j] = __builtin_bit_cast(float, (unsigned)a[j]);
+        else {
+            v[2 * j] = T == SM_TYPE_BF16 ? bf16_to_f32(a[j] & 0xffffu) : f16_to_f32(a[j] & 0xffffu);
+            v[2 * j + 1] = T == SM_TYPE_BF16 ? __builtin_bit_cast(float, (unsigned)a[j] & 0xffff0000u) : f16_to_f32(a[j] >> 16);
+        }
+    }
+}
 // eight consecutive elements of a row as fp32 (type: SM_TYPE_*); `valid` of them exist, the others are 0
 template <int T>
 __device__ __forceinline__ void load8(const void* base, size_t off, int valid, float* v) {
     if (valid >= 8) {
         if constexpr (T == SM_TYPE_F32) {
             const u32x4_u* p = reinterpret_cast<const u32x4_u*>(static_cast<const float*>(base) + off);
-            const u32x4 a = p[0], b = p[1];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                v[j] = __builtin_bit_cast(float, (unsigned)a[j]);
-                v[4 + j] = __builtin_bit_cast(float, (unsigned)b[j]);
-            }
+            unpack<T>(p[0], v);
+            unpack<T>(p[1], v + 4);
         } else {
-            const u32x4 a = *reinterpret_cast<const u32x4_u*>(static_cast<const uint16_t*>(base) + off);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const unsigned lo = a[j] & 0xffffu, hi = a[j] >> 16;
-                v[2 * j] = T == SM_TYPE_BF16 ? bf16_to_f32(lo) : f16_to_f32(lo);
-                v[2 * j + 1] = T == SM_TYPE_BF16 ? bf16_to_f32(hi) : f16_to_f32(hi);
-            }
+            unpack<T>(*reinterpret_cast<const u32x4_u*>(static_cast<const uint16_t*>(base) + off), v);
         }
         return;
     }
@@ -250,29 +253,57 @@ struct MatmulArgs {
     int kb_per_split;
 };
 
+// four results of a row in one store (results start at any element: aligned to theirs only); fewer at the row's end
 __device__ __forceinline__ void store4(const MatmulArgs& g, int m, int n, f32x4 v) {
     const int cnt = g.N - n;
+    const size_t at = (size_t)m * g.out_stride + n;
     if (g.out_type == SM_TYPE_F32) {
-        float* o = static_cast<float*>(g.out) + (size_t)m * g.out_stride + n;
+        float* o = static_cast<float*>(g.out) + at;
+        if (cnt >= 4) {
+            if (g.accumulate) {
+                const u32x4 old = *reinterpret_cast<const u32x4_u*>(o);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (j < cnt) o[j] = g.accumulate ? o[j] + v[j] : v[j];
-    } else {
-        uint16_t* o = static_cast<uint16_t*>(g.out) + (size_t)m * g.out_stride + n;
-        const bool bf = g.out_type == SM_TYPE_BF16;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (j < cnt) {
-                float x = v[j];
-                if (g.accumulate) x += bf ? bf16_to_f32(o[j]) : f16_to_f32(o[j]);
-                o[j] = (uint16_t)(bf ? f32_to_bf16(x) : f32_to_f16(x));
+                for (int j = 0; j < 4; ++j) v[j] += __builtin_bit_cast(float, (unsigned)old[j]);
             }
+            u32x4 w;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = __builtin_bit_cast(unsigned, (float)v[j]);
+            *reinterpret_cast<u32x4_u*>(o) = w;
+            return;
+        }
+        for (int j = 0; j < cnt; ++j) o[j] = g.accumulate ? o[j] + v[j] : v[j];
+    } else {
+        uint16_t* o = static_cast<uint16_t*>(g.out) + at;
+        const bool bf = g.out_type == SM_TYPE_BF16;
+        if (cnt >= 4) {
+            if (g.accumulate) {
+                const u32x2 old = *reinterpret_cast<const u32x2_u*>(o);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const unsigned h = (old[j >> 1] >> (16 * (j & 1))) & 0xffffu;
+                    v[j] += bf ? bf16_to_f32(h) : f16_to_f32(h);
+                }
+            }
+            u32x2 w;
+            w[0] = bf ? f32_to_bf16(v[0]) | (f32_to_bf16(v[1]) << 16) : f32_to_f16(v[0]) | (f32_to_f16(v[1]) << 16);
+            w[1] = bf ? f32_to_bf16(v[2]) | (f32_to_bf16(v[3]) << 16) : f32_to_f16(v[2]) | (f32_to_f16(v[3]) << 16);
+            *reinterpret_cast<u32x2_u*>(o) = w;
+            return;
+        }
+        for (int j = 0; j < cnt; ++j) {
+            float x = v[j];
+            if (g.accumulate) x += bf ? bf16_to_f32(o[j]) : f16_to_f32(o[j]);
+            o[j] = (uint16_t)(bf ? f32_to_bf16(x) : f32_to_f16(x));
+        }
     }
 }
 
-// direct loads into LDS are counted as vector-memory operations: a wave waits for its own before the barrier that hands
-// the stage to the others
-__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// Direct loads into LDS are counted as vector-memory operations and finish in their order: a wave waits for its own (all but
+// the LEFT newest) before the barrier that hands a stage to the others.
+template <int LEFT>
+__device__ __forceinline__ void wait_loads() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LEFT) : "memory");
+}
 
 // An operand's 32 codes of a lane as bf16, scaled by 2^(byte - 127): e4m3 / e5m2 have 4 / 3 significant bits, bf16 has 8 and
 // fp32's exponents, so this is exact. scale: the byte in the exponent field of a float.
@@ -281,6 +312,9 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 struct Wide {
     bf16x8 p[4];
 };
+__device__ __forceinline__ i32x8 join(u32x4 lo, u32x4 hi) {
+    return i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+}
 template <int F>
 __device__ __forceinline__ Wide widen(i32x8 v, float scale) {
     Wide w;
@@ -318,16 +352,29 @@ __device__ __forceinline__ f32x4 mfma_block(i32x8 bfrag, i32x8 afrag, f32x4 c, i
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(bfrag, afrag, c, SM_FP8_E4M3, FA, OP, sb, OP, sa);
 }
 
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const void* base) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)0xfffffff0u, 0x00020000);
+}
+
+// 16 bytes per lane from rsrc + voff + soff to LDS bytes dst + 16 lane (the builtin exists in the device pass only)
+__device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t rsrc, uint8_t* dst, unsigned voff, int soff) {
+#ifdef __HIP_DEVICE_COMPILE__
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)dst, 16, (int)voff, soff, 0, 0);
+#endif
+}
+
 // BM x BN output tile per block, waves WM x WN; a stage = one block of 128 along K of both operands, double-buffered in
 // LDS and filled by direct loads (16 bytes per lane, no registers). LDS rows are 128 bytes; the 16-byte chunk c of row r
 // sits at chunk c ^ (r & 7), so that the eight lanes of a read phase hit eight different chunk columns. A lane's 32 bytes of
 // an operand row are chunks g and g + 4 (g = lane / 16): the same permutation of k on both sides leaves the sum as it is,
 // and a block of 128 has ONE scale, so it does not matter which quarter a lane holds.
-template <int BM, int BN, int WM, int WN, int FA, bool F32S, bool NATIVE>
+enum { SCALE_POW2, SCALE_F32_ROWS, SCALE_F32_TILES };      // how the scales of a launch are held (fp32: B's blocks)
+
+template <int BM, int BN, int WM, int WN, int NST, int FA, int SC, bool NATIVE>
 __global__ __launch_bounds__(WM* WN * 64) void fp8_matmul_kernel(MatmulArgs g) {
     constexpr int NT = WM * WN * 64;
     constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
-    __shared__ __align__(16) uint8_t lds[2][(BM + BN) * 128];
+    __shared__ __align__(16) uint8_t lds[NST][(BM + BN) * 128];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave % WM, wn = wave / WM;
     const int mt = (g.M + BM - 1) / BM, nt = (g.N + BN - 1) / BN;
@@ -337,22 +384,27 @@ __global__ __launch_bounds__(WM* WN * 64) void fp8_matmul_kernel(MatmulArgs g) {
     const int m0 = (group * 8 + in % gm) * BM, n0 = in / gm * BN;
     const int kb0 = blockIdx.y * g.kb_per_split, kb1 = min(g.KB, kb0 + g.kb_per_split);
 
-    // one direct load moves 64 lanes x 16 bytes = 8 rows; lane i's data lands at byte 16 i of the wave's kilobyte
-    constexpr int NL = (BM + BN) * 128 / (NT * 16);
-    const uint8_t* src[NL];
+    // One direct load moves 64 lanes x 16 bytes = 8 rows; lane i's data lands at byte 16 i of the wave's kilobyte. Buffer loads: a
+    // uniform base (the tile's first row), a 32-bit offset per lane (256 rows of the longest pitch stay below 2^32) and the
+    // block of 128 as scalar offset - no 64-bit vector arithmetic in the loop. Rows behind the last are the last one again.
+    constexpr int RW = NT / 8;                                   // rows all waves load at a time
+    constexpr int NLA = BM / RW, NLB = BN / RW;
+    static_assert(BM % RW == 0 && BN % RW == 0, "whole loads");
+    const int r8 = lane >> 3, c16 = ((lane & 7) ^ r8) << 4;
+    const __amdgpu_buffer_rsrc_t asrc = tile_rsrc(g.a + (size_t)m0 * g.a_pitch), bsrc = tile_rsrc(g.b + (size_t)n0 * g.b_pitch);
+    unsigned va[NLA], vb[NLB];
 #pragma unroll
-    for (int i = 0; i < NL; ++i) {
-        const int rowbase = (i * (NT / 64) + wave) * 8, r8 = lane >> 3, c = (lane & 7) ^ r8;      // rowbase: wave-uniform
-        src[i] = (rowbase < BM ? g.a + (size_t)min(m0 + rowbase + r8, g.M - 1) * g.a_pitch
-                               : g.b + (size_t)min(n0 + rowbase - BM + r8, g.N - 1) * g.b_pitch) + (size_t)kb0 * 128 + c * 16;
-    }
-    auto stage = [&](int buf) {
+    for (int i = 0; i < NLA; ++i) va[i] = (unsigned)min(i * RW + wave * 8 + r8, g.M - 1 - m0) * (unsigned)g.a_pitch + c16;
 #pragma unroll
-        for (int i = 0; i < NL; ++i) {
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src[i],
-                                             (__attribute__((address_space(3))) void*)(lds[buf] + (i * (NT / 64) + wave) * 1024), 16, 0, 0);
-            src[i] += 128;
-        }
+    for (int i = 0; i < NLB; ++i) vb[i] = (unsigned)min(i * RW + wave * 8 + r8, g.N - 1 - n0) * (unsigned)g.b_pitch + c16;
+    auto stage = [&](int buf, int kb) {
+        uint8_t* dst = lds[buf] + wave * 1024;
+#pragma unroll
+        for (int i = 0; i < NLA; ++i)
+            load_to_lds(asrc, dst + i * RW * 128, va[i], kb * 128);
+#pragma unroll
+        for (int i = 0; i < NLB; ++i)
+            load_to_lds(bsrc, dst + BM * 128 + i * RW * 128, vb[i], kb * 128);
     };
     f32x4 acc[TN][TM];
 #pragma unroll
@@ -361,108 +413,111 @@ __global__ __launch_bounds__(WM* WN * 64) void fp8_matmul_kernel(MatmulArgs g) {
         for (int j = 0; j < TM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
     const int lr = lane & 15, lg = lane >> 4;
-    int arow[TM], brow[TN];      // scale rows of this lane
+    // The scales of the next four blocks (power-of-two: a dword per row) or the next block (fp32) are loaded a step ahead.
+    // rows of A: one per lane and row tile; rows of B: likewise, or - fp32, whose factors meet the result - the lane's four
+    // result columns; fp32 scales per tile: one for the wave (its columns lie within one tile).
+    constexpr bool F32S = SC != SCALE_POW2;
+    constexpr int NB = SC == SCALE_POW2 ? TN : SC == SCALE_F32_ROWS ? 4 * TN : 1;
+    unsigned arow[TM], brow[NB];
 #pragma unroll
-    for (int j = 0; j < TM; ++j) arow[j] = min(m0 + (wm * TM + j) * 16 + lr, g.M - 1);
+    for (int j = 0; j < TM; ++j) arow[j] = (unsigned)min(m0 + (wm * TM + j) * 16 + lr, g.M - 1) * 4u;
 #pragma unroll
-    for (int i = 0; i < TN; ++i) brow[i] = min(n0 + (wn * TN + i) * 16 + lr, g.N - 1) >> g.b_shift;
-
-    int sa[TM], sb[TN];
-    auto load_scales = [&](int kq) {
-        const uint32_t* pa = static_cast<const uint32_t*>(g.as) + (size_t)kq * g.M;
-        const uint32_t* pb = static_cast<const uint32_t*>(g.bs) + (size_t)kq * g.bs_rows;
+    for (int i = 0; i < NB; ++i) {
+        const int n = n0 + wn * TN * 16 + (SC == SCALE_POW2 ? i * 16 + lr : SC == SCALE_F32_ROWS ? (i >> 2) * 16 + lg * 4 + (i & 3) : 0);
+        brow[i] = (unsigned)(min(n, g.N - 1) >> g.b_shift) * 4u;
+    }
+    int sa[TM], sb[NB], sa_next[TM], sb_next[NB];
+    auto load_scales = [&](int row, int* pa_out, int* pb_out) {      // row: of the scale arrays (kb / 4 or kb)
+        const __amdgpu_buffer_rsrc_t pa = tile_rsrc(static_cast<const char*>(g.as) + (size_t)row * g.M * 4);
+        const __amdgpu_buffer_rsrc_t pb = tile_rsrc(static_cast<const char*>(g.bs) + (size_t)row * g.bs_rows * 4);
 #pragma unroll
-        for (int j = 0; j < TM; ++j) sa[j] = (int)pa[arow[j]];
+        for (int j = 0; j < TM; ++j) pa_out[j] = (int)__builtin_amdgcn_raw_buffer_load_b32(pa, arow[j], 0, 0);
 #pragma unroll
-        for (int i = 0; i < TN; ++i) sb[i] = (int)pb[brow[i]];
+        for (int i = 0; i < NB; ++i) pb_out[i] = (int)__builtin_amdgcn_raw_buffer_load_b32(pb, brow[i], 0, 0);
     };
-    auto frag = [&](const uint8_t* base, int row) {
-        const u32x4 lo = *reinterpret_cast<const u32x4*>(base + row * 128 + ((lg ^ (row & 7)) << 4));
-        const u32x4 hi = *reinterpret_cast<const u32x4*>(base + row * 128 + (((lg + 4) ^ (row & 7)) << 4));
-        return i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+    auto take_scales = [&]() {
+#pragma unroll
+        for (int j = 0; j < TM; ++j) sa[j] = sa_next[j];
+#pragma unroll
+        for (int i = 0; i < NB; ++i) sb[i] = sb_next[i];
     };
-    // fp32 scales: the block's sum on its own, then one multiply-add per element with sa[m] sb[n]
-    f32x4 fb[TN];
-    float fa[TM];
-    auto block_scales = [&](int kb) {
-        const float* pa = static_cast<const float*>(g.as) + (size_t)kb * g.M;
-        const float* pb = static_cast<const float*>(g.bs) + (size_t)kb * g.bs_rows;
-#pragma unroll
-        for (int i = 0; i < TN; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) fb[i][e] = pb[min(n0 + (wn * TN + i) * 16 + lg * 4 + e, g.N - 1) >> g.b_shift];
-#pragma unroll
-        for (int j = 0; j < TM; ++j) fa[j] = pa[arow[j]];
+    // a tile of 16 rows is 2 KB of LDS; the swizzle depends on the row within it only
+    const int f0 = lr * 128 + ((lg ^ (lr & 7)) << 4), f1 = lr * 128 + (((lg + 4) ^ (lr & 7)) << 4);
+    auto frag = [&](const uint8_t* base, int tile) {
+        return join(*reinterpret_cast<const u32x4*>(base + tile * 2048 + f0), *reinterpret_cast<const u32x4*>(base + tile * 2048 + f1));
     };
-    auto add_block = [&](f32x4& c, f32x4 d, float sam, f32x4 sbn) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) c[e] = fmaf(d[e], sam * sbn[e], c[e]);
-    };
-    auto compute = [&](auto opc, int buf, int kb) {
+    const auto as_float = [](int v) { return __builtin_bit_cast(float, v); };
+    // One block of 128. On entry b holds its fragments of B and a the first one of A; every fragment is read from LDS one group
+    // of matrix instructions before its use. With the last fragments of A in registers the stage is done with: the
+    // waves meet (the next stage has arrived, NST - 2 younger ones are still on their way), the loads of stage k + NST start into
+    // the buffer just freed, and the next step's first fragments are read under this step's last matrix instructions.
+    constexpr int NL = NLA + NLB;
+    int cur = 0;
+    i32x8 b[TN], a;
+    auto step = [&](auto opc, int k) {
         constexpr int OP = decltype(opc)::value;
+        const int buf = NST == 2 || NST == 4 ? OP % NST : cur, nbuf = NST == 2 || NST == 4 ? (OP + 1) % NST : cur + 1 == NST ? 0 : cur + 1;
+        cur = nbuf;
         const uint8_t* la = lds[buf];
-        const uint8_t* lb = la + BM * 128;
-        if constexpr (NATIVE) {
-            i32x8 bf[TN];
+        const uint8_t* na = lds[nbuf];
+        if constexpr (F32S) load_scales(min(k + 1, kb1 - 1), sa_next, sb_next);
+        else if constexpr (OP == 1) load_scales(min(k + 3, kb1 - 1) >> 2, sa_next, sb_next);
+        Wide bw[NATIVE ? 1 : TN];
+        if constexpr (!NATIVE) {
 #pragma unroll
-            for (int i = 0; i < TN; ++i) bf[i] = frag(lb, (wn * TN + i) * 16 + lr);
-            if constexpr (!F32S) {
-#pragma unroll
-                for (int j = 0; j < TM; ++j) {
-                    const i32x8 af = frag(la, (wm * TM + j) * 16 + lr);
-#pragma unroll
-                    for (int i = 0; i < TN; ++i) acc[i][j] = mfma_block<OP, FA>(bf[i], af, acc[i][j], sb[i], sa[j]);
-                }
-            } else {
-                block_scales(kb);
-#pragma unroll
-                for (int j = 0; j < TM; ++j) {
-                    const i32x8 af = frag(la, (wm * TM + j) * 16 + lr);
-#pragma unroll
-                    for (int i = 0; i < TN; ++i)
-                        add_block(acc[i][j], mfma_block<0, FA>(bf[i], af, f32x4{0.f, 0.f, 0.f, 0.f}, 0x7f7f7f7f, 0x7f7f7f7f), fa[j], fb[i]);
-                }
-            }
-        } else {
-            Wide bw[TN];
-#pragma unroll
-            for (int i = 0; i < TN; ++i)
-                bw[i] = widen<SM_FP8_E4M3>(frag(lb, (wn * TN + i) * 16 + lr), F32S ? 1.f : byte_scale<OP>(sb[i]));
-            if constexpr (F32S) block_scales(kb);
-#pragma unroll
-            for (int j = 0; j < TM; ++j) {
-                const Wide aw = widen<FA>(frag(la, (wm * TM + j) * 16 + lr), F32S ? 1.f : byte_scale<OP>(sa[j]));
-#pragma unroll
-                for (int i = 0; i < TN; ++i) {
-                    if constexpr (F32S) add_block(acc[i][j], mfma_wide(bw[i], aw, f32x4{0.f, 0.f, 0.f, 0.f}), fa[j], fb[i]);
-                    else acc[i][j] = mfma_wide(bw[i], aw, acc[i][j]);
-                }
-            }
+            for (int i = 0; i < TN; ++i) bw[i] = widen<SM_FP8_E4M3>(b[i], F32S ? 1.f : byte_scale<OP>(sb[i]));
         }
+#pragma unroll
+        for (int j = 0; j < TM; ++j) {
+            i32x8 next;
+            if (j + 1 < TM) {
+                next = frag(la, wm * TM + j + 1);
+            } else {
+                wait_loads<(NST - 2) * NL>();
+                __syncthreads();
+                stage(buf, min(k + NST, kb1 - 1));      // (behind the end: the last block again, read by nobody)
+                next = frag(na, wm * TM);
+            }
+            Wide aw;
+            if constexpr (!NATIVE) aw = widen<FA>(a, F32S ? 1.f : byte_scale<OP>(sa[j]));
+#pragma unroll
+            for (int i = 0; i < TN; ++i) {
+                const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+                f32x4 c = F32S ? zero : acc[i][j];
+                if constexpr (!NATIVE) c = mfma_wide(bw[i], aw, c);
+                else if constexpr (F32S) c = mfma_block<0, FA>(b[i], a, c, 0x7f7f7f7f, 0x7f7f7f7f);
+                else c = mfma_block<OP, FA>(b[i], a, c, sb[i], sa[j]);
+                if constexpr (F32S) {
+                    // the block's sum on its own, then one multiply-add per element with sa[m] sb[n]
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        acc[i][j][e] = fmaf(c[e], as_float(sa[j]) * as_float(sb[SC == SCALE_F32_ROWS ? 4 * i + e : 0]), acc[i][j][e]);
+                } else {
+                    acc[i][j] = c;
+                }
+                if (j + 1 == TM) b[i] = frag(na + BM * 128, wn * TN + i);
+            }
+            a = next;
+        }
+        if constexpr (F32S || OP == 3) take_scales();
     };
     if (kb0 < kb1) {
-        stage(0);
-        if constexpr (!F32S) load_scales(kb0 >> 2);
-        wait_loads();
+#pragma unroll
+        for (int i = 0; i < NST; ++i) stage(i, min(kb0 + i, kb1 - 1));
+        load_scales(F32S ? kb0 : kb0 >> 2, sa, sb);
+        wait_loads<(NST - 1) * NL>();
         __syncthreads();
-        int buf = 0;
+        a = frag(lds[0], wm * TM);
+#pragma unroll
+        for (int i = 0; i < TN; ++i) b[i] = frag(lds[0] + BM * 128, wn * TN + i);
         // kb0 is a multiple of 4: block kb's scale byte is byte kb % 4 of its dword, a constant of the unrolled step
         for (int kb = kb0; kb < kb1; kb += 4) {
-            auto step = [&](auto opc) {
-                const int k = kb + decltype(opc)::value;
-                if (k >= kb1) return;
-                if (k + 1 < kb1) stage(buf ^ 1);
-                compute(opc, buf, k);
-                if (decltype(opc)::value == 3 && !F32S && k + 1 < kb1) load_scales((k + 1) >> 2);
-                wait_loads();
-                __syncthreads();
-                buf ^= 1;
-            };
-            step(std::integral_constant<int, 0>{});
-            step(std::integral_constant<int, 1>{});
-            step(std::integral_constant<int, 2>{});
-            step(std::integral_constant<int, 3>{});
+            step(std::integral_constant<int, 0>{}, kb);
+            if (kb + 1 < kb1) step(std::integral_constant<int, 1>{}, kb + 1);
+            if (kb + 2 < kb1) step(std::integral_constant<int, 2>{}, kb + 2);
+            if (kb + 3 < kb1) step(std::integral_constant<int, 3>{}, kb + 3);
         }
+        wait_loads<0>();      // no load into this block's LDS may outlive it
     }
 #pragma unroll
     for (int j = 0; j < TM; ++j) {
@@ -480,6 +535,154 @@ __global__ __launch_bounds__(WM* WN * 64) void fp8_matmul_kernel(MatmulArgs g) {
             } else {
                 store4(g, m, n, acc[i][j]);
             }
+        }
+    }
+}
+
+// Few rows of A (M <= 16 TM): the product is a stream through B, which is read once, straight into the matrix instructions'
+// operand registers - no LDS, no barrier until the end. A block owns 16 rows of B; its eight waves take the blocks of 128
+// along K in turn (together 1 KB of every row at a time) and U of them are in flight per wave. X: what A is - codes (SM_FP8_*
+// + 8) or raw values (SM_TYPE_*), which every wave quantises on its way into the operand (their block maximum needs two cross-lane steps): one launch
+// for a layer's forward pass. Bound by HBM: the codes of B.
+constexpr int STREAM_WAVES = 8;
+struct StreamArgs {
+    MatmulArgs g;
+    const void* x;          // raw rows (or null)
+    size_t x_stride;
+    int K;
+};
+template <int X, int TM, bool F32S, int U>
+__global__ __launch_bounds__(STREAM_WAVES * 64) void fp8_stream_kernel(StreamArgs t) {
+    constexpr bool RAW = X < 8;
+    constexpr int FA = X == 8 + SM_FP8_E5M2 ? SM_FP8_E5M2 : SM_FP8_E4M3;
+    const MatmulArgs& g = t.g;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lr = lane & 15, lg = lane >> 4;
+    const int n0 = blockIdx.x * 16;
+    const int kb0 = blockIdx.y * g.kb_per_split, kb1 = min(g.KB, kb0 + g.kb_per_split);
+    const int brow = min(n0 + lr, g.N - 1);
+    const uint8_t* bp = g.b + (size_t)brow * g.b_pitch + lg * 16;
+    f32x4 acc[TM];
+#pragma unroll
+    for (int j = 0; j < TM; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    // NB blocks, STREAM_WAVES apart: all loads first, then the arithmetic. FULL: K covers the blocks (raw rows end inside the last one).
+    constexpr int RV = RAW ? (X == SM_TYPE_F32 ? 8 : 4) : 2;       // 16-byte vectors of A per lane and block
+    auto group = [&](auto nbc, auto fullc, int kb) {
+        constexpr int NB = decltype(nbc)::value;
+        constexpr bool FULL = decltype(fullc)::value;
+        u32x4 bv[NB][2], av[NB][TM][RV];
+        int sbyte[NB], sa[NB][TM];
+        f32x4 fb[NB];
+#pragma unroll
+        for (int u = 0; u < NB; ++u) {
+            const int k = kb + u * STREAM_WAVES;
+            bv[u][0] = *reinterpret_cast<const u32x4*>(bp + (size_t)k * 128);
+            bv[u][1] = *reinterpret_cast<const u32x4*>(bp + (size_t)k * 128 + 64);
+            if constexpr (F32S) {
+                const float* pb = static_cast<const float*>(g.bs) + (size_t)k * g.bs_rows;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) fb[u][e] = pb[min(n0 + lg * 4 + e, g.N - 1) >> g.b_shift];
+            } else {
+                sbyte[u] = static_cast<const uint8_t*>(g.bs)[scale_at(k, brow >> g.b_shift, g.bs_rows)];
+            }
+#pragma unroll
+            for (int j = 0; j < TM; ++j) {
+                const int m = min(j * 16 + lr, g.M - 1);
+                if constexpr (RAW) {
+                    // the same places of the block as B's chunks: elements 16 lg ... + 15 and 64 + 16 lg ... + 15
+                    const int c = k * 128 + lg * 16;
+                    if constexpr (FULL) {
+                        constexpr int ES = X == SM_TYPE_F32 ? 4 : 2;
+                        const char* xp = static_cast<const char*>(t.x) + ((size_t)m * t.x_stride + c) * ES;
+#pragma unroll
+                        for (int q = 0; q < RV; ++q)
+                            av[u][j][q] = *reinterpret_cast<const u32x4_u*>(xp + (q < RV / 2 ? q * 16 : 64 * ES + (q - RV / 2) * 16));
+                    }
+                } else {
+                    const uint8_t* ap = g.a + (size_t)m * g.a_pitch + (size_t)k * 128 + lg * 16;
+                    av[u][j][0] = *reinterpret_cast<const u32x4*>(ap);
+                    av[u][j][1] = *reinterpret_cast<const u32x4*>(ap + 64);
+                    if constexpr (F32S) sa[u][j] = __builtin_bit_cast(int, static_cast<const float*>(g.as)[(size_t)k * g.M + m]);
+                    else sa[u][j] = static_cast<const uint8_t*>(g.as)[scale_at(k, m, g.M)];
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < NB; ++u) {
+            const Wide bw = widen<SM_FP8_E4M3>(join(bv[u][0], bv[u][1]), F32S ? 1.f : __builtin_bit_cast(float, (unsigned)sbyte[u] << 23));
+#pragma unroll
+            for (int j = 0; j < TM; ++j) {
+                i32x8 codes;
+                int byte;
+                if constexpr (RAW) {
+                    float v[32];
+                    if constexpr (FULL) {
+#pragma unroll
+                        for (int q = 0; q < RV; ++q) unpack<X>(av[u][j][q], v + q * (32 / RV));
+                    } else {
+                        const int k = kb + u * STREAM_WAVES, c = k * 128 + lg * 16, m = min(j * 16 + lr, g.M - 1);
+                        const size_t row = (size_t)m * t.x_stride;
+                        load8<X>(t.x, row + c, t.K - c, v);
+                        load8<X>(t.x, row + c + 8, t.K - c - 8, v + 8);
+                        load8<X>(t.x, row + c + 64, t.K - c - 64, v + 16);
+                        load8<X>(t.x, row + c + 72, t.K - c - 72, v + 24);
+                    }
+                    float m = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) m = fmaxf(m, finite_abs(v[i]));
+                    m = fmaxf(m, __shfl_xor(m, 16, 64));
+                    m = fmaxf(m, __shfl_xor(m, 32, 64));
+                    const int e = block_exponent(m, 8);
+                    byte = e + 127;
+                    const float inv = inv_pow2(e);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const u32x2 w = cvt8(v + 8 * q, inv, SM_FP8_E4M3);
+                        codes[2 * q] = (int)w[0];
+                        codes[2 * q + 1] = (int)w[1];
+                    }
+                } else {
+                    codes = join(av[u][j][0], av[u][j][1]);
+                    byte = sa[u][j];
+                }
+                if constexpr (F32S) {
+                    const f32x4 d = mfma_wide(bw, widen<FA>(codes, 1.f), f32x4{0.f, 0.f, 0.f, 0.f});
+                    const float fa = __builtin_bit_cast(float, byte);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[j][e] = fmaf(d[e], fa * fb[u][e], acc[j][e]);
+                } else {
+                    acc[j] = mfma_wide(bw, widen<FA>(codes, __builtin_bit_cast(float, (unsigned)byte << 23)), acc[j]);
+                }
+            }
+        }
+    };
+    constexpr std::integral_constant<bool, true> full{};
+    const int kbf = RAW ? min(kb1, t.K >> 7) : kb1;       // blocks that K covers whole
+    int kb = kb0 + wave;
+    for (; kb + (U - 1) * STREAM_WAVES < kbf; kb += STREAM_WAVES * U) group(std::integral_constant<int, U>{}, full, kb);
+    if constexpr (U > 2)
+        for (; kb + STREAM_WAVES < kbf; kb += STREAM_WAVES * 2) group(std::integral_constant<int, 2>{}, full, kb);
+    for (; kb < kbf; kb += STREAM_WAVES) group(std::integral_constant<int, 1>{}, full, kb);
+    if constexpr (RAW)
+        if (kb < kb1) group(std::integral_constant<int, 1>{}, std::integral_constant<bool, false>{}, kb);
+    // the waves' sums, added in their order
+    __shared__ f32x4 part[STREAM_WAVES][TM][64];
+#pragma unroll
+    for (int j = 0; j < TM; ++j) part[wave][j][lane] = acc[j];
+    __syncthreads();
+    for (int j = wave; j < TM; j += STREAM_WAVES) {
+        f32x4 s = part[0][j][lane];
+#pragma unroll
+        for (int w = 1; w < STREAM_WAVES; ++w) s += part[w][j][lane];
+        const int m = j * 16 + lr, n = n0 + lg * 4;
+        if (m >= g.M || n >= g.N) continue;
+        if (gridDim.y > 1) {
+            float* o = g.ws + ((size_t)blockIdx.y * g.M + m) * g.N + n;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (n + e < g.N) o[e] = s[e];
+        } else {
+            store4(g, m, n, s);
         }
     }
 }
@@ -507,24 +710,87 @@ __global__ __launch_bounds__(256) void fp8_matmul_empty_kernel(MatmulArgs g) {
     if (id < per_row * g.M) store4(g, (int)(id / per_row), (int)(id % per_row) * 4, f32x4{0.f, 0.f, 0.f, 0.f});
 }
 
+// Which kernel takes an M x N x 128 KB product, and in how many slices of K. Measured on MI355X (us):
+//                                        256 x 256   256 x 128   128 x 128   64 x 64
+//   8192^3      bf16 result, 2^e scales        413         488         499       921
+//   4096^3      bf16 result, 2^e scales         59          71          70       126
+//   4096^3      f16 result, fp32 scales        317         123         133       201   (256 x 256 spills)
+//   2048^3      bf16 result, 2^e scales         33          22          17        18
+//   512 x 4096 x 4096, bf16                     50          31          26        18
+// A 256-row tile takes a CU, two 128 x 128 tiles share one: the large tile is taken where its rounds over the 256 CUs are not
+// emptier than the small one's by more than what it gains (1.2 x); below 192 tiles of 128 x 128 the chip is filled with
+// 64 x 64 ones, and where even those are few (a weight gradient of small layers) K is split, at least eight blocks a slice, and
+// the slices are added by a second kernel (128 x 256 x 8192: 27 us in one slice).
+// Up to 64 rows the stream kernel: it reads B once at any M.
+enum { TILE_STREAM, TILE_64, TILE_128, TILE_256 };
 struct Plan {
-    int bm, bn, splits, kb_per_split;
+    int kind, splits, kb_per_split;
 };
 static Plan matmul_plan(int M, int N, int KB) {
-    Plan p{128, 128, 1, KB};
+    const auto tiles = [&](long long bm, long long bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
+    const auto fill = [](long long t, long long slots) { return (double)t / (double)((t + slots - 1) / slots * slots); };
+    Plan p{TILE_64, 1, KB};
+    long long t = tiles(64, 64);
+    if (M <= 64) {
+        p.kind = TILE_STREAM;
+        t = (N + 15) / 16;
+    } else if (tiles(128, 128) >= 192) {
+        p.kind = 1.2 * fill(tiles(256, 256), 256) >= fill(tiles(128, 128), 512) ? TILE_256 : TILE_128;
+        return p;
+    }
+    if (t <= 128 && KB >= 16) {
+        const long long want = std::min<long long>(256 / t, KB / (p.kind == TILE_STREAM ? 32 : 8));
+        if (want > 1) {
+            p.kb_per_split = (int)((KB + want - 1) / want + 3) / 4 * 4;      // (whole dwords of scale bytes)
+            p.splits = (KB + p.kb_per_split - 1) / p.kb_per_split;
+        }
+    }
     return p;
 }
 
-template <int BM, int BN, int WM, int WN, bool NATIVE>
-static void launch_matmul(const MatmulArgs& g, int a_fmt, bool f32s, int splits, hipStream_t s) {
-    const dim3 grid((unsigned)(((g.M + BM - 1) / BM) * ((g.N + BN - 1) / BN)), (unsigned)splits), block(WM * WN * 64);
-    if (f32s) {
-        if (a_fmt == SM_FP8_E4M3) hipLaunchKernelGGL((fp8_matmul_kernel<BM, BN, WM, WN, 0, true, NATIVE>), grid, block, 0, s, g);
-        else hipLaunchKernelGGL((fp8_matmul_kernel<BM, BN, WM, WN, 1, true, NATIVE>), grid, block, 0, s, g);
+template <int X, int TM, bool F32S>
+static void launch_stream(const StreamArgs& t, int splits, hipStream_t s) {
+    constexpr int U = X < 8 ? (X == SM_TYPE_F32 ? 2 : 4) : (TM == 1 ? 4 : 2);
+    hipLaunchKernelGGL((fp8_stream_kernel<X, TM, F32S, U>), dim3((unsigned)((t.g.N + 15) / 16), (unsigned)splits), dim3(STREAM_WAVES * 64), 0, s, t);
+}
+template <int TM>
+static void launch_stream_codes(const StreamArgs& t, int a_fmt, bool f32s, int splits, hipStream_t s) {
+    if (a_fmt == SM_FP8_E4M3) {
+        if (f32s) launch_stream<8 + SM_FP8_E4M3, TM, true>(t, splits, s);
+        else launch_stream<8 + SM_FP8_E4M3, TM, false>(t, splits, s);
     } else {
-        if (a_fmt == SM_FP8_E4M3) hipLaunchKernelGGL((fp8_matmul_kernel<BM, BN, WM, WN, 0, false, NATIVE>), grid, block, 0, s, g);
-        else hipLaunchKernelGGL((fp8_matmul_kernel<BM, BN, WM, WN, 1, false, NATIVE>), grid, block, 0, s, g);
+        if (f32s) launch_stream<8 + SM_FP8_E5M2, TM, true>(t, splits, s);
+        else launch_stream<8 + SM_FP8_E5M2, TM, false>(t, splits, s);
     }
+}
+static void launch_reduce(const MatmulArgs& g, int splits, hipStream_t s) {
+    const size_t quads = (size_t)(g.N + 3) / 4 * g.M;
+    hipLaunchKernelGGL(fp8_matmul_reduce_kernel, dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, s, g, splits);
+}
+
+template <int BM, int BN, int WM, int WN, int NST, bool NATIVE, bool F32S>
+static void launch_matmul(const MatmulArgs& g, int a_fmt, int splits, hipStream_t s) {
+    const dim3 grid((unsigned)(((g.M + BM - 1) / BM) * ((g.N + BN - 1) / BN)), (unsigned)splits), block(WM * WN * 64);
+    const auto go = [&](auto fa, auto sc) {
+        hipLaunchKernelGGL((fp8_matmul_kernel<BM, BN, WM, WN, NST, decltype(fa)::value, decltype(sc)::value, NATIVE>), grid, block, 0, s, g);
+    };
+    const auto with_format = [&](auto sc) {
+        if (a_fmt == SM_FP8_E4M3) go(std::integral_constant<int, SM_FP8_E4M3>{}, sc);
+        else go(std::integral_constant<int, SM_FP8_E5M2>{}, sc);
+    };
+    if constexpr (!F32S) with_format(std::integral_constant<int, SCALE_POW2>{});
+    else if (g.b_shift == 0) with_format(std::integral_constant<int, SCALE_F32_ROWS>{});
+    else with_format(std::integral_constant<int, SCALE_F32_TILES>{});
+}
+
+template <bool NATIVE>
+static void launch_tile(int kind, const MatmulArgs& g, int a_fmt, bool f32s, int splits, hipStream_t s) {
+    if (kind == TILE_256 && !f32s) launch_matmul<256, 256, 2, 4, 2, NATIVE, false>(g, a_fmt, splits, s);
+    else if (kind == TILE_256) launch_matmul<256, 128, 4, 2, 3, NATIVE, true>(g, a_fmt, splits, s);
+    else if (kind == TILE_128 && !f32s) launch_matmul<128, 128, 2, 2, 2, NATIVE, false>(g, a_fmt, splits, s);
+    else if (kind == TILE_128) launch_matmul<128, 128, 2, 2, 2, NATIVE, true>(g, a_fmt, splits, s);
+    else if (!f32s) launch_matmul<64, 64, 2, 2, 4, NATIVE, false>(g, a_fmt, splits, s);
+    else launch_matmul<64, 64, 2, 2, 4, NATIVE, true>(g, a_fmt, splits, s);
 }
 
 template <int T>
@@ -591,12 +857,69 @@ int sm_fp8_matmul(const void* a, const void* a_scale, int a_fmt, size_t a_pitch,
     const sm::Plan p = sm::matmul_plan(M, N, KB);
     if (p.splits > 1 && (ws == nullptr || ws_bytes < (size_t)p.splits * M * N * sizeof(float))) return (int)hipErrorInvalidValue;
     g.kb_per_split = p.kb_per_split;
-    sm::launch_matmul<128, 128, 2, 2, false>(g, a_fmt, scale_f32 != 0, p.splits, s);
-    SM_LAUNCH_CHECK();
-    if (p.splits > 1) {
-        hipLaunchKernelGGL(sm::fp8_matmul_reduce_kernel, dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, s, g, p.splits);
-        SM_LAUNCH_CHECK();
+    const bool f32s = scale_f32 != 0;
+    if (p.kind == sm::TILE_STREAM) {
+        const sm::StreamArgs t{g, nullptr, 0, K};
+        if (M <= 16) sm::launch_stream_codes<1>(t, a_fmt, f32s, p.splits, s);
+        else if (M <= 32) sm::launch_stream_codes<2>(t, a_fmt, f32s, p.splits, s);
+        else sm::launch_stream_codes<4>(t, a_fmt, f32s, p.splits, s);
+    } else {
+        // The 8-bit matrix instruction aligns the products of eight neighbouring k to the largest of them and keeps 13 bits below
+        // its leading one (measured; so does the older 16x16x32 form), fp32 beyond that: relative to sum |a||b| an error of
+        // 2^-19 (normal data) to 2^-15 (log-normal, sigma 2) at K = 128, falling with sqrt(K). It is taken where the result
+        // is bf16 - half a step is 2^-9 - and K >= 1024, where it stays inside what a plain fp32 sum of K terms may lose.
+        // Every other product widens the codes to bf16 (exact, scale included) and sums in fp32 throughout, at half the rate.
+        if (out_type == SM_TYPE_BF16 && KB >= 8) sm::launch_tile<true>(p.kind, g, a_fmt, f32s, p.splits, s);
+        else sm::launch_tile<false>(p.kind, g, a_fmt, f32s, p.splits, s);
     }
+    SM_LAUNCH_CHECK();
+    if (p.splits > 1) sm::launch_reduce(g, p.splits, s);
+    SM_LAUNCH_CHECK();
+    return 0;
+}
+
+// rows up to which a layer's forward pass quantises inside the product
+static constexpr int LINEAR_FUSED_ROWS = 16;
+
+size_t sm_fp8_linear_ws_bytes(int M, int N, int K) {
+    if (M <= 0 || N <= 0 || K <= 0) return 0;
+    const size_t slabs = sm_fp8_matmul_ws_bytes(M, N, K);
+    if (M <= LINEAR_FUSED_ROWS) return slabs;
+    const size_t KB = ((size_t)K + 127) / 128;
+    return (slabs + 15) / 16 * 16 + (size_t)M * KB * 128 + (KB + 3) / 4 * M * 4;
+}
+
+int sm_fp8_linear(const void* x, int x_type, size_t x_stride, const void* w, const void* w_scale, int w_tiles, size_t w_pitch, int M,
+                  int N, int K, void* out, int out_type, size_t out_stride, void* ws, size_t ws_bytes, void* stream) {
+    if (M < 0 || N < 0 || K < 0 || x_type < 0 || x_type > SM_TYPE_F16 || out_type < 0 || out_type > SM_TYPE_F16)
+        return (int)hipErrorInvalidValue;
+    if (M == 0 || N == 0) return 0;
+    if (K > 0 && (x == nullptr || x_stride < (size_t)K || (ws == nullptr && sm_fp8_linear_ws_bytes(M, N, K) > 0) ||
+                  ws_bytes < sm_fp8_linear_ws_bytes(M, N, K)))
+        return (int)hipErrorInvalidValue;
+    const int KB = (K + 127) / 128;
+    if (K == 0 || M > LINEAR_FUSED_ROWS) {
+        const size_t slabs = (sm_fp8_matmul_ws_bytes(M, N, K) + 15) / 16 * 16;
+        char* q = (char*)ws + slabs;
+        char* qs = q + (size_t)M * KB * 128;
+        if (K > 0)
+            if (const int e = sm_fp8_quantize(x, x_type, M, K, x_stride, SM_FP8_E4M3, 0, q, qs, nullptr, nullptr, stream)) return e;
+        return sm_fp8_matmul(q, qs, SM_FP8_E4M3, (size_t)KB * 128, w, w_scale, w_tiles, w_pitch, 0, M, N, K, out, out_type, out_stride, 0,
+                             ws, slabs, stream);
+    }
+    if (out == nullptr || out_stride < (size_t)N || w == nullptr || w_scale == nullptr || w_pitch < (size_t)KB * 128 || w_pitch % 16 ||
+        (uintptr_t)w % 16)
+        return (int)hipErrorInvalidValue;
+    hipStream_t s = (hipStream_t)stream;
+    const sm::Plan p = sm::matmul_plan(M, N, KB);
+    sm::StreamArgs t{{nullptr, (const uint8_t*)w, nullptr, w_scale, out, (float*)ws, 0, w_pitch, out_stride, M, N, KB, w_tiles ? 7 : 0,
+                      w_tiles ? (N + 127) / 128 : N, out_type, 0, p.kb_per_split}, x, x_stride, K};
+    if (x_type == SM_TYPE_F32) sm::launch_stream<SM_TYPE_F32, 1, false>(t, p.splits, s);
+    else if (x_type == SM_TYPE_BF16) sm::launch_stream<SM_TYPE_BF16, 1, false>(t, p.splits, s);
+    else sm::launch_stream<SM_TYPE_F16, 1, false>(t, p.splits, s);
+    SM_LAUNCH_CHECK();
+    if (p.splits > 1) sm::launch_reduce(t.g, p.splits, s);
+    SM_LAUNCH_CHECK();
     return 0;
 }
 

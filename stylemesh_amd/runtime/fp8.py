@@ -26,16 +26,13 @@ def _blocks(n: int) -> int:
 
 def _check_device(*tensors):
     """Launches go to the CURRENT device's current stream: tensors of another device (or of the host) are refused."""
-    cur = None
     for t in tensors:
         if t is None:
             continue
         if not t.is_cuda:
             raise ValueError("device tensors only (there is no CPU form)")
-        if cur is None:
-            cur = torch.cuda.current_device()
-        if t.device.index != cur:
-            raise ValueError(f"a tensor lives on {t.device}, the current device is cuda:{cur}")
+        if t.get_device() != torch.cuda.current_device():
+            raise ValueError(f"a tensor lives on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
 
 
 class Fp8Matrix:
@@ -47,7 +44,7 @@ class Fp8Matrix:
     (row, block kb) at [kb / 4, row, kb % 4], KB = ceil(cols / 128), S = rows or ceil(rows / 128) - or float32 scales [KB, S].
     The tensors are used as they are, no copy is taken."""
 
-    __slots__ = ("data", "scale", "cols", "block")
+    __slots__ = ("data", "scale", "cols", "block", "_ptrs")
 
     def __init__(self, data: torch.Tensor, scale: torch.Tensor, cols: int, block: str = "rows"):
         if block not in ("rows", "tiles"):
@@ -67,6 +64,7 @@ class Fp8Matrix:
         if scale.device != data.device:
             raise ValueError(f"codes on {data.device}, scales on {scale.device}")
         self.data, self.scale, self.cols, self.block = data, scale, int(cols), block
+        self._ptrs = (data.data_ptr(), scale.data_ptr())      # (of tensors this object keeps)
 
     @property
     def rows(self) -> int:
@@ -225,8 +223,7 @@ def matmul_fp8(a: Fp8Matrix, b: Fp8Matrix, out: torch.Tensor | None = None, out_
     need = ops.lib.sm_fp8_matmul_ws_bytes(M, N, K)
     # (scratch of this call's own: two captured graphs, or two streams, never share slabs)
     ws = torch.empty(need, dtype=torch.uint8, device=a.device) if need else None
-    hip.check(ops.lib.sm_fp8_matmul(a.data.data_ptr(), a.scale.data_ptr(), _FMT_ID[a.data.dtype], a.data.shape[1],
-                                    b.data.data_ptr(), b.scale.data_ptr(), int(b.block == "tiles"), b.data.shape[1],
+    hip.check(ops.lib.sm_fp8_matmul(*a._ptrs, _FMT_ID[a.data.dtype], a.data.shape[1], *b._ptrs, int(b.block == "tiles"), b.data.shape[1],
                                     int(a.scale.dtype == torch.float32), M, N, K, out.data_ptr(), _TYPE_ID[out.dtype],
                                     out.stride(0) if M > 1 else N, int(accumulate), ptr(ws), need, hip.stream()), "sm_fp8_matmul")
     return out
@@ -244,11 +241,27 @@ def linear_fp8_fwd(x: torch.Tensor, weight: Fp8Matrix, out_dtype=None, keep_tran
     from the same read of x."""
     _weight_arg(weight)
     _matrix_arg(x, "x")
-    if x.shape[1] != weight.cols:
-        raise ValueError(f"x has {x.shape[1]} columns, the weight {weight.cols}")
-    n, t = _quantize(x, "rows", "e4m3", True, keep_transposed)
-    y = matmul_fp8(n, weight, out_dtype=out_dtype or x.dtype)
-    return (y, t) if keep_transposed else y
+    M, K = x.shape
+    if K != weight.cols:
+        raise ValueError(f"x has {K} columns, the weight {weight.cols}")
+    if out_dtype is None:
+        out_dtype = x.dtype
+    if keep_transposed:
+        n, t = _quantize(x, "rows", "e4m3", True, True)
+        return matmul_fp8(n, weight, out_dtype=out_dtype), t
+    if out_dtype not in _TYPE_ID:
+        raise ValueError(f"out_dtype={out_dtype}: float32, bfloat16 or float16")
+    _check_device(weight.data)
+    N = weight.rows
+    y = torch.empty(M, N, dtype=out_dtype, device=x.device)
+    if M and N:
+        lib = ops.lib
+        need = lib.sm_fp8_linear_ws_bytes(M, N, K)
+        ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None      # of this call's own, as matmul_fp8's
+        hip.check(lib.sm_fp8_linear(x.data_ptr(), _TYPE_ID[x.dtype], x.stride(0) if M > 1 else K, *weight._ptrs,
+                                    int(weight.block == "tiles"), weight.data.shape[1], M, N, K, y.data_ptr(), _TYPE_ID[out_dtype], N,
+                                    None if ws is None else ws.data_ptr(), need, hip.stream()), "sm_fp8_linear")
+    return y
 
 
 def linear_fp8_bwd(dy: torch.Tensor, x_t: Fp8Matrix | None, weight_t: Fp8Matrix | None, fmt: str = "e4m3", dx_dtype=None,
