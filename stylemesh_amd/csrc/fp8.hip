@@ -132,48 +132,163 @@ struct QuantArgs {
     uint8_t *q, *qs, *qt, *qts;
 };
 
-// One 128 x 128 tile per block of 256 threads: thread t holds rows 8 (t / 16) ... + 7, columns 8 (t % 16) ... + 7 in registers
-// (x is read once whatever is produced). Row maxima: 16 lanes of a row; column maxima: registers, then the wave's four row
-// groups, then the four waves through LDS; tile maximum: all. The transposed codes go through a 128 x (128 + 16) byte LDS
-// image so that both results leave as whole 128-byte lines.
-// Bound by HBM: cols * rows * (sizeof(x) + 1 per result).
-template <int T, bool TILES, bool Q, bool QT>
-__global__ __launch_bounds__(256) void fp8_quantize_kernel(QuantArgs a) {
-    const int tid = threadIdx.x, rg = tid >> 4, cg = tid & 15, wave = tid >> 6;
-    const int tr = blockIdx.y * 128, tc = blockIdx.x * 128;
-    const int top = a.fmt == SM_FP8_E4M3 ? 8 : 15;
-    const int c0 = tc + cg * 8;
-    float v[8][8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int r = tr + rg * 8 + i;
-        load8<T>(a.x, (size_t)r * a.stride + c0, r < a.rows ? a.cols - c0 : 0, v[i]);
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+typedef short s16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+
+// Magnitudes compare like their bits: a dword holds one fp32 or two 16-bit ones, and maxima are integer maxima.
+template <int T>
+__device__ __forceinline__ unsigned mag(unsigned d) { return d & (T == SM_TYPE_F32 ? 0x7fffffffu : 0x7fff7fffu); }
+template <int T>
+__device__ __forceinline__ unsigned mag_max(unsigned a, unsigned b) {
+    if constexpr (T == SM_TYPE_F32) return max(a, b);
+    else return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+}
+template <int T>
+constexpr unsigned inf_bits = T == SM_TYPE_F32 ? 0x7f800000u : T == SM_TYPE_BF16 ? 0x7f80u : 0x7c00u;
+template <int T>
+__device__ __forceinline__ unsigned mag_both(unsigned m) { return T == SM_TYPE_F32 ? m : max(m & 0xffffu, m >> 16); }   // of a dword's values
+template <int T>
+__device__ __forceinline__ unsigned mag_finite(unsigned m) {      // non-finite values -> 0
+    if constexpr (T == SM_TYPE_F32) return m >= inf_bits<T> ? 0u : m;
+    else return ((m & 0xffffu) >= inf_bits<T> ? 0u : m & 0xffffu) | ((m >> 16) >= inf_bits<T> ? 0u : m & 0xffff0000u);
+}
+template <int T>
+__device__ __forceinline__ float mag_float(unsigned m) {
+    return T == SM_TYPE_F32 ? __builtin_bit_cast(float, m) : T == SM_TYPE_BF16 ? bf16_to_f32(m) : f16_to_f32(m);
+}
+// max over the 16 lanes of a row of the wave (data-parallel moves, no LDS)
+template <int T>
+__device__ __forceinline__ unsigned row16_max(unsigned m) {
+    m = mag_max<T>(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0x128, 0xf, 0xf, false));      // row_ror 8, 4, 2, 1
+    m = mag_max<T>(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0x124, 0xf, 0xf, false));
+    m = mag_max<T>(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0x122, 0xf, 0xf, false));
+    return mag_max<T>(m, (unsigned)__builtin_amdgcn_update_dpp(0, (int)m, 0x121, 0xf, 0xf, false));
+}
+
+// Two finite values divided by 2^e -> two codes: one instruction, round to nearest even (scale: the float 2^e, normal).
+// 16-bit types: v = the dword of both; fp32: v and w.
+template <int T, bool HI>
+__device__ __forceinline__ s16x2 cvt_scaled(unsigned v, unsigned w, float scale, s16x2 old, int fmt) {
+    if (fmt == SM_FP8_E4M3) {
+        if constexpr (T == SM_TYPE_F32) return __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(old, __builtin_bit_cast(float, v), __builtin_bit_cast(float, w), scale, HI);
+        else if constexpr (T == SM_TYPE_BF16) return __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(old, __builtin_bit_cast(bf16x2, v), scale, HI);
+        else return __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(old, __builtin_bit_cast(f16x2, v), scale, HI);
     }
-    __shared__ float red[4][128];
-    __shared__ __align__(16) uint8_t img[QT ? 128 * 144 : 16];
-    float rmax[8], cmax[8];
+    if constexpr (T == SM_TYPE_F32) return __builtin_amdgcn_cvt_scalef32_pk_bf8_f32(old, __builtin_bit_cast(float, v), __builtin_bit_cast(float, w), scale, HI);
+    else if constexpr (T == SM_TYPE_BF16) return __builtin_amdgcn_cvt_scalef32_pk_bf8_bf16(old, __builtin_bit_cast(bf16x2, v), scale, HI);
+    else return __builtin_amdgcn_cvt_scalef32_pk_bf8_f16(old, __builtin_bit_cast(f16x2, v), scale, HI);
+}
+// Eight values of a row (16-bit: 4 dwords, fp32: 8) -> eight codes. plain: all finite and the scale a normal float; otherwise
+// each value is scaled and selected on its own.
+template <int T>
+__device__ __forceinline__ u32x2 codes8(const unsigned* d, int e, int fmt, bool plain) {
+    u32x2 r;
+    if (plain) {
+        const float scale = __builtin_bit_cast(float, (unsigned)(e + 127) << 23);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        float m = 0.f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) m = fmaxf(m, finite_abs(v[i][j]));
-        if (!TILES && Q) {
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+        for (int h = 0; h < 2; ++h) {
+            s16x2 c = {0, 0};
+            if constexpr (T == SM_TYPE_F32) {
+                c = cvt_scaled<T, false>(d[4 * h], d[4 * h + 1], scale, c, fmt);
+                c = cvt_scaled<T, true>(d[4 * h + 2], d[4 * h + 3], scale, c, fmt);
+            } else {
+                c = cvt_scaled<T, false>(d[2 * h], 0, scale, c, fmt);
+                c = cvt_scaled<T, true>(d[2 * h + 1], 0, scale, c, fmt);
+            }
+            r[h] = __builtin_bit_cast(unsigned, c);
         }
-        rmax[i] = m;
+        return r;
     }
+    float v[8];
+#pragma unroll
+    for (int q = 0; q < (T == SM_TYPE_F32 ? 2 : 1); ++q) unpack<T>(u32x4{d[4 * q], d[4 * q + 1], d[4 * q + 2], d[4 * q + 3]}, v + 4 * q);
+    return cvt8(v, inv_pow2(e), fmt);
+}
+
+// One tile of 16 RPT rows x 128 columns per block of 256 threads: thread t holds rows RPT (t / 16) ... and columns
+// 8 (t % 16) ... + 7 as they came (all its loads in flight together; x is read once whatever is produced). Maxima are taken on
+// the bits, two 16-bit values per instruction: a block row's 16 lanes by data-parallel moves; columns in registers, then
+// the wave's four row groups, then the four waves through LDS; tiles over everything. The scaled conversion instruction does the rest
+// (about three instructions an element where it was twenty). The transposed codes turn through a 128 x 128 byte LDS image
+// whose 8-byte units are swizzled by their column group, and both results leave as whole 128-byte lines.
+// Bound by HBM: rows * cols * (sizeof(x) + 1 per result). Transposes and tiles need RPT = 8 (128 rows); rows alone take RPT = 1
+// where that leaves too few blocks (16 x 4096 fp32: 8.2 -> 3 us).
+template <int T, bool TILES, bool Q, bool QT, int RPT>
+__global__ __launch_bounds__(256) void fp8_quantize_kernel(QuantArgs a) {
+    static_assert(RPT == 8 || (!TILES && !QT), "column blocks need 128 rows");
+    constexpr int ND = T == SM_TYPE_F32 ? 8 : 4;      // dwords of eight values
+    constexpr int ES = T == SM_TYPE_F32 ? 4 : 2;
+    const int tid = threadIdx.x, rg = tid >> 4, cg = tid & 15, wave = tid >> 6;
+    const int tr = blockIdx.y * 16 * RPT, tc = blockIdx.x * 128, c0 = tc + cg * 8;
+    const int top = a.fmt == SM_FP8_E4M3 ? 8 : 15;
+    unsigned d[RPT][ND];
+    if (c0 + 8 <= a.cols) {
+#pragma unroll
+        for (int i = 0; i < RPT; ++i) {
+            const int r = min(tr + rg * RPT + i, a.rows - 1);
+            const u32x4_u* p = reinterpret_cast<const u32x4_u*>(static_cast<const char*>(a.x) + ((size_t)r * a.stride + c0) * ES);
+#pragma unroll
+            for (int q = 0; q < ND / 4; ++q) {
+                const u32x4 w = p[q];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) d[i][4 * q + j] = w[j];
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < RPT; ++i) {
+            const int r = min(tr + rg * RPT + i, a.rows - 1);
+#pragma unroll
+            for (int j = 0; j < ND; ++j) {
+                const size_t at = (size_t)r * a.stride + c0;
+                if constexpr (T == SM_TYPE_F32) {
+                    d[i][j] = c0 + j < a.cols ? static_cast<const unsigned*>(a.x)[at + j] : 0u;
+                } else {
+                    const uint16_t* p = static_cast<const uint16_t*>(a.x) + at;
+                    d[i][j] = (c0 + 2 * j < a.cols ? (unsigned)p[2 * j] : 0u) | (c0 + 2 * j + 1 < a.cols ? (unsigned)p[2 * j + 1] << 16 : 0u);
+                }
+            }
+        }
+    }
+    unsigned rmax[RPT], all = 0;
+#pragma unroll
+    for (int i = 0; i < RPT; ++i) {
+        if (tr + rg * RPT + i >= a.rows) {      // (behind the last row: zeros)
+#pragma unroll
+            for (int j = 0; j < ND; ++j) d[i][j] = 0;
+        }
+        unsigned m = 0;
+#pragma unroll
+        for (int j = 0; j < ND; ++j) m = mag_max<T>(m, mag<T>(d[i][j]));
+        rmax[i] = m;
+        all = mag_max<T>(all, m);
+    }
+    // a wave that holds infinities or NaN takes its maxima again without them, and converts value by value
+    const bool finite = !__any(mag_both<T>(all) >= inf_bits<T>);
+    if (!finite) {
+        all = 0;
+#pragma unroll
+        for (int i = 0; i < RPT; ++i) {
+            unsigned m = 0;
+#pragma unroll
+            for (int j = 0; j < ND; ++j) m = mag_max<T>(m, mag_finite<T>(mag<T>(d[i][j])));
+            rmax[i] = m;
+            all = mag_max<T>(all, m);
+        }
+    }
+    __shared__ unsigned red[4][QT && !TILES ? 16 * ND : 1];
+    __shared__ __align__(16) uint8_t img[QT ? 128 * 128 : 16];
     const int cblocks = (a.cols + 127) >> 7, rblocks = (a.rows + 127) >> 7;
     int tile_e = 0;
     if constexpr (TILES) {
-        float m = rmax[0];
+        unsigned m = mag_both<T>(all);
 #pragma unroll
-        for (int i = 1; i < 8; ++i) m = fmaxf(m, rmax[i]);
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+        for (int o = 32; o > 0; o >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, o, 64));
         if ((tid & 63) == 0) red[wave][0] = m;
         __syncthreads();
-        tile_e = block_exponent(fmaxf(fmaxf(red[0][0], red[1][0]), fmaxf(red[2][0], red[3][0])), top);
+        tile_e = block_exponent(mag_float<T>(max(max(red[0][0], red[1][0]), max(red[2][0], red[3][0]))), top);
         if (tid < 4) {      // thread 0: this tile's byte; the row's / column's last tile also fills the dword's unused bytes
             if (Q && (tid == 0 || ((int)blockIdx.x + tid < (cblocks + 3) / 4 * 4 && (int)blockIdx.x == cblocks - 1)))
                 a.qs[scale_at(blockIdx.x + tid, blockIdx.y, rblocks)] = tid == 0 ? (uint8_t)(tile_e + 127) : (uint8_t)127;
@@ -184,11 +299,11 @@ __global__ __launch_bounds__(256) void fp8_quantize_kernel(QuantArgs a) {
     if constexpr (Q) {
         const size_t pitch = (size_t)cblocks * 128;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int r = tr + rg * 8 + i;
-            const int e = TILES ? tile_e : block_exponent(rmax[i], top);
+        for (int i = 0; i < RPT; ++i) {
+            const int r = tr + rg * RPT + i;
+            const int e = TILES ? tile_e : block_exponent(mag_float<T>(mag_both<T>(row16_max<T>(rmax[i]))), top);
             if (r < a.rows) {
-                *reinterpret_cast<u32x2*>(a.q + (size_t)r * pitch + c0) = cvt8(v[i], inv_pow2(e), a.fmt);
+                *reinterpret_cast<u32x2*>(a.q + (size_t)r * pitch + c0) = codes8<T>(d[i], e, a.fmt, finite && e > -127);
                 if (!TILES && cg < 4 && (cg == 0 || ((int)blockIdx.x == cblocks - 1 && (int)blockIdx.x + cg < (cblocks + 3) / 4 * 4)))
                     a.qs[scale_at(blockIdx.x + cg, r, a.rows)] = cg == 0 ? (uint8_t)(e + 127) : (uint8_t)127;
             }
@@ -197,42 +312,49 @@ __global__ __launch_bounds__(256) void fp8_quantize_kernel(QuantArgs a) {
     if constexpr (QT) {
         if constexpr (!TILES) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                float m = 0.f;
+            for (int j = 0; j < ND; ++j) {
+                unsigned m = 0;
+                if (finite) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) m = fmaxf(m, finite_abs(v[i][j]));
-                m = fmaxf(m, __shfl_xor(m, 16, 64));
-                m = fmaxf(m, __shfl_xor(m, 32, 64));
-                cmax[j] = m;
-            }
-            if ((tid & 63) < 16) {
+                    for (int i = 0; i < RPT; ++i) m = mag_max<T>(m, mag<T>(d[i][j]));
+                } else {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) red[wave][cg * 8 + j] = cmax[j];
+                    for (int i = 0; i < RPT; ++i) m = mag_max<T>(m, mag_finite<T>(mag<T>(d[i][j])));
+                }
+                m = mag_max<T>(m, (unsigned)__shfl_xor((int)m, 16, 64));
+                m = mag_max<T>(m, (unsigned)__shfl_xor((int)m, 32, 64));
+                if ((tid & 63) < 16) red[wave][cg * ND + j] = m;
             }
             __syncthreads();
         }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int cl = cg * 8 + j;
+        for (int j = 0; j < 8; ++j) {      // column j of the thread: its eight rows, packed as a row of the transpose
+            const int cl = cg * 8 + j, dj = T == SM_TYPE_F32 ? j : j >> 1;
             int e = tile_e;
             if (!TILES) {
-                e = block_exponent(fmaxf(fmaxf(red[0][cl], red[1][cl]), fmaxf(red[2][cl], red[3][cl])), top);
+                unsigned m = mag_max<T>(mag_max<T>(red[0][cg * ND + dj], red[1][cg * ND + dj]), mag_max<T>(red[2][cg * ND + dj], red[3][cg * ND + dj]));
+                if constexpr (T != SM_TYPE_F32) m = j & 1 ? m >> 16 : m & 0xffffu;
+                e = block_exponent(mag_float<T>(m), top);
                 if (tc + cl < a.cols && rg < 4 && (rg == 0 || ((int)blockIdx.y == rblocks - 1 && (int)blockIdx.y + rg < (rblocks + 3) / 4 * 4)))
                     a.qts[scale_at(blockIdx.y + rg, tc + cl, a.cols)] = rg == 0 ? (uint8_t)(e + 127) : (uint8_t)127;
             }
-            float t[8];
+            unsigned t[ND];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) t[i] = v[i][j];
-            *reinterpret_cast<u32x2*>(img + cl * 144 + rg * 8) = cvt8(t, inv_pow2(e), a.fmt);
+            for (int i = 0; i < ND; ++i) {
+                if constexpr (T == SM_TYPE_F32) t[i] = d[i][j];
+                else t[i] = j & 1 ? (d[2 * i][dj] >> 16) | (d[2 * i + 1][dj] & 0xffff0000u) : (d[2 * i][dj] & 0xffffu) | (d[2 * i + 1][dj] << 16);
+            }
+            *reinterpret_cast<u32x2*>(img + cl * 128 + (rg ^ cg) * 8) = codes8<T>(t, e, a.fmt, finite && e > -127);
         }
         __syncthreads();
         const size_t pitch = (size_t)rblocks * 128;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {      // 8 lanes write a column's 128 bytes
-            const int cl = i * 32 + (tid >> 3);
-            if (tc + cl < a.cols)
-                *reinterpret_cast<u32x4*>(a.qt + (size_t)(tc + cl) * pitch + tr + (tid & 7) * 16) =
-                    *reinterpret_cast<const u32x4*>(img + cl * 144 + (tid & 7) * 16);
+            const int cl = i * 32 + (tid >> 3), p = tid & 7, g = cl >> 3;
+            // units 2 p and 2 p + 1 of the column lie in the pair p ^ (g / 2), the other way round for odd g
+            u32x4 w = *reinterpret_cast<const u32x4*>(img + cl * 128 + (p ^ (g >> 1)) * 16);
+            if (g & 1) w = u32x4{w[2], w[3], w[0], w[1]};
+            if (tc + cl < a.cols) *reinterpret_cast<u32x4*>(a.qt + (size_t)(tc + cl) * pitch + tr + p * 16) = w;
         }
     }
 }
@@ -308,7 +430,6 @@ __device__ __forceinline__ void wait_loads() {
 // An operand's 32 codes of a lane as bf16, scaled by 2^(byte - 127): e4m3 / e5m2 have 4 / 3 significant bits, bf16 has 8 and
 // fp32's exponents, so this is exact. scale: the byte in the exponent field of a float.
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 struct Wide {
     bf16x8 p[4];
 };
@@ -340,10 +461,14 @@ __device__ __forceinline__ float byte_scale(int dword) {      // byte OP of a sc
     const unsigned u = (unsigned)dword >> (8 * OP);
     return __builtin_bit_cast(float, (u & 255u) << 23);
 }
-__device__ __forceinline__ f32x4 mfma_wide(const Wide& b, const Wide& a, f32x4 c) {
+// c[i] += b[i] a over a block of 128 for N rows of tiles: the four instructions of one result depend on each other, so the
+// tiles take turns
+template <int N>
+__device__ __forceinline__ void mfma_wide(const Wide* b, const Wide& a, f32x4* c) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b.p[i], a.p[i], c, 0, 0, 0);
-    return c;
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int i = 0; i < N; ++i) c[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[i].p[q], a.p[q], c[i], 0, 0, 0);
 }
 
 template <int OP, int FA>
@@ -478,22 +603,27 @@ __global__ __launch_bounds__(WM* WN * 64) void fp8_matmul_kernel(MatmulArgs g) {
                 stage(buf, min(k + NST, kb1 - 1));      // (behind the end: the last block again, read by nobody)
                 next = frag(na, wm * TM);
             }
-            Wide aw;
-            if constexpr (!NATIVE) aw = widen<FA>(a, F32S ? 1.f : byte_scale<OP>(sa[j]));
+            f32x4 c[TN];
+#pragma unroll
+            for (int i = 0; i < TN; ++i) c[i] = F32S ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[i][j];
+            if constexpr (!NATIVE) {
+                mfma_wide<TN>(bw, widen<FA>(a, F32S ? 1.f : byte_scale<OP>(sa[j])), c);
+            } else {
+#pragma unroll
+                for (int i = 0; i < TN; ++i) {
+                    if constexpr (F32S) c[i] = mfma_block<0, FA>(b[i], a, c[i], 0x7f7f7f7f, 0x7f7f7f7f);
+                    else c[i] = mfma_block<OP, FA>(b[i], a, c[i], sb[i], sa[j]);
+                }
+            }
 #pragma unroll
             for (int i = 0; i < TN; ++i) {
-                const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-                f32x4 c = F32S ? zero : acc[i][j];
-                if constexpr (!NATIVE) c = mfma_wide(bw[i], aw, c);
-                else if constexpr (F32S) c = mfma_block<0, FA>(b[i], a, c, 0x7f7f7f7f, 0x7f7f7f7f);
-                else c = mfma_block<OP, FA>(b[i], a, c, sb[i], sa[j]);
                 if constexpr (F32S) {
                     // the block's sum on its own, then one multiply-add per element with sa[m] sb[n]
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        acc[i][j][e] = fmaf(c[e], as_float(sa[j]) * as_float(sb[SC == SCALE_F32_ROWS ? 4 * i + e : 0]), acc[i][j][e]);
+                        acc[i][j][e] = fmaf(c[i][e], as_float(sa[j]) * as_float(sb[SC == SCALE_F32_ROWS ? 4 * i + e : 0]), acc[i][j][e]);
                 } else {
-                    acc[i][j] = c;
+                    acc[i][j] = c[i];
                 }
                 if (j + 1 == TM) b[i] = frag(na + BM * 128, wn * TN + i);
             }
@@ -540,10 +670,11 @@ __global__ __launch_bounds__(WM* WN * 64) void fp8_matmul_kernel(MatmulArgs g) {
 }
 
 // Few rows of A (M <= 16 TM): the product is a stream through B, which is read once, straight into the matrix instructions'
-// operand registers - no LDS, no barrier until the end. A block owns 16 rows of B; its eight waves take the blocks of 128
+// operand registers - no LDS, no barrier until the end. A block owns 16 TB rows of B; its eight waves take the blocks of 128
 // along K in turn (together 1 KB of every row at a time) and U of them are in flight per wave. X: what A is - codes (SM_FP8_*
-// + 8) or raw values (SM_TYPE_*), which every wave quantises on its way into the operand (their block maximum needs two cross-lane steps): one launch
-// for a layer's forward pass. Bound by HBM: the codes of B.
+// + 8) or raw values (SM_TYPE_*), which every wave quantises on its way into the operand (their block maximum needs two
+// cross-lane steps): one launch for a layer's forward pass. Bound by HBM: the codes of B; A comes from the caches once per
+// block, which is why 16 and more rows of A take TB = 2 where B is long enough to fill the chip so.
 constexpr int STREAM_WAVES = 8;
 struct StreamArgs {
     MatmulArgs g;
@@ -551,39 +682,102 @@ struct StreamArgs {
     size_t x_stride;
     int K;
 };
-template <int X, int TM, bool F32S, int U>
+// A lane's 32 raw values of block kb of row m -> codes and the block's scale byte (the same in the four lanes that share the
+// row). r: the values as loaded; FULL = false: the row ends inside the block and they are read here.
+template <int X, int RV, bool FULL>
+__device__ __forceinline__ void quantize_rows(const StreamArgs& t, const u32x4* r, int kb, int m, int lg, i32x8& codes, int& byte) {
+    float v[32];
+    if constexpr (FULL) {
+        unsigned top = 0;
+#pragma unroll
+        for (int q = 0; q < RV; ++q)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top = mag_max<X>(top, mag<X>(r[q][i]));
+        top = mag_both<X>(top);
+        if (!__any(top >= inf_bits<X>)) {
+            top = max(top, (unsigned)__shfl_xor((int)top, 16, 64));
+            top = max(top, (unsigned)__shfl_xor((int)top, 32, 64));
+            const int e = block_exponent(mag_float<X>(top), 8);
+            byte = e + 127;
+            if (!__any(e == -127)) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    unsigned d[8];
+#pragma unroll
+                    for (int i = 0; i < (RV == 8 ? 8 : 4); ++i) d[i] = RV == 8 ? r[2 * q + (i >> 2)][i & 3] : r[q][i];
+                    const u32x2 w = codes8<X>(d, e, SM_FP8_E4M3, true);
+                    codes[2 * q] = (int)w[0];
+                    codes[2 * q + 1] = (int)w[1];
+                }
+                return;
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < RV; ++q) unpack<X>(r[q], v + q * (32 / RV));
+    } else {
+        const int c = kb * 128 + lg * 16;
+        const size_t row = (size_t)m * t.x_stride;
+        load8<X>(t.x, row + c, t.K - c, v);
+        load8<X>(t.x, row + c + 8, t.K - c - 8, v + 8);
+        load8<X>(t.x, row + c + 64, t.K - c - 64, v + 16);
+        load8<X>(t.x, row + c + 72, t.K - c - 72, v + 24);
+    }
+    float a = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) a = fmaxf(a, finite_abs(v[i]));
+    a = fmaxf(a, __shfl_xor(a, 16, 64));
+    a = fmaxf(a, __shfl_xor(a, 32, 64));
+    const int e = block_exponent(a, 8);
+    byte = e + 127;
+    const float inv = inv_pow2(e);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const u32x2 w = cvt8(v + 8 * q, inv, SM_FP8_E4M3);
+        codes[2 * q] = (int)w[0];
+        codes[2 * q + 1] = (int)w[1];
+    }
+}
+
+template <int X, int TM, int TB, bool F32S, bool NATIVE, int U>
 __global__ __launch_bounds__(STREAM_WAVES * 64) void fp8_stream_kernel(StreamArgs t) {
     constexpr bool RAW = X < 8;
     constexpr int FA = X == 8 + SM_FP8_E5M2 ? SM_FP8_E5M2 : SM_FP8_E4M3;
     const MatmulArgs& g = t.g;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lr = lane & 15, lg = lane >> 4;
-    const int n0 = blockIdx.x * 16;
+    const int n0 = blockIdx.x * 16 * TB;
     const int kb0 = blockIdx.y * g.kb_per_split, kb1 = min(g.KB, kb0 + g.kb_per_split);
-    const int brow = min(n0 + lr, g.N - 1);
-    const uint8_t* bp = g.b + (size_t)brow * g.b_pitch + lg * 16;
-    f32x4 acc[TM];
+    int brow[TB];
 #pragma unroll
-    for (int j = 0; j < TM; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < TB; ++i) brow[i] = min(n0 + i * 16 + lr, g.N - 1);
+    f32x4 acc[TM][TB];
+#pragma unroll
+    for (int j = 0; j < TM; ++j)
+#pragma unroll
+        for (int i = 0; i < TB; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 
     // NB blocks, STREAM_WAVES apart: all loads first, then the arithmetic. FULL: K covers the blocks (raw rows end inside the last one).
     constexpr int RV = RAW ? (X == SM_TYPE_F32 ? 8 : 4) : 2;       // 16-byte vectors of A per lane and block
     auto group = [&](auto nbc, auto fullc, int kb) {
         constexpr int NB = decltype(nbc)::value;
         constexpr bool FULL = decltype(fullc)::value;
-        u32x4 bv[NB][2], av[NB][TM][RV];
-        int sbyte[NB], sa[NB][TM];
-        f32x4 fb[NB];
+        u32x4 bv[NB][TB][2], av[NB][TM][RV];
+        int sb[NB][TB], sa[NB][TM];
+        f32x4 fb[NB][TB];
 #pragma unroll
         for (int u = 0; u < NB; ++u) {
             const int k = kb + u * STREAM_WAVES;
-            bv[u][0] = *reinterpret_cast<const u32x4*>(bp + (size_t)k * 128);
-            bv[u][1] = *reinterpret_cast<const u32x4*>(bp + (size_t)k * 128 + 64);
-            if constexpr (F32S) {
-                const float* pb = static_cast<const float*>(g.bs) + (size_t)k * g.bs_rows;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) fb[u][e] = pb[min(n0 + lg * 4 + e, g.N - 1) >> g.b_shift];
-            } else {
-                sbyte[u] = static_cast<const uint8_t*>(g.bs)[scale_at(k, brow >> g.b_shift, g.bs_rows)];
+            for (int i = 0; i < TB; ++i) {
+                const uint8_t* bp = g.b + (size_t)brow[i] * g.b_pitch + (size_t)k * 128 + lg * 16;
+                bv[u][i][0] = *reinterpret_cast<const u32x4*>(bp);
+                bv[u][i][1] = *reinterpret_cast<const u32x4*>(bp + 64);
+                if constexpr (F32S) {
+                    const float* pb = static_cast<const float*>(g.bs) + (size_t)k * g.bs_rows;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) fb[u][i][e] = pb[min(n0 + i * 16 + lg * 4 + e, g.N - 1) >> g.b_shift];
+                } else {
+                    sb[u][i] = static_cast<const uint8_t*>(g.bs)[scale_at(k, brow[i] >> g.b_shift, g.bs_rows)];
+                }
             }
 #pragma unroll
             for (int j = 0; j < TM; ++j) {
@@ -609,49 +803,41 @@ __global__ __launch_bounds__(STREAM_WAVES * 64) void fp8_stream_kernel(StreamArg
         }
 #pragma unroll
         for (int u = 0; u < NB; ++u) {
-            const Wide bw = widen<SM_FP8_E4M3>(join(bv[u][0], bv[u][1]), F32S ? 1.f : __builtin_bit_cast(float, (unsigned)sbyte[u] << 23));
+            i32x8 bc[TB];
+            Wide bw[NATIVE ? 1 : TB];
+#pragma unroll
+            for (int i = 0; i < TB; ++i) {
+                bc[i] = join(bv[u][i][0], bv[u][i][1]);
+                if constexpr (!NATIVE) bw[i] = widen<SM_FP8_E4M3>(bc[i], F32S ? 1.f : __builtin_bit_cast(float, (unsigned)sb[u][i] << 23));
+            }
 #pragma unroll
             for (int j = 0; j < TM; ++j) {
                 i32x8 codes;
                 int byte;
                 if constexpr (RAW) {
-                    float v[32];
-                    if constexpr (FULL) {
-#pragma unroll
-                        for (int q = 0; q < RV; ++q) unpack<X>(av[u][j][q], v + q * (32 / RV));
-                    } else {
-                        const int k = kb + u * STREAM_WAVES, c = k * 128 + lg * 16, m = min(j * 16 + lr, g.M - 1);
-                        const size_t row = (size_t)m * t.x_stride;
-                        load8<X>(t.x, row + c, t.K - c, v);
-                        load8<X>(t.x, row + c + 8, t.K - c - 8, v + 8);
-                        load8<X>(t.x, row + c + 64, t.K - c - 64, v + 16);
-                        load8<X>(t.x, row + c + 72, t.K - c - 72, v + 24);
-                    }
-                    float m = 0.f;
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) m = fmaxf(m, finite_abs(v[i]));
-                    m = fmaxf(m, __shfl_xor(m, 16, 64));
-                    m = fmaxf(m, __shfl_xor(m, 32, 64));
-                    const int e = block_exponent(m, 8);
-                    byte = e + 127;
-                    const float inv = inv_pow2(e);
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const u32x2 w = cvt8(v + 8 * q, inv, SM_FP8_E4M3);
-                        codes[2 * q] = (int)w[0];
-                        codes[2 * q + 1] = (int)w[1];
-                    }
+                    quantize_rows<X, RV, FULL>(t, av[u][j], kb + u * STREAM_WAVES, min(j * 16 + lr, g.M - 1), lg, codes, byte);
                 } else {
                     codes = join(av[u][j][0], av[u][j][1]);
                     byte = sa[u][j];
                 }
-                if constexpr (F32S) {
-                    const f32x4 d = mfma_wide(bw, widen<FA>(codes, 1.f), f32x4{0.f, 0.f, 0.f, 0.f});
-                    const float fa = __builtin_bit_cast(float, byte);
+                f32x4 c[TB];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[j][e] = fmaf(d[e], fa * fb[u][e], acc[j][e]);
+                for (int i = 0; i < TB; ++i) c[i] = F32S ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[j][i];
+                if constexpr (NATIVE) {
+#pragma unroll
+                    for (int i = 0; i < TB; ++i) c[i] = mfma_block<0, FA>(bc[i], codes, c[i], sb[u][i], byte);
                 } else {
-                    acc[j] = mfma_wide(bw, widen<FA>(codes, __builtin_bit_cast(float, (unsigned)byte << 23)), acc[j]);
+                    mfma_wide<TB>(bw, widen<FA>(codes, F32S ? 1.f : __builtin_bit_cast(float, (unsigned)byte << 23)), c);
+                }
+#pragma unroll
+                for (int i = 0; i < TB; ++i) {
+                    if constexpr (F32S) {
+                        const float fa = __builtin_bit_cast(float, byte);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[j][i][e] = fmaf(c[i][e], fa * fb[u][i][e], acc[j][i][e]);
+                    } else {
+                        acc[j][i] = c[i];
+                    }
                 }
             }
         }
@@ -662,19 +848,22 @@ __global__ __launch_bounds__(STREAM_WAVES * 64) void fp8_stream_kernel(StreamArg
     for (; kb + (U - 1) * STREAM_WAVES < kbf; kb += STREAM_WAVES * U) group(std::integral_constant<int, U>{}, full, kb);
     if constexpr (U > 2)
         for (; kb + STREAM_WAVES < kbf; kb += STREAM_WAVES * 2) group(std::integral_constant<int, 2>{}, full, kb);
-    for (; kb < kbf; kb += STREAM_WAVES) group(std::integral_constant<int, 1>{}, full, kb);
+    if constexpr (U > 1)
+        for (; kb < kbf; kb += STREAM_WAVES) group(std::integral_constant<int, 1>{}, full, kb);
     if constexpr (RAW)
         if (kb < kb1) group(std::integral_constant<int, 1>{}, std::integral_constant<bool, false>{}, kb);
     // the waves' sums, added in their order
-    __shared__ f32x4 part[STREAM_WAVES][TM][64];
+    __shared__ f32x4 part[STREAM_WAVES][TM * TB][64];
 #pragma unroll
-    for (int j = 0; j < TM; ++j) part[wave][j][lane] = acc[j];
+    for (int j = 0; j < TM; ++j)
+#pragma unroll
+        for (int i = 0; i < TB; ++i) part[wave][j * TB + i][lane] = acc[j][i];
     __syncthreads();
-    for (int j = wave; j < TM; j += STREAM_WAVES) {
-        f32x4 s = part[0][j][lane];
+    for (int q = wave; q < TM * TB; q += STREAM_WAVES) {
+        f32x4 s = part[0][q][lane];
 #pragma unroll
-        for (int w = 1; w < STREAM_WAVES; ++w) s += part[w][j][lane];
-        const int m = j * 16 + lr, n = n0 + lg * 4;
+        for (int w = 1; w < STREAM_WAVES; ++w) s += part[w][q][lane];
+        const int m = q / TB * 16 + lr, n = n0 + q % TB * 16 + lg * 4;
         if (m >= g.M || n >= g.N) continue;
         if (gridDim.y > 1) {
             float* o = g.ws + ((size_t)blockIdx.y * g.M + m) * g.N + n;
@@ -748,20 +937,35 @@ static Plan matmul_plan(int M, int N, int KB) {
     return p;
 }
 
-template <int X, int TM, bool F32S>
+// (a bf16 result of K >= 1024 takes the 8-bit matrix instruction: see sm_fp8_matmul)
+static bool native_result(int out_type, int KB) { return out_type == SM_TYPE_BF16 && KB >= 8; }
+
+template <int X, int TM, int TB, bool F32S, bool NATIVE, int U>
 static void launch_stream(const StreamArgs& t, int splits, hipStream_t s) {
-    constexpr int U = X < 8 ? (X == SM_TYPE_F32 ? 2 : 4) : (TM == 1 ? 4 : 2);
-    hipLaunchKernelGGL((fp8_stream_kernel<X, TM, F32S, U>), dim3((unsigned)((t.g.N + 15) / 16), (unsigned)splits), dim3(STREAM_WAVES * 64), 0, s, t);
+    hipLaunchKernelGGL((fp8_stream_kernel<X, TM, TB, F32S, NATIVE, U>), dim3((unsigned)((t.g.N + 16 * TB - 1) / (16 * TB)), (unsigned)splits),
+                       dim3(STREAM_WAVES * 64), 0, s, t);
 }
-template <int TM>
-static void launch_stream_codes(const StreamArgs& t, int a_fmt, bool f32s, int splits, hipStream_t s) {
-    if (a_fmt == SM_FP8_E4M3) {
-        if (f32s) launch_stream<8 + SM_FP8_E4M3, TM, true>(t, splits, s);
-        else launch_stream<8 + SM_FP8_E4M3, TM, false>(t, splits, s);
-    } else {
-        if (f32s) launch_stream<8 + SM_FP8_E5M2, TM, true>(t, splits, s);
-        else launch_stream<8 + SM_FP8_E5M2, TM, false>(t, splits, s);
-    }
+template <int X>
+static void launch_stream_raw(const StreamArgs& t, int splits, hipStream_t s) {
+    constexpr int U = X == SM_TYPE_F32 ? 2 : 4;
+    if (native_result(t.g.out_type, t.g.KB)) launch_stream<X, 1, 1, false, true, U>(t, splits, s);
+    else launch_stream<X, 1, 1, false, false, U>(t, splits, s);
+}
+template <int X, bool NATIVE>
+static void launch_stream_pow2(const StreamArgs& t, int splits, hipStream_t s) {
+    const bool wide = (t.g.N + 31) / 32 >= 192;       // 32 rows of B per block still fill the chip
+    if (t.g.M <= 16) launch_stream<X, 1, 1, false, NATIVE, 4>(t, splits, s);
+    else if (t.g.M <= 32) wide ? launch_stream<X, 2, 2, false, NATIVE, 2>(t, splits, s) : launch_stream<X, 2, 1, false, NATIVE, 2>(t, splits, s);
+    else wide ? launch_stream<X, 4, 2, false, NATIVE, 1>(t, splits, s) : launch_stream<X, 4, 1, false, NATIVE, 2>(t, splits, s);
+}
+template <int X>
+static void launch_stream_codes(const StreamArgs& t, bool f32s, int splits, hipStream_t s) {
+    if (!f32s) {
+        if (native_result(t.g.out_type, t.g.KB)) launch_stream_pow2<X, true>(t, splits, s);
+        else launch_stream_pow2<X, false>(t, splits, s);
+    } else if (t.g.M <= 16) launch_stream<X, 1, 1, true, false, 4>(t, splits, s);
+    else if (t.g.M <= 32) launch_stream<X, 2, 1, true, false, 2>(t, splits, s);
+    else launch_stream<X, 4, 1, true, false, 2>(t, splits, s);
 }
 static void launch_reduce(const MatmulArgs& g, int splits, hipStream_t s) {
     const size_t quads = (size_t)(g.N + 3) / 4 * g.M;
@@ -795,16 +999,18 @@ static void launch_tile(int kind, const MatmulArgs& g, int a_fmt, bool f32s, int
 
 template <int T>
 static int launch_quantize(const QuantArgs& a, int tiles, hipStream_t s) {
-    const dim3 grid((unsigned)((a.cols + 127) / 128), (unsigned)((a.rows + 127) / 128));
+    const unsigned cb = (unsigned)((a.cols + 127) / 128);
+    const dim3 grid(cb, (unsigned)((a.rows + 127) / 128)), block(256);
     const bool q = a.q != nullptr, qt = a.qt != nullptr;
     if (tiles) {
-        if (q && qt) hipLaunchKernelGGL((fp8_quantize_kernel<T, true, true, true>), grid, dim3(256), 0, s, a);
-        else if (q) hipLaunchKernelGGL((fp8_quantize_kernel<T, true, true, false>), grid, dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((fp8_quantize_kernel<T, true, false, true>), grid, dim3(256), 0, s, a);
+        if (q && qt) hipLaunchKernelGGL((fp8_quantize_kernel<T, true, true, true, 8>), grid, block, 0, s, a);
+        else if (q) hipLaunchKernelGGL((fp8_quantize_kernel<T, true, true, false, 8>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((fp8_quantize_kernel<T, true, false, true, 8>), grid, block, 0, s, a);
     } else {
-        if (q && qt) hipLaunchKernelGGL((fp8_quantize_kernel<T, false, true, true>), grid, dim3(256), 0, s, a);
-        else if (q) hipLaunchKernelGGL((fp8_quantize_kernel<T, false, true, false>), grid, dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((fp8_quantize_kernel<T, false, false, true>), grid, dim3(256), 0, s, a);
+        if (q && qt) hipLaunchKernelGGL((fp8_quantize_kernel<T, false, true, true, 8>), grid, block, 0, s, a);
+        else if (qt) hipLaunchKernelGGL((fp8_quantize_kernel<T, false, false, true, 8>), grid, block, 0, s, a);
+        else if ((size_t)grid.x * grid.y >= 1024) hipLaunchKernelGGL((fp8_quantize_kernel<T, false, true, false, 8>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((fp8_quantize_kernel<T, false, true, false, 1>), dim3(cb, (unsigned)((a.rows + 15) / 16)), block, 0, s, a);
     }
     SM_LAUNCH_CHECK();
     return 0;
@@ -860,16 +1066,15 @@ int sm_fp8_matmul(const void* a, const void* a_scale, int a_fmt, size_t a_pitch,
     const bool f32s = scale_f32 != 0;
     if (p.kind == sm::TILE_STREAM) {
         const sm::StreamArgs t{g, nullptr, 0, K};
-        if (M <= 16) sm::launch_stream_codes<1>(t, a_fmt, f32s, p.splits, s);
-        else if (M <= 32) sm::launch_stream_codes<2>(t, a_fmt, f32s, p.splits, s);
-        else sm::launch_stream_codes<4>(t, a_fmt, f32s, p.splits, s);
+        if (a_fmt == SM_FP8_E4M3) sm::launch_stream_codes<8 + SM_FP8_E4M3>(t, f32s, p.splits, s);
+        else sm::launch_stream_codes<8 + SM_FP8_E5M2>(t, f32s, p.splits, s);
     } else {
         // The 8-bit matrix instruction aligns the products of eight neighbouring k to the largest of them and keeps 13 bits below
         // its leading one (measured; so does the older 16x16x32 form), fp32 beyond that: relative to sum |a||b| an error of
         // 2^-19 (normal data) to 2^-15 (log-normal, sigma 2) at K = 128, falling with sqrt(K). It is taken where the result
         // is bf16 - half a step is 2^-9 - and K >= 1024, where it stays inside what a plain fp32 sum of K terms may lose.
         // Every other product widens the codes to bf16 (exact, scale included) and sums in fp32 throughout, at half the rate.
-        if (out_type == SM_TYPE_BF16 && KB >= 8) sm::launch_tile<true>(p.kind, g, a_fmt, f32s, p.splits, s);
+        if (sm::native_result(out_type, KB)) sm::launch_tile<true>(p.kind, g, a_fmt, f32s, p.splits, s);
         else sm::launch_tile<false>(p.kind, g, a_fmt, f32s, p.splits, s);
     }
     SM_LAUNCH_CHECK();
@@ -914,9 +1119,9 @@ int sm_fp8_linear(const void* x, int x_type, size_t x_stride, const void* w, con
     const sm::Plan p = sm::matmul_plan(M, N, KB);
     sm::StreamArgs t{{nullptr, (const uint8_t*)w, nullptr, w_scale, out, (float*)ws, 0, w_pitch, out_stride, M, N, KB, w_tiles ? 7 : 0,
                       w_tiles ? (N + 127) / 128 : N, out_type, 0, p.kb_per_split}, x, x_stride, K};
-    if (x_type == SM_TYPE_F32) sm::launch_stream<SM_TYPE_F32, 1, false>(t, p.splits, s);
-    else if (x_type == SM_TYPE_BF16) sm::launch_stream<SM_TYPE_BF16, 1, false>(t, p.splits, s);
-    else sm::launch_stream<SM_TYPE_F16, 1, false>(t, p.splits, s);
+    if (x_type == SM_TYPE_F32) sm::launch_stream_raw<SM_TYPE_F32>(t, p.splits, s);
+    else if (x_type == SM_TYPE_BF16) sm::launch_stream_raw<SM_TYPE_BF16>(t, p.splits, s);
+    else sm::launch_stream_raw<SM_TYPE_F16>(t, p.splits, s);
     SM_LAUNCH_CHECK();
     if (p.splits > 1) sm::launch_reduce(t.g, p.splits, s);
     SM_LAUNCH_CHECK();
