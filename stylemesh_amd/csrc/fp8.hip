@@ -801,6 +801,7 @@ __global__ __launch_bounds__(STREAM_WAVES * 64) void fp8_stream_kernel(StreamArg
                 }
             }
         }
+        __builtin_amdgcn_sched_barrier(0);      // (left alone the compiler sinks half of the loads between the products)
 #pragma unroll
         for (int u = 0; u < NB; ++u) {
             i32x8 bc[TB];

@@ -8,10 +8,11 @@ scratch) from torch's allocator and synchronises nothing. There is no autograd n
 """
 from __future__ import annotations
 
+from functools import lru_cache
+
 import torch
 
 from . import hip, ops
-from .hip import ptr
 
 BLOCK = 128
 FORMATS = {"e4m3": torch.float8_e4m3fn, "e5m2": torch.float8_e5m2}
@@ -65,6 +66,14 @@ class Fp8Matrix:
             raise ValueError(f"codes on {data.device}, scales on {scale.device}")
         self.data, self.scale, self.cols, self.block = data, scale, int(cols), block
         self._ptrs = (data.data_ptr(), scale.data_ptr())      # (of tensors this object keeps)
+
+    @classmethod
+    def _made(cls, data, scale, cols, block):
+        """Of tensors this module laid out itself: nothing to check."""
+        m = cls.__new__(cls)
+        m.data, m.scale, m.cols, m.block = data, scale, cols, block
+        m._ptrs = (data.data_ptr(), scale.data_ptr())
+        return m
 
     @property
     def rows(self) -> int:
@@ -138,17 +147,19 @@ def pack_scale_bytes(e: torch.Tensor) -> torch.Tensor:
 
 
 def _matrix_arg(x, what):
+    """x: a matrix the kernels read or write; returns its row stride in elements"""
     if not torch.is_tensor(x) or x.dim() != 2 or x.dtype not in _TYPE_ID:
         raise ValueError(f"{what} must be a float32 / bfloat16 / float16 matrix, got "
                          f"{(x.dtype, tuple(x.shape)) if torch.is_tensor(x) else type(x)}")
+    (rows, cols), (sr, sc) = x.shape, x.stride()
     # (the stride of a dimension of one element means nothing)
-    if (x.shape[1] > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
+    if (cols > 1 and sc != 1) or (rows > 1 and sr < cols):
         raise ValueError(f"{what} must have unit column stride and rows that do not overlap, got strides {x.stride()} for "
                          f"{tuple(x.shape)}; pass .contiguous(), or transpose=True for a transposed matrix")
-    if max(x.shape) > _MAX_DIM:
+    if rows > _MAX_DIM or cols > _MAX_DIM:
         raise ValueError(f"{what}: {tuple(x.shape)} has a dimension above {_MAX_DIM}")
     _check_device(x)
-    return x
+    return sr if rows > 1 else max(cols, 1)
 
 
 def _empty(rows, cols, fmt, block, device):
@@ -158,7 +169,7 @@ def _empty(rows, cols, fmt, block, device):
 
 
 def _quantize(x, block, fmt, plain, transpose):
-    x = _matrix_arg(x, "x")
+    stride = _matrix_arg(x, "x")
     if fmt not in FORMATS:
         raise ValueError(f"fmt={fmt!r}: 'e4m3' or 'e5m2'")
     if block not in ("rows", "tiles"):
@@ -166,12 +177,12 @@ def _quantize(x, block, fmt, plain, transpose):
     rows, cols = x.shape
     q, qs = _empty(rows, cols, fmt, block, x.device) if plain else (None, None)
     qt, qts = _empty(cols, rows, fmt, block, x.device) if transpose else (None, None)
-    stride = x.stride(0) if rows > 1 else max(cols, 1)
     if rows and cols:
+        n = (q.data_ptr(), qs.data_ptr()) if plain else (None, None)
+        t = (qt.data_ptr(), qts.data_ptr()) if transpose else (None, None)
         hip.check(ops.lib.sm_fp8_quantize(x.data_ptr(), _TYPE_ID[x.dtype], rows, cols, stride, _FMT_ID[FORMATS[fmt]],
-                                          int(block == "tiles"), ptr(q), ptr(qs), ptr(qt), ptr(qts), hip.stream()),
-                  "sm_fp8_quantize")
-    return (Fp8Matrix(q, qs, cols, block) if plain else None, Fp8Matrix(qt, qts, rows, block) if transpose else None)
+                                          int(block == "tiles"), *n, *t, hip.stream()), "sm_fp8_quantize")
+    return (Fp8Matrix._made(q, qs, cols, block) if plain else None, Fp8Matrix._made(qt, qts, rows, block) if transpose else None)
 
 
 def fp8_quantize(x: torch.Tensor, block: str = "rows", fmt: str = "e4m3", transpose: bool = False) -> Fp8Matrix:
@@ -187,6 +198,16 @@ def fp8_quantize_both(x: torch.Tensor, block: str = "rows", fmt: str = "e4m3"):
     """(``fp8_quantize(x)``, ``fp8_quantize(x, transpose=True)``) from one read of ``x``: what a training step needs of its
     activations and output gradients (rows) and of its weights (tiles)."""
     return _quantize(x, block, fmt, True, True)
+
+
+@lru_cache(maxsize=4096)      # (a function of the sizes alone)
+def _matmul_ws(M, N, K):
+    return hip.lib.sm_fp8_matmul_ws_bytes(M, N, K)
+
+
+@lru_cache(maxsize=4096)
+def _linear_ws(M, N, K):
+    return hip.lib.sm_fp8_linear_ws_bytes(M, N, K)
 
 
 def matmul_fp8(a: Fp8Matrix, b: Fp8Matrix, out: torch.Tensor | None = None, out_dtype=None, accumulate: bool = False) -> torch.Tensor:
@@ -211,21 +232,23 @@ def matmul_fp8(a: Fp8Matrix, b: Fp8Matrix, out: torch.Tensor | None = None, out_
     if out is None:
         if accumulate:
             raise ValueError("accumulate needs out")
-        out = torch.empty(M, N, dtype=out_dtype or torch.bfloat16, device=a.device)
-        if out.dtype not in _TYPE_ID:
+        if out_dtype is None:
+            out_dtype = torch.bfloat16
+        if out_dtype not in _TYPE_ID:
             raise ValueError(f"out_dtype={out_dtype}: float32, bfloat16 or float16")
+        out, stride = torch.empty((M, N), dtype=out_dtype, device=a.data.device), max(N, 1)
     else:
-        _matrix_arg(out, "out")
+        stride = _matrix_arg(out, "out")
         if tuple(out.shape) != (M, N) or (out_dtype is not None and out.dtype != out_dtype):
             raise ValueError(f"out is {out.dtype} {tuple(out.shape)}, the product {out_dtype or out.dtype} {(M, N)}")
     if M == 0 or N == 0:
         return out
-    need = ops.lib.sm_fp8_matmul_ws_bytes(M, N, K)
+    need = _matmul_ws(M, N, K)
     # (scratch of this call's own: two captured graphs, or two streams, never share slabs)
     ws = torch.empty(need, dtype=torch.uint8, device=a.device) if need else None
     hip.check(ops.lib.sm_fp8_matmul(*a._ptrs, _FMT_ID[a.data.dtype], a.data.shape[1], *b._ptrs, int(b.block == "tiles"), b.data.shape[1],
                                     int(a.scale.dtype == torch.float32), M, N, K, out.data_ptr(), _TYPE_ID[out.dtype],
-                                    out.stride(0) if M > 1 else N, int(accumulate), ptr(ws), need, hip.stream()), "sm_fp8_matmul")
+                                    stride, int(accumulate), None if ws is None else ws.data_ptr(), need, hip.stream()), "sm_fp8_matmul")
     return out
 
 
@@ -240,7 +263,7 @@ def linear_fp8_fwd(x: torch.Tensor, weight: Fp8Matrix, out_dtype=None, keep_tran
     (default: x's). ``keep_transposed``: returns (y, q(x^T)), the second for ``linear_fp8_bwd``'s weight gradient - quantised
     from the same read of x."""
     _weight_arg(weight)
-    _matrix_arg(x, "x")
+    stride = _matrix_arg(x, "x")
     M, K = x.shape
     if K != weight.cols:
         raise ValueError(f"x has {K} columns, the weight {weight.cols}")
@@ -253,12 +276,11 @@ def linear_fp8_fwd(x: torch.Tensor, weight: Fp8Matrix, out_dtype=None, keep_tran
         raise ValueError(f"out_dtype={out_dtype}: float32, bfloat16 or float16")
     _check_device(weight.data)
     N = weight.rows
-    y = torch.empty(M, N, dtype=out_dtype, device=x.device)
+    y = torch.empty((M, N), dtype=out_dtype, device=x.device)
     if M and N:
-        lib = ops.lib
-        need = lib.sm_fp8_linear_ws_bytes(M, N, K)
+        need = _linear_ws(M, N, K)
         ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None      # of this call's own, as matmul_fp8's
-        hip.check(lib.sm_fp8_linear(x.data_ptr(), _TYPE_ID[x.dtype], x.stride(0) if M > 1 else K, *weight._ptrs,
+        hip.check(ops.lib.sm_fp8_linear(x.data_ptr(), _TYPE_ID[x.dtype], stride, *weight._ptrs,
                                     int(weight.block == "tiles"), weight.data.shape[1], M, N, K, y.data_ptr(), _TYPE_ID[out_dtype], N,
                                     None if ws is None else ws.data_ptr(), need, hip.stream()), "sm_fp8_linear")
     return y

@@ -10,20 +10,23 @@ that is not finite is not an error (finding out would synchronise): the coeffici
 """
 from __future__ import annotations
 
-import ctypes as C
 import math
+from array import array
+from operator import attrgetter
 
+import numpy as np
 import torch
 
 from . import hip, ops
 
 _TYPE_ID = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}           # SM_TYPE_*
+_SIZE = (4, 2, 2)
+_T = torch.Tensor
+_dtype, _shape = attrgetter("dtype"), attrgetter("shape")
 
 
 def _dense(t) -> bool:
-    """One element per address of a range: contiguous, or a permutation of a contiguous tensor."""
-    if t.is_contiguous():
-        return True
+    """One element per address of a range: a permutation of a contiguous tensor."""
     want = 1
     for st, sz in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz > 1):
         if st != want:
@@ -32,16 +35,38 @@ def _dense(t) -> bool:
     return True
 
 
-def _check(tensors, what):
-    for t in tensors:
-        if t.dtype not in _TYPE_ID:
-            raise ValueError(f"{what}: {t.dtype} tensor (float32, bfloat16 or float16)")
-        if not t.is_cuda:
+class _Table:
+    """Pointers, element counts and types of a list of tensors as the library reads them. A list is walked once per attribute
+    with C-level maps: a model's few hundred tensors are handed over anew every step, and at a microsecond a tensor the walk
+    would be the operator's time."""
+
+    def __init__(self, tensors, what):
+        try:
+            self.types = array("i", [_TYPE_ID[d] for d in map(_dtype, tensors)])
+        except KeyError as e:
+            raise ValueError(f"{what}: {e.args[0]} tensor (float32, bfloat16 or float16)") from None
+        devices = set(map(_T.get_device, tensors))
+        if -1 in devices:
             raise ValueError(f"{what}: device tensors only (there is no CPU form)")
-        if t.device.index != torch.cuda.current_device():
-            raise ValueError(f"{what}: a tensor lives on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
-        if not _dense(t):
-            raise ValueError(f"{what}: strides {t.stride()} of {tuple(t.shape)} leave gaps or overlap")
+        if devices and devices != {torch.cuda.current_device()}:
+            raise ValueError(f"{what}: tensors on devices {sorted(devices)}, the current device is cuda:{torch.cuda.current_device()}")
+        self.contiguous = list(map(_T.is_contiguous, tensors))
+        if not all(self.contiguous):
+            for t, ok in zip(tensors, self.contiguous):
+                if not ok and not _dense(t):
+                    raise ValueError(f"{what}: strides {t.stride()} of {tuple(t.shape)} leave gaps or overlap")
+        self.ptrs = array("Q", map(_T.data_ptr, tensors))
+        self.numel = array("Q", map(_T.numel, tensors))
+        self.n = len(tensors)
+
+    def spans(self):
+        start = np.frombuffer(self.ptrs, dtype=np.uint64)
+        size = np.asarray(_SIZE, dtype=np.uint64)[np.frombuffer(self.types, dtype=np.int32)]
+        return start, start + np.frombuffer(self.numel, dtype=np.uint64) * size
+
+
+def _address(a) -> int | None:
+    return a.buffer_info()[0] if len(a) else None
 
 
 def _norm_kind(norm_type) -> int:
@@ -60,6 +85,28 @@ def _max_norm(v) -> float:
     return v
 
 
+def _refuse_overlap(g: _Table, o: _Table):
+    """What is written must be written once: an output that overlaps another output, or a gradient other than its own
+    (the same tensor listed twice, for one), has no defined result."""
+    if g.n == 0:
+        return
+    os_, oe = o.spans()
+    live = np.nonzero(oe > os_)[0]
+    if live.size == 0:
+        return
+    order = live[np.argsort(os_[live], kind="stable")]
+    ss, ee = os_[order], oe[order]
+    if (ee[:-1] > ss[1:]).any():
+        raise ValueError("two of the tensors to be written overlap (a gradient listed twice?)")
+    if o is g:
+        return
+    gs, ge = g.spans()
+    lo, hi = np.searchsorted(ee, gs, "right"), np.searchsorted(ss, ge, "left")      # outputs that gradient i touches
+    for i in np.nonzero((hi > lo) & (ge > gs))[0]:
+        if hi[i] - lo[i] > 1 or order[lo[i]] != i or os_[i] != gs[i]:
+            raise ValueError("an output overlaps a gradient that is not its own")
+
+
 class GradClip:
     """The call's tables for gradients that stay where they are (an arena's views, ``zero_grad(set_to_none=False)``): checked
     and laid out once, used every step. Keeps the tensors alive; ``grads`` may hold None (a parameter without a gradient).
@@ -74,69 +121,50 @@ class GradClip:
             out = list(out)
             if len(out) != len(grads):
                 raise ValueError(f"{len(grads)} gradients, {len(out)} outputs")
-        pairs = [(g, g if out is None else out[i]) for i, g in enumerate(grads) if g is not None]
-        self.grads, self.out = [g for g, _ in pairs], [o for _, o in pairs]
-        _check(self.grads, "grads")
-        self.device = torch.device("cuda", torch.cuda.current_device())
-        if out is not None:
-            if any(o is None for o in self.out):
+        if type(None) in set(map(type, grads)):
+            out = None if out is None else [o for o, g in zip(out, grads) if g is not None]
+            grads = [g for g in grads if g is not None]
+        self.grads, self.out = grads, grads if out is None else out
+        g = self._g = _Table(grads, "grads")
+        if out is None or not grads:
+            o = self._o = g
+        else:
+            if type(None) in set(map(type, out)):
                 raise ValueError("an output is missing for a gradient that is there")
-            _check(self.out, "out")
-            for g, o in pairs:
-                if o.shape != g.shape or (o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous())):
-                    raise ValueError(f"out {tuple(o.shape)} / {o.stride()} does not match its gradient {tuple(g.shape)} / {g.stride()}")
-                if o.data_ptr() == g.data_ptr() and o.dtype != g.dtype and g.numel():
-                    raise ValueError("an output that is its gradient must have its type")
-        self._refuse_overlap(pairs)
-        n = len(pairs)
-        self._n = n
-        self._in = (C.c_void_p * n)(*[g.data_ptr() for g in self.grads])
-        self._outp = (C.c_void_p * n)(*[o.data_ptr() for o in self.out])
-        self._numel = (C.c_size_t * n)(*[g.numel() for g in self.grads])
-        self._types = (C.c_int * n)(*[_TYPE_ID[g.dtype] for g in self.grads])
-        self._out_types = (C.c_int * n)(*[_TYPE_ID[o.dtype] for o in self.out])
-        self._ws = torch.empty(ops.lib.sm_grad_norm_ws_bytes(n), dtype=torch.uint8, device=self.device)
+            o = self._o = _Table(out, "out")
+            if list(map(_shape, grads)) != list(map(_shape, out)):
+                raise ValueError("an output has not the shape of its gradient")
+            if not (all(g.contiguous) and all(o.contiguous)):
+                for a, b, ca, cb in zip(grads, out, g.contiguous, o.contiguous):
+                    if not (ca and cb) and a.stride() != b.stride():
+                        raise ValueError(f"out with strides {b.stride()} does not match its gradient's {a.stride()}")
+            same = np.frombuffer(g.ptrs, dtype=np.uint64) == np.frombuffer(o.ptrs, dtype=np.uint64)
+            if (same & (np.frombuffer(g.numel, dtype=np.uint64) > 0) & (np.frombuffer(g.types, np.int32) != np.frombuffer(o.types, np.int32))).any():
+                raise ValueError("an output that is its gradient must have its type")
+        _refuse_overlap(g, o)
+        self.device = torch.device("cuda", torch.cuda.current_device())
+        self._args = (_address(g.ptrs), _address(o.ptrs), _address(g.numel), _address(g.types), _address(o.types), g.n)
+        self._ws = torch.empty(ops.lib.sm_grad_norm_ws_bytes(g.n), dtype=torch.uint8, device=self.device)
+        self._ws_args = (self._ws.data_ptr(), self._ws.numel())
 
-    @staticmethod
-    def _refuse_overlap(pairs):
-        """What is written must be written once: an output that overlaps another output, or a gradient other than its own
-        (the same tensor listed twice, for one), has no defined result."""
-        span = lambda t: (t.data_ptr(), t.data_ptr() + t.numel() * t.element_size())
-        outs = sorted(span(o) + (i,) for i, (_, o) in enumerate(pairs) if o.numel())
-        for (_, e0, _), (s1, _, _) in zip(outs, outs[1:]):
-            if s1 < e0:
-                raise ValueError("two of the tensors to be written overlap (a gradient listed twice?)")
-        ins = sorted(span(g) + (i,) for i, (g, _) in enumerate(pairs) if g.numel())
-        k = 0
-        for s, e, i in outs:
-            while k < len(ins) and ins[k][1] <= s and ins[k][0] < s:
-                k += 1
-            j = k
-            while j < len(ins) and ins[j][0] < e:
-                if ins[j][1] > s and (ins[j][2] != i or ins[j][0] != s):
-                    raise ValueError("an output overlaps a gradient that is not its own")
-                j += 1
-
-    def _current(self):
+    def _result(self):
         if torch.cuda.current_device() != self.device.index:
             raise ValueError(f"the plan's tensors live on {self.device}, the current device is cuda:{torch.cuda.current_device()}")
+        return torch.empty((), dtype=torch.float32, device=self.device)
 
     def norm(self, norm_type=2.0) -> torch.Tensor:
         """The global norm as a float32 device scalar."""
         kind = _norm_kind(norm_type)
-        self._current()
-        out = torch.empty((), dtype=torch.float32, device=self.device)
-        hip.check(ops.lib.sm_grad_norm(self._in, self._numel, self._types, self._n, kind, self._ws.data_ptr(), self._ws.numel(),
-                                       out.data_ptr(), hip.stream()), "sm_grad_norm")
+        out = self._result()
+        gp, _, numel, types, _, n = self._args
+        hip.check(ops.lib.sm_grad_norm(gp, numel, types, n, kind, *self._ws_args, out.data_ptr(), hip.stream()), "sm_grad_norm")
         return out
 
     def clip(self, max_norm, norm_type=2.0) -> torch.Tensor:
         """Clips, and returns the norm BEFORE clipping (float32 device scalar)."""
         kind, max_norm = _norm_kind(norm_type), _max_norm(max_norm)
-        self._current()
-        out = torch.empty((), dtype=torch.float32, device=self.device)
-        hip.check(ops.lib.sm_grad_clip(self._in, self._outp, self._numel, self._types, self._out_types, self._n, kind, max_norm,
-                                       self._ws.data_ptr(), self._ws.numel(), out.data_ptr(), hip.stream()), "sm_grad_clip")
+        out = self._result()
+        hip.check(ops.lib.sm_grad_clip(*self._args, kind, max_norm, *self._ws_args, out.data_ptr(), hip.stream()), "sm_grad_clip")
         return out
 
 
@@ -144,13 +172,10 @@ def grad_norm(grads, norm_type=2.0) -> torch.Tensor:
     """The global norm of a list of gradients (``GradClip.norm`` for a list that changes from call to call; None entries are
     skipped; the same tensor listed twice counts twice)."""
     kind = _norm_kind(norm_type)
-    grads = [g for g in grads if g is not None]
-    _check(grads, "grads")
-    n = len(grads)
-    ws = torch.empty(ops.lib.sm_grad_norm_ws_bytes(n), dtype=torch.uint8, device="cuda")
+    t = _Table([g for g in grads if g is not None], "grads")
+    ws = torch.empty(ops.lib.sm_grad_norm_ws_bytes(t.n), dtype=torch.uint8, device="cuda")
     out = torch.empty((), dtype=torch.float32, device="cuda")
-    hip.check(ops.lib.sm_grad_norm((C.c_void_p * n)(*[g.data_ptr() for g in grads]), (C.c_size_t * n)(*[g.numel() for g in grads]),
-                                   (C.c_int * n)(*[_TYPE_ID[g.dtype] for g in grads]), n, kind, ws.data_ptr(), ws.numel(),
+    hip.check(ops.lib.sm_grad_norm(_address(t.ptrs), _address(t.numel), _address(t.types), t.n, kind, ws.data_ptr(), ws.numel(),
                                    out.data_ptr(), hip.stream()), "sm_grad_norm")
     return out
 
