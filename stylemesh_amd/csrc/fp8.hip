@@ -420,11 +420,12 @@ __device__ __forceinline__ void store4(const MatmulArgs& g, int m, int n, f32x4 
     }
 }
 
-// Direct loads into LDS are counted as vector-memory operations and finish in their order: a wave waits for its own (all but
-// the LEFT newest) before the barrier that hands a stage to the others.
+// Direct loads into LDS are counted as vector-memory operations and finish in their order. The waves of a block meet with
+// their own loads - all but the LEFT newest - landed and their LDS reads done: after it every wave may read the stage
+// those loads filled and overwrite the one those reads came from. (__syncthreads would wait for every load in flight.)
 template <int LEFT>
-__device__ __forceinline__ void wait_loads() {
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LEFT) : "memory");
+__device__ __forceinline__ void meet() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory");
 }
 
 // An operand's 32 codes of a lane as bf16, scaled by 2^(byte - 127): e4m3 / e5m2 have 4 / 3 significant bits, bf16 has 8 and
@@ -598,8 +599,7 @@ __global__ __launch_bounds__(WM* WN * 64) void fp8_matmul_kernel(MatmulArgs g) {
             if (j + 1 < TM) {
                 next = frag(la, wm * TM + j + 1);
             } else {
-                wait_loads<(NST - 2) * NL>();
-                __syncthreads();
+                meet<(NST - 2) * NL>();
                 stage(buf, min(k + NST, kb1 - 1));      // (behind the end: the last block again, read by nobody)
                 next = frag(na, wm * TM);
             }
@@ -635,8 +635,7 @@ __global__ __launch_bounds__(WM* WN * 64) void fp8_matmul_kernel(MatmulArgs g) {
 #pragma unroll
         for (int i = 0; i < NST; ++i) stage(i, min(kb0 + i, kb1 - 1));
         load_scales(F32S ? kb0 : kb0 >> 2, sa, sb);
-        wait_loads<(NST - 1) * NL>();
-        __syncthreads();
+        meet<(NST - 1) * NL>();
         a = frag(lds[0], wm * TM);
 #pragma unroll
         for (int i = 0; i < TN; ++i) b[i] = frag(lds[0] + BM * 128, wn * TN + i);
@@ -647,7 +646,7 @@ __global__ __launch_bounds__(WM* WN * 64) void fp8_matmul_kernel(MatmulArgs g) {
             if (kb + 2 < kb1) step(std::integral_constant<int, 2>{}, kb + 2);
             if (kb + 3 < kb1) step(std::integral_constant<int, 3>{}, kb + 3);
         }
-        wait_loads<0>();      // no load into this block's LDS may outlive it
+        meet<0>();      // no load into this block's LDS may outlive it
     }
 #pragma unroll
     for (int j = 0; j < TM; ++j) {
@@ -911,7 +910,8 @@ __global__ __launch_bounds__(256) void fp8_matmul_empty_kernel(MatmulArgs g) {
 // emptier than the small one's by more than what it gains (1.2 x); below 192 tiles of 128 x 128 the chip is filled with
 // 64 x 64 ones, and where even those are few (a weight gradient of small layers) K is split, at least eight blocks a slice, and
 // the slices are added by a second kernel (128 x 256 x 8192: 27 us in one slice).
-// Up to 64 rows the stream kernel: it reads B once at any M.
+// Up to 32 rows the stream kernel, which needs no LDS and keeps more of B in flight (32 x 4096 x 4096: 9.6 against 12.3 us); above,
+// its rereads of A through the caches cost more (37 x 8200 x 5001: 25 against 20 us).
 enum { TILE_STREAM, TILE_64, TILE_128, TILE_256 };
 struct Plan {
     int kind, splits, kb_per_split;
@@ -921,15 +921,15 @@ static Plan matmul_plan(int M, int N, int KB) {
     const auto fill = [](long long t, long long slots) { return (double)t / (double)((t + slots - 1) / slots * slots); };
     Plan p{TILE_64, 1, KB};
     long long t = tiles(64, 64);
-    if (M <= 64) {
+    if (M <= 32) {
         p.kind = TILE_STREAM;
         t = (N + 15) / 16;
     } else if (tiles(128, 128) >= 192) {
         p.kind = 1.2 * fill(tiles(256, 256), 256) >= fill(tiles(128, 128), 512) ? TILE_256 : TILE_128;
         return p;
     }
-    if (t <= 128 && KB >= 16) {
-        const long long want = std::min<long long>(256 / t, KB / (p.kind == TILE_STREAM ? 32 : 8));
+    if (t <= (p.kind == TILE_STREAM ? 128 : 192) && KB >= 16) {
+        const long long want = std::min<long long>(384 / t, KB / (p.kind == TILE_STREAM ? 32 : 8));
         if (want > 1) {
             p.kb_per_split = (int)((KB + want - 1) / want + 3) / 4 * 4;      // (whole dwords of scale bytes)
             p.splits = (KB + p.kb_per_split - 1) / p.kb_per_split;
@@ -956,8 +956,7 @@ template <int X, bool NATIVE>
 static void launch_stream_pow2(const StreamArgs& t, int splits, hipStream_t s) {
     const bool wide = (t.g.N + 31) / 32 >= 192;       // 32 rows of B per block still fill the chip
     if (t.g.M <= 16) launch_stream<X, 1, 1, false, NATIVE, 4>(t, splits, s);
-    else if (t.g.M <= 32) wide ? launch_stream<X, 2, 2, false, NATIVE, 2>(t, splits, s) : launch_stream<X, 2, 1, false, NATIVE, 2>(t, splits, s);
-    else wide ? launch_stream<X, 4, 2, false, NATIVE, 1>(t, splits, s) : launch_stream<X, 4, 1, false, NATIVE, 2>(t, splits, s);
+    else wide ? launch_stream<X, 2, 2, false, NATIVE, 2>(t, splits, s) : launch_stream<X, 2, 1, false, NATIVE, 2>(t, splits, s);
 }
 template <int X>
 static void launch_stream_codes(const StreamArgs& t, bool f32s, int splits, hipStream_t s) {
@@ -965,8 +964,7 @@ static void launch_stream_codes(const StreamArgs& t, bool f32s, int splits, hipS
         if (native_result(t.g.out_type, t.g.KB)) launch_stream_pow2<X, true>(t, splits, s);
         else launch_stream_pow2<X, false>(t, splits, s);
     } else if (t.g.M <= 16) launch_stream<X, 1, 1, true, false, 4>(t, splits, s);
-    else if (t.g.M <= 32) launch_stream<X, 2, 1, true, false, 2>(t, splits, s);
-    else launch_stream<X, 4, 1, true, false, 2>(t, splits, s);
+    else launch_stream<X, 2, 1, true, false, 2>(t, splits, s);
 }
 static void launch_reduce(const MatmulArgs& g, int splits, hipStream_t s) {
     const size_t quads = (size_t)(g.N + 3) / 4 * g.M;

@@ -9,6 +9,7 @@
 // Sums are held in 64 bits: squares of fp32 gradients over- and underflow fp32 (|g| > 1.8e19, < 1e-23) where the norm
 // does not, and the 64-bit multiply-add runs at the fp32 rate on this chip - both kernels are bound by HBM.
 #include <cmath>
+#include <type_traits>
 
 #include "common.h"
 
@@ -27,7 +28,7 @@ struct GradTable {
     void* out[GN_TENSORS];
     unsigned long long n[GN_TENSORS];
     int first[GN_TENSORS + 1];       // first chunk of each tensor
-    uint8_t type[GN_TENSORS];        // SM_TYPE_* of in, of out << 4
+    unsigned type[GN_TENSORS];       // SM_TYPE_* of in, of out << 4
     int count;
     int chunk_log2;                  // elements per chunk
 };
@@ -36,10 +37,17 @@ __device__ __forceinline__ double gn_combine(double a, double b, bool inf) {
     if (!inf) return a + b;
     return (b > a || b != b) ? b : a;      // a NaN stays
 }
-__device__ __forceinline__ double gn_take(double acc, float v, bool inf) {
-    if (!inf) return fma((double)v, (double)v, acc);
-    const float a = fabsf(v);
-    return gn_combine(acc, (double)a, true);
+template <bool INF>
+__device__ __forceinline__ double gn_take(double acc, float v) {
+    if constexpr (!INF) return fma((double)v, (double)v, acc);
+    else return gn_combine(acc, (double)fabsf(v), true);
+}
+// f(type as a constant), chosen once per chunk: the loops inside have no branch left
+template <class F>
+__device__ __forceinline__ void gn_typed(unsigned type, F f) {
+    if (type == SM_TYPE_F32) f(std::integral_constant<int, SM_TYPE_F32>{});
+    else if (type == SM_TYPE_BF16) f(std::integral_constant<int, SM_TYPE_BF16>{});
+    else f(std::integral_constant<int, SM_TYPE_F16>{});
 }
 __device__ __forceinline__ double gn_block(double v, bool inf) {
     __shared__ double red[4];
@@ -58,27 +66,51 @@ __device__ __forceinline__ unsigned gn_down(float f, int type) {
     const unsigned u = __builtin_bit_cast(unsigned, f);
     return (u & 0x7fffffffu) > 0x7f800000u ? ((u >> 16) | 0x40u) : (u + 0x7fffu + ((u >> 16) & 1u)) >> 16;
 }
-// elements i ... i + 7 of a tensor as fp32
-__device__ __forceinline__ void gn_load8(const void* p, size_t i, int type, float* v) {
-    if (type == SM_TYPE_F32) {
-        const g_u32x4_u* q = reinterpret_cast<const g_u32x4_u*>(static_cast<const float*>(p) + i);
-        const g_u32x4 a = q[0], b = q[1];
+// elements i ... i + 7 of a tensor as they are, and as fp32
+template <int T>
+struct Raw8 {
+    g_u32x4 d[T == SM_TYPE_F32 ? 2 : 1];
+    __device__ __forceinline__ void load(const void* p, size_t i) {
+        const g_u32x4_u* q = reinterpret_cast<const g_u32x4_u*>(static_cast<const char*>(p) + i * (T == SM_TYPE_F32 ? 4 : 2));
+        d[0] = q[0];
+        if constexpr (T == SM_TYPE_F32) d[1] = q[1];
+    }
+    __device__ __forceinline__ void get(float* v) const {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            v[j] = __builtin_bit_cast(float, (unsigned)a[j]);
-            v[4 + j] = __builtin_bit_cast(float, (unsigned)b[j]);
-        }
-    } else {
-        const g_u32x4 a = *reinterpret_cast<const g_u32x4_u*>(static_cast<const uint16_t*>(p) + i);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            v[2 * j] = gn_up(a[j] & 0xffffu, type);
-            v[2 * j + 1] = gn_up(a[j] >> 16, type);
+            if constexpr (T == SM_TYPE_F32) {
+                v[j] = __builtin_bit_cast(float, (unsigned)d[0][j]);
+                v[4 + j] = __builtin_bit_cast(float, (unsigned)d[1][j]);
+            } else {
+                v[2 * j] = gn_up(d[0][j] & 0xffffu, T);
+                v[2 * j + 1] = gn_up(d[0][j] >> 16, T);
+            }
         }
     }
-}
+};
 __device__ __forceinline__ float gn_load1(const void* p, size_t i, int type) {
     return type == SM_TYPE_F32 ? static_cast<const float*>(p)[i] : gn_up(static_cast<const uint16_t*>(p)[i], type);
+}
+template <int O>
+__device__ __forceinline__ void gn_store8(void* p, size_t i, const float* v, bool past) {
+    g_u32x4_u* o = reinterpret_cast<g_u32x4_u*>(static_cast<char*>(p) + i * (O == SM_TYPE_F32 ? 4 : 2));
+    g_u32x4 a, b;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if constexpr (O == SM_TYPE_F32) {
+            a[j] = __builtin_bit_cast(unsigned, v[j]);
+            b[j] = __builtin_bit_cast(unsigned, v[4 + j]);
+        } else {
+            a[j] = gn_down(v[2 * j], O) | (gn_down(v[2 * j + 1], O) << 16);
+        }
+    }
+    if (past) {
+        __builtin_nontemporal_store(a, o);
+        if constexpr (O == SM_TYPE_F32) __builtin_nontemporal_store(b, o + 1);
+    } else {
+        o[0] = a;
+        if constexpr (O == SM_TYPE_F32) o[1] = b;
+    }
 }
 __device__ __forceinline__ int gn_tensor_of(const GradTable& t, int chunk) {
     int lo = 0, hi = t.count;              // last tensor with first <= chunk (an empty tensor has no chunk)
@@ -89,23 +121,42 @@ __device__ __forceinline__ int gn_tensor_of(const GradTable& t, int chunk) {
     return lo;
 }
 
-__global__ __launch_bounds__(256) void grad_norm_partial_kernel(GradTable t, int inf, double* __restrict__ partial) {
+template <bool INF>
+__global__ __launch_bounds__(256) void grad_norm_partial_kernel(GradTable t, double* __restrict__ partial) {
     double acc = 0.0;
     for (int c = blockIdx.x; c < t.first[t.count]; c += gridDim.x) {
         const int k = gn_tensor_of(t, c);
         const size_t begin = (size_t)(c - t.first[k]) << t.chunk_log2;
         const size_t end = min((size_t)t.n[k], begin + ((size_t)1 << t.chunk_log2));
-        const int type = t.type[k] & 15;
-        size_t i = begin + threadIdx.x * 8;
-        for (; i + 8 <= end; i += 2048) {
-            float v[8];
-            gn_load8(t.in[k], i, type, v);
+        const void* in = t.in[k];
+        gn_typed(t.type[k] & 15u, [&](auto tc) {
+            constexpr int T = decltype(tc)::value;
+            size_t i = begin + threadIdx.x * 8;
+            // four rounds of loads in flight
+            for (; i + 3 * 2048 + 8 <= end; i += 4 * 2048) {
+                Raw8<T> r[4];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) acc = gn_take(acc, v[j], inf != 0);
-        }
-        for (; i < end; ++i) acc = gn_take(acc, gn_load1(t.in[k], i, type), inf != 0);     // (only the thread the end falls to)
+                for (int u = 0; u < 4; ++u) r[u].load(in, i + u * 2048);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    float v[8];
+                    r[u].get(v);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) acc = gn_take<INF>(acc, v[j]);
+                }
+            }
+            for (; i + 8 <= end; i += 2048) {
+                Raw8<T> r;
+                float v[8];
+                r.load(in, i);
+                r.get(v);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) acc = gn_take<INF>(acc, v[j]);
+            }
+            for (; i < end; ++i) acc = gn_take<INF>(acc, gn_load1(in, i, T));      // (only the thread the end falls to)
+        });
     }
-    acc = gn_block(acc, inf != 0);
+    acc = gn_block(acc, INF);
     if (threadIdx.x == 0) partial[blockIdx.x] = acc;
 }
 
@@ -128,40 +179,47 @@ __global__ __launch_bounds__(256) void grad_clip_kernel(GradTable t, const doubl
     const double q = max_norm / (norm + 1e-6);
     const float coef = q > 1.0 ? 1.f : (float)q;          // a NaN norm stays NaN, as in the arithmetic it stands for
     if (in_place && coef == 1.f) return;                   // x 1 in place is what is there
-    const int total = t.first[t.count];
-    for (int c = blockIdx.x; c < total; c += gridDim.x) {
+    // from the last chunk backwards: the norm's pass ended there, and what it read last may still be in the 256 MB cache
+    for (int c = t.first[t.count] - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x) {
         const int k = gn_tensor_of(t, c);
         const size_t begin = (size_t)(c - t.first[k]) << t.chunk_log2;
         const size_t end = min((size_t)t.n[k], begin + ((size_t)1 << t.chunk_log2));
-        const int type = t.type[k] & 15, otype = t.type[k] >> 4;
-        size_t i = begin + threadIdx.x * 8;
-        for (; i + 8 <= end; i += 2048) {
-            float v[8];
-            gn_load8(t.in[k], i, type, v);
+        const void* in = t.in[k];
+        void* out = t.out[k];
+        gn_typed(t.type[k] & 15u, [&](auto tc) {
+            constexpr int T = decltype(tc)::value;
+            gn_typed(t.type[k] >> 4, [&](auto oc) {
+                constexpr int O = decltype(oc)::value;
+                size_t i = begin + threadIdx.x * 8;
+                for (; i + 2048 + 8 <= end; i += 2 * 2048) {
+                    Raw8<T> r[2];
+                    r[0].load(in, i);
+                    r[1].load(in, i + 2048);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] *= coef;
-            if (otype == SM_TYPE_F32) {
-                g_u32x4_u* o = reinterpret_cast<g_u32x4_u*>(static_cast<float*>(t.out[k]) + i);
-                g_u32x4 a, b;
+                    for (int u = 0; u < 2; ++u) {
+                        float v[8];
+                        r[u].get(v);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    a[j] = __builtin_bit_cast(unsigned, v[j]);
-                    b[j] = __builtin_bit_cast(unsigned, v[4 + j]);
+                        for (int j = 0; j < 8; ++j) v[j] *= coef;
+                        gn_store8<O>(out, i + u * 2048, v, !in_place);
+                    }
                 }
-                o[0] = a;
-                o[1] = b;
-            } else {
-                g_u32x4 a;
+                for (; i + 8 <= end; i += 2048) {
+                    Raw8<T> r;
+                    float v[8];
+                    r.load(in, i);
+                    r.get(v);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) a[j] = gn_down(v[2 * j], otype) | (gn_down(v[2 * j + 1], otype) << 16);
-                *reinterpret_cast<g_u32x4_u*>(static_cast<uint16_t*>(t.out[k]) + i) = a;
-            }
-        }
-        for (; i < end; ++i) {
-            const float x = gn_load1(t.in[k], i, type) * coef;
-            if (otype == SM_TYPE_F32) static_cast<float*>(t.out[k])[i] = x;
-            else static_cast<uint16_t*>(t.out[k])[i] = (uint16_t)gn_down(x, otype);
-        }
+                    for (int j = 0; j < 8; ++j) v[j] *= coef;
+                    gn_store8<O>(out, i, v, !in_place);
+                }
+                for (; i < end; ++i) {
+                    const float x = gn_load1(in, i, T) * coef;
+                    if constexpr (O == SM_TYPE_F32) static_cast<float*>(out)[i] = x;
+                    else static_cast<uint16_t*>(out)[i] = (uint16_t)gn_down(x, O);
+                }
+            });
+        });
     }
 }
 
@@ -169,9 +227,10 @@ __global__ __launch_bounds__(256) void grad_clip_kernel(GradTable t, const doubl
 
 namespace {
 
-// chunks of 4096 elements (two rounds of a block's 8-element loads), or as many more as keep a launch's chunks within an int
+// chunks of 4096 elements (two rounds of a block's 8-element loads) for short lists, 8192 for long ones, or as many more as
+// keep a launch's chunks within an int
 int chunk_log2_of(unsigned long long total) {
-    int l = 12;
+    int l = total >= (8ull << 20) ? 13 : 12;
     while ((total >> l) > (1ull << 28)) ++l;
     return l;
 }
@@ -187,7 +246,7 @@ int fill_table(sm::GradTable& t, const void* const* in, void* const* out, const 
         t.out[i] = out == nullptr ? nullptr : out[first + i];
         t.n[i] = numel[first + i];
         const int ty = types[first + i], oty = out_types == nullptr ? ty : out_types[first + i];
-        t.type[i] = (uint8_t)(ty | (oty << 4));
+        t.type[i] = (unsigned)(ty | (oty << 4));
         t.first[i + 1] = t.first[i] + (int)((numel[first + i] + ((size_t)1 << chunk_log2) - 1) >> chunk_log2);
     }
     return t.first[count];
@@ -213,7 +272,8 @@ int launch_partials(const void* const* grads, const size_t* numel, const int* ty
         if (chunks == 0) continue;
         const int blocks = chunks < sm::GN_PARTIALS ? chunks : sm::GN_PARTIALS;
         if ((size_t)(*n_partial + blocks) > ws_doubles) return (int)hipErrorInvalidValue;
-        hipLaunchKernelGGL(sm::grad_norm_partial_kernel, dim3((unsigned)blocks), dim3(256), 0, s, t, inf, ws + *n_partial);
+        if (inf) hipLaunchKernelGGL(sm::grad_norm_partial_kernel<true>, dim3((unsigned)blocks), dim3(256), 0, s, t, ws + *n_partial);
+        else hipLaunchKernelGGL(sm::grad_norm_partial_kernel<false>, dim3((unsigned)blocks), dim3(256), 0, s, t, ws + *n_partial);
         SM_LAUNCH_CHECK();
         *n_partial += blocks;
     }
