@@ -157,6 +157,21 @@ int sm_adam_fused(float* p, float* g, float* m, float* v, size_t n, const size_t
                   int zero_grad, float* sumsq_out, const float* dev_hyper, const int32_t* touched,
                   int touched_chunk_log2, void* stream);
 
+/* sm_adam_fused of a CLIPPED gradient (Trainer(gradient_clip_val=...) of the reference's pytorch_lightning: the total gradient -
+ * mean data term + regulariser - of all layers is scaled by min(1, max_norm / (its norm + 1e-6)) before the optimizer step).
+ * sm_adam_grad_clip: clip_out (device, 2 floats) = {norm, coefficient} of grad_scale g + reg_coef p over the arena, or its
+ * flagged chunks (touched as sm_adam_fused takes it), sums in 64 bits, the same bits every time; ws:
+ * sm_adam_grad_clip_ws_bytes() bytes, 8-byte aligned, of this call's own. sm_adam_fused_clipped: sm_adam_fused with every
+ * gradient times clip[1] (1: bit for bit sm_adam_fused). */
+size_t sm_adam_grad_clip_ws_bytes(void);
+int sm_adam_grad_clip(const float* p, const float* g, size_t n, const size_t* seg_end, const float* reg_coef, int n_seg, float grad_scale,
+                      const int32_t* touched, int touched_chunk_log2, double max_norm, void* ws, size_t ws_bytes, float* clip_out, void* stream);
+int sm_adam_fused_clipped(float* p, float* g, float* m, float* v, size_t n, const size_t* seg_end,
+                          const float* reg_coef, int n_seg, float lr, double beta1, double beta2, float eps,
+                          double bias_corr1, double bias_corr2, float grad_scale, float clamp_lo, float clamp_hi,
+                          int zero_grad, float* sumsq_out, const float* dev_hyper, const int32_t* touched,
+                          int touched_chunk_log2, const float* clip, void* stream);
+
 /* Device-side step counter of the fused update for hipGraph replay (torch.optim.Adam's state['step'] and the
  * bias corrections of model/model.py:387-395's optimizer): state = {lr, step} (device, 2 doubles). Adds 1 to the
  * step and writes dev_hyper = {lr / (1 - beta1^step), 1 / sqrt(1 - beta2^step)} (2 floats, computed in double as

@@ -357,7 +357,8 @@ __global__ __launch_bounds__(256) void adam_kernel(float* __restrict__ p, float*
                                                    float grad_scale, float lo, float hi, int zero_grad,
                                                    float* __restrict__ sumsq, const float* __restrict__ dev_hyper,
                                                    int tiles_per_block, const int32_t* __restrict__ touched,
-                                                   int touched_log2) {
+                                                   int touched_log2, const float* __restrict__ clip) {
+    const float clip_coef = ADAM && clip ? clip[1] : 1.f;      // (x 1 leaves every gradient as it is)
     if (ADAM && dev_hyper) {   // step-dependent scalars from device memory: the launch can be replayed from a hipGraph
         lr_over_bc1 = dev_hyper[0];
         inv_sqrt_bc2 = dev_hyper[1];
@@ -442,7 +443,7 @@ __global__ __launch_bounds__(256) void adam_kernel(float* __restrict__ p, float*
                 const int k = seg_of(segs, i0 + j);
                 float x = pv[u][j];
                 if (ADAM) {
-                    const float gr = fmaf(gv[u][j], grad_scale, segs.reg[k] * x);  // data term (+ mean over ranks) + reg
+                    const float gr = fmaf(gv[u][j], grad_scale, segs.reg[k] * x) * clip_coef;  // data term (+ mean over ranks) + reg
                     mv[u][j] = fmaf(gr - mv[u][j], one_minus_beta1, mv[u][j]);          // exp_avg.lerp_(grad, 1 - beta1)
                     vv[u][j] = fmaf(gr * gr, one_minus_beta2, vv[u][j] * beta2);        // exp_avg_sq.mul_(b2).addcmul_(g, g, 1-b2)
                     const float denom = sqrtf(vv[u][j]) * inv_sqrt_bc2 + eps;
@@ -511,7 +512,8 @@ __global__ __launch_bounds__(256) void adam_sparse_kernel(float* __restrict__ p,
                                                           float one_minus_beta2, float eps, float inv_sqrt_bc2,
                                                           float grad_scale, float lo, float hi, int zero_grad,
                                                           float* __restrict__ sumsq, const float* __restrict__ dev_hyper,
-                                                          const int32_t* __restrict__ touched) {
+                                                          const int32_t* __restrict__ touched, const float* __restrict__ clip) {
+    const float clip_coef = clip ? clip[1] : 1.f;
     if (dev_hyper) {
         lr_over_bc1 = dev_hyper[0];
         inv_sqrt_bc2 = dev_hyper[1];
@@ -574,7 +576,7 @@ __global__ __launch_bounds__(256) void adam_sparse_kernel(float* __restrict__ p,
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 float x = pv[u][j];
-                const float gr = fmaf(gv[u][j], grad_scale, reg * x);          // data term (+ mean over ranks) + reg
+                const float gr = fmaf(gv[u][j], grad_scale, reg * x) * clip_coef;          // data term (+ mean over ranks) + reg
                 mv[u][j] = fmaf(gr - mv[u][j], one_minus_beta1, mv[u][j]);          // exp_avg.lerp_(grad, 1 - beta1)
                 vv[u][j] = fmaf(gr * gr, one_minus_beta2, vv[u][j] * beta2);        // exp_avg_sq.mul_(b2).addcmul_(g, g, 1-b2)
                 const float denom = sqrtf(vv[u][j]) * inv_sqrt_bc2 + eps;
@@ -605,6 +607,56 @@ __global__ __launch_bounds__(256) void adam_sparse_kernel(float* __restrict__ p,
         __syncthreads();
         const float s_ = block_sum(sq);
         if (threadIdx.x == 0 && s_ != 0.f) atomicAdd(sumsq + k, s_);
+    }
+}
+
+// ---- the norm of the gradient sm_adam_fused is about to apply, and the clip coefficient -------------------------------
+// gr = grad_scale g + reg_coef p, the update's own expression, over the whole arena or its flagged chunks (elsewhere p and g
+// are zero); sums in 64 bits, one partial per block, added by one block in their order: no atomics, the same bits every time
+// - ranks that hold the same sums get the same coefficient. Bound by HBM: 8 bytes per element of the flagged chunks.
+constexpr int CLIP_BLOCKS = 1024;
+__global__ __launch_bounds__(256) void adam_grad_partial_kernel(const float* __restrict__ p, const float* __restrict__ g, size_t n, Segs segs,
+                                                                float grad_scale, const int32_t* __restrict__ touched, int touched_log2,
+                                                                double* __restrict__ partial) {
+    double acc = 0.0;
+    for (size_t i0 = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4; i0 < n; i0 += (size_t)gridDim.x * 1024) {
+        if (touched != nullptr && touched[i0 >> touched_log2] == 0) continue;
+        float pv[4] = {0.f, 0.f, 0.f, 0.f}, gv[4] = {0.f, 0.f, 0.f, 0.f};
+        if (i0 + 4 <= n) {
+            *reinterpret_cast<float4*>(pv) = *reinterpret_cast<const float4*>(p + i0);
+            *reinterpret_cast<float4*>(gv) = *reinterpret_cast<const float4*>(g + i0);
+        } else {
+            for (int j = 0; i0 + j < n; ++j) {
+                pv[j] = p[i0 + j];
+                gv[j] = g[i0 + j];
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float gr = fmaf(gv[j], grad_scale, segs.reg[seg_of(segs, i0 + j)] * pv[j]);
+            acc = fma((double)gr, (double)gr, acc);
+        }
+    }
+    __shared__ double red[4];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) acc += __shfl_down(acc, o, 64);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = acc;
+    __syncthreads();
+    if (threadIdx.x == 0) partial[blockIdx.x] = red[0] + red[1] + red[2] + red[3];
+}
+
+__global__ __launch_bounds__(256) void adam_grad_clip_kernel(const double* __restrict__ partial, int n, double max_norm, float* __restrict__ out) {
+    double acc = 0.0;
+    for (int i = threadIdx.x; i < n; i += 256) acc += partial[i];
+    __shared__ double red[4];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) acc += __shfl_down(acc, o, 64);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = acc;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const double norm = sqrt(red[0] + red[1] + red[2] + red[3]), q = max_norm / (norm + 1e-6);
+        out[0] = (float)norm;
+        out[1] = q > 1.0 ? 1.f : (float)q;
     }
 }
 
@@ -728,10 +780,10 @@ static int make_segs(sm::Segs& s, size_t n, const size_t* seg_end, const float* 
     return 0;
 }
 
-int sm_adam_fused(float* p, float* g, float* m, float* v, size_t n, const size_t* seg_end, const float* reg_coef,
+static int adam_fused_impl(float* p, float* g, float* m, float* v, size_t n, const size_t* seg_end, const float* reg_coef,
                   int n_seg, float lr, double beta1, double beta2, float eps, double bias_corr1, double bias_corr2,
                   float grad_scale, float clamp_lo, float clamp_hi, int zero_grad, float* sumsq_out,
-                  const float* dev_hyper, const int32_t* touched, int touched_chunk_log2, void* stream) {
+                  const float* dev_hyper, const int32_t* touched, int touched_chunk_log2, const float* clip, void* stream) {
     if (touched != nullptr && (touched_chunk_log2 < 2 || touched_chunk_log2 > 24)) return (int)hipErrorInvalidValue;
     sm::Segs s;
     if (int e = make_segs(s, n, seg_end, reg_coef, n_seg)) return e;
@@ -757,7 +809,7 @@ int sm_adam_fused(float* p, float* g, float* m, float* v, size_t n, const size_t
             if (t.first_block[n_seg] > 0)
                 hipLaunchKernelGGL(sm::adam_sparse_kernel, dim3((unsigned)t.first_block[n_seg]), dim3(256), 0, (hipStream_t)stream,
                                    p, g, m, v, n, s, t, lr_over_bc1, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), eps,
-                                   inv_sqrt_bc2, grad_scale, clamp_lo, clamp_hi, zero_grad, sumsq_out, dev_hyper, touched);
+                                   inv_sqrt_bc2, grad_scale, clamp_lo, clamp_hi, zero_grad, sumsq_out, dev_hyper, touched, clip);
             SM_LAUNCH_CHECK();
             return 0;
         }
@@ -766,7 +818,44 @@ int sm_adam_fused(float* p, float* g, float* m, float* v, size_t n, const size_t
     const size_t blocks = ((n + 1023) / 1024 + tpb - 1) / tpb;
     hipLaunchKernelGGL(sm::adam_kernel<true>, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, p, g, m, v, n,
                        s, lr_over_bc1, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), eps, inv_sqrt_bc2,
-                       grad_scale, clamp_lo, clamp_hi, zero_grad, sumsq_out, dev_hyper, tpb, touched, touched_chunk_log2);
+                       grad_scale, clamp_lo, clamp_hi, zero_grad, sumsq_out, dev_hyper, tpb, touched, touched_chunk_log2,
+                       clip);
+    SM_LAUNCH_CHECK();
+    return 0;
+}
+
+int sm_adam_fused(float* p, float* g, float* m, float* v, size_t n, const size_t* seg_end, const float* reg_coef,
+                  int n_seg, float lr, double beta1, double beta2, float eps, double bias_corr1, double bias_corr2,
+                  float grad_scale, float clamp_lo, float clamp_hi, int zero_grad, float* sumsq_out,
+                  const float* dev_hyper, const int32_t* touched, int touched_chunk_log2, void* stream) {
+    return adam_fused_impl(p, g, m, v, n, seg_end, reg_coef, n_seg, lr, beta1, beta2, eps, bias_corr1, bias_corr2, grad_scale, clamp_lo,
+                           clamp_hi, zero_grad, sumsq_out, dev_hyper, touched, touched_chunk_log2, nullptr, stream);
+}
+
+int sm_adam_fused_clipped(float* p, float* g, float* m, float* v, size_t n, const size_t* seg_end, const float* reg_coef,
+                  int n_seg, float lr, double beta1, double beta2, float eps, double bias_corr1, double bias_corr2,
+                  float grad_scale, float clamp_lo, float clamp_hi, int zero_grad, float* sumsq_out,
+                  const float* dev_hyper, const int32_t* touched, int touched_chunk_log2, const float* clip, void* stream) {
+    if (clip == nullptr) return (int)hipErrorInvalidValue;
+    return adam_fused_impl(p, g, m, v, n, seg_end, reg_coef, n_seg, lr, beta1, beta2, eps, bias_corr1, bias_corr2, grad_scale, clamp_lo,
+                           clamp_hi, zero_grad, sumsq_out, dev_hyper, touched, touched_chunk_log2, clip, stream);
+}
+
+size_t sm_adam_grad_clip_ws_bytes(void) { return sm::CLIP_BLOCKS * sizeof(double); }
+
+int sm_adam_grad_clip(const float* p, const float* g, size_t n, const size_t* seg_end, const float* reg_coef, int n_seg, float grad_scale,
+                      const int32_t* touched, int touched_chunk_log2, double max_norm, void* ws, size_t ws_bytes, float* clip_out, void* stream) {
+    if (!(max_norm >= 0.0) || clip_out == nullptr || ws == nullptr || ws_bytes < sm::CLIP_BLOCKS * sizeof(double) || n == 0 ||
+        (touched != nullptr && (touched_chunk_log2 < 2 || touched_chunk_log2 > 24)))
+        return (int)hipErrorInvalidValue;
+    sm::Segs s;
+    if (int e = make_segs(s, n, seg_end, reg_coef, n_seg)) return e;
+    const size_t tiles = (n + 1023) / 1024;
+    const int blocks = (int)(tiles < (size_t)sm::CLIP_BLOCKS ? tiles : (size_t)sm::CLIP_BLOCKS);
+    hipLaunchKernelGGL(sm::adam_grad_partial_kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, p, g, n, s, grad_scale, touched,
+                       touched_chunk_log2, (double*)ws);
+    SM_LAUNCH_CHECK();
+    hipLaunchKernelGGL(sm::adam_grad_clip_kernel, dim3(1), dim3(256), 0, (hipStream_t)stream, (const double*)ws, blocks, max_norm, clip_out);
     SM_LAUNCH_CHECK();
     return 0;
 }
@@ -803,7 +892,7 @@ int sm_clamp_sumsq(float* p, size_t n, const size_t* seg_end, int n_seg, float c
     const size_t blocks = ((n + 1023) / 1024 + tpb - 1) / tpb;
     hipLaunchKernelGGL(sm::adam_kernel<false>, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, p,
                        (float*)nullptr, (float*)nullptr, (float*)nullptr, n, s, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, clamp_lo,
-                       clamp_hi, 0, sumsq_out, (const float*)nullptr, tpb, (const int32_t*)nullptr, 0);
+                       clamp_hi, 0, sumsq_out, (const float*)nullptr, tpb, (const int32_t*)nullptr, 0, (const float*)nullptr);
     SM_LAUNCH_CHECK();
     return 0;
 }

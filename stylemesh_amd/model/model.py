@@ -52,6 +52,7 @@ class FusedTextureAdam:
         self.module = module
         self.param_groups = [{"lr": lr, "initial_lr": lr, "params": list(module.texture.parameters())}]
         self.world_size = 1
+        self.gradient_clip_val = 0.0      # > 0: norm of the total gradient (data term + regulariser, all layers) is clipped to it
 
     def zero_grad(self, set_to_none=False):
         pass   # the fused update leaves a zeroed gradient arena
@@ -62,6 +63,7 @@ class FusedTextureAdam:
         eng = self.module._engine
         eng.cfg.learning_rate = self.param_groups[0]["lr"]
         eng.cfg.decay_gamma, eng.epoch = 1.0, 0    # the scheduler owns the learning rate
+        eng.gradient_clip_val = float(self.gradient_clip_val)
         reducer = getattr(self.module, "grad_reducer", None)
         if eng.use_deferred_exchange(reducer):
             # STYLEMESH_DEFERRED_EXCHANGE=1 with an owner-aware reducer: critical exchange of the shared chunks, the
@@ -305,6 +307,7 @@ class TextureOptimizationStyleTransferPipeline(_Base):
         if opt is not None:   # the scheduler owns the learning rate: the split update's early half needs THIS step's
             eng.cfg.learning_rate = opt.param_groups[0]["lr"]
             eng.cfg.decay_gamma, eng.epoch = 1.0, 0
+            eng.gradient_clip_val = float(opt.gradient_clip_val)     # (a clipped step has no early half)
         losses = dict(eng.step_compute(batch, self.grad_reducer))   # device tensors that stay valid: no copies
         losses["total"] = losses["content"] + losses["style"] + losses["tex_reg"]
         self._log_losses(losses, "train", log_idx)

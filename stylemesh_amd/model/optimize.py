@@ -136,7 +136,8 @@ def main(args):
     else:
         model.grad_reducer = make_sparse_grad_reducer(comm, world)
 
-    trainer = MiniTrainer(max_epochs=args.max_epochs, logger=logger, device=device, rank=rank, world_size=world)
+    trainer = MiniTrainer(max_epochs=args.max_epochs, logger=logger, device=device, rank=rank, world_size=world,
+                          gradient_clip_val=args.gradient_clip_val)
     _mark("model built")
     trainer.fit(model, dm)
     _mark("fit done")
@@ -152,6 +153,7 @@ def build_parser():
     # the Trainer flags the reference's scripts use (scripts/train/*.sh:1,14)
     parser.add_argument('--gpus', default=1, type=int)
     parser.add_argument('--max_epochs', default=1, type=int)
+    parser.add_argument('--gradient_clip_val', default=0.0, type=float)
     parser.add_argument('--default_root_dir', default=".", type=str)
     parser.add_argument('--version', default=0, type=int)
     # custom flags: names, defaults and parsing of model/optimize.py:244-290

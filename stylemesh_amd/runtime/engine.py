@@ -49,8 +49,11 @@ class EngineConfig:
     learning_rate: float = 1.0
     decay_gamma: float = 0.1
     decay_step_size: int = 30
+    gradient_clip_val: float = 0.0      # > 0: the total gradient's norm is clipped to this before the update (Lightning's Trainer flag)
 
     def validate(self):
+        if not float(self.gradient_clip_val) >= 0.0:
+            raise ValueError(f"gradient_clip_val={self.gradient_clip_val}: a number >= 0 (0 = no clipping)")
         if self.style_pyramid_mode not in ("single", "multi"):
             raise ValueError(f"Unsupported style_pyramid_mode: {self.style_pyramid_mode}")
         if self.gram_mode not in ("current", "average"):
@@ -172,6 +175,11 @@ class StepEngine:
         self.view_key = None
         self._last_batch = None
         self.step_count = 0
+        # gradient clipping (0: off): the update waits for the whole gradient's norm, so the split update and the overlapped
+        # exchanges, which update a part of the arena before the rest of the gradient exists, are off with it
+        self.gradient_clip_val = float(cfg.gradient_clip_val)
+        self.grad_clip = torch.zeros(2, device=device)      # {norm of the last clipped step's total gradient, coefficient}
+        self._clip_ws = torch.empty(ops.adam_grad_clip_ws_bytes(), dtype=torch.uint8, device=device)
         self.epoch = 0
         # device scalars: [content, style] weighted loss accumulators, per-layer sum of squares of the texture
         # ... and, behind them in the same buffer (one fill zeroes all of it every step), the per-layer max |x| bounds
@@ -1449,7 +1457,7 @@ class StepEngine:
             self._hyper_step = self.step_count
             # the capture bakes in the flags pointer and the sparse-vs-dense choice: part of the key
             touched, tl2 = self._touched_arg()
-            key = (world_size, None if touched is None else touched.data_ptr(), tl2)
+            key = (world_size, None if touched is None else touched.data_ptr(), tl2, self.gradient_clip_val)
             if self._opt_graph is None or self._opt_graph[0] != key:
                 if getattr(self, "_opt_warm", 0) < 1:      # one eager run before capturing
                     self._opt_warm = 1
@@ -1492,7 +1500,7 @@ class StepEngine:
         ``_optimizer_launch`` then only walks the view's own chunks. Call after ``loss_tensors()`` (which reads the
         sum of squares this zeroes)."""
         self._adam_early_pending = False
-        if not (self.split_update and self.sparse_update and self.touched is not None and self._view_flags is not None
+        if not (self.gradient_clip_val == 0.0 and self.split_update and self.sparse_update and self.touched is not None and self._view_flags is not None
                 and not self._can_graph() and not torch.cuda.is_current_stream_capturing()
                 and self.view is not None and self._overlap_pays([lv for lv in self.view if lv.active])):
             return
@@ -1530,14 +1538,24 @@ class StepEngine:
         if dev_hyper is not None:
             ops.adam_hyper_step(self._hyper_state, dev_hyper)
         touched, tl2 = self._touched_arg()
+        clip = self._clip_launch(world_size, touched, tl2)
         ops.adam_fused(self.arena.p, self.arena.g, self.arena.m, self.arena.v, self.arena.seg_end, self.reg_coef,
                        self.lr, self.step_count, grad_scale=1.0 / world_size, sumsq_out=self.sumsq,
-                       dev_hyper=dev_hyper, touched=touched, touched_log2=tl2)
+                       dev_hyper=dev_hyper, touched=touched, touched_log2=tl2, clip=clip)
+
+    def _clip_launch(self, world_size, touched, touched_log2):
+        """Norm and clip coefficient of the gradient the update is about to apply (None: clipping is off)."""
+        if self.gradient_clip_val == 0.0:
+            return None
+        ops.adam_grad_clip(self.arena.p, self.arena.g, self.arena.seg_end, self.reg_coef, self.gradient_clip_val, self.grad_clip,
+                           self._clip_ws, grad_scale=1.0 / world_size, touched=touched, touched_log2=touched_log2)
+        return self.grad_clip
 
     def use_pipelined_exchange(self, reducer) -> bool:
         """Multi-GPU tail of the step as pipelined exchange + update? (identical on every rank: it depends on the
         reducer's chunk count - the all-reduced union of the ranks' footprints - and on configuration only)"""
-        if reducer is None or not hasattr(reducer, "pipelined") or self._can_graph() or self.pipeline_exchange is False:
+        if (reducer is None or not hasattr(reducer, "pipelined") or self._can_graph() or self.pipeline_exchange is False
+                or self.gradient_clip_val != 0.0):
             return False
         if self.pipeline_exchange is True:
             return True
@@ -1553,7 +1571,7 @@ class StepEngine:
         OPT-IN (STYLEMESH_DEFERRED_EXCHANGE=1; identical on every rank: configuration and the all-reduced chunk lists only):
         functional and bit-identical to exchange-then-update over gloo (tests/test_distributed_cpu.py), never timed over
         RCCL on separate GPUs - the same status as the pipelined exchange."""
-        return (self.deferred_exchange and reducer is not None and getattr(reducer, "owner_aware", False)
+        return (self.deferred_exchange and self.gradient_clip_val == 0.0 and reducer is not None and getattr(reducer, "owner_aware", False)
                 and self.touched is not None and self.sparse_update and not self._can_graph() and reducer.ready)
 
     def _chunk_update(self, world_size, with_sumsq=True):
@@ -1727,7 +1745,7 @@ class StepEngine:
         SMALL steps (one 256 x 341 level: 1.1 ms of GPU work against 0.65 - 1.1 ms of interpreter + ctypes time for its
         ~70 launches), which run on one stream: no side streams, no split update (``_overlap_pays``), no graphs, no
         per-launch timers, one rank."""
-        if self.step_programs == "0" or reducer is not None or self.use_graphs or self.view is None or self.overlap_style:
+        if self.step_programs == "0" or self.gradient_clip_val != 0.0 or reducer is not None or self.use_graphs or self.view is None or self.overlap_style:
             return None
         if (ops.CONV_TIMER is not None and ops.CONV_TIMER.enabled) or getattr(self, "phase_timer", None) is not None:
             return None

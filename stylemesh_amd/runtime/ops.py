@@ -236,8 +236,8 @@ def adam_hyper(lr, step, beta1=0.9, beta2=0.999):
 
 
 def adam_fused(p, g, m, v, seg_end, reg_coef, lr, step, grad_scale=1.0, beta1=0.9, beta2=0.999, eps=1e-8,
-               zero_grad=True, sumsq_out=None, dev_hyper=None, lo=0, hi=None, touched=None, touched_log2=0):
-    """``lo`` / ``hi``: update only arena elements [lo, hi) (multiples of 4; the pipelined multi-GPU exchange updates
+               zero_grad=True, sumsq_out=None, dev_hyper=None, lo=0, hi=None, touched=None, touched_log2=0, clip=None):
+    """``clip`` (``adam_grad_clip``'s result): every gradient is scaled by its coefficient first. ``lo`` / ``hi``: update only arena elements [lo, hi) (multiples of 4; the pipelined multi-GPU exchange updates
     the arena range by range) - same kernel on offset pointers, segment ends shifted and clipped to the range.
     ``touched``: int32 flag per 2^touched_log2 floats of the WHOLE arena; chunks with flag 0 are skipped (exact only for
     elements with p = g = m = v = 0, see sm_adam_fused). ``g`` may be None: the data-term gradient is zero wherever
@@ -260,10 +260,37 @@ def adam_fused(p, g, m, v, seg_end, reg_coef, lr, step, grad_scale=1.0, beta1=0.
     # algorithmic bytes: 7 (6 without the gradient arena) streams x 4 B per element of the FLAGGED chunks; the flagged share
     # is a device quantity: the launch is recorded with the whole range's bytes and bench.py scales by the share it reads
     tag = "adam_dense" if touched is None else ("adam_early(x flagged share)" if g is None else "adam_closing(x flagged share)")
+    if clip is not None:
+        _hbm_timed(tag, n * (28 if g is not None else 24), lambda: hip.check(
+            lib.sm_adam_fused_clipped(ptr(p), ptr(g), ptr(m), ptr(v), n, hip.size_array(seg_end), hip.float_array(reg_coef),
+                                      len(seg_end), lr, beta1, beta2, eps, bc1, bc2, grad_scale, CLAMP_LO, CLAMP_HI, int(zero_grad),
+                                      ptr(sumsq_out), ptr(dev_hyper), ptr(touched), touched_log2, ptr(clip), hip.stream()),
+            "sm_adam_fused_clipped"))
+        return
     _hbm_timed(tag, n * (28 if g is not None else 24), lambda: hip.check(
         lib.sm_adam_fused(ptr(p), ptr(g), ptr(m), ptr(v), n, hip.size_array(seg_end), hip.float_array(reg_coef),
                           len(seg_end), lr, beta1, beta2, eps, bc1, bc2, grad_scale, CLAMP_LO, CLAMP_HI, int(zero_grad),
                           ptr(sumsq_out), ptr(dev_hyper), ptr(touched), touched_log2, hip.stream()), "sm_adam_fused"))
+
+
+def adam_grad_clip(p, g, seg_end, reg_coef, max_norm, clip_out, ws, grad_scale=1.0, touched=None, touched_log2=0):
+    """Norm of the total gradient ``grad_scale * g + reg_coef * p`` that ``adam_fused`` would apply (64-bit sums), and the
+    coefficient min(1, max_norm / (norm + 1e-6)), into ``clip_out`` (float32 [2], device) for ``adam_fused(clip=...)``; ``ws``:
+    uint8 scratch of ``adam_grad_clip_ws_bytes()`` bytes. ``touched``: as for ``adam_fused``."""
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError(f"max_norm={max_norm}: a number >= 0")
+    assert clip_out.dtype == torch.float32 and clip_out.numel() >= 2 and p.numel() == g.numel()
+    if touched is not None:
+        assert touched.dtype == torch.int32 and touched.numel() * (1 << touched_log2) >= p.numel()
+    _hbm_timed("adam_grad_clip(x flagged share)", p.numel() * 8, lambda: hip.check(
+        lib.sm_adam_grad_clip(ptr(p), ptr(g), p.numel(), hip.size_array(seg_end), hip.float_array(reg_coef), len(seg_end), grad_scale,
+                              ptr(touched), touched_log2, max_norm, ptr(ws), ws.numel(), ptr(clip_out), hip.stream()),
+        "sm_adam_grad_clip"))
+
+
+def adam_grad_clip_ws_bytes() -> int:
+    return lib.sm_adam_grad_clip_ws_bytes()
 
 
 def adam_hyper_step(state, dev_hyper, beta1=0.9, beta2=0.999):

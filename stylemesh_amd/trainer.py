@@ -73,7 +73,13 @@ class JsonlLogger:
 
 class MiniTrainer:
     def __init__(self, max_epochs=1, logger=None, device=None, rank=0, world_size=1, limit_train_batches=None,
-                 limit_val_batches=None, progress=True):
+                 limit_val_batches=None, progress=True, gradient_clip_val=0.0):
+        """``gradient_clip_val`` (Lightning's Trainer flag; 0 / None: off): the gradients' global 2-norm is clipped to it between
+        backward and the optimizer step - inside the fused update for the texture pipeline, in place on ``param.grad``
+        (``runtime.gradclip.clip_grad_norm``) for any other module."""
+        self.gradient_clip_val = 0.0 if gradient_clip_val is None else float(gradient_clip_val)
+        if not self.gradient_clip_val >= 0.0:
+            raise ValueError(f"gradient_clip_val={gradient_clip_val}: a number >= 0 (0 = no clipping)")
         self.max_epochs, self.rank, self.world_size = max_epochs, rank, world_size
         self.logger = logger if logger is not None else JsonlLogger()
         self.device = device if device is not None else (torch.device("cuda", 0) if torch.cuda.is_available() else "cpu")
@@ -177,6 +183,9 @@ class MiniTrainer:
         opt, sched = optimizers[0], (schedulers[0] if schedulers else None)
         if hasattr(opt, "world_size"):
             opt.world_size = self.world_size
+        fused_clip = hasattr(opt, "gradient_clip_val")
+        if fused_clip:
+            opt.gradient_clip_val = self.gradient_clip_val
         def now():
             if self.device != "cpu" and torch.cuda.is_available():
                 torch.cuda.synchronize()
@@ -217,6 +226,9 @@ class MiniTrainer:
                 if not out.get("backward_done", False):    # (the fused module has deposited its gradients already)
                     out["loss"].backward()
                 t_e = time.perf_counter() if timing else 0.0
+                if self.gradient_clip_val and not fused_clip:
+                    from .runtime.gradclip import clip_grad_norm
+                    clip_grad_norm([q.grad for group in opt.param_groups for q in group["params"]], self.gradient_clip_val)
                 opt.step()
                 self.global_step += 1
                 if timing:

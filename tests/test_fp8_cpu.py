@@ -99,3 +99,44 @@ def test_scale_bytes_round_trip():
     assert torch.equal(got[e < 255], want[e < 255]) and torch.isnan(got[e == 255]).all()
     t = fp8.Fp8Matrix.from_parts(torch.zeros(300, 700, dtype=torch.uint8).view(E4), e[:3, :6], "tiles").transposed()
     assert t.shape == (700, 300) and torch.equal(t.scales()[e[:3, :6].t() < 255], want[:3, :6].t()[e[:3, :6].t() < 255].float())
+
+
+def test_gradient_clip_flag_and_entry_refusals():
+    import ctypes as C
+    from stylemesh_amd.model.optimize import build_parser
+    base = ["--style_image_path", "synthetic:1:8x8"]
+    assert build_parser().parse_args(base).gradient_clip_val == 0.0
+    assert build_parser().parse_args(base + ["--gradient_clip_val", "0.5"]).gradient_clip_val == 0.5
+    lib = hip.lib
+    buf = torch.zeros(1 << 16, dtype=torch.uint8)
+    p = buf.data_ptr() + (-buf.data_ptr()) % 16
+    one = lambda t, v: (t * 1)(v)
+    ptrs, n, ty = one(C.c_void_p, p), one(C.c_size_t, 16), one(C.c_int, 0)
+    need = lib.sm_grad_norm_ws_bytes(1)
+    bad_ty, half = one(C.c_int, 3), one(C.c_int, 1)
+    other = one(C.c_void_p, p + 4096)
+    assert lib.sm_grad_norm(ptrs, n, ty, -1, 0, p, need, p, None) != 0
+    assert lib.sm_grad_norm(ptrs, n, bad_ty, 1, 0, p, need, p, None) != 0
+    assert lib.sm_grad_norm(None, n, ty, 1, 0, p, need, p, None) != 0
+    assert lib.sm_grad_norm(one(C.c_void_p, None), n, ty, 1, 0, p, need, p, None) != 0
+    assert lib.sm_grad_norm(ptrs, n, ty, 1, 0, p, 0, p, None) != 0
+    assert lib.sm_grad_norm(ptrs, n, ty, 1, 0, None, need, p, None) != 0
+    assert lib.sm_grad_norm(ptrs, n, ty, 1, 0, p, need, None, None) != 0
+    assert lib.sm_grad_norm(ptrs, one(C.c_size_t, 1 << 41), ty, 1, 0, p, need, p, None) != 0
+    clip = lambda out, oty, mx, ws: lib.sm_grad_clip(ptrs, out, n, ty, oty, 1, 0, mx, p, ws, p, None)
+    assert clip(other, ty, -1.0, need) != 0 and clip(other, ty, float("nan"), need) != 0 and clip(None, ty, 1.0, need) != 0
+    assert clip(other, bad_ty, 1.0, need) != 0 and clip(ptrs, half, 1.0, need) != 0 and clip(other, ty, 1.0, 8 * 0) != 0
+    seg, reg = one(C.c_size_t, 64), one(C.c_float, 0.0)
+    g = lambda **k: lib.sm_adam_grad_clip(p, p, k.get("n", 64), seg, reg, 1, 1.0, k.get("t"), k.get("l", 0), k.get("m", 1.0), k.get("ws", p),
+                                          k.get("wb", 1 << 15), k.get("out", p), None)
+    for bad in (dict(n=0), dict(n=63), dict(t=p, l=1), dict(t=p, l=25), dict(m=-1.0), dict(m=float("nan")), dict(ws=None), dict(wb=8), dict(out=None)):
+        assert g(**bad) != 0, bad
+
+
+def test_gradient_lists_of_host_tensors_are_refused():
+    from stylemesh_amd.runtime import gradclip
+    t = torch.ones(4)
+    for f in (lambda: gradclip.clip_grad_norm([t], 1.0), lambda: gradclip.grad_norm([t]), lambda: gradclip.GradClip([t]),
+              lambda: gradclip.clip_grad_norm([t], -1.0), lambda: gradclip.clip_grad_norm([t], 1.0, 3.0), lambda: gradclip.GradClip([t], [])):
+        with pytest.raises(ValueError):
+            f()
