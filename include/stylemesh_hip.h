@@ -776,6 +776,15 @@ size_t sm_fp8_linear_ws_bytes(int M, int N, int K);
 int sm_fp8_linear(const void* x, int x_type, size_t x_stride, const void* w, const void* w_scale, int w_tiles, size_t w_pitch, int M,
                   int N, int K, void* out, int out_type, size_t out_stride, void* ws, size_t ws_bytes, void* stream);
 
+/* Its backward pass (M, N, K > 0): dx[M][K] = q(dy) W from W's transpose wt [K][N], dw[N][K] = q(dy^T) q(x^T)^T (+= with accumulate,
+ * fp32) from the transposed activations xt [K][M], both e4m3 with power-of-two scales; dy [M][N] is read once and quantised in
+ * fmt. dx or dw may be NULL (not computed; its operand is not looked at). ws: sm_fp8_linear_backward_ws_bytes(M, N, K, dx
+ * wanted, dw wanted) bytes, 16-byte aligned, of this call's own. */
+size_t sm_fp8_linear_backward_ws_bytes(int M, int N, int K, int need_dx, int need_dw);
+int sm_fp8_linear_backward(const void* dy, int dy_type, size_t dy_stride, int fmt, int M, int N, int K, const void* wt, const void* wt_scale,
+                           int wt_tiles, size_t wt_pitch, const void* xt, const void* xt_scale, int xt_tiles, size_t xt_pitch, void* dx,
+                           int dx_type, size_t dx_stride, float* dw, size_t dw_stride, int accumulate, void* ws, size_t ws_bytes, void* stream);
+
 /* ---- G1: the global norm of many gradient tensors, and clipping by it (csrc/gradnorm.hip) -------------------
  * What Trainer(gradient_clip_val=...) of the reference's pytorch_lightning does between backward and the optimizer step
  * (torch.nn.utils.clip_grad_norm_). grads / out / numel / types (SM_TYPE_*) / out_types: HOST arrays of n entries, read during

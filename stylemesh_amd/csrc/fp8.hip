@@ -303,7 +303,7 @@ __global__ __launch_bounds__(256) void fp8_quantize_kernel(QuantArgs a) {
             const int r = tr + rg * RPT + i;
             const int e = TILES ? tile_e : block_exponent(mag_float<T>(mag_both<T>(row16_max<T>(rmax[i]))), top);
             if (r < a.rows) {
-                *reinterpret_cast<u32x2*>(a.q + (size_t)r * pitch + c0) = codes8<T>(d[i], e, a.fmt, finite && e > -127);
+                *reinterpret_cast<u32x2*>(a.q + (size_t)r * pitch + c0) = codes8<T>(d[i], e, a.fmt, finite && !__any(e == -127));
                 if (!TILES && cg < 4 && (cg == 0 || ((int)blockIdx.x == cblocks - 1 && (int)blockIdx.x + cg < (cblocks + 3) / 4 * 4)))
                     a.qs[scale_at(blockIdx.x + cg, r, a.rows)] = cg == 0 ? (uint8_t)(e + 127) : (uint8_t)127;
             }
@@ -344,7 +344,7 @@ __global__ __launch_bounds__(256) void fp8_quantize_kernel(QuantArgs a) {
                 if constexpr (T == SM_TYPE_F32) t[i] = d[i][j];
                 else t[i] = j & 1 ? (d[2 * i][dj] >> 16) | (d[2 * i + 1][dj] & 0xffff0000u) : (d[2 * i][dj] & 0xffffu) | (d[2 * i + 1][dj] << 16);
             }
-            *reinterpret_cast<u32x2*>(img + cl * 128 + (rg ^ cg) * 8) = codes8<T>(t, e, a.fmt, finite && e > -127);
+            *reinterpret_cast<u32x2*>(img + cl * 128 + (rg ^ cg) * 8) = codes8<T>(t, e, a.fmt, finite && !__any(e == -127));
         }
         __syncthreads();
         const size_t pitch = (size_t)rblocks * 128;
@@ -1124,6 +1124,53 @@ int sm_fp8_linear(const void* x, int x_type, size_t x_stride, const void* w, con
     SM_LAUNCH_CHECK();
     if (p.splits > 1) sm::launch_reduce(t.g, p.splits, s);
     SM_LAUNCH_CHECK();
+    return 0;
+}
+
+// workspace of a backward pass: both quantised forms of dy, then one product's slabs (the products run one after the other)
+static size_t bwd_layout(int M, int N, int K, bool need_dx, bool need_dw, size_t* qs, size_t* t, size_t* ts, size_t* slabs) {
+    const auto up = [](size_t b) { return (b + 255) / 256 * 256; };
+    const size_t nb = ((size_t)N + 127) / 128, mb = ((size_t)M + 127) / 128;
+    size_t at = 0;
+    if (need_dx) {
+        at = up((size_t)M * nb * 128);
+        *qs = at;
+        at += up((nb + 3) / 4 * M * 4);
+    }
+    *t = at;
+    if (need_dw) {
+        at += up((size_t)N * mb * 128);
+        *ts = at;
+        at += up((mb + 3) / 4 * N * 4);
+    }
+    *slabs = at;
+    return at + std::max(need_dx ? sm_fp8_matmul_ws_bytes(M, K, N) : 0, need_dw ? sm_fp8_matmul_ws_bytes(N, K, M) : 0);
+}
+
+size_t sm_fp8_linear_backward_ws_bytes(int M, int N, int K, int need_dx, int need_dw) {
+    if (M <= 0 || N <= 0 || K <= 0) return 0;
+    size_t qs, t, ts, slabs;
+    return bwd_layout(M, N, K, need_dx != 0, need_dw != 0, &qs, &t, &ts, &slabs);
+}
+
+int sm_fp8_linear_backward(const void* dy, int dy_type, size_t dy_stride, int fmt, int M, int N, int K, const void* wt, const void* wt_scale,
+                           int wt_tiles, size_t wt_pitch, const void* xt, const void* xt_scale, int xt_tiles, size_t xt_pitch, void* dx,
+                           int dx_type, size_t dx_stride, float* dw, size_t dw_stride, int accumulate, void* ws, size_t ws_bytes, void* stream) {
+    if (M <= 0 || N <= 0 || K <= 0 || (dx == nullptr && dw == nullptr)) return (int)hipErrorInvalidValue;
+    size_t qs = 0, t = 0, ts = 0, slabs = 0;
+    if (ws == nullptr || (uintptr_t)ws % 16 || ws_bytes < bwd_layout(M, N, K, dx != nullptr, dw != nullptr, &qs, &t, &ts, &slabs))
+        return (int)hipErrorInvalidValue;
+    char* w = (char*)ws;
+    if (const int e = sm_fp8_quantize(dy, dy_type, M, N, dy_stride, fmt, 0, dx ? w : nullptr, dx ? w + qs : nullptr, dw ? w + t : nullptr,
+                                      dw ? w + ts : nullptr, stream))
+        return e;
+    if (dx)
+        if (const int e = sm_fp8_matmul(w, w + qs, fmt, ((size_t)N + 127) / 128 * 128, wt, wt_scale, wt_tiles, wt_pitch, 0, M, K, N, dx, dx_type,
+                                        dx_stride, 0, w + slabs, ws_bytes - slabs, stream))
+            return e;
+    if (dw)
+        return sm_fp8_matmul(w + t, w + ts, fmt, ((size_t)M + 127) / 128 * 128, xt, xt_scale, xt_tiles, xt_pitch, 0, N, K, M, dw, SM_TYPE_F32,
+                             dw_stride, accumulate, w + slabs, ws_bytes - slabs, stream);
     return 0;
 }
 

@@ -71,7 +71,7 @@ const Entry ENTRIES[] = {
     SM_ENTRY(sm_gram_masked_split2_grouped), SM_ENTRY(sm_style_loss), SM_ENTRY(sm_gram_backward),
     SM_ENTRY(sm_gram_backward_split), SM_ENTRY(sm_style_loss_grouped), SM_ENTRY(sm_gram_backward_split2_grouped),
     SM_ENTRY(sm_mse_masked), SM_ENTRY(sm_copy_floats), SM_ENTRY(sm_zero_floats),
-    SM_ENTRY(sm_fp8_quantize), SM_ENTRY(sm_fp8_matmul), SM_ENTRY(sm_fp8_linear), SM_ENTRY(sm_grad_norm), SM_ENTRY(sm_grad_clip),
+    SM_ENTRY(sm_fp8_quantize), SM_ENTRY(sm_fp8_matmul), SM_ENTRY(sm_fp8_linear), SM_ENTRY(sm_fp8_linear_backward), SM_ENTRY(sm_grad_norm), SM_ENTRY(sm_grad_clip),
     SM_ENTRY(sm_adam_grad_clip), SM_ENTRY(sm_adam_fused_clipped),
 };
 constexpr int N_ENTRIES = (int)(sizeof(ENTRIES) / sizeof(ENTRIES[0]));

@@ -210,6 +210,11 @@ def _linear_ws(M, N, K):
     return hip.lib.sm_fp8_linear_ws_bytes(M, N, K)
 
 
+@lru_cache(maxsize=4096)
+def _backward_ws(M, N, K, dx, dw):
+    return hip.lib.sm_fp8_linear_backward_ws_bytes(M, N, K, int(dx), int(dw))
+
+
 def matmul_fp8(a: Fp8Matrix, b: Fp8Matrix, out: torch.Tensor | None = None, out_dtype=None, accumulate: bool = False) -> torch.Tensor:
     """[M, N] = A B^T for A [M, K] (``rows`` scales, e4m3 or e5m2) and B [N, K] (e4m3, ``rows`` or ``tiles`` scales), both with
     power-of-two or both with float32 scales; fp32 accumulate, one rounding to ``out_dtype`` (float32 / bfloat16 / float16;
@@ -293,21 +298,54 @@ def linear_fp8_bwd(dy: torch.Tensor, x_t: Fp8Matrix | None, weight_t: Fp8Matrix 
     dw [N, K] = q(dy^T) q(x^T)^T in float32 from ``x_t`` = [K, M] (``keep_transposed``). ``fmt``: format of the gradient's
     codes. ``dw`` / ``accumulate``: write into, or add to, an existing float32 gradient. Either of ``x_t`` / ``weight_t`` may be
     None: that gradient is not computed and None is returned in its place."""
-    _matrix_arg(dy, "dy")
+    stride = _matrix_arg(dy, "dy")
     M, N = dy.shape
     if x_t is None and weight_t is None:
         raise ValueError("nothing to compute: both x_t and weight_t are None")
-    if weight_t is not None and _weight_arg(weight_t, "weight_t").cols != N:
-        raise ValueError(f"dy has {N} columns, weight_t {weight_t.cols}")
+    if fmt not in FORMATS:
+        raise ValueError(f"fmt={fmt!r}: 'e4m3' or 'e5m2'")
+    K = (weight_t if weight_t is not None else _weight_arg(x_t, "x_t")).rows
+    dx = None
+    if weight_t is not None:
+        if _weight_arg(weight_t, "weight_t").cols != N:
+            raise ValueError(f"dy has {N} columns, weight_t {weight_t.cols}")
+        if dx_dtype is None:
+            dx_dtype = dy.dtype
+        if dx_dtype not in _TYPE_ID:
+            raise ValueError(f"dx_dtype={dx_dtype}: float32, bfloat16 or float16")
     if x_t is not None:
-        if _weight_arg(x_t, "x_t").cols != M:
-            raise ValueError(f"dy has {M} rows, x_t {x_t.cols} columns")
-        if dw is not None and dw.dtype != torch.float32:
-            raise ValueError(f"dw must be float32, got {dw.dtype}")
+        if _weight_arg(x_t, "x_t").cols != M or x_t.rows != K:
+            raise ValueError(f"dy has {M} rows and the layer {K} inputs, x_t is {x_t.shape}")
+        if dw is not None and (dw.dtype != torch.float32 or tuple(dw.shape) != (N, K)):
+            raise ValueError(f"dw must be float32 {(N, K)}, got {dw.dtype} {tuple(dw.shape)}")
+        if accumulate and dw is None:
+            raise ValueError("accumulate needs dw")
     elif dw is not None:
         raise ValueError("dw given, but no x_t to compute it from")
-    n, t = _quantize(dy, "rows", fmt, weight_t is not None, x_t is not None)
-    dx = matmul_fp8(n, weight_t, out_dtype=dx_dtype or dy.dtype) if weight_t is not None else None
-    if x_t is not None:
-        dw = matmul_fp8(t, x_t, out=dw, out_dtype=torch.float32, accumulate=accumulate)
+    if K > _MAX_DIM:
+        raise ValueError(f"a dimension above {_MAX_DIM}")
+    dw_stride = _matrix_arg(dw, "dw") if dw is not None else max(K, 1)
+    _check_device(None if weight_t is None else weight_t.data, None if x_t is None else x_t.data)
+    if not (M and N and K):      # a gradient without elements, or a sum without terms
+        if weight_t is not None:
+            dx = torch.zeros((M, K), dtype=dx_dtype, device=dy.device)
+        if x_t is not None:
+            if dw is None:
+                dw = torch.zeros((N, K), dtype=torch.float32, device=dy.device)
+            elif not accumulate:
+                dw.zero_()
+        return dx, dw
+    none = (None, None)
+    wt, wt_args = (weight_t._ptrs, (int(weight_t.block == "tiles"), weight_t.data.shape[1])) if weight_t is not None else (none, (0, 0))
+    xt, xt_args = (x_t._ptrs, (int(x_t.block == "tiles"), x_t.data.shape[1])) if x_t is not None else (none, (0, 0))
+    if weight_t is not None:
+        dx = torch.empty((M, K), dtype=dx_dtype, device=dy.device)
+    if x_t is not None and dw is None:
+        dw = torch.empty((N, K), dtype=torch.float32, device=dy.device)
+    need = _backward_ws(M, N, K, weight_t is not None, x_t is not None)
+    ws = torch.empty(need, dtype=torch.uint8, device=dy.device)      # of this call's own, as matmul_fp8's
+    hip.check(ops.lib.sm_fp8_linear_backward(
+        dy.data_ptr(), _TYPE_ID[dy.dtype], stride, _FMT_ID[FORMATS[fmt]], M, N, K, *wt, *wt_args, *xt, *xt_args,
+        None if dx is None else dx.data_ptr(), 0 if dx is None else _TYPE_ID[dx_dtype], K, None if dw is None else dw.data_ptr(), dw_stride,
+        int(accumulate), ws.data_ptr(), need, hip.stream()), "sm_fp8_linear_backward")
     return dx, dw

@@ -22,7 +22,7 @@ from . import hip, ops
 _TYPE_ID = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}           # SM_TYPE_*
 _SIZE = (4, 2, 2)
 _T = torch.Tensor
-_dtype, _shape = attrgetter("dtype"), attrgetter("shape")
+_dtype = attrgetter("dtype")
 
 
 def _dense(t) -> bool:
@@ -41,10 +41,13 @@ class _Table:
     would be the operator's time."""
 
     def __init__(self, tensors, what):
-        try:
+        kinds = set(map(_dtype, tensors))
+        if not kinds <= _TYPE_ID.keys():
+            raise ValueError(f"{what}: {[str(d) for d in kinds - _TYPE_ID.keys()]} (float32, bfloat16 or float16)")
+        if len(kinds) == 1:
+            self.types = array("i", [_TYPE_ID[kinds.pop()]]) * len(tensors)
+        else:
             self.types = array("i", [_TYPE_ID[d] for d in map(_dtype, tensors)])
-        except KeyError as e:
-            raise ValueError(f"{what}: {e.args[0]} tensor (float32, bfloat16 or float16)") from None
         devices = set(map(_T.get_device, tensors))
         if -1 in devices:
             raise ValueError(f"{what}: device tensors only (there is no CPU form)")
@@ -110,8 +113,8 @@ def _refuse_overlap(g: _Table, o: _Table):
 class GradClip:
     """The call's tables for gradients that stay where they are (an arena's views, ``zero_grad(set_to_none=False)``): checked
     and laid out once, used every step. Keeps the tensors alive; ``grads`` may hold None (a parameter without a gradient).
-    ``out``: one tensor per gradient (same shape and element order) that receives the clipped values, of any of the three
-    types; None: the gradients themselves are scaled in place (where nothing is clipped the second pass ends at once).
+    ``out``: one tensor per gradient that receives the clipped values, of any of the three types (both contiguous with as
+    many elements, or the same shape and strides); None: the gradients themselves are scaled in place (where nothing is clipped the second pass ends at once).
     Concurrent use of ONE plan on two streams is not allowed (its scratch is its own); two plans over the same gradients are
     independent."""
 
@@ -132,12 +135,12 @@ class GradClip:
             if type(None) in set(map(type, out)):
                 raise ValueError("an output is missing for a gradient that is there")
             o = self._o = _Table(out, "out")
-            if list(map(_shape, grads)) != list(map(_shape, out)):
-                raise ValueError("an output has not the shape of its gradient")
+            if g.numel != o.numel:
+                raise ValueError("an output has not as many elements as its gradient")
             if not (all(g.contiguous) and all(o.contiguous)):
                 for a, b, ca, cb in zip(grads, out, g.contiguous, o.contiguous):
-                    if not (ca and cb) and a.stride() != b.stride():
-                        raise ValueError(f"out with strides {b.stride()} does not match its gradient's {a.stride()}")
+                    if not (ca and cb) and (a.shape != b.shape or a.stride() != b.stride()):
+                        raise ValueError(f"out {tuple(b.shape)} / {b.stride()} does not match its gradient {tuple(a.shape)} / {a.stride()}")
             same = np.frombuffer(g.ptrs, dtype=np.uint64) == np.frombuffer(o.ptrs, dtype=np.uint64)
             if (same & (np.frombuffer(g.numel, dtype=np.uint64) > 0) & (np.frombuffer(g.types, np.int32) != np.frombuffer(o.types, np.int32))).any():
                 raise ValueError("an output that is its gradient must have its type")

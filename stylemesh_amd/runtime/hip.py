@@ -120,6 +120,8 @@ SIGNATURES = {
     "sm_fp8_matmul": [_vp, _vp, _i, _sz, _vp, _vp, _i, _sz, _i, _i, _i, _i, _vp, _i, _sz, _i, _vp, _sz, _vp],
     "sm_fp8_linear_ws_bytes": [_i, _i, _i],
     "sm_fp8_linear": [_vp, _i, _sz, _vp, _vp, _i, _sz, _i, _i, _i, _vp, _i, _sz, _vp, _sz, _vp],
+    "sm_fp8_linear_backward_ws_bytes": [_i, _i, _i, _i, _i],
+    "sm_fp8_linear_backward": [_vp, _i, _sz, _i, _i, _i, _i, _vp, _vp, _i, _sz, _vp, _vp, _i, _sz, _vp, _i, _sz, _vp, _sz, _i, _vp, _sz, _vp],
     "sm_grad_norm_ws_bytes": [_i],
     "sm_grad_norm": [_vp, _vp, _vp, _i, _i, _vp, _sz, _vp, _vp],
     "sm_grad_clip": [_vp, _vp, _vp, _vp, _vp, _i, _i, _d, _vp, _sz, _vp, _vp],
@@ -133,7 +135,7 @@ PURE_HOST = {"sm_fmap_row_stride", "sm_fmap_plane", "sm_abi_version", "sm_sizeof
              "sm_conv_split2_tile_positions", "sm_plane_tile_positions", "sm_gram_num_slabs", "sm_gram_workspace_slabs",
              "sm_gram_split_num_slabs", "sm_gram_backward_split_ws_bytes", "sm_reproject_blocks", "sm_flags_compact_ws_ints",
              "sm_comm_unique_id_bytes", "sm_cover_segments_ws_bytes", "sm_view_lists_ws_bytes", "sm_call_id",
-             "sm_call_n_args", "sm_device_link", "sm_fp8_matmul_ws_bytes", "sm_fp8_linear_ws_bytes",
+             "sm_call_n_args", "sm_device_link", "sm_fp8_matmul_ws_bytes", "sm_fp8_linear_ws_bytes", "sm_fp8_linear_backward_ws_bytes",
              "sm_adam_grad_clip_ws_bytes", "sm_grad_norm_ws_bytes"}
 
 

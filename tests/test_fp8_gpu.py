@@ -412,3 +412,40 @@ def test_training_step_of_a_layer():
         coef = min(1.0, max_norm / (rn + 1e-6))
         assert ((dw.double() - raw.double() * coef).abs() <= 2.0 ** -22 * raw.double().abs() + 1e-44).all()
         wd -= lr * dw
+
+
+def test_linear_backward_without_elements():
+    fp8 = _fp8()
+    q = lambda m, k, block="rows": fp8.fp8_quantize(torch.zeros(m, k, device="cuda"), block)
+    for M, N, K in ((0, 5, 7), (3, 0, 7), (3, 5, 0)):
+        dy = torch.ones(M, N, device="cuda")
+        dx, dw = fp8.linear_fp8_bwd(dy, q(K, M), q(K, N, "tiles"))
+        assert dx.shape == (M, K) and dw.shape == (N, K) and not dx.any() and not dw.any()
+        old = torch.full((N, K), 3.0, device="cuda")
+        assert fp8.linear_fp8_bwd(dy, q(K, M), None, dw=old, accumulate=True)[1] is old and (old == 3.0).all()
+        assert not fp8.linear_fp8_bwd(dy, q(K, M), None, dw=old)[1].any()
+
+
+def test_products_on_a_side_stream_and_interleaved():
+    """Two streams at once, each with split products, quantisers and backward passes of its own: no scratch is shared."""
+    fp8 = _fp8()
+    g = torch.Generator().manual_seed(8)
+    mk = lambda *s: torch.randint(-4, 5, s, generator=g).float().cuda()
+    x, w, dy = [mk(100, 9000) for _ in range(2)], mk(64, 9000), mk(100, 64)
+    w8, w8t = fp8.fp8_quantize_both(w, "tiles")
+    def work(i):
+        y, xt = fp8.linear_fp8_fwd(x[i], w8, out_dtype=torch.float32, keep_transposed=True)
+        return (y,) + fp8.linear_fp8_bwd(dy, xt, w8t)
+    want = [work(i) for i in range(2)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = [[], []]
+        for r in range(6):
+            for i, s in enumerate(streams):
+                with torch.cuda.stream(s):
+                    got[i].append(work(i))
+        torch.cuda.synchronize()
+        for i in range(2):
+            for res in got[i]:
+                assert all(torch.equal(a, b) for a, b in zip(res, want[i]))
