@@ -497,7 +497,7 @@ __device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t rsrc, uint8_t
 enum { SCALE_POW2, SCALE_F32_ROWS, SCALE_F32_TILES };      // how the scales of a launch are held (fp32: B's blocks)
 
 template <int BM, int BN, int WM, int WN, int NST, int FA, int SC, bool NATIVE>
-__global__ __launch_bounds__(WM* WN * 64) void fp8_matmul_kernel(MatmulArgs g) {
+__device__ __forceinline__ void matmul_tile(const MatmulArgs& g, int block) {
     constexpr int NT = WM * WN * 64;
     constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
     __shared__ __align__(16) uint8_t lds[NST][(BM + BN) * 128];
@@ -505,7 +505,7 @@ __global__ __launch_bounds__(WM* WN * 64) void fp8_matmul_kernel(MatmulArgs g) {
     const int wm = wave % WM, wn = wave / WM;
     const int mt = (g.M + BM - 1) / BM, nt = (g.N + BN - 1) / BN;
     // XCD-contiguous shares of the tiles, walked in groups of 8 rows of tiles: the blocks of an XCD share operand rows in its L2
-    const int id = xcd_linear(blockIdx.x, mt * nt);
+    const int id = xcd_linear(block, mt * nt);
     const int group = id / (8 * nt), gm = min(8, mt - group * 8), in = id - group * 8 * nt;
     const int m0 = (group * 8 + in % gm) * BM, n0 = in / gm * BN;
     const int kb0 = blockIdx.y * g.kb_per_split, kb1 = min(g.KB, kb0 + g.kb_per_split);
@@ -666,6 +666,20 @@ __global__ __launch_bounds__(WM* WN * 64) void fp8_matmul_kernel(MatmulArgs g) {
             }
         }
     }
+}
+
+template <int BM, int BN, int WM, int WN, int NST, int FA, int SC, bool NATIVE>
+__global__ __launch_bounds__(WM* WN * 64) void fp8_matmul_kernel(MatmulArgs g) {
+    matmul_tile<BM, BN, WM, WN, NST, FA, SC, NATIVE>(g, blockIdx.x);
+}
+
+// Two products in one launch (a small layer's two gradients, neither of which fills the chip): the first blocks0 blocks are the
+// first one's
+template <int BM, int BN, int WM, int WN, int NST, int FA, int SC, bool NATIVE>
+__global__ __launch_bounds__(WM* WN * 64) void fp8_matmul_pair_kernel(MatmulArgs g0, MatmulArgs g1, int blocks0) {
+    const bool first = (int)blockIdx.x < blocks0;
+    const MatmulArgs g = first ? g0 : g1;
+    matmul_tile<BM, BN, WM, WN, NST, FA, SC, NATIVE>(g, first ? blockIdx.x : blockIdx.x - blocks0);
 }
 
 // Few rows of A (M <= 16 TM): the product is a stream through B, which is read once, straight into the matrix instructions'
@@ -938,7 +952,11 @@ static Plan matmul_plan(int M, int N, int KB) {
     return p;
 }
 
-// (a bf16 result of K >= 1024 takes the 8-bit matrix instruction: see sm_fp8_matmul)
+// The 8-bit matrix instruction aligns the products of eight neighbouring k to the largest of them and keeps 13 bits below its
+// leading one (measured; so does the older 16x16x32 form), fp32 beyond that: relative to sum |a||b| an rms error of 2^-19
+// (normal data) to 2^-15 (log-normal, sigma 2) at K = 128, falling with sqrt(K). It is taken where the result is bf16 - half
+// a step is 2^-9 - and K >= 1024, where it stays inside what a plain fp32 sum of K terms may lose (K 2^-23 sum |a||b|).
+// Every other product widens the codes to bf16 (exact, scale included) and sums in fp32 throughout, at half the rate.
 static bool native_result(int out_type, int KB) { return out_type == SM_TYPE_BF16 && KB >= 8; }
 
 template <int X, int TM, int TB, bool F32S, bool NATIVE, int U>
@@ -1039,47 +1057,63 @@ size_t sm_fp8_matmul_ws_bytes(int M, int N, int K) {
     return p.splits > 1 ? (size_t)p.splits * M * N * sizeof(float) : 0;
 }
 
+// checks a product's arguments and plans it (M, N, K > 0)
+static int prepare_product(sm::MatmulArgs& g, sm::Plan& p, const void* a, const void* a_scale, int a_fmt, size_t a_pitch, const void* b,
+                           const void* b_scale, int b_tiles, size_t b_pitch, int M, int N, int K, void* out, int out_type, size_t out_stride,
+                           int accumulate, void* ws, size_t ws_bytes) {
+    const int KB = (K + 127) / 128;
+    if (out_type < 0 || out_type > SM_TYPE_F16 || (a_fmt != SM_FP8_E4M3 && a_fmt != SM_FP8_E5M2) || out == nullptr || out_stride < (size_t)N ||
+        a == nullptr || b == nullptr || a_scale == nullptr || b_scale == nullptr || a_pitch < (size_t)KB * 128 || b_pitch < (size_t)KB * 128 ||
+        a_pitch % 16 || b_pitch % 16 || (uintptr_t)a % 16 || (uintptr_t)b % 16)
+        return (int)hipErrorInvalidValue;
+    p = sm::matmul_plan(M, N, KB);
+    if (p.splits > 1 && (ws == nullptr || ws_bytes < (size_t)p.splits * M * N * sizeof(float))) return (int)hipErrorInvalidValue;
+    g = sm::MatmulArgs{(const uint8_t*)a, (const uint8_t*)b, a_scale, b_scale, out, (float*)ws, a_pitch, b_pitch, out_stride, M, N, KB,
+                       b_tiles ? 7 : 0, b_tiles ? (N + 127) / 128 : N, out_type, accumulate, p.kb_per_split};
+    return 0;
+}
+
+static int run_product(const sm::MatmulArgs& g, const sm::Plan& p, int a_fmt, bool f32s, int K, hipStream_t s) {
+    if (p.kind == sm::TILE_STREAM) {
+        const sm::StreamArgs t{g, nullptr, 0, K};
+        if (a_fmt == SM_FP8_E4M3) sm::launch_stream_codes<8 + SM_FP8_E4M3>(t, f32s, p.splits, s);
+        else sm::launch_stream_codes<8 + SM_FP8_E5M2>(t, f32s, p.splits, s);
+    } else if (sm::native_result(g.out_type, g.KB)) {
+        sm::launch_tile<true>(p.kind, g, a_fmt, f32s, p.splits, s);
+    } else {
+        sm::launch_tile<false>(p.kind, g, a_fmt, f32s, p.splits, s);
+    }
+    SM_LAUNCH_CHECK();
+    if (p.splits > 1) sm::launch_reduce(g, p.splits, s);
+    SM_LAUNCH_CHECK();
+    return 0;
+}
+
 int sm_fp8_matmul(const void* a, const void* a_scale, int a_fmt, size_t a_pitch, const void* b, const void* b_scale, int b_tiles,
                   size_t b_pitch, int scale_f32, int M, int N, int K, void* out, int out_type, size_t out_stride, int accumulate,
                   void* ws, size_t ws_bytes, void* stream) {
     if (M < 0 || N < 0 || K < 0 || out_type < 0 || out_type > SM_TYPE_F16 || (a_fmt != SM_FP8_E4M3 && a_fmt != SM_FP8_E5M2))
         return (int)hipErrorInvalidValue;
     if (M == 0 || N == 0) return 0;
-    if (out == nullptr || out_stride < (size_t)N) return (int)hipErrorInvalidValue;
     hipStream_t s = (hipStream_t)stream;
-    const int KB = (K + 127) / 128;
-    sm::MatmulArgs g{(const uint8_t*)a, (const uint8_t*)b, a_scale, b_scale, out, (float*)ws, a_pitch, b_pitch, out_stride, M, N, KB,
-                     b_tiles ? 7 : 0, b_tiles ? (N + 127) / 128 : N, out_type, accumulate, KB};
-    const size_t quads = (size_t)(N + 3) / 4 * M;
+    sm::MatmulArgs g{};
     if (K == 0) {
+        if (out == nullptr || out_stride < (size_t)N) return (int)hipErrorInvalidValue;
+        g.out = out;
+        g.out_stride = out_stride;
+        g.M = M;
+        g.N = N;
+        g.out_type = out_type;
+        const size_t quads = (size_t)(N + 3) / 4 * M;
         if (!accumulate) hipLaunchKernelGGL(sm::fp8_matmul_empty_kernel, dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, s, g);
         SM_LAUNCH_CHECK();
         return 0;
     }
-    if (a == nullptr || b == nullptr || a_scale == nullptr || b_scale == nullptr || a_pitch < (size_t)KB * 128 ||
-        b_pitch < (size_t)KB * 128 || a_pitch % 16 || b_pitch % 16 || (uintptr_t)a % 16 || (uintptr_t)b % 16)
-        return (int)hipErrorInvalidValue;
-    const sm::Plan p = sm::matmul_plan(M, N, KB);
-    if (p.splits > 1 && (ws == nullptr || ws_bytes < (size_t)p.splits * M * N * sizeof(float))) return (int)hipErrorInvalidValue;
-    g.kb_per_split = p.kb_per_split;
-    const bool f32s = scale_f32 != 0;
-    if (p.kind == sm::TILE_STREAM) {
-        const sm::StreamArgs t{g, nullptr, 0, K};
-        if (a_fmt == SM_FP8_E4M3) sm::launch_stream_codes<8 + SM_FP8_E4M3>(t, f32s, p.splits, s);
-        else sm::launch_stream_codes<8 + SM_FP8_E5M2>(t, f32s, p.splits, s);
-    } else {
-        // The 8-bit matrix instruction aligns the products of eight neighbouring k to the largest of them and keeps 13 bits below
-        // its leading one (measured; so does the older 16x16x32 form), fp32 beyond that: relative to sum |a||b| an error of
-        // 2^-19 (normal data) to 2^-15 (log-normal, sigma 2) at K = 128, falling with sqrt(K). It is taken where the result
-        // is bf16 - half a step is 2^-9 - and K >= 1024, where it stays inside what a plain fp32 sum of K terms may lose.
-        // Every other product widens the codes to bf16 (exact, scale included) and sums in fp32 throughout, at half the rate.
-        if (sm::native_result(out_type, KB)) sm::launch_tile<true>(p.kind, g, a_fmt, f32s, p.splits, s);
-        else sm::launch_tile<false>(p.kind, g, a_fmt, f32s, p.splits, s);
-    }
-    SM_LAUNCH_CHECK();
-    if (p.splits > 1) sm::launch_reduce(g, p.splits, s);
-    SM_LAUNCH_CHECK();
-    return 0;
+    sm::Plan p;
+    if (const int e = prepare_product(g, p, a, a_scale, a_fmt, a_pitch, b, b_scale, b_tiles, b_pitch, M, N, K, out, out_type, out_stride, accumulate,
+                                      ws, ws_bytes))
+        return e;
+    return run_product(g, p, a_fmt, scale_f32 != 0, K, s);
 }
 
 // rows up to which a layer's forward pass quantises inside the product
@@ -1161,16 +1195,35 @@ int sm_fp8_linear_backward(const void* dy, int dy_type, size_t dy_stride, int fm
     if (ws == nullptr || (uintptr_t)ws % 16 || ws_bytes < bwd_layout(M, N, K, dx != nullptr, dw != nullptr, &qs, &t, &ts, &slabs))
         return (int)hipErrorInvalidValue;
     char* w = (char*)ws;
+    const hipStream_t s = (hipStream_t)stream;
+    sm::MatmulArgs gx{}, gw{};
+    sm::Plan px{}, pw{};
+    if (dx)
+        if (const int e = prepare_product(gx, px, w, w + qs, fmt, ((size_t)N + 127) / 128 * 128, wt, wt_scale, wt_tiles, wt_pitch, M, K, N, dx, dx_type,
+                                          dx_stride, 0, w + slabs, ws_bytes - slabs))
+            return e;
+    if (dw)
+        if (const int e = prepare_product(gw, pw, w + t, w + ts, fmt, ((size_t)M + 127) / 128 * 128, xt, xt_scale, xt_tiles, xt_pitch, N, K, M, dw,
+                                          SM_TYPE_F32, dw_stride, accumulate, w + slabs, ws_bytes - slabs))
+            return e;
     if (const int e = sm_fp8_quantize(dy, dy_type, M, N, dy_stride, fmt, 0, dx ? w : nullptr, dx ? w + qs : nullptr, dw ? w + t : nullptr,
                                       dw ? w + ts : nullptr, stream))
         return e;
+    // two products of small tiles, neither of which fills the chip: one launch (1029 x 517 x 1283: 8.3 + 8.2 -> 12.8 us)
+    if (dx && dw && px.kind == sm::TILE_64 && pw.kind == sm::TILE_64 && px.splits == 1 && pw.splits == 1 && !sm::native_result(dx_type, gx.KB)) {
+        const int b0 = ((gx.M + 63) / 64) * ((gx.N + 63) / 64), b1 = ((gw.M + 63) / 64) * ((gw.N + 63) / 64);
+        if (fmt == SM_FP8_E4M3)
+            hipLaunchKernelGGL((sm::fp8_matmul_pair_kernel<64, 64, 2, 2, 4, SM_FP8_E4M3, sm::SCALE_POW2, false>), dim3((unsigned)(b0 + b1)), dim3(256),
+                               0, s, gx, gw, b0);
+        else
+            hipLaunchKernelGGL((sm::fp8_matmul_pair_kernel<64, 64, 2, 2, 4, SM_FP8_E5M2, sm::SCALE_POW2, false>), dim3((unsigned)(b0 + b1)), dim3(256),
+                               0, s, gx, gw, b0);
+        SM_LAUNCH_CHECK();
+        return 0;
+    }
     if (dx)
-        if (const int e = sm_fp8_matmul(w, w + qs, fmt, ((size_t)N + 127) / 128 * 128, wt, wt_scale, wt_tiles, wt_pitch, 0, M, K, N, dx, dx_type,
-                                        dx_stride, 0, w + slabs, ws_bytes - slabs, stream))
-            return e;
-    if (dw)
-        return sm_fp8_matmul(w + t, w + ts, fmt, ((size_t)M + 127) / 128 * 128, xt, xt_scale, xt_tiles, xt_pitch, 0, N, K, M, dw, SM_TYPE_F32,
-                             dw_stride, accumulate, w + slabs, ws_bytes - slabs, stream);
+        if (const int e = run_product(gx, px, fmt, false, N, s)) return e;
+    if (dw) return run_product(gw, pw, fmt, false, M, s);
     return 0;
 }
 

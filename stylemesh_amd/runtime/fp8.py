@@ -25,15 +25,18 @@ def _blocks(n: int) -> int:
     return -(-n // BLOCK)
 
 
-def _check_device(*tensors):
+def _check_device(*devices):
     """Launches go to the CURRENT device's current stream: tensors of another device (or of the host) are refused."""
-    for t in tensors:
-        if t is None:
+    cur = None
+    for d in devices:
+        if d is None:
             continue
-        if not t.is_cuda:
+        if d < 0:
             raise ValueError("device tensors only (there is no CPU form)")
-        if t.get_device() != torch.cuda.current_device():
-            raise ValueError(f"a tensor lives on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+        if cur is None:
+            cur = torch.cuda.current_device()
+        if d != cur:
+            raise ValueError(f"a tensor lives on cuda:{d}, the current device is cuda:{cur}")
 
 
 class Fp8Matrix:
@@ -45,7 +48,7 @@ class Fp8Matrix:
     (row, block kb) at [kb / 4, row, kb % 4], KB = ceil(cols / 128), S = rows or ceil(rows / 128) - or float32 scales [KB, S].
     The tensors are used as they are, no copy is taken."""
 
-    __slots__ = ("data", "scale", "cols", "block", "_ptrs")
+    __slots__ = ("data", "scale", "cols", "block", "_ptrs", "_pitch", "_tiles", "_device", "_weight")
 
     def __init__(self, data: torch.Tensor, scale: torch.Tensor, cols: int, block: str = "rows"):
         if block not in ("rows", "tiles"):
@@ -64,15 +67,20 @@ class Fp8Matrix:
                              f"{tuple(scale.shape)}")
         if scale.device != data.device:
             raise ValueError(f"codes on {data.device}, scales on {scale.device}")
-        self.data, self.scale, self.cols, self.block = data, scale, int(cols), block
-        self._ptrs = (data.data_ptr(), scale.data_ptr())      # (of tensors this object keeps)
+        self._set(data, scale, int(cols), block)
+
+    def _set(self, data, scale, cols, block):
+        self.data, self.scale, self.cols, self.block = data, scale, cols, block
+        # what every call hands to the library, of the tensors this object keeps
+        self._ptrs, self._pitch, self._tiles = (data.data_ptr(), scale.data_ptr()), data.shape[1], int(block == "tiles")
+        self._device = data.get_device()                                                     # (-1: host)
+        self._weight = data.dtype == torch.float8_e4m3fn and scale.dtype == torch.uint8      # can be a layer's weight
 
     @classmethod
     def _made(cls, data, scale, cols, block):
         """Of tensors this module laid out itself: nothing to check."""
         m = cls.__new__(cls)
-        m.data, m.scale, m.cols, m.block = data, scale, cols, block
-        m._ptrs = (data.data_ptr(), scale.data_ptr())
+        m._set(data, scale, cols, block)
         return m
 
     @property
@@ -158,7 +166,7 @@ def _matrix_arg(x, what):
                          f"{tuple(x.shape)}; pass .contiguous(), or transpose=True for a transposed matrix")
     if rows > _MAX_DIM or cols > _MAX_DIM:
         raise ValueError(f"{what}: {tuple(x.shape)} has a dimension above {_MAX_DIM}")
-    _check_device(x)
+    _check_device(x.get_device())
     return sr if rows > 1 else max(cols, 1)
 
 
@@ -233,7 +241,7 @@ def matmul_fp8(a: Fp8Matrix, b: Fp8Matrix, out: torch.Tensor | None = None, out_
     M, N, K = a.rows, b.rows, a.cols
     if max(M, N) > _MAX_DIM:
         raise ValueError(f"a dimension above {_MAX_DIM}")
-    _check_device(a.data, b.data, out)
+    _check_device(a._device, b._device)
     if out is None:
         if accumulate:
             raise ValueError("accumulate needs out")
@@ -251,14 +259,14 @@ def matmul_fp8(a: Fp8Matrix, b: Fp8Matrix, out: torch.Tensor | None = None, out_
     need = _matmul_ws(M, N, K)
     # (scratch of this call's own: two captured graphs, or two streams, never share slabs)
     ws = torch.empty(need, dtype=torch.uint8, device=a.device) if need else None
-    hip.check(ops.lib.sm_fp8_matmul(*a._ptrs, _FMT_ID[a.data.dtype], a.data.shape[1], *b._ptrs, int(b.block == "tiles"), b.data.shape[1],
+    hip.check(ops.lib.sm_fp8_matmul(*a._ptrs, _FMT_ID[a.data.dtype], a._pitch, *b._ptrs, b._tiles, b._pitch,
                                     int(a.scale.dtype == torch.float32), M, N, K, out.data_ptr(), _TYPE_ID[out.dtype],
                                     stride, int(accumulate), None if ws is None else ws.data_ptr(), need, hip.stream()), "sm_fp8_matmul")
     return out
 
 
 def _weight_arg(w, what="weight"):
-    if not isinstance(w, Fp8Matrix) or w.data.dtype != torch.float8_e4m3fn or w.scale.dtype != torch.uint8:
+    if not isinstance(w, Fp8Matrix) or not w._weight:
         raise ValueError(f"{what} must be an e4m3 Fp8Matrix with power-of-two scales")
     return w
 
@@ -279,14 +287,14 @@ def linear_fp8_fwd(x: torch.Tensor, weight: Fp8Matrix, out_dtype=None, keep_tran
         return matmul_fp8(n, weight, out_dtype=out_dtype), t
     if out_dtype not in _TYPE_ID:
         raise ValueError(f"out_dtype={out_dtype}: float32, bfloat16 or float16")
-    _check_device(weight.data)
+    _check_device(weight._device)
     N = weight.rows
-    y = torch.empty((M, N), dtype=out_dtype, device=x.device)
+    y = x.new_empty((M, N), dtype=out_dtype)
     if M and N:
         need = _linear_ws(M, N, K)
         ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None      # of this call's own, as matmul_fp8's
         hip.check(ops.lib.sm_fp8_linear(x.data_ptr(), _TYPE_ID[x.dtype], stride, *weight._ptrs,
-                                    int(weight.block == "tiles"), weight.data.shape[1], M, N, K, y.data_ptr(), _TYPE_ID[out_dtype], N,
+                                    weight._tiles, weight._pitch, M, N, K, y.data_ptr(), _TYPE_ID[out_dtype], N,
                                     None if ws is None else ws.data_ptr(), need, hip.stream()), "sm_fp8_linear")
     return y
 
@@ -325,7 +333,7 @@ def linear_fp8_bwd(dy: torch.Tensor, x_t: Fp8Matrix | None, weight_t: Fp8Matrix 
     if K > _MAX_DIM:
         raise ValueError(f"a dimension above {_MAX_DIM}")
     dw_stride = _matrix_arg(dw, "dw") if dw is not None else max(K, 1)
-    _check_device(None if weight_t is None else weight_t.data, None if x_t is None else x_t.data)
+    _check_device(None if weight_t is None else weight_t._device, None if x_t is None else x_t._device)
     if not (M and N and K):      # a gradient without elements, or a sum without terms
         if weight_t is not None:
             dx = torch.zeros((M, K), dtype=dx_dtype, device=dy.device)
@@ -336,8 +344,8 @@ def linear_fp8_bwd(dy: torch.Tensor, x_t: Fp8Matrix | None, weight_t: Fp8Matrix 
                 dw.zero_()
         return dx, dw
     none = (None, None)
-    wt, wt_args = (weight_t._ptrs, (int(weight_t.block == "tiles"), weight_t.data.shape[1])) if weight_t is not None else (none, (0, 0))
-    xt, xt_args = (x_t._ptrs, (int(x_t.block == "tiles"), x_t.data.shape[1])) if x_t is not None else (none, (0, 0))
+    wt, wt_args = (weight_t._ptrs, (weight_t._tiles, weight_t._pitch)) if weight_t is not None else (none, (0, 0))
+    xt, xt_args = (x_t._ptrs, (x_t._tiles, x_t._pitch)) if x_t is not None else (none, (0, 0))
     if weight_t is not None:
         dx = torch.empty((M, K), dtype=dx_dtype, device=dy.device)
     if x_t is not None and dw is None:
