@@ -180,15 +180,19 @@ __device__ __forceinline__ s16x2 cvt_scaled(unsigned v, unsigned w, float scale,
     else if constexpr (T == SM_TYPE_BF16) return __builtin_amdgcn_cvt_scalef32_pk_bf8_bf16(old, __builtin_bit_cast(bf16x2, v), scale, HI);
     else return __builtin_amdgcn_cvt_scalef32_pk_bf8_f16(old, __builtin_bit_cast(f16x2, v), scale, HI);
 }
-// Eight values of a row (16-bit: 4 dwords, fp32: 8) -> eight codes. plain: all finite and the scale a normal float; otherwise
-// each value is scaled and selected on its own.
-template <int T>
-__device__ __forceinline__ u32x2 codes8(const unsigned* d, int e, int fmt, bool plain) {
-    u32x2 r;
+// N values (four or eight) of a row (16-bit: N / 2 dwords, fp32: N) -> N codes. plain: all finite and the scale a normal float;
+// otherwise each value is scaled and selected on its own.
+template <int T, int N>
+struct Codes {
+    unsigned w[N / 4];
+};
+template <int T, int N>
+__device__ __forceinline__ Codes<T, N> encode(const unsigned* d, int e, int fmt, bool plain) {
+    Codes<T, N> r;
     if (plain) {
         const float scale = __builtin_bit_cast(float, (unsigned)(e + 127) << 23);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < N / 4; ++h) {
             s16x2 c = {0, 0};
             if constexpr (T == SM_TYPE_F32) {
                 c = cvt_scaled<T, false>(d[4 * h], d[4 * h + 1], scale, c, fmt);
@@ -197,31 +201,46 @@ __device__ __forceinline__ u32x2 codes8(const unsigned* d, int e, int fmt, bool 
                 c = cvt_scaled<T, false>(d[2 * h], 0, scale, c, fmt);
                 c = cvt_scaled<T, true>(d[2 * h + 1], 0, scale, c, fmt);
             }
-            r[h] = __builtin_bit_cast(unsigned, c);
+            r.w[h] = __builtin_bit_cast(unsigned, c);
         }
         return r;
     }
-    float v[8];
+    const float inv = inv_pow2(e);
 #pragma unroll
-    for (int q = 0; q < (T == SM_TYPE_F32 ? 2 : 1); ++q) unpack<T>(u32x4{d[4 * q], d[4 * q + 1], d[4 * q + 2], d[4 * q + 3]}, v + 4 * q);
-    return cvt8(v, inv_pow2(e), fmt);
+    for (int h = 0; h < N / 4; ++h) {
+        float v[8];
+        if constexpr (T == SM_TYPE_F32) unpack<T>(u32x4{d[4 * h], d[4 * h + 1], d[4 * h + 2], d[4 * h + 3]}, v);
+        else unpack<T>(u32x4{d[2 * h], d[2 * h + 1], 0u, 0u}, v);
+        const int w = cvt2<false>(v[0] * inv, v[1] * inv, 0, fmt);
+        r.w[h] = (unsigned)cvt2<true>(v[2] * inv, v[3] * inv, w, fmt);
+    }
+    return r;
+}
+template <int T>
+__device__ __forceinline__ u32x2 codes8(const unsigned* d, int e, int fmt, bool plain) {
+    const Codes<T, 8> c = encode<T, 8>(d, e, fmt, plain);
+    return u32x2{c.w[0], c.w[1]};
 }
 
-// One tile of 16 RPT rows x 128 columns per block of 256 threads: thread t holds rows RPT (t / 16) ... and columns
-// 8 (t % 16) ... + 7 as they came (all its loads in flight together; x is read once whatever is produced). Maxima are taken on
-// the bits, two 16-bit values per instruction: a block row's 16 lanes by data-parallel moves; columns in registers, then
-// the wave's four row groups, then the four waves through LDS; tiles over everything. The scaled conversion instruction does the rest
-// (about three instructions an element where it was twenty). The transposed codes turn through a 128 x 128 byte LDS image
-// whose 8-byte units are swizzled by their column group, and both results leave as whole 128-byte lines.
-// Bound by HBM: rows * cols * (sizeof(x) + 1 per result). Transposes and tiles need RPT = 8 (128 rows); rows alone take RPT = 1
-// where that leaves too few blocks (16 x 4096 fp32: 8.2 -> 3 us).
-template <int T, bool TILES, bool Q, bool QT, int RPT>
-__global__ __launch_bounds__(256) void fp8_quantize_kernel(QuantArgs a) {
-    static_assert(RPT == 8 || (!TILES && !QT), "column blocks need 128 rows");
+// One tile of ROWS rows x 128 columns per block: thread t holds rows RPT (t / 16) ... and columns 8 (t % 16) ... + 7 as they came
+// (all its loads in flight together; x is read once whatever is produced). Maxima are taken on the bits, two 16-bit
+// values per instruction: a block row's 16 lanes by data-parallel moves; columns in registers, then the wave's four row
+// groups, then the waves through LDS; tiles over everything. The scaled conversion instruction does the rest (about three
+// instructions an element where it was twenty). The transposed codes turn through a 128 x 128 byte LDS image whose 8-byte units are
+// swizzled by their column group, and both results leave as whole 128-byte lines.
+// Bound by HBM: rows * cols * (sizeof(x) + 1 per result); 8192^2 bf16 both ways 58 us (4.6 TB/s, a copy of that size 5.3).
+// Transposes and tiles take ROWS = 128, RPT = 4: with fewer tiles than CUs a thread's instructions bound it (1029 x 517 fp32 both
+// ways 9.1 us at RPT = 8, 7.2 at 4; no difference at 8192^2). Rows alone take RPT = 8, and 16 rows a block, RPT = 1, where
+// 128 leave too few blocks (16 x 4096 fp32: 8.2 -> 2.7 us).
+template <int T, bool TILES, bool Q, bool QT, int RPT, int ROWS>
+__global__ __launch_bounds__(16 * ROWS / RPT) void fp8_quantize_kernel(QuantArgs a) {
+    static_assert(ROWS == 128 || (!TILES && !QT), "column blocks need 128 rows");
+    static_assert(!QT || RPT == 4, "a dword of a column per thread");
+    constexpr int NT = 16 * ROWS / RPT, NW = NT / 64;
     constexpr int ND = T == SM_TYPE_F32 ? 8 : 4;      // dwords of eight values
     constexpr int ES = T == SM_TYPE_F32 ? 4 : 2;
     const int tid = threadIdx.x, rg = tid >> 4, cg = tid & 15, wave = tid >> 6;
-    const int tr = blockIdx.y * 16 * RPT, tc = blockIdx.x * 128, c0 = tc + cg * 8;
+    const int tr = blockIdx.y * ROWS, tc = blockIdx.x * 128, c0 = tc + cg * 8;
     const int top = a.fmt == SM_FP8_E4M3 ? 8 : 15;
     unsigned d[RPT][ND];
     if (c0 + 8 <= a.cols) {
@@ -278,7 +297,7 @@ __global__ __launch_bounds__(256) void fp8_quantize_kernel(QuantArgs a) {
             all = mag_max<T>(all, m);
         }
     }
-    __shared__ unsigned red[4][QT && !TILES ? 16 * ND : 1];
+    __shared__ unsigned red[NW][QT && !TILES ? 16 * ND : 1];
     __shared__ __align__(16) uint8_t img[QT ? 128 * 128 : 16];
     const int cblocks = (a.cols + 127) >> 7, rblocks = (a.rows + 127) >> 7;
     int tile_e = 0;
@@ -288,7 +307,10 @@ __global__ __launch_bounds__(256) void fp8_quantize_kernel(QuantArgs a) {
         for (int o = 32; o > 0; o >>= 1) m = max(m, (unsigned)__shfl_xor((int)m, o, 64));
         if ((tid & 63) == 0) red[wave][0] = m;
         __syncthreads();
-        tile_e = block_exponent(mag_float<T>(max(max(red[0][0], red[1][0]), max(red[2][0], red[3][0]))), top);
+        m = red[0][0];
+#pragma unroll
+        for (int w = 1; w < NW; ++w) m = max(m, red[w][0]);
+        tile_e = block_exponent(mag_float<T>(m), top);
         if (tid < 4) {      // thread 0: this tile's byte; the row's / column's last tile also fills the dword's unused bytes
             if (Q && (tid == 0 || ((int)blockIdx.x + tid < (cblocks + 3) / 4 * 4 && (int)blockIdx.x == cblocks - 1)))
                 a.qs[scale_at(blockIdx.x + tid, blockIdx.y, rblocks)] = tid == 0 ? (uint8_t)(tile_e + 127) : (uint8_t)127;
@@ -328,29 +350,33 @@ __global__ __launch_bounds__(256) void fp8_quantize_kernel(QuantArgs a) {
             __syncthreads();
         }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {      // column j of the thread: its eight rows, packed as a row of the transpose
+        for (int j = 0; j < 8; ++j) {      // column j of the thread: its rows, packed as a row of the transpose
             const int cl = cg * 8 + j, dj = T == SM_TYPE_F32 ? j : j >> 1;
             int e = tile_e;
             if (!TILES) {
-                unsigned m = mag_max<T>(mag_max<T>(red[0][cg * ND + dj], red[1][cg * ND + dj]), mag_max<T>(red[2][cg * ND + dj], red[3][cg * ND + dj]));
+                unsigned m = red[0][cg * ND + dj];
+#pragma unroll
+                for (int w = 1; w < NW; ++w) m = mag_max<T>(m, red[w][cg * ND + dj]);
                 if constexpr (T != SM_TYPE_F32) m = j & 1 ? m >> 16 : m & 0xffffu;
                 e = block_exponent(mag_float<T>(m), top);
                 if (tc + cl < a.cols && rg < 4 && (rg == 0 || ((int)blockIdx.y == rblocks - 1 && (int)blockIdx.y + rg < (rblocks + 3) / 4 * 4)))
                     a.qts[scale_at(blockIdx.y + rg, tc + cl, a.cols)] = rg == 0 ? (uint8_t)(e + 127) : (uint8_t)127;
             }
-            unsigned t[ND];
+            constexpr int NR = T == SM_TYPE_F32 ? RPT : RPT / 2;
+            unsigned t[NR];
 #pragma unroll
-            for (int i = 0; i < ND; ++i) {
+            for (int i = 0; i < NR; ++i) {
                 if constexpr (T == SM_TYPE_F32) t[i] = d[i][j];
                 else t[i] = j & 1 ? (d[2 * i][dj] >> 16) | (d[2 * i + 1][dj] & 0xffff0000u) : (d[2 * i][dj] & 0xffffu) | (d[2 * i + 1][dj] << 16);
             }
-            *reinterpret_cast<u32x2*>(img + cl * 128 + (rg ^ cg) * 8) = codes8<T>(t, e, a.fmt, finite && !__any(e == -127));
+            *reinterpret_cast<unsigned*>(img + cl * 128 + ((rg >> 1) ^ cg) * 8 + (rg & 1) * 4) =
+                encode<T, 4>(t, e, a.fmt, finite && !__any(e == -127)).w[0];
         }
         __syncthreads();
         const size_t pitch = (size_t)rblocks * 128;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {      // 8 lanes write a column's 128 bytes
-            const int cl = i * 32 + (tid >> 3), p = tid & 7, g = cl >> 3;
+        for (int i = 0; i < 1024 / NT; ++i) {      // 8 lanes write a column's 128 bytes
+            const int cl = i * (NT / 8) + (tid >> 3), p = tid & 7, g = cl >> 3;
             // units 2 p and 2 p + 1 of the column lie in the pair p ^ (g / 2), the other way round for odd g
             u32x4 w = *reinterpret_cast<const u32x4*>(img + cl * 128 + (p ^ (g >> 1)) * 16);
             if (g & 1) w = u32x4{w[2], w[3], w[0], w[1]};
@@ -1017,17 +1043,17 @@ static void launch_tile(int kind, const MatmulArgs& g, int a_fmt, bool f32s, int
 template <int T>
 static int launch_quantize(const QuantArgs& a, int tiles, hipStream_t s) {
     const unsigned cb = (unsigned)((a.cols + 127) / 128);
-    const dim3 grid(cb, (unsigned)((a.rows + 127) / 128)), block(256);
+    const dim3 grid(cb, (unsigned)((a.rows + 127) / 128));
     const bool q = a.q != nullptr, qt = a.qt != nullptr;
     if (tiles) {
-        if (q && qt) hipLaunchKernelGGL((fp8_quantize_kernel<T, true, true, true, 8>), grid, block, 0, s, a);
-        else if (q) hipLaunchKernelGGL((fp8_quantize_kernel<T, true, true, false, 8>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((fp8_quantize_kernel<T, true, false, true, 8>), grid, block, 0, s, a);
+        if (q && qt) hipLaunchKernelGGL((fp8_quantize_kernel<T, true, true, true, 4, 128>), grid, dim3(512), 0, s, a);
+        else if (q) hipLaunchKernelGGL((fp8_quantize_kernel<T, true, true, false, 4, 128>), grid, dim3(512), 0, s, a);
+        else hipLaunchKernelGGL((fp8_quantize_kernel<T, true, false, true, 4, 128>), grid, dim3(512), 0, s, a);
     } else {
-        if (q && qt) hipLaunchKernelGGL((fp8_quantize_kernel<T, false, true, true, 8>), grid, block, 0, s, a);
-        else if (qt) hipLaunchKernelGGL((fp8_quantize_kernel<T, false, false, true, 8>), grid, block, 0, s, a);
-        else if ((size_t)grid.x * grid.y >= 1024) hipLaunchKernelGGL((fp8_quantize_kernel<T, false, true, false, 8>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((fp8_quantize_kernel<T, false, true, false, 1>), dim3(cb, (unsigned)((a.rows + 15) / 16)), block, 0, s, a);
+        if (q && qt) hipLaunchKernelGGL((fp8_quantize_kernel<T, false, true, true, 4, 128>), grid, dim3(512), 0, s, a);
+        else if (qt) hipLaunchKernelGGL((fp8_quantize_kernel<T, false, false, true, 4, 128>), grid, dim3(512), 0, s, a);
+        else if ((size_t)grid.x * grid.y >= 1024) hipLaunchKernelGGL((fp8_quantize_kernel<T, false, true, false, 8, 128>), grid, dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((fp8_quantize_kernel<T, false, true, false, 1, 16>), dim3(cb, (unsigned)((a.rows + 15) / 16)), dim3(256), 0, s, a);
     }
     SM_LAUNCH_CHECK();
     return 0;
