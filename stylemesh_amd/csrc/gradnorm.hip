@@ -293,7 +293,7 @@ int sm_grad_norm(const void* const* grads, const size_t* numel, const int* types
                  float* norm_out, void* stream) {
     unsigned long long total;
     if (const int e = check_list(grads, numel, types, n, &total)) return e;
-    if (norm_out == nullptr || ws == nullptr) return (int)hipErrorInvalidValue;
+    if (norm_out == nullptr || ws == nullptr || (uintptr_t)ws % 8) return (int)hipErrorInvalidValue;
     hipStream_t s = (hipStream_t)stream;
     int n_partial = 0;
     if (const int e = launch_partials(grads, numel, types, n, inf_norm, chunk_log2_of(total), (double*)ws, ws_bytes / sizeof(double), &n_partial, s))
@@ -307,7 +307,7 @@ int sm_grad_clip(const void* const* grads, void* const* out, const size_t* numel
                  int inf_norm, double max_norm, void* ws, size_t ws_bytes, float* norm_out, void* stream) {
     unsigned long long total;
     if (const int e = check_list(grads, numel, types, n, &total)) return e;
-    if (norm_out == nullptr || ws == nullptr || !(max_norm >= 0.0) || (n > 0 && (out == nullptr || out_types == nullptr)))
+    if (norm_out == nullptr || ws == nullptr || (uintptr_t)ws % 8 || !(max_norm >= 0.0) || (n > 0 && (out == nullptr || out_types == nullptr)))
         return (int)hipErrorInvalidValue;
     int in_place = 1;
     for (int i = 0; i < n; ++i) {

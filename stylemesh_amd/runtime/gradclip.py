@@ -115,8 +115,7 @@ class GradClip:
     and laid out once, used every step. Keeps the tensors alive; ``grads`` may hold None (a parameter without a gradient).
     ``out``: one tensor per gradient that receives the clipped values, of any of the three types (both contiguous with as
     many elements, or the same shape and strides); None: the gradients themselves are scaled in place (where nothing is clipped the second pass ends at once).
-    Concurrent use of ONE plan on two streams is not allowed (its scratch is its own); two plans over the same gradients are
-    independent."""
+    Calls on two streams need the caller's ordering only where both write the same outputs: each has scratch of its own."""
 
     def __init__(self, grads, out=None):
         grads = list(grads)
@@ -147,27 +146,28 @@ class GradClip:
         _refuse_overlap(g, o)
         self.device = torch.device("cuda", torch.cuda.current_device())
         self._args = (_address(g.ptrs), _address(o.ptrs), _address(g.numel), _address(g.types), _address(o.types), g.n)
-        self._ws = torch.empty(ops.lib.sm_grad_norm_ws_bytes(g.n), dtype=torch.uint8, device=self.device)
-        self._ws_args = (self._ws.data_ptr(), self._ws.numel())
+        self._ws_bytes = ops.lib.sm_grad_norm_ws_bytes(g.n)
 
     def _result(self):
+        """(norm, scratch) of one call: two streams, or two captured graphs, of one plan share nothing"""
         if torch.cuda.current_device() != self.device.index:
             raise ValueError(f"the plan's tensors live on {self.device}, the current device is cuda:{torch.cuda.current_device()}")
-        return torch.empty((), dtype=torch.float32, device=self.device)
+        return (torch.empty((), dtype=torch.float32, device=self.device),
+                torch.empty(self._ws_bytes, dtype=torch.uint8, device=self.device))
 
     def norm(self, norm_type=2.0) -> torch.Tensor:
         """The global norm as a float32 device scalar."""
         kind = _norm_kind(norm_type)
-        out = self._result()
+        out, ws = self._result()
         gp, _, numel, types, _, n = self._args
-        hip.check(ops.lib.sm_grad_norm(gp, numel, types, n, kind, *self._ws_args, out.data_ptr(), hip.stream()), "sm_grad_norm")
+        hip.check(ops.lib.sm_grad_norm(gp, numel, types, n, kind, ws.data_ptr(), self._ws_bytes, out.data_ptr(), hip.stream()), "sm_grad_norm")
         return out
 
     def clip(self, max_norm, norm_type=2.0) -> torch.Tensor:
         """Clips, and returns the norm BEFORE clipping (float32 device scalar)."""
         kind, max_norm = _norm_kind(norm_type), _max_norm(max_norm)
-        out = self._result()
-        hip.check(ops.lib.sm_grad_clip(*self._args, kind, max_norm, *self._ws_args, out.data_ptr(), hip.stream()), "sm_grad_clip")
+        out, ws = self._result()
+        hip.check(ops.lib.sm_grad_clip(*self._args, kind, max_norm, ws.data_ptr(), self._ws_bytes, out.data_ptr(), hip.stream()), "sm_grad_clip")
         return out
 
 

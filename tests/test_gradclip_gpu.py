@@ -215,3 +215,29 @@ def test_more_than_two_to_the_31_elements():
     assert float(gc.clip_grad_norm([g], 1.0)) == 13.0
     ref = torch.tensor([4.0, 12.0, 3.0]) / 13.0
     assert ((g[[0, 1 << 31, n - 1]].float().cpu() - ref).abs() <= 2.0 ** -8 * ref).all() and float(g[1:100].abs().sum()) == 0
+
+
+def test_one_plan_in_two_graphs():
+    """Two captured graphs of the SAME plan on two streams at once: neither uses the other's partial sums."""
+    gc = _mod()
+    src = _grads([3_000_001, 12, 50_000], ("f32", "bf16"))
+    plan = gc.GradClip(src)
+    want = [plan.norm(), plan.norm(math.inf)]
+    st = [torch.cuda.Stream(), torch.cuda.Stream()]
+    graphs, norms = [], []
+    for kind, s in zip((2.0, math.inf), st):
+        s.wait_stream(torch.cuda.current_stream())
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr, stream=s):
+            norms.append(plan.norm(kind))
+        graphs.append(gr)
+    for r in range(4):
+        for n in norms:
+            n.zero_()
+        torch.cuda.synchronize()
+        for gr, s in zip(graphs, st):
+            with torch.cuda.stream(s):
+                gr.replay()
+        eager = plan.norm()
+        torch.cuda.synchronize()
+        assert torch.equal(eager, want[0]) and all(torch.equal(a, b) for a, b in zip(norms, want))
