@@ -756,13 +756,15 @@ int sm_tex_sample_mip(const float* const* levels, const int* level_w, const int*
  * one scale per 128 x 128 tile instead of per row and block. x is read once. A block's scale is the smallest power of two
  * 2^e, e in [-127, 127], with max |x| <= 448 2^e (e5m2: 57344 2^e), 1 for a block of zeros; the codes are x 2^-e rounded to
  * nearest even. NaN and infinities do not take part in the maximum; NaN becomes NaN, an infinity NaN (e4m3) / infinity (e5m2).
- * q, qt: 16-byte aligned. */
+ * q, qt: 16-byte aligned. rows, cols: at most 65535 * 128. */
 int sm_fp8_quantize(const void* x, int x_type, int rows, int cols, size_t x_stride, int fmt, int tiles, void* q, void* q_scale,
                     void* qt, void* qt_scale, void* stream);
 /* out[M][N] (out_type, row stride out_stride elements) = A B^T, or out += A B^T (accumulate), A [M][K] with scales per row and
- * block, B [N][K] (e4m3) per row and block or per tile (b_tiles); fp32 accumulate, one rounding to out_type. scale_f32: both
- * scale arrays are floats. a, b: 16-byte aligned, pitches multiples of 16 and at least K rounded up to 128. ws:
- * sm_fp8_matmul_ws_bytes(M, N, K) bytes (0: may be NULL) of scratch of this call's own. K = 0: zeros / out as it is. */
+ * block, B [N][K] (e4m3) per row and block or per tile (b_tiles); fp32 accumulate, one rounding to out_type. A bf16 result of
+ * K > 896 takes the 8-bit matrix instruction, whose sum of eight products keeps 13 bits below the largest of them; every other
+ * one widens the codes to bf16, which is exact, and sums in fp32. scale_f32: both scale arrays are floats. a, b: 16-byte
+ * aligned, scales 4-byte aligned, pitches multiples of 16, at least K rounded up to 128 and at most 0xfffff0; M, N < 2^30.
+ * ws: sm_fp8_matmul_ws_bytes(M, N, K) bytes (0: may be NULL) of scratch of this call's own. K = 0: zeros / out as it is. */
 size_t sm_fp8_matmul_ws_bytes(int M, int N, int K);
 int sm_fp8_matmul(const void* a, const void* a_scale, int a_fmt, size_t a_pitch, const void* b, const void* b_scale, int b_tiles,
                   size_t b_pitch, int scale_f32, int M, int N, int K, void* out, int out_type, size_t out_stride, int accumulate,

@@ -515,8 +515,8 @@ __device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t rsrc, uint8_t
 #endif
 }
 
-// BM x BN output tile per block, waves WM x WN; a stage = one block of 128 along K of both operands, double-buffered in
-// LDS and filled by direct loads (16 bytes per lane, no registers). LDS rows are 128 bytes; the 16-byte chunk c of row r
+// BM x BN output tile per block, waves WM x WN; a stage = one block of 128 along K of both operands, in a ring of NST
+// stages in LDS, filled by direct loads (16 bytes per lane, no registers). LDS rows are 128 bytes; the 16-byte chunk c of row r
 // sits at chunk c ^ (r & 7), so that the eight lanes of a read phase hit eight different chunk columns. A lane's 32 bytes of
 // an operand row are chunks g and g + 4 (g = lane / 16): the same permutation of k on both sides leaves the sum as it is,
 // and a block of 128 has ONE scale, so it does not matter which quarter a lane holds.
@@ -1063,13 +1063,16 @@ static int launch_quantize(const QuantArgs& a, int tiles, hipStream_t s) {
 
 extern "C" {
 
+static constexpr int MAX_QUANTIZED = 65535 * 128;      // rows / columns of a quantised matrix: the grid's second dimension, in 128s
+
 int sm_fp8_quantize(const void* x, int x_type, int rows, int cols, size_t x_stride, int fmt, int tiles, void* q, void* q_scale,
                     void* qt, void* qt_scale, void* stream) {
     if (rows < 0 || cols < 0 || x_type < 0 || x_type > SM_TYPE_F16 || (fmt != SM_FP8_E4M3 && fmt != SM_FP8_E5M2) ||
         (q == nullptr) != (q_scale == nullptr) || (qt == nullptr) != (qt_scale == nullptr) || (q == nullptr && qt == nullptr))
         return (int)hipErrorInvalidValue;
     if (rows == 0 || cols == 0) return 0;
-    if (x == nullptr || x_stride < (size_t)cols || (rows + 127) / 128 > 65535) return (int)hipErrorInvalidValue;
+    if (x == nullptr || x_stride < (size_t)cols || rows > MAX_QUANTIZED || cols > MAX_QUANTIZED || (uintptr_t)q % 16 || (uintptr_t)qt % 16)
+        return (int)hipErrorInvalidValue;
     const sm::QuantArgs a{x, x_stride, rows, cols, fmt, (uint8_t*)q, (uint8_t*)q_scale, (uint8_t*)qt, (uint8_t*)qt_scale};
     hipStream_t s = (hipStream_t)stream;
     if (x_type == SM_TYPE_F32) return sm::launch_quantize<SM_TYPE_F32>(a, tiles, s);
@@ -1079,18 +1082,23 @@ int sm_fp8_quantize(const void* x, int x_type, int rows, int cols, size_t x_stri
 
 size_t sm_fp8_matmul_ws_bytes(int M, int N, int K) {
     if (M <= 0 || N <= 0 || K <= 0) return 0;
-    const sm::Plan p = sm::matmul_plan(M, N, (K + 127) / 128);
+    const sm::Plan p = sm::matmul_plan(M, N, (int)(((size_t)K + 127) / 128));
     return p.splits > 1 ? (size_t)p.splits * M * N * sizeof(float) : 0;
 }
+
+// offsets from a tile's first row (256 rows) and from a row of scales are 32 bits
+static constexpr size_t MAX_PITCH = 0xfffff0;
+static constexpr int MAX_ROWS = (1 << 30) - 1;
 
 // checks a product's arguments and plans it (M, N, K > 0)
 static int prepare_product(sm::MatmulArgs& g, sm::Plan& p, const void* a, const void* a_scale, int a_fmt, size_t a_pitch, const void* b,
                            const void* b_scale, int b_tiles, size_t b_pitch, int M, int N, int K, void* out, int out_type, size_t out_stride,
                            int accumulate, void* ws, size_t ws_bytes) {
-    const int KB = (K + 127) / 128;
+    const int KB = (int)(((size_t)K + 127) / 128);
     if (out_type < 0 || out_type > SM_TYPE_F16 || (a_fmt != SM_FP8_E4M3 && a_fmt != SM_FP8_E5M2) || out == nullptr || out_stride < (size_t)N ||
         a == nullptr || b == nullptr || a_scale == nullptr || b_scale == nullptr || a_pitch < (size_t)KB * 128 || b_pitch < (size_t)KB * 128 ||
-        a_pitch % 16 || b_pitch % 16 || (uintptr_t)a % 16 || (uintptr_t)b % 16)
+        a_pitch % 16 || b_pitch % 16 || (uintptr_t)a % 16 || (uintptr_t)b % 16 || (uintptr_t)a_scale % 4 || (uintptr_t)b_scale % 4 ||
+        a_pitch > MAX_PITCH || b_pitch > MAX_PITCH || M > MAX_ROWS || N > MAX_ROWS)
         return (int)hipErrorInvalidValue;
     p = sm::matmul_plan(M, N, KB);
     if (p.splits > 1 && (ws == nullptr || ws_bytes < (size_t)p.splits * M * N * sizeof(float))) return (int)hipErrorInvalidValue;
@@ -1159,9 +1167,9 @@ int sm_fp8_linear(const void* x, int x_type, size_t x_stride, const void* w, con
         return (int)hipErrorInvalidValue;
     if (M == 0 || N == 0) return 0;
     if (K > 0 && (x == nullptr || x_stride < (size_t)K || (ws == nullptr && sm_fp8_linear_ws_bytes(M, N, K) > 0) ||
-                  ws_bytes < sm_fp8_linear_ws_bytes(M, N, K)))
+                  ws_bytes < sm_fp8_linear_ws_bytes(M, N, K) || (uintptr_t)ws % 16))
         return (int)hipErrorInvalidValue;
-    const int KB = (K + 127) / 128;
+    const int KB = (int)(((size_t)K + 127) / 128);
     if (K == 0 || M > LINEAR_FUSED_ROWS) {
         const size_t slabs = (sm_fp8_matmul_ws_bytes(M, N, K) + 15) / 16 * 16;
         char* q = (char*)ws + slabs;
@@ -1172,7 +1180,7 @@ int sm_fp8_linear(const void* x, int x_type, size_t x_stride, const void* w, con
                              ws, slabs, stream);
     }
     if (out == nullptr || out_stride < (size_t)N || w == nullptr || w_scale == nullptr || w_pitch < (size_t)KB * 128 || w_pitch % 16 ||
-        (uintptr_t)w % 16)
+        (uintptr_t)w % 16 || N > MAX_ROWS)
         return (int)hipErrorInvalidValue;
     hipStream_t s = (hipStream_t)stream;
     const sm::Plan p = sm::matmul_plan(M, N, KB);

@@ -48,7 +48,7 @@ class Fp8Matrix:
     (row, block kb) at [kb / 4, row, kb % 4], KB = ceil(cols / 128), S = rows or ceil(rows / 128) - or float32 scales [KB, S].
     The tensors are used as they are, no copy is taken."""
 
-    __slots__ = ("data", "scale", "cols", "block", "_ptrs", "_pitch", "_tiles", "_device", "_weight")
+    __slots__ = ("_data", "_scale", "_cols", "_block", "_ptrs", "_pitch", "_tiles", "_device", "_weight")
 
     def __init__(self, data: torch.Tensor, scale: torch.Tensor, cols: int, block: str = "rows"):
         if block not in ("rows", "tiles"):
@@ -65,13 +65,15 @@ class Fp8Matrix:
         if want is None or tuple(scale.shape) != want or not scale.is_contiguous():
             raise ValueError(f"scales must be contiguous uint8 {(-(-kb // 4), s, 4)} or float32 {(kb, s)}, got {scale.dtype} "
                              f"{tuple(scale.shape)}")
+        if scale.data_ptr() % 4:
+            raise ValueError("scales must start on a 4-byte boundary")
         if scale.device != data.device:
             raise ValueError(f"codes on {data.device}, scales on {scale.device}")
         self._set(data, scale, int(cols), block)
 
     def _set(self, data, scale, cols, block):
-        self.data, self.scale, self.cols, self.block = data, scale, cols, block
-        # what every call hands to the library, of the tensors this object keeps
+        self._data, self._scale, self._cols, self._block = data, scale, cols, block
+        # what every call hands to the library, of the tensors this object keeps (and never exchanges: the properties are read-only)
         self._ptrs, self._pitch, self._tiles = (data.data_ptr(), scale.data_ptr()), data.shape[1], int(block == "tiles")
         self._device = data.get_device()                                                     # (-1: host)
         self._weight = data.dtype == torch.float8_e4m3fn and scale.dtype == torch.uint8      # can be a layer's weight
@@ -82,6 +84,11 @@ class Fp8Matrix:
         m = cls.__new__(cls)
         m._set(data, scale, cols, block)
         return m
+
+    data = property(lambda self: self._data)
+    scale = property(lambda self: self._scale)
+    cols = property(lambda self: self._cols)
+    block = property(lambda self: self._block)
 
     @property
     def rows(self) -> int:
@@ -110,6 +117,8 @@ class Fp8Matrix:
         if scale.dtype == torch.float32:
             packed = scale.t().contiguous()
         elif scale.dtype in (torch.uint8, torch.int32):
+            if scale.dtype == torch.int32 and scale.numel() and not 0 <= int(scale.min()) <= int(scale.max()) <= 255:
+                raise ValueError("exponent bytes lie in 0 ... 255")
             packed = pack_scale_bytes(scale)
         else:
             raise ValueError(f"scales of type {scale.dtype}: float32, or exponent bytes as uint8 / int32")
@@ -197,7 +206,8 @@ def fp8_quantize(x: torch.Tensor, block: str = "rows", fmt: str = "e4m3", transp
     """``x`` [rows, cols] (float32 / bfloat16 / float16, unit column stride, any row stride) - or, with ``transpose``, its
     transpose - as an ``Fp8Matrix`` with power-of-two scales: per block the smallest power of two that brings the largest
     finite magnitude into the format's range; x / scale is exact, the code is it rounded to nearest even. NaN stays NaN, an
-    infinity becomes NaN (e4m3 has none) or infinity (e5m2); neither touches its neighbours' scale."""
+    infinity becomes NaN (e4m3 has none) or infinity (e5m2); neither touches its neighbours' scale. (A magnitude from
+    1.9375 * 2^127 on rounds up to 2^128, which fp32 does not hold: its products are infinite.)"""
     n, t = _quantize(x, block, fmt, not transpose, transpose)
     return t if transpose else n
 
@@ -226,7 +236,9 @@ def _backward_ws(M, N, K, dx, dw):
 def matmul_fp8(a: Fp8Matrix, b: Fp8Matrix, out: torch.Tensor | None = None, out_dtype=None, accumulate: bool = False) -> torch.Tensor:
     """[M, N] = A B^T for A [M, K] (``rows`` scales, e4m3 or e5m2) and B [N, K] (e4m3, ``rows`` or ``tiles`` scales), both with
     power-of-two or both with float32 scales; fp32 accumulate, one rounding to ``out_dtype`` (float32 / bfloat16 / float16;
-    default bfloat16). ``out``: result of that type and shape, unit column stride; ``accumulate``: added to it (in fp32, then
+    default bfloat16). A bfloat16 result of K > 896 takes the 8-bit matrix instruction, whose sum of eight products keeps 13 bits
+    below the largest of them (far inside the result's half step); every other one widens the codes exactly and sums in fp32.
+    ``out``: result of that type and shape, unit column stride; ``accumulate``: added to it (in fp32, then
     rounded once)."""
     if not isinstance(a, Fp8Matrix) or not isinstance(b, Fp8Matrix):
         raise ValueError("matmul_fp8 takes two Fp8Matrix operands")
@@ -239,7 +251,7 @@ def matmul_fp8(a: Fp8Matrix, b: Fp8Matrix, out: torch.Tensor | None = None, out_
     if a.scale.dtype != b.scale.dtype:
         raise ValueError(f"one operand has {a.scale.dtype} scales, the other {b.scale.dtype}")
     M, N, K = a.rows, b.rows, a.cols
-    if max(M, N) > _MAX_DIM:
+    if max(M, N, K) > _MAX_DIM:
         raise ValueError(f"a dimension above {_MAX_DIM}")
     _check_device(a._device, b._device)
     if out is None:

@@ -140,3 +140,36 @@ def test_gradient_lists_of_host_tensors_are_refused():
               lambda: gradclip.clip_grad_norm([t], -1.0), lambda: gradclip.clip_grad_norm([t], 1.0, 3.0), lambda: gradclip.GradClip([t], [])):
         with pytest.raises(ValueError):
             f()
+
+
+def test_a_matrix_keeps_its_tensors():
+    """Pointers are taken once, so the tensors cannot be exchanged; scales that are read as dwords start on one."""
+    m = mat(4, 200)
+    for name in ("data", "scale", "cols", "block"):
+        with pytest.raises(AttributeError):
+            setattr(m, name, getattr(m, name))
+    d = torch.zeros(4, 256, dtype=torch.uint8).view(E4)
+    with pytest.raises(ValueError):
+        fp8.Fp8Matrix(d, torch.zeros(17, dtype=torch.uint8)[1:].view(1, 4, 4), 200)
+    for e in (256, -1):
+        with pytest.raises(ValueError):
+            fp8.Fp8Matrix.from_parts(d, torch.full((4, 2), e, dtype=torch.int32))
+
+
+def test_c_entry_limits():
+    """Sizes, pitches and alignments whose offsets the kernels could not hold."""
+    lib = hip.lib
+    buf = torch.zeros(1 << 12, dtype=torch.uint8)
+    p = buf.data_ptr() + (-buf.data_ptr()) % 16
+    q = lambda rows, cols, a=p, b=p: lib.sm_fp8_quantize(p, 0, rows, cols, 1 << 31, 0, 0, a, p, b, p, None)
+    big = 65535 * 128 + 1
+    assert q(big, 1) != 0 and q(1, big) != 0 and q((1 << 31) - 1, 1) != 0 and q(1, (1 << 31) - 1) != 0 and q(1, 1, a=p + 8) != 0 and q(1, 1, b=p + 4) != 0
+    ok = [p, p, 0, 256, p, p, 0, 256, 0, 40, 6, 200, p, 0, 6, 0, None, 0, None]
+    m = lambda **k: lib.sm_fp8_matmul(*[k.get(f"a{i}", v) for i, v in enumerate(ok)])
+    for bad in (dict(a1=p + 1), dict(a5=p + 2), dict(a3=1 << 24), dict(a7=1 << 24), dict(a9=1 << 30), dict(a10=1 << 30, a14=1 << 30),
+                dict(a11=(1 << 31) - 1, a3=1 << 31, a7=1 << 31)):
+        assert m(**bad) != 0, bad
+    ok2 = [p, 0, 200, p, p, 0, 256, 40, 6, 200, p, 0, 6, p, 1 << 30, None]
+    f = lambda **k: lib.sm_fp8_linear(*[k.get(f"a{i}", v) for i, v in enumerate(ok2)])
+    for bad in (dict(a13=p + 8), dict(a14=100), dict(a2=199), dict(a6=128), dict(a3=p + 8), dict(a7=4, a3=p + 8), dict(a7=4, a6=250), dict(a7=4, a8=1 << 30, a12=1 << 30)):
+        assert f(**bad) != 0, bad

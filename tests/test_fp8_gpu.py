@@ -449,3 +449,51 @@ def test_products_on_a_side_stream_and_interleaved():
         for i in range(2):
             for res in got[i]:
                 assert all(torch.equal(a, b) for a, b in zip(res, want[i]))
+
+
+@pytest.mark.parametrize("M", [1, 7, 16, 17, 40])
+@pytest.mark.parametrize("K", [1, 129, 1100])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_linear_forward_of_views(M, K, dtype):
+    """Inputs that start at any element and whose rows lie further apart, on both sides of the fused rule's border."""
+    fp8 = _fp8()
+    big, w = _rand(M + 2, K + 9, 41, DT[dtype], spread=0.5), _rand(70, K, 42, spread=0.5)
+    w8 = fp8.fp8_quantize(w.cuda(), "tiles")
+    x = big[1:M + 1, 3:K + 3]
+    xv, wv = R.requantized(x), R.requantized(w, "tiles")
+    ref = xv @ wv.t()
+    for out_dtype in (torch.bfloat16, torch.float32):
+        y = fp8.linear_fp8_fwd(big.cuda()[1:M + 1, 3:K + 3], w8, out_dtype=out_dtype)
+        assert ((y.double().cpu() - ref).abs() <= R.matmul_bound(xv, wv, out_dtype, ref)).all()
+
+
+@pytest.mark.parametrize("M", [1, 16, 20, 40, 200])
+@pytest.mark.parametrize("bad", ["nan", "inf"])
+def test_linear_forward_long_rows_with_nan_and_inf(M, bad):
+    """K where a bfloat16 result takes the 8-bit instruction: a NaN or an infinity fills its own row with NaN and nothing else."""
+    fp8 = _fp8()
+    x, w = _rand(M, 2000, 51, torch.bfloat16, spread=0.5).cuda(), _rand(90, 2000, 52, spread=0.5).cuda()
+    w8 = fp8.fp8_quantize(w, "tiles")
+    y = fp8.linear_fp8_fwd(x, w8)
+    assert torch.isfinite(y).all()
+    x[M // 2, 1999] = float(bad)
+    yb = fp8.linear_fp8_fwd(x, w8)
+    keep = [i for i in range(M) if i != M // 2]
+    assert torch.isnan(yb[M // 2]).all() and torch.equal(yb[keep], y[keep])
+
+
+@pytest.mark.parametrize("M,N,K", [(1800, 1930, 1100), (4000, 4000, 1100), (4000, 3900, 520)])
+@pytest.mark.parametrize("scale", ["e8m0", "f32"])
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+def test_matmul_large_tiles(M, N, K, scale, out):
+    """Sizes that take the larger tiles, both arithmetics; the reference covers rows and columns at the tiles' borders."""
+    fp8 = _fp8()
+    for fmt, block in (("e4m3", "rows"), ("e5m2", "tiles")):
+        a, b, av, bv = _operands(fp8, M, N, K, block, fmt, scale, seed=60)
+        y = fp8.matmul_fp8(a, b, out_dtype=DT[out]).double().cpu()
+        rows = sorted({0, 15, 16, 63, 127, 128, 255, 256, 1000, M - 129, M - 128, M - 17, M - 2, M - 1})
+        ref = av[rows] @ bv.t()
+        assert ((y[rows] - ref).abs() <= R.matmul_bound(av[rows], bv, DT[out], ref)).all()
+        cols = sorted({0, 15, 63, 64, 127, 128, 255, 256, 1001, N - 130, N - 3, N - 1})
+        ref = av @ bv[cols].t()
+        assert ((y[:, cols] - ref).abs() <= R.matmul_bound(av, bv[cols], DT[out], ref)).all()
