@@ -11,18 +11,16 @@ that is not finite is not an error (finding out would synchronise): the coeffici
 from __future__ import annotations
 
 import math
-from array import array
-from operator import attrgetter
 
-import numpy as np
 import torch
 
 from . import hip, ops
 
-_TYPE_ID = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}           # SM_TYPE_*
-_SIZE = (4, 2, 2)
-_T = torch.Tensor
-_dtype = attrgetter("dtype")
+try:
+    from .. import _tensor_list
+except ImportError as e:
+    raise ImportError("stylemesh_amd/_tensor_list.so is missing or does not fit this torch: build it with "
+                      "`python -c 'import __graft_entry__ as g; g.build()'` or stylemesh_amd/csrc/build.sh") from e
 
 
 def _dense(t) -> bool:
@@ -36,40 +34,26 @@ def _dense(t) -> bool:
 
 
 class _Table:
-    """Pointers, element counts and types of a list of tensors as the library reads them. A list is walked once per attribute
-    with C-level maps: a model's few hundred tensors are handed over anew every step, and at a microsecond a tensor the walk
-    would be the operator's time."""
+    """Pointers, element counts and types of a list of tensors as the library reads them (csrc/tensor_list.cpp: one walk in
+    native code)."""
 
     def __init__(self, tensors, what):
-        kinds = set(map(_dtype, tensors))
-        if not kinds <= _TYPE_ID.keys():
-            raise ValueError(f"{what}: {[str(d) for d in kinds - _TYPE_ID.keys()]} (float32, bfloat16 or float16)")
-        if len(kinds) == 1:
-            self.types = array("i", [_TYPE_ID[kinds.pop()]]) * len(tensors)
-        else:
-            self.types = array("i", [_TYPE_ID[d] for d in map(_dtype, tensors)])
-        devices = set(map(_T.get_device, tensors))
-        if -1 in devices:
-            raise ValueError(f"{what}: device tensors only (there is no CPU form)")
-        if devices and devices != {torch.cuda.current_device()}:
-            raise ValueError(f"{what}: tensors on devices {sorted(devices)}, the current device is cuda:{torch.cuda.current_device()}")
-        self.contiguous = list(map(_T.is_contiguous, tensors))
-        if not all(self.contiguous):
-            for t, ok in zip(tensors, self.contiguous):
-                if not ok and not _dense(t):
+        self.packed, at, odd, device, self.contiguous = _tensor_list.pack(tensors)
+        if odd >= 0:
+            t = tensors[odd]
+            raise ValueError(f"{what}: entry {odd} is {t.dtype}, {t.layout} (strided float32, bfloat16 or float16)")
+        self.n = n = len(tensors)
+        if n:
+            if device == -1:
+                raise ValueError(f"{what}: device tensors only (there is no CPU form)")
+            if device != torch.cuda.current_device():
+                raise ValueError(f"{what}: tensors on {sorted(set(str(t.device) for t in tensors))}, the current device is "
+                                 f"cuda:{torch.cuda.current_device()}")
+        self.ptrs, self.numel, self.types = (at, at + 8 * n, at + 16 * n) if n else (None, None, None)
+        if not self.contiguous:
+            for t in tensors:
+                if not t.is_contiguous() and not _dense(t):
                     raise ValueError(f"{what}: strides {t.stride()} of {tuple(t.shape)} leave gaps or overlap")
-        self.ptrs = array("Q", map(_T.data_ptr, tensors))
-        self.numel = array("Q", map(_T.numel, tensors))
-        self.n = len(tensors)
-
-    def spans(self):
-        start = np.frombuffer(self.ptrs, dtype=np.uint64)
-        size = np.asarray(_SIZE, dtype=np.uint64)[np.frombuffer(self.types, dtype=np.int32)]
-        return start, start + np.frombuffer(self.numel, dtype=np.uint64) * size
-
-
-def _address(a) -> int | None:
-    return a.buffer_info()[0] if len(a) else None
 
 
 def _norm_kind(norm_type) -> int:
@@ -88,26 +72,10 @@ def _max_norm(v) -> float:
     return v
 
 
-def _refuse_overlap(g: _Table, o: _Table):
-    """What is written must be written once: an output that overlaps another output, or a gradient other than its own
-    (the same tensor listed twice, for one), has no defined result."""
-    if g.n == 0:
-        return
-    os_, oe = o.spans()
-    live = np.nonzero(oe > os_)[0]
-    if live.size == 0:
-        return
-    order = live[np.argsort(os_[live], kind="stable")]
-    ss, ee = os_[order], oe[order]
-    if (ee[:-1] > ss[1:]).any():
-        raise ValueError("two of the tensors to be written overlap (a gradient listed twice?)")
-    if o is g:
-        return
-    gs, ge = g.spans()
-    lo, hi = np.searchsorted(ee, gs, "right"), np.searchsorted(ss, ge, "left")      # outputs that gradient i touches
-    for i in np.nonzero((hi > lo) & (ge > gs))[0]:
-        if hi[i] - lo[i] > 1 or order[lo[i]] != i or os_[i] != gs[i]:
-            raise ValueError("an output overlaps a gradient that is not its own")
+# What is written must be written once: an output that overlaps another output, or a gradient other than its own (the same
+# tensor listed twice, for one), has no defined result.
+_WRONG = (None, "an output has not as many elements as its gradient", "an output that is its gradient must have its type",
+          "two of the tensors to be written overlap (a gradient listed twice?)", "an output overlaps a gradient that is not its own")
 
 
 class GradClip:
@@ -134,18 +102,15 @@ class GradClip:
             if type(None) in set(map(type, out)):
                 raise ValueError("an output is missing for a gradient that is there")
             o = self._o = _Table(out, "out")
-            if g.numel != o.numel:
-                raise ValueError("an output has not as many elements as its gradient")
-            if not (all(g.contiguous) and all(o.contiguous)):
-                for a, b, ca, cb in zip(grads, out, g.contiguous, o.contiguous):
-                    if not (ca and cb) and (a.shape != b.shape or a.stride() != b.stride()):
+            if not (g.contiguous and o.contiguous):
+                for a, b in zip(grads, out):
+                    if not (a.is_contiguous() and b.is_contiguous()) and (a.shape != b.shape or a.stride() != b.stride()):
                         raise ValueError(f"out {tuple(b.shape)} / {b.stride()} does not match its gradient {tuple(a.shape)} / {a.stride()}")
-            same = np.frombuffer(g.ptrs, dtype=np.uint64) == np.frombuffer(o.ptrs, dtype=np.uint64)
-            if (same & (np.frombuffer(g.numel, dtype=np.uint64) > 0) & (np.frombuffer(g.types, np.int32) != np.frombuffer(o.types, np.int32))).any():
-                raise ValueError("an output that is its gradient must have its type")
-        _refuse_overlap(g, o)
+        wrong = _tensor_list.check_outputs(g.packed, o.packed)
+        if wrong:
+            raise ValueError(_WRONG[wrong])
         self.device = torch.device("cuda", torch.cuda.current_device())
-        self._args = (_address(g.ptrs), _address(o.ptrs), _address(g.numel), _address(g.types), _address(o.types), g.n)
+        self._args = (g.ptrs, o.ptrs, g.numel, g.types, o.types, g.n)
         self._ws_bytes = ops.lib.sm_grad_norm_ws_bytes(g.n)
 
     def _result(self):
@@ -178,7 +143,7 @@ def grad_norm(grads, norm_type=2.0) -> torch.Tensor:
     t = _Table([g for g in grads if g is not None], "grads")
     ws = torch.empty(ops.lib.sm_grad_norm_ws_bytes(t.n), dtype=torch.uint8, device="cuda")
     out = torch.empty((), dtype=torch.float32, device="cuda")
-    hip.check(ops.lib.sm_grad_norm(_address(t.ptrs), _address(t.numel), _address(t.types), t.n, kind, ws.data_ptr(), ws.numel(),
+    hip.check(ops.lib.sm_grad_norm(t.ptrs, t.numel, t.types, t.n, kind, ws.data_ptr(), ws.numel(),
                                    out.data_ptr(), hip.stream()), "sm_grad_norm")
     return out
 

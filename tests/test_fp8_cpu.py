@@ -173,3 +173,53 @@ def test_c_entry_limits():
     f = lambda **k: lib.sm_fp8_linear(*[k.get(f"a{i}", v) for i, v in enumerate(ok2)])
     for bad in (dict(a13=p + 8), dict(a14=100), dict(a2=199), dict(a6=128), dict(a3=p + 8), dict(a7=4, a3=p + 8), dict(a7=4, a6=250), dict(a7=4, a8=1 << 30, a12=1 << 30)):
         assert f(**bad) != 0, bad
+
+
+def test_tensor_list_walk():
+    """The native walk over a list: what it reports of host tensors, odd types and non-tensors."""
+    import struct
+    from stylemesh_amd import _tensor_list as tl
+    packed, at, odd, device, contiguous = tl.pack([torch.ones(3), torch.ones(2, 5).half(), torch.ones(4).bfloat16()])
+    assert struct.unpack("3i", packed[48:]) == (0, 2, 1) and odd == -1 and device == -1 and contiguous and at
+    assert tl.pack([]) [2:] == (-1, -2, True)
+    assert tl.pack([torch.ones(3), torch.ones(3).double()])[2] == 1
+    assert tl.pack([torch.ones(3).to_sparse()])[2] == 0
+    for bad in ([1], [None], [torch.ones(1), "x"]):
+        with pytest.raises(ValueError):
+            tl.pack(bad)
+    for f in (lambda: tl.pack((torch.ones(1),)), lambda: tl.check_outputs(b"123", b""), lambda: tl.check_outputs([], b"")):
+        with pytest.raises(TypeError):
+            f()
+
+
+def test_outputs_of_a_list_against_every_pair():
+    """Overlap of outputs with each other and with other entries' inputs, against the quadratic definition."""
+    import random
+    import struct
+    from stylemesh_amd import _tensor_list as tl
+    rng = random.Random(3)
+    table = lambda e: b"".join(struct.pack(f"{len(e)}{c}", *[x[i] for x in e]) for i, c in enumerate("QQi"))
+    seen = set()
+    for _ in range(3000):
+        n = rng.randint(0, 5)
+        span = rng.choice([60, 400])
+        g = [(rng.randrange(span), rng.choice([0, 1, 5, 9]), rng.randrange(3)) for _ in range(n)]
+        o = [rng.choice([e, (rng.randrange(span), e[1], rng.randrange(3))]) for e in g]
+        if n and rng.random() < 0.05:
+            o[0] = (o[0][0], o[0][1] + 1, o[0][2])
+        end = lambda e: e[0] + e[1] * (2 if e[2] else 4)
+        hit = lambda a, b: a[1] and b[1] and a[0] < end(b) and b[0] < end(a)
+        want = 0
+        if any(a[1] != b[1] for a, b in zip(g, o)):
+            want = 1
+        elif any(a[1] and a[0] == b[0] and a[2] != b[2] for a, b in zip(g, o)):
+            want = 2
+        elif any(hit(o[i], o[j]) for i in range(n) for j in range(i)):
+            want = 3
+        elif any(hit(g[i], o[j]) and (i != j or g[i][0] != o[j][0]) for i in range(n) for j in range(n)):
+            want = 4
+        assert tl.check_outputs(table(g), table(o)) == want, (g, o)
+        t = table(g)
+        assert tl.check_outputs(t, t) == (3 if any(hit(g[i], g[j]) for i in range(n) for j in range(i)) else 0)
+        seen.add(want)
+    assert seen == {0, 1, 2, 3, 4}
