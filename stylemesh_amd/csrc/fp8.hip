@@ -222,31 +222,14 @@ __device__ __forceinline__ u32x2 codes8(const unsigned* d, int e, int fmt, bool 
     return u32x2{c.w[0], c.w[1]};
 }
 
-// One tile of ROWS rows x 128 columns per block: thread t holds rows RPT (t / 16) ... and columns 8 (t % 16) ... + 7 as they came
-// (all its loads in flight together; x is read once whatever is produced). Maxima are taken on the bits, two 16-bit
-// values per instruction: a block row's 16 lanes by data-parallel moves; columns in registers, then the wave's four row
-// groups, then the waves through LDS; tiles over everything. The scaled conversion instruction does the rest (about three
-// instructions an element where it was twenty). The transposed codes turn through a 128 x 128 byte LDS image whose 8-byte units are
-// swizzled by their column group, and both results leave as whole 128-byte lines.
-// Bound by HBM: rows * cols * (sizeof(x) + 1 per result); 8192^2 bf16 both ways 58 us (4.6 TB/s, a copy of that size 5.3).
-// Transposes and tiles take ROWS = 128, RPT = 4: with fewer tiles than CUs a thread's instructions bound it (1029 x 517 fp32 both
-// ways 9.1 us at RPT = 8, 7.2 at 4; no difference at 8192^2). Rows alone take RPT = 8, and 16 rows a block, RPT = 1, where
-// 128 leave too few blocks (16 x 4096 fp32: 8.2 -> 2.7 us).
-template <int T, bool TILES, bool Q, bool QT, int RPT, int ROWS>
-__global__ __launch_bounds__(16 * ROWS / RPT) void fp8_quantize_kernel(QuantArgs a) {
-    static_assert(ROWS == 128 || (!TILES && !QT), "column blocks need 128 rows");
-    static_assert(!QT || RPT == 4, "a dword of a column per thread");
-    constexpr int NT = 16 * ROWS / RPT, NW = NT / 64;
-    constexpr int ND = T == SM_TYPE_F32 ? 8 : 4;      // dwords of eight values
+// columns c0 ... c0 + 7 of rows r0 ... r0 + RPT - 1 as they are, all loads in flight together; zeros outside the matrix
+template <int T, int RPT, int ND>
+__device__ __forceinline__ void load_rows(const QuantArgs& a, int r0, int c0, unsigned (&d)[RPT][ND]) {
     constexpr int ES = T == SM_TYPE_F32 ? 4 : 2;
-    const int tid = threadIdx.x, rg = tid >> 4, cg = tid & 15, wave = tid >> 6;
-    const int tr = blockIdx.y * ROWS, tc = blockIdx.x * 128, c0 = tc + cg * 8;
-    const int top = a.fmt == SM_FP8_E4M3 ? 8 : 15;
-    unsigned d[RPT][ND];
     if (c0 + 8 <= a.cols) {
 #pragma unroll
         for (int i = 0; i < RPT; ++i) {
-            const int r = min(tr + rg * RPT + i, a.rows - 1);
+            const int r = min(r0 + i, a.rows - 1);
             const u32x4_u* p = reinterpret_cast<const u32x4_u*>(static_cast<const char*>(a.x) + ((size_t)r * a.stride + c0) * ES);
 #pragma unroll
             for (int q = 0; q < ND / 4; ++q) {
@@ -258,7 +241,7 @@ __global__ __launch_bounds__(16 * ROWS / RPT) void fp8_quantize_kernel(QuantArgs
     } else {
 #pragma unroll
         for (int i = 0; i < RPT; ++i) {
-            const int r = min(tr + rg * RPT + i, a.rows - 1);
+            const int r = min(r0 + i, a.rows - 1);
 #pragma unroll
             for (int j = 0; j < ND; ++j) {
                 const size_t at = (size_t)r * a.stride + c0;
@@ -271,13 +254,39 @@ __global__ __launch_bounds__(16 * ROWS / RPT) void fp8_quantize_kernel(QuantArgs
             }
         }
     }
+#pragma unroll
+    for (int i = 0; i < RPT; ++i)
+        if (r0 + i >= a.rows)
+#pragma unroll
+            for (int j = 0; j < ND; ++j) d[i][j] = 0;
+}
+
+// One tile of ROWS rows x 128 columns per block: thread t holds rows RPT (t / 16) ... and columns 8 (t % 16) ... + 7 as they came
+// (all its loads in flight together; x is read once whatever is produced). Maxima are taken on the bits, two 16-bit
+// values per instruction: a block row's 16 lanes by data-parallel moves; columns in registers, then the wave's four row
+// groups, then the waves through LDS; tiles over everything. The scaled conversion instruction does the rest (about three
+// instructions an element where it was twenty). The transposed codes turn through a 128 x 128 byte LDS image whose 8-byte units are
+// swizzled by their column group, and both results leave as whole 128-byte lines.
+// A column's exponent is found by one thread and read back by the sixteen that hold its rows (each on its own: 4096^2 bf16 both
+// ways 19.7 -> 17.6 us, the LDS reads and integer instructions of it).
+// Bound by HBM: rows * cols * (sizeof(x) + 1 per result); 8192^2 bf16 both ways 60 us, 4.5 TB/s (a copy of that size: 5.3).
+// Transposes and tiles take ROWS = 128, RPT = 4: with few tiles a thread's instructions bound it (1029 x 517 fp32 both
+// ways 9.1 us at RPT = 8, 7.2 at 4; no difference at 8192^2). Rows alone take RPT = 8, and 16 rows a block, RPT = 1, where
+// 128 leave too few blocks (16 x 4096 fp32: 8.2 -> 2.7 us).
+template <int T, bool TILES, bool Q, bool QT, int RPT, int ROWS>
+__device__ __forceinline__ void quantize_tile(const QuantArgs& a, const int bx, const int by) {
+    static_assert(ROWS == 128 || (!TILES && !QT), "column blocks need 128 rows");
+    static_assert(!QT || RPT == 4, "a dword of a column per thread");
+    constexpr int NT = 16 * ROWS / RPT, NW = NT / 64;
+    constexpr int ND = T == SM_TYPE_F32 ? 8 : 4;      // dwords of eight values
+    const int tid = threadIdx.x, rg = tid >> 4, cg = tid & 15, wave = tid >> 6;
+    const int tr = by * ROWS, tc = bx * 128, c0 = tc + cg * 8;
+    const int top = a.fmt == SM_FP8_E4M3 ? 8 : 15;
+    unsigned d[RPT][ND];
+    load_rows<T, RPT>(a, tr + rg * RPT, c0, d);
     unsigned rmax[RPT], all = 0;
 #pragma unroll
     for (int i = 0; i < RPT; ++i) {
-        if (tr + rg * RPT + i >= a.rows) {      // (behind the last row: zeros)
-#pragma unroll
-            for (int j = 0; j < ND; ++j) d[i][j] = 0;
-        }
         unsigned m = 0;
 #pragma unroll
         for (int j = 0; j < ND; ++j) m = mag_max<T>(m, mag<T>(d[i][j]));
@@ -299,6 +308,7 @@ __global__ __launch_bounds__(16 * ROWS / RPT) void fp8_quantize_kernel(QuantArgs
     }
     __shared__ unsigned red[NW][QT && !TILES ? 16 * ND : 1];
     __shared__ __align__(16) uint8_t img[QT ? 128 * 128 : 16];
+    __shared__ __align__(16) int exponent[QT && !TILES ? 128 : 4];
     const int cblocks = (a.cols + 127) >> 7, rblocks = (a.rows + 127) >> 7;
     int tile_e = 0;
     if constexpr (TILES) {
@@ -312,10 +322,10 @@ __global__ __launch_bounds__(16 * ROWS / RPT) void fp8_quantize_kernel(QuantArgs
         for (int w = 1; w < NW; ++w) m = max(m, red[w][0]);
         tile_e = block_exponent(mag_float<T>(m), top);
         if (tid < 4) {      // thread 0: this tile's byte; the row's / column's last tile also fills the dword's unused bytes
-            if (Q && (tid == 0 || ((int)blockIdx.x + tid < (cblocks + 3) / 4 * 4 && (int)blockIdx.x == cblocks - 1)))
-                a.qs[scale_at(blockIdx.x + tid, blockIdx.y, rblocks)] = tid == 0 ? (uint8_t)(tile_e + 127) : (uint8_t)127;
-            if (QT && (tid == 0 || ((int)blockIdx.y + tid < (rblocks + 3) / 4 * 4 && (int)blockIdx.y == rblocks - 1)))
-                a.qts[scale_at(blockIdx.y + tid, blockIdx.x, cblocks)] = tid == 0 ? (uint8_t)(tile_e + 127) : (uint8_t)127;
+            if (Q && (tid == 0 || (bx + tid < (cblocks + 3) / 4 * 4 && bx == cblocks - 1)))
+                a.qs[scale_at(bx + tid, by, rblocks)] = tid == 0 ? (uint8_t)(tile_e + 127) : (uint8_t)127;
+            if (QT && (tid == 0 || (by + tid < (rblocks + 3) / 4 * 4 && by == rblocks - 1)))
+                a.qts[scale_at(by + tid, bx, cblocks)] = tid == 0 ? (uint8_t)(tile_e + 127) : (uint8_t)127;
         }
     }
     if constexpr (Q) {
@@ -326,8 +336,8 @@ __global__ __launch_bounds__(16 * ROWS / RPT) void fp8_quantize_kernel(QuantArgs
             const int e = TILES ? tile_e : block_exponent(mag_float<T>(mag_both<T>(row16_max<T>(rmax[i]))), top);
             if (r < a.rows) {
                 *reinterpret_cast<u32x2*>(a.q + (size_t)r * pitch + c0) = codes8<T>(d[i], e, a.fmt, finite && !__any(e == -127));
-                if (!TILES && cg < 4 && (cg == 0 || ((int)blockIdx.x == cblocks - 1 && (int)blockIdx.x + cg < (cblocks + 3) / 4 * 4)))
-                    a.qs[scale_at(blockIdx.x + cg, r, a.rows)] = cg == 0 ? (uint8_t)(e + 127) : (uint8_t)127;
+                if (!TILES && cg < 4 && (cg == 0 || (bx == cblocks - 1 && bx + cg < (cblocks + 3) / 4 * 4)))
+                    a.qs[scale_at(bx + cg, r, a.rows)] = cg == 0 ? (uint8_t)(e + 127) : (uint8_t)127;
             }
         }
     }
@@ -348,20 +358,31 @@ __global__ __launch_bounds__(16 * ROWS / RPT) void fp8_quantize_kernel(QuantArgs
                 if ((tid & 63) < 16) red[wave][cg * ND + j] = m;
             }
             __syncthreads();
+            if (tid < 128) {      // a thread per column
+                unsigned m = 0;
+#pragma unroll
+                for (int w = 0; w < NW; ++w) m = mag_max<T>(m, red[w][T == SM_TYPE_F32 ? tid : tid >> 1]);
+                if constexpr (T != SM_TYPE_F32) m = tid & 1 ? m >> 16 : m & 0xffffu;
+                exponent[tid] = block_exponent(mag_float<T>(m), top);
+                if (tc + tid < a.cols) {
+                    a.qts[scale_at(by, tc + tid, a.cols)] = (uint8_t)(exponent[tid] + 127);
+                    if (by == rblocks - 1)      // the dword's unused bytes
+                        for (int k = rblocks; k & 3; ++k) a.qts[scale_at(k, tc + tid, a.cols)] = 127;
+                }
+            }
+            __syncthreads();
         }
+        int es[8];
+        bool plain = finite;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            es[j] = TILES ? tile_e : exponent[cg * 8 + j];
+            plain = plain && es[j] != -127;
+        }
+        plain = __all(plain);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {      // column j of the thread: its rows, packed as a row of the transpose
             const int cl = cg * 8 + j, dj = T == SM_TYPE_F32 ? j : j >> 1;
-            int e = tile_e;
-            if (!TILES) {
-                unsigned m = red[0][cg * ND + dj];
-#pragma unroll
-                for (int w = 1; w < NW; ++w) m = mag_max<T>(m, red[w][cg * ND + dj]);
-                if constexpr (T != SM_TYPE_F32) m = j & 1 ? m >> 16 : m & 0xffffu;
-                e = block_exponent(mag_float<T>(m), top);
-                if (tc + cl < a.cols && rg < 4 && (rg == 0 || ((int)blockIdx.y == rblocks - 1 && (int)blockIdx.y + rg < (rblocks + 3) / 4 * 4)))
-                    a.qts[scale_at(blockIdx.y + rg, tc + cl, a.cols)] = rg == 0 ? (uint8_t)(e + 127) : (uint8_t)127;
-            }
             constexpr int NR = T == SM_TYPE_F32 ? RPT : RPT / 2;
             unsigned t[NR];
 #pragma unroll
@@ -370,7 +391,7 @@ __global__ __launch_bounds__(16 * ROWS / RPT) void fp8_quantize_kernel(QuantArgs
                 else t[i] = j & 1 ? (d[2 * i][dj] >> 16) | (d[2 * i + 1][dj] & 0xffff0000u) : (d[2 * i][dj] & 0xffffu) | (d[2 * i + 1][dj] << 16);
             }
             *reinterpret_cast<unsigned*>(img + cl * 128 + ((rg >> 1) ^ cg) * 8 + (rg & 1) * 4) =
-                encode<T, 4>(t, e, a.fmt, finite && !__any(e == -127)).w[0];
+                encode<T, 4>(t, es[j], a.fmt, plain).w[0];
         }
         __syncthreads();
         const size_t pitch = (size_t)rblocks * 128;
@@ -382,6 +403,98 @@ __global__ __launch_bounds__(16 * ROWS / RPT) void fp8_quantize_kernel(QuantArgs
             if (g & 1) w = u32x4{w[2], w[3], w[0], w[1]};
             if (tc + cl < a.cols) *reinterpret_cast<u32x4*>(a.qt + (size_t)(tc + cl) * pitch + tr + p * 16) = w;
         }
+    }
+}
+
+template <int T, bool TILES, bool Q, bool QT, int RPT, int ROWS>
+__global__ __launch_bounds__(16 * ROWS / RPT) void fp8_quantize_kernel(QuantArgs a) {
+    quantize_tile<T, TILES, Q, QT, RPT, ROWS>(a, blockIdx.x, blockIdx.y);
+}
+
+// 128 rows x 32 columns of the transpose: thread t holds rows 2 (t / 4), + 1 and columns 8 (t % 4) ... + 7; as above otherwise. The
+// image's 32-byte units are swizzled by the column group.
+template <int T>
+__device__ __forceinline__ void quantize_columns(const QuantArgs& a, const int bx, const int by) {
+    constexpr int ND = T == SM_TYPE_F32 ? 8 : 4;
+    const int tid = threadIdx.x, rg = tid >> 2, cg = tid & 3, wave = tid >> 6;
+    const int tr = by * 128, tc = bx * 32;
+    const int top = a.fmt == SM_FP8_E4M3 ? 8 : 15;
+    const int rblocks = (a.rows + 127) >> 7;
+    unsigned d[2][ND];
+    load_rows<T, 2>(a, tr + rg * 2, tc + cg * 8, d);
+    unsigned all = 0;
+#pragma unroll
+    for (int j = 0; j < ND; ++j) all = mag_max<T>(all, mag_max<T>(mag<T>(d[0][j]), mag<T>(d[1][j])));
+    const bool finite = !__any(mag_both<T>(all) >= inf_bits<T>);
+    __shared__ unsigned red[4][4 * ND];
+    __shared__ __align__(16) int exponent[32];
+    __shared__ __align__(16) uint8_t img[32 * 128];
+#pragma unroll
+    for (int j = 0; j < ND; ++j) {
+        unsigned m = finite ? mag_max<T>(mag<T>(d[0][j]), mag<T>(d[1][j])) : mag_max<T>(mag_finite<T>(mag<T>(d[0][j])), mag_finite<T>(mag<T>(d[1][j])));
+#pragma unroll
+        for (int o = 4; o < 64; o <<= 1) m = mag_max<T>(m, (unsigned)__shfl_xor((int)m, o, 64));
+        if ((tid & 63) < 4) red[wave][cg * ND + j] = m;
+    }
+    __syncthreads();
+    if (tid < 32) {      // a thread per column
+        const int dj = T == SM_TYPE_F32 ? tid : tid >> 1;
+        unsigned m = mag_max<T>(mag_max<T>(red[0][dj], red[1][dj]), mag_max<T>(red[2][dj], red[3][dj]));
+        if constexpr (T != SM_TYPE_F32) m = tid & 1 ? m >> 16 : m & 0xffffu;
+        const int e = block_exponent(mag_float<T>(m), top);
+        exponent[tid] = e;
+        if (tc + tid < a.cols) {
+            a.qts[scale_at(by, tc + tid, a.cols)] = (uint8_t)(e + 127);
+            if (by == rblocks - 1)      // the dword's unused bytes
+                for (int k = rblocks; k & 3; ++k) a.qts[scale_at(k, tc + tid, a.cols)] = 127;
+        }
+    }
+    __syncthreads();
+    int es[8];
+    bool plain = finite;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        es[j] = exponent[cg * 8 + j];
+        plain = plain && es[j] != -127;
+    }
+    plain = __all(plain);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int cl = cg * 8 + j, dj = T == SM_TYPE_F32 ? j : j >> 1, e = es[j];
+        unsigned c;
+        if (plain) {
+            const float scale = __builtin_bit_cast(float, (unsigned)(e + 127) << 23);
+            unsigned v, w = 0;
+            if constexpr (T == SM_TYPE_F32) v = d[0][j], w = d[1][j];
+            else v = j & 1 ? (d[0][dj] >> 16) | (d[1][dj] & 0xffff0000u) : (d[0][dj] & 0xffffu) | (d[1][dj] << 16);
+            c = __builtin_bit_cast(unsigned, cvt_scaled<T, false>(v, w, scale, s16x2{0, 0}, a.fmt));
+        } else {
+            float v[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) v[i] = mag_float<T>(T == SM_TYPE_F32 ? d[i][j] : j & 1 ? d[i][dj] >> 16 : d[i][dj] & 0xffffu);
+            const float inv = inv_pow2(e);
+            c = (unsigned)cvt2<false>(v[0] * inv, v[1] * inv, 0, a.fmt);
+        }
+        *reinterpret_cast<uint16_t*>(img + cl * 128 + ((rg * 2) ^ (cg * 32))) = (uint16_t)c;
+    }
+    __syncthreads();
+    const int cl = tid >> 3, p = tid & 7;
+    if (tc + cl < a.cols)
+        *reinterpret_cast<u32x4*>(a.qt + (size_t)(tc + cl) * ((size_t)rblocks * 128) + tr + p * 16) =
+            *reinterpret_cast<const u32x4*>(img + cl * 128 + ((p * 16) ^ ((cl >> 3) * 32)));
+}
+
+// A small matrix row-wise and / or transposed: the first blocks_q blocks take 16 rows x 128 columns of the row-wise result, the others
+// 128 x 32 of the transpose. x is read twice, the second time from the caches.
+template <int T>
+__global__ __launch_bounds__(256) void fp8_quantize_small_kernel(QuantArgs a, int blocks_q) {
+    const int b = blockIdx.x;
+    if (b < blocks_q) {
+        const int cblocks = (a.cols + 127) >> 7;
+        quantize_tile<T, false, true, false, 1, 16>(a, b % cblocks, b / cblocks);
+    } else {
+        const int ct = (a.cols + 31) >> 5, t = b - blocks_q;
+        quantize_columns<T>(a, t % ct, t / ct);
     }
 }
 
@@ -1050,9 +1163,16 @@ static int launch_quantize(const QuantArgs& a, int tiles, hipStream_t s) {
         else if (q) hipLaunchKernelGGL((fp8_quantize_kernel<T, true, true, false, 4, 128>), grid, dim3(512), 0, s, a);
         else hipLaunchKernelGGL((fp8_quantize_kernel<T, true, false, true, 4, 128>), grid, dim3(512), 0, s, a);
     } else {
-        if (q && qt) hipLaunchKernelGGL((fp8_quantize_kernel<T, false, true, true, 4, 128>), grid, dim3(512), 0, s, a);
+        const size_t n = (size_t)grid.x * grid.y;
+        // fewer tiles of 128 x 128 than half the CUs: small blocks (fp32 / bf16, both ways, us: 300 x 300 6.1 -> 4.6 / 6.2 -> 4.1,
+        // 1029 x 517 6.5 -> 5.5 / 7.4 -> 5.2, 1024 x 1024 6.5 -> 5.8 / 6.0 -> 4.8; 2048 x 1536 9.1 -> 10.1 / 7.2 -> 8.3)
+        if (qt && n < 128) {
+            const unsigned bq = q ? cb * (unsigned)((a.rows + 15) / 16) : 0;
+            const unsigned bt = (unsigned)((a.cols + 31) / 32) * grid.y;
+            hipLaunchKernelGGL(fp8_quantize_small_kernel<T>, dim3(bq + bt), dim3(256), 0, s, a, (int)bq);
+        } else if (q && qt) hipLaunchKernelGGL((fp8_quantize_kernel<T, false, true, true, 4, 128>), grid, dim3(512), 0, s, a);
         else if (qt) hipLaunchKernelGGL((fp8_quantize_kernel<T, false, false, true, 4, 128>), grid, dim3(512), 0, s, a);
-        else if ((size_t)grid.x * grid.y >= 1024) hipLaunchKernelGGL((fp8_quantize_kernel<T, false, true, false, 8, 128>), grid, dim3(256), 0, s, a);
+        else if (n >= 1024) hipLaunchKernelGGL((fp8_quantize_kernel<T, false, true, false, 8, 128>), grid, dim3(256), 0, s, a);
         else hipLaunchKernelGGL((fp8_quantize_kernel<T, false, true, false, 1, 16>), dim3(cb, (unsigned)((a.rows + 15) / 16)), dim3(256), 0, s, a);
     }
     SM_LAUNCH_CHECK();
