@@ -497,3 +497,26 @@ def test_matmul_large_tiles(M, N, K, scale, out):
         cols = sorted({0, 15, 63, 64, 127, 128, 255, 256, 1001, N - 130, N - 3, N - 1})
         ref = av @ bv[cols].t()
         assert ((y[:, cols] - ref).abs() <= R.matmul_bound(av, bv[cols], DT[out], ref)).all()
+
+
+@pytest.mark.parametrize("rows,cols", [(1500, 1500), (129, 16400), (4300, 515)])
+@pytest.mark.parametrize("dtype,fmt", [("f32", "e4m3"), ("bf16", "e5m2"), ("f16", "e4m3")])
+def test_quantize_large_is_the_definition(rows, cols, dtype, fmt):
+    """Enough tiles for the large blocks' form; NaN, infinities, a zero row and column, and subnormal scales among them."""
+    fp8 = _fp8()
+    x = _rand(rows, cols, rows + cols, DT[dtype], spread=1.0)
+    x[7], x[:, 130] = 0, 0
+    x[100, 3], x[101, 140], x[128, cols - 1] = float("nan"), float("inf"), float("-inf")
+    if dtype == "f32":
+        x[:, 5] *= 2.0 ** -140
+        x[20] *= 2.0 ** -140
+    xd = x.cuda()
+    n, t = fp8.fp8_quantize_both(xd, "rows", fmt)
+    _check_matrix(n, x, "rows", fmt)
+    _check_matrix(t, x.t(), "rows", fmt)
+    q = fp8.fp8_quantize(xd, "rows", fmt, transpose=True)
+    assert torch.equal(q.data.view(torch.uint8), t.data.view(torch.uint8)) and torch.equal(q.scale, t.scale)
+    assert torch.equal(fp8.fp8_quantize(xd, "rows", fmt).data.view(torch.uint8), n.data.view(torch.uint8))
+    a, b = fp8.fp8_quantize_both(xd, "tiles", fmt)
+    _check_matrix(a, x, "tiles", fmt)
+    _check_matrix(b, x.t(), "tiles", fmt)
