@@ -4,7 +4,7 @@
 //
 //   norm = sqrt(sum over all tensors of g^2)  or  max |g|        coef = min(1, max_norm / (norm + 1e-6))        out = g coef
 //
-// Two kernels per 120 tensors: per-block partial sums, then the scaling pass, whose every block adds the same partial sums in
+// Two kernels per 200 tensors: per-block partial sums, then the scaling pass, whose every block adds the same partial sums in
 // the same order (a few KB from L2) instead of waiting for a third launch. No atomics: the norm has the same bits every time.
 // Sums are held in 64 bits: squares of fp32 gradients over- and underflow fp32 (|g| > 1.8e19, < 1e-23) where the norm
 // does not, and the 64-bit multiply-add runs at the fp32 rate on this chip - both kernels are bound by HBM.
@@ -20,17 +20,27 @@ typedef g_u32x4 g_u32x4_u __attribute__((aligned(2)));      // gradient views st
 typedef unsigned g_u32x2 __attribute__((ext_vector_type(2)));
 typedef g_u32x2 g_u32x2_u __attribute__((aligned(2)));
 
-constexpr int GN_TENSORS = 120;      // per launch: the table travels in the kernel arguments (no device copy to keep alive)
+// tensors per launch: the table travels in the kernel arguments (4 KB; no device copy to keep alive), 20 bytes a tensor. With 32
+// bytes and 120 tensors a list of 161 takes four launches instead of two (99 991 bf16 elements each: 35 -> 24 us).
+constexpr int GN_TENSORS = 200;
 constexpr int GN_PARTIALS = 1024;    // at most this many partial sums per call and launch
 
 struct GradTable {
-    const void* in[GN_TENSORS];
-    void* out[GN_TENSORS];
-    unsigned long long n[GN_TENSORS];
+    unsigned in_lo[GN_TENSORS], out_lo[GN_TENSORS];
+    unsigned hi[GN_TENSORS];         // bits 32 ... 47 of in and, above them, of out: device addresses have 48 bits
+    unsigned tail[GN_TENSORS];       // elements of the last chunk | SM_TYPE_* of in << 16 | of out << 20
     int first[GN_TENSORS + 1];       // first chunk of each tensor
-    unsigned type[GN_TENSORS];       // SM_TYPE_* of in, of out << 4
     int count;
-    int chunk_log2;                  // elements per chunk
+    int chunk_log2;                  // elements per chunk, at most 2^13
+};
+static_assert(sizeof(GradTable) <= 4096 - 48, "with the kernels' other arguments within 4 KB");
+
+// chunk c of the table's tensors
+struct Chunk {
+    const void* in;
+    void* out;
+    size_t begin, end;               // elements of the tensor
+    unsigned in_type, out_type;
 };
 
 __device__ __forceinline__ double gn_combine(double a, double b, bool inf) {
@@ -121,17 +131,29 @@ __device__ __forceinline__ int gn_tensor_of(const GradTable& t, int chunk) {
     return lo;
 }
 
+__device__ __forceinline__ Chunk gn_chunk(const GradTable& t, int c) {
+    const int k = gn_tensor_of(t, c);
+    const unsigned hi = t.hi[k], tail = t.tail[k];
+    Chunk r;
+    r.in = reinterpret_cast<const void*>((unsigned long long)t.in_lo[k] | (unsigned long long)(hi & 0xffffu) << 32);
+    r.out = reinterpret_cast<void*>((unsigned long long)t.out_lo[k] | (unsigned long long)(hi >> 16) << 32);
+    r.begin = (size_t)(c - t.first[k]) << t.chunk_log2;
+    r.end = r.begin + (c + 1 == t.first[k + 1] ? tail & 0xffffu : 1u << t.chunk_log2);
+    r.in_type = tail >> 16 & 15u;
+    r.out_type = tail >> 20;
+    return r;
+}
+
 template <bool INF>
 __global__ __launch_bounds__(256) void grad_norm_partial_kernel(GradTable t, double* __restrict__ partial) {
     double acc = 0.0;
     for (int c = blockIdx.x; c < t.first[t.count]; c += gridDim.x) {
-        const int k = gn_tensor_of(t, c);
-        const size_t begin = (size_t)(c - t.first[k]) << t.chunk_log2;
-        const size_t end = min((size_t)t.n[k], begin + ((size_t)1 << t.chunk_log2));
-        const void* in = t.in[k];
-        gn_typed(t.type[k] & 15u, [&](auto tc) {
+        const Chunk k = gn_chunk(t, c);
+        const void* in = k.in;
+        const size_t end = k.end;
+        gn_typed(k.in_type, [&](auto tc) {
             constexpr int T = decltype(tc)::value;
-            size_t i = begin + threadIdx.x * 8;
+            size_t i = k.begin + threadIdx.x * 8;
             // four rounds of loads in flight
             for (; i + 3 * 2048 + 8 <= end; i += 4 * 2048) {
                 Raw8<T> r[4];
@@ -181,16 +203,15 @@ __global__ __launch_bounds__(256) void grad_clip_kernel(GradTable t, const doubl
     if (in_place && coef == 1.f) return;                   // x 1 in place is what is there
     // from the last chunk backwards: the norm's pass ended there, and what it read last may still be in the 256 MB cache
     for (int c = t.first[t.count] - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x) {
-        const int k = gn_tensor_of(t, c);
-        const size_t begin = (size_t)(c - t.first[k]) << t.chunk_log2;
-        const size_t end = min((size_t)t.n[k], begin + ((size_t)1 << t.chunk_log2));
-        const void* in = t.in[k];
-        void* out = t.out[k];
-        gn_typed(t.type[k] & 15u, [&](auto tc) {
+        const Chunk k = gn_chunk(t, c);
+        const void* in = k.in;
+        void* out = k.out;
+        const size_t end = k.end;
+        gn_typed(k.in_type, [&](auto tc) {
             constexpr int T = decltype(tc)::value;
-            gn_typed(t.type[k] >> 4, [&](auto oc) {
+            gn_typed(k.out_type, [&](auto oc) {
                 constexpr int O = decltype(oc)::value;
-                size_t i = begin + threadIdx.x * 8;
+                size_t i = k.begin + threadIdx.x * 8;
                 for (; i + 2048 + 8 <= end; i += 2 * 2048) {
                     Raw8<T> r[2];
                     r[0].load(in, i);
@@ -227,13 +248,9 @@ __global__ __launch_bounds__(256) void grad_clip_kernel(GradTable t, const doubl
 
 namespace {
 
-// chunks of 4096 elements (two rounds of a block's 8-element loads) for short lists, 8192 for long ones, or as many more as
-// keep a launch's chunks within an int
-int chunk_log2_of(unsigned long long total) {
-    int l = total >= (8ull << 20) ? 13 : 12;
-    while ((total >> l) > (1ull << 28)) ++l;
-    return l;
-}
+// chunks of 4096 elements (two rounds of a block's 8-element loads) for short lists, 8192 for long ones (a call's 2^40 elements
+// are 2^27 chunks)
+int chunk_log2_of(unsigned long long total) { return total >= (8ull << 20) ? 13 : 12; }
 
 // table of tensors [first, first + count) of a call; returns its chunks
 int fill_table(sm::GradTable& t, const void* const* in, void* const* out, const size_t* numel, const int* types, const int* out_types,
@@ -242,12 +259,15 @@ int fill_table(sm::GradTable& t, const void* const* in, void* const* out, const 
     t.chunk_log2 = chunk_log2;
     t.first[0] = 0;
     for (int i = 0; i < count; ++i) {
-        t.in[i] = in[first + i];
-        t.out[i] = out == nullptr ? nullptr : out[first + i];
-        t.n[i] = numel[first + i];
+        const size_t n = numel[first + i];
+        const int chunks = (int)((n + ((size_t)1 << chunk_log2) - 1) >> chunk_log2);
+        const uint64_t a = n ? (uint64_t)in[first + i] : 0, b = n && out != nullptr ? (uint64_t)out[first + i] : 0;
         const int ty = types[first + i], oty = out_types == nullptr ? ty : out_types[first + i];
-        t.type[i] = (unsigned)(ty | (oty << 4));
-        t.first[i + 1] = t.first[i] + (int)((numel[first + i] + ((size_t)1 << chunk_log2) - 1) >> chunk_log2);
+        t.in_lo[i] = (unsigned)a;
+        t.out_lo[i] = (unsigned)b;
+        t.hi[i] = (unsigned)(a >> 32) | (unsigned)(b >> 32) << 16;
+        t.tail[i] = chunks ? (unsigned)(n - ((size_t)(chunks - 1) << chunk_log2)) | (unsigned)ty << 16 | (unsigned)oty << 20 : 0;
+        t.first[i + 1] = t.first[i] + chunks;
     }
     return t.first[count];
 }
@@ -256,7 +276,8 @@ int check_list(const void* const* in, const size_t* numel, const int* types, int
     *total = 0;
     if (n < 0 || (n > 0 && (in == nullptr || numel == nullptr || types == nullptr))) return (int)hipErrorInvalidValue;
     for (int i = 0; i < n; ++i) {
-        if (types[i] < 0 || types[i] > SM_TYPE_F16 || (numel[i] > 0 && in[i] == nullptr)) return (int)hipErrorInvalidValue;
+        if (types[i] < 0 || types[i] > SM_TYPE_F16 || (numel[i] > 0 && (in[i] == nullptr || (uint64_t)in[i] >> 48 != 0 || numel[i] >> 40)))
+            return (int)hipErrorInvalidValue;
         *total += numel[i];
     }
     return *total >> 40 ? (int)hipErrorInvalidValue : 0;
@@ -311,7 +332,7 @@ int sm_grad_clip(const void* const* grads, void* const* out, const size_t* numel
         return (int)hipErrorInvalidValue;
     int in_place = 1;
     for (int i = 0; i < n; ++i) {
-        if (out_types[i] < 0 || out_types[i] > SM_TYPE_F16 || (numel[i] > 0 && out[i] == nullptr)) return (int)hipErrorInvalidValue;
+        if (out_types[i] < 0 || out_types[i] > SM_TYPE_F16 || (numel[i] > 0 && (out[i] == nullptr || (uint64_t)out[i] >> 48 != 0))) return (int)hipErrorInvalidValue;
         if (numel[i] == 0) continue;
         if (out[i] != grads[i]) in_place = 0;
         else if (out_types[i] != types[i]) return (int)hipErrorInvalidValue;

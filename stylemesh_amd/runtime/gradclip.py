@@ -1,6 +1,6 @@
 """The global norm over many gradient tensors and clipping by it (``sm_grad_norm`` / ``sm_grad_clip``; csrc/gradnorm.hip):
 ``Trainer(gradient_clip_val=...)`` of the reference's pytorch_lightning (requirements.txt:76), i.e.
-``torch.nn.utils.clip_grad_norm_``, as two launches per 120 tensors with no host synchronisation.
+``torch.nn.utils.clip_grad_norm_``, as two launches per 200 tensors with no host synchronisation.
 
     norm = sqrt(sum of all squares) or max |g|;   out = g * min(1, max_norm / (norm + 1e-6))
 

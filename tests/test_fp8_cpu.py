@@ -223,3 +223,17 @@ def test_outputs_of_a_list_against_every_pair():
         assert tl.check_outputs(t, t) == (3 if any(hit(g[i], g[j]) for i in range(n) for j in range(i)) else 0)
         seen.add(want)
     assert seen == {0, 1, 2, 3, 4}
+
+
+def test_gradient_list_limits():
+    """Sizes and addresses the packed table could not hold come back as an error."""
+    import ctypes as C
+    lib = hip.lib
+    p = 1 << 20
+    arr = lambda t, *v: (t * len(v))(*v)
+    ty = arr(C.c_int, 0, 0)
+    norm = lambda ptrs, n: lib.sm_grad_norm(arr(C.c_void_p, *ptrs), arr(C.c_size_t, *n), ty, 2, 0, p, 1 << 14, p, None)
+    assert norm((p, 1 << 48), (4, 4)) != 0 and norm((p, p), (1 << 63, 1 << 63)) != 0 and norm((p, p), (1 << 40, 4)) != 0
+    clip = lambda out: lib.sm_grad_clip(arr(C.c_void_p, p, p), arr(C.c_void_p, *out), arr(C.c_size_t, 4, 4), ty, ty, 2, 0, 1.0, p, 1 << 14, p, None)
+    assert clip((p, 1 << 50)) != 0
+    assert lib.sm_grad_norm(arr(C.c_void_p, p, p), arr(C.c_size_t, 4, 4), ty, 2, 0, p + 4, 1 << 14, p, None) != 0
