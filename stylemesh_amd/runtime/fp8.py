@@ -19,6 +19,7 @@ FORMATS = {"e4m3": torch.float8_e4m3fn, "e5m2": torch.float8_e5m2}
 _FMT_ID = {torch.float8_e4m3fn: 0, torch.float8_e5m2: 1}                      # SM_FP8_*
 _TYPE_ID = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}           # SM_TYPE_*
 _MAX_DIM = 65535 * 128       # rows / columns of a matrix (the quantiser's grid)
+_NONE = (None, None)
 
 
 def _blocks(n: int) -> int:
@@ -48,7 +49,7 @@ class Fp8Matrix:
     (row, block kb) at [kb / 4, row, kb % 4], KB = ceil(cols / 128), S = rows or ceil(rows / 128) - or float32 scales [KB, S].
     The tensors are used as they are, no copy is taken."""
 
-    __slots__ = ("_data", "_scale", "_cols", "_block", "_ptrs", "_pitch", "_tiles", "_device", "_weight")
+    __slots__ = ("_data", "_scale", "_rows", "_cols", "_tiles", "_fmt", "_f32", "_ptrs", "_pitch", "_device")
 
     def __init__(self, data: torch.Tensor, scale: torch.Tensor, cols: int, block: str = "rows"):
         if block not in ("rows", "tiles"):
@@ -69,34 +70,24 @@ class Fp8Matrix:
             raise ValueError("scales must start on a 4-byte boundary")
         if scale.device != data.device:
             raise ValueError(f"codes on {data.device}, scales on {scale.device}")
-        self._set(data, scale, int(cols), block)
+        self._set(data, scale, data.shape[0], int(cols), int(block == "tiles"), _FMT_ID[data.dtype], int(scale.dtype == torch.float32),
+                  (data.data_ptr(), scale.data_ptr()), data.get_device())
 
-    def _set(self, data, scale, cols, block):
-        self._data, self._scale, self._cols, self._block = data, scale, cols, block
-        # what every call hands to the library, of the tensors this object keeps (and never exchanges: the properties are read-only)
-        self._ptrs, self._pitch, self._tiles = (data.data_ptr(), scale.data_ptr()), data.shape[1], int(block == "tiles")
-        self._device = data.get_device()                                                     # (-1: host)
-        self._weight = data.dtype == torch.float8_e4m3fn and scale.dtype == torch.uint8      # can be a layer's weight
-
-    @classmethod
-    def _made(cls, data, scale, cols, block):
-        """Of tensors this module laid out itself: nothing to check."""
-        m = cls.__new__(cls)
-        m._set(data, scale, cols, block)
-        return m
+    def _set(self, data, scale, rows, cols, tiles, fmt, f32, ptrs, device):
+        # what every call hands to the library, of the tensors this object keeps (and never exchanges: the properties are
+        # read-only); device -1: host
+        self._data, self._scale, self._rows, self._cols, self._tiles, self._fmt, self._f32 = data, scale, rows, cols, tiles, fmt, f32
+        self._ptrs, self._pitch, self._device = ptrs, -(-cols // BLOCK) * BLOCK, device
 
     data = property(lambda self: self._data)
     scale = property(lambda self: self._scale)
+    rows = property(lambda self: self._rows)
     cols = property(lambda self: self._cols)
-    block = property(lambda self: self._block)
-
-    @property
-    def rows(self) -> int:
-        return self.data.shape[0]
+    block = property(lambda self: "tiles" if self._tiles else "rows")
 
     @property
     def shape(self):
-        return (self.data.shape[0], self.cols)
+        return (self._rows, self._cols)
 
     @property
     def device(self):
@@ -165,7 +156,7 @@ def pack_scale_bytes(e: torch.Tensor) -> torch.Tensor:
 
 def _matrix_arg(x, what):
     """x: a matrix the kernels read or write; returns its row stride in elements"""
-    if not torch.is_tensor(x) or x.dim() != 2 or x.dtype not in _TYPE_ID:
+    if not isinstance(x, torch.Tensor) or x.dtype not in _TYPE_ID or x.dim() != 2:
         raise ValueError(f"{what} must be a float32 / bfloat16 / float16 matrix, got "
                          f"{(x.dtype, tuple(x.shape)) if torch.is_tensor(x) else type(x)}")
     (rows, cols), (sr, sc) = x.shape, x.stride()
@@ -179,10 +170,15 @@ def _matrix_arg(x, what):
     return sr if rows > 1 else max(cols, 1)
 
 
-def _empty(rows, cols, fmt, block, device):
-    kb, s = _blocks(cols), rows if block == "rows" else _blocks(rows)
-    return (torch.empty(rows, kb * BLOCK, dtype=FORMATS[fmt], device=device),
-            torch.empty(-(-kb // 4), s, 4, dtype=torch.uint8, device=device))
+_new = Fp8Matrix.__new__
+
+
+def _room(rows, cols, dtype, tiles, device):
+    """codes, scales and their pointers of a matrix to be written"""
+    kb = -(-cols // BLOCK)
+    q = torch.empty((rows, kb * BLOCK), dtype=dtype, device=device)
+    s = torch.empty(((kb + 3) // 4, -(-rows // BLOCK) if tiles else rows, 4), dtype=torch.uint8, device=device)
+    return q, s, (q.data_ptr(), s.data_ptr())
 
 
 def _quantize(x, block, fmt, plain, transpose):
@@ -191,15 +187,20 @@ def _quantize(x, block, fmt, plain, transpose):
         raise ValueError(f"fmt={fmt!r}: 'e4m3' or 'e5m2'")
     if block not in ("rows", "tiles"):
         raise ValueError(f"block={block!r}: 'rows' or 'tiles'")
-    rows, cols = x.shape
-    q, qs = _empty(rows, cols, fmt, block, x.device) if plain else (None, None)
-    qt, qts = _empty(cols, rows, fmt, block, x.device) if transpose else (None, None)
+    (rows, cols), device, dtype, tiles = x.shape, x.device, FORMATS[fmt], int(block == "tiles")
+    fid, n, t, np, tp = _FMT_ID[dtype], None, None, _NONE, _NONE
+    if plain:
+        q, s, np = _room(rows, cols, dtype, tiles, device)
+        n = _new(Fp8Matrix)
+        n._set(q, s, rows, cols, tiles, fid, 0, np, device.index)
+    if transpose:
+        q, s, tp = _room(cols, rows, dtype, tiles, device)
+        t = _new(Fp8Matrix)
+        t._set(q, s, cols, rows, tiles, fid, 0, tp, device.index)
     if rows and cols:
-        n = (q.data_ptr(), qs.data_ptr()) if plain else (None, None)
-        t = (qt.data_ptr(), qts.data_ptr()) if transpose else (None, None)
-        hip.check(ops.lib.sm_fp8_quantize(x.data_ptr(), _TYPE_ID[x.dtype], rows, cols, stride, _FMT_ID[FORMATS[fmt]],
-                                          int(block == "tiles"), *n, *t, hip.stream()), "sm_fp8_quantize")
-    return (Fp8Matrix._made(q, qs, cols, block) if plain else None, Fp8Matrix._made(qt, qts, rows, block) if transpose else None)
+        hip.check(ops.lib.sm_fp8_quantize(x.data_ptr(), _TYPE_ID[x.dtype], rows, cols, stride, fid, tiles, *np, *tp, hip.stream()),
+                  "sm_fp8_quantize")
+    return n, t
 
 
 def fp8_quantize(x: torch.Tensor, block: str = "rows", fmt: str = "e4m3", transpose: bool = False) -> Fp8Matrix:
@@ -242,15 +243,15 @@ def matmul_fp8(a: Fp8Matrix, b: Fp8Matrix, out: torch.Tensor | None = None, out_
     rounded once)."""
     if not isinstance(a, Fp8Matrix) or not isinstance(b, Fp8Matrix):
         raise ValueError("matmul_fp8 takes two Fp8Matrix operands")
-    if a.block != "rows":
+    if a._tiles:
         raise ValueError("the first operand needs row scales")
-    if b.data.dtype != torch.float8_e4m3fn:
+    if b._fmt != 0:
         raise ValueError("the second operand must be e4m3")
-    if a.cols != b.cols:
+    M, N, K = a._rows, b._rows, a._cols
+    if K != b._cols:
         raise ValueError(f"inner dimensions differ: {a.shape} x {b.shape}^T")
-    if a.scale.dtype != b.scale.dtype:
+    if a._f32 != b._f32:
         raise ValueError(f"one operand has {a.scale.dtype} scales, the other {b.scale.dtype}")
-    M, N, K = a.rows, b.rows, a.cols
     if max(M, N, K) > _MAX_DIM:
         raise ValueError(f"a dimension above {_MAX_DIM}")
     _check_device(a._device, b._device)
@@ -261,7 +262,7 @@ def matmul_fp8(a: Fp8Matrix, b: Fp8Matrix, out: torch.Tensor | None = None, out_
             out_dtype = torch.bfloat16
         if out_dtype not in _TYPE_ID:
             raise ValueError(f"out_dtype={out_dtype}: float32, bfloat16 or float16")
-        out, stride = torch.empty((M, N), dtype=out_dtype, device=a.data.device), max(N, 1)
+        out, stride = torch.empty((M, N), dtype=out_dtype, device=a._data.device), max(N, 1)
     else:
         stride = _matrix_arg(out, "out")
         if tuple(out.shape) != (M, N) or (out_dtype is not None and out.dtype != out_dtype):
@@ -271,14 +272,13 @@ def matmul_fp8(a: Fp8Matrix, b: Fp8Matrix, out: torch.Tensor | None = None, out_
     need = _matmul_ws(M, N, K)
     # (scratch of this call's own: two captured graphs, or two streams, never share slabs)
     ws = torch.empty(need, dtype=torch.uint8, device=a.device) if need else None
-    hip.check(ops.lib.sm_fp8_matmul(*a._ptrs, _FMT_ID[a.data.dtype], a._pitch, *b._ptrs, b._tiles, b._pitch,
-                                    int(a.scale.dtype == torch.float32), M, N, K, out.data_ptr(), _TYPE_ID[out.dtype],
-                                    stride, int(accumulate), None if ws is None else ws.data_ptr(), need, hip.stream()), "sm_fp8_matmul")
+    hip.check(ops.lib.sm_fp8_matmul(*a._ptrs, a._fmt, a._pitch, *b._ptrs, b._tiles, b._pitch, a._f32, M, N, K,
+                                    out.data_ptr(), _TYPE_ID[out.dtype], stride, int(accumulate), None if ws is None else ws.data_ptr(), need, hip.stream()), "sm_fp8_matmul")
     return out
 
 
 def _weight_arg(w, what="weight"):
-    if not isinstance(w, Fp8Matrix) or not w._weight:
+    if not isinstance(w, Fp8Matrix) or w._fmt != 0 or w._f32:
         raise ValueError(f"{what} must be an e4m3 Fp8Matrix with power-of-two scales")
     return w
 
@@ -290,8 +290,8 @@ def linear_fp8_fwd(x: torch.Tensor, weight: Fp8Matrix, out_dtype=None, keep_tran
     _weight_arg(weight)
     stride = _matrix_arg(x, "x")
     M, K = x.shape
-    if K != weight.cols:
-        raise ValueError(f"x has {K} columns, the weight {weight.cols}")
+    if K != weight._cols:
+        raise ValueError(f"x has {K} columns, the weight {weight._cols}")
     if out_dtype is None:
         out_dtype = x.dtype
     if keep_transposed:
@@ -300,7 +300,7 @@ def linear_fp8_fwd(x: torch.Tensor, weight: Fp8Matrix, out_dtype=None, keep_tran
     if out_dtype not in _TYPE_ID:
         raise ValueError(f"out_dtype={out_dtype}: float32, bfloat16 or float16")
     _check_device(weight._device)
-    N = weight.rows
+    N = weight._rows
     y = x.new_empty((M, N), dtype=out_dtype)
     if M and N:
         need = _linear_ws(M, N, K)
@@ -355,9 +355,8 @@ def linear_fp8_bwd(dy: torch.Tensor, x_t: Fp8Matrix | None, weight_t: Fp8Matrix 
             elif not accumulate:
                 dw.zero_()
         return dx, dw
-    none = (None, None)
-    wt, wt_args = (weight_t._ptrs, (weight_t._tiles, weight_t._pitch)) if weight_t is not None else (none, (0, 0))
-    xt, xt_args = (x_t._ptrs, (x_t._tiles, x_t._pitch)) if x_t is not None else (none, (0, 0))
+    wt, wt_args = (weight_t._ptrs, (weight_t._tiles, weight_t._pitch)) if weight_t is not None else (_NONE, (0, 0))
+    xt, xt_args = (x_t._ptrs, (x_t._tiles, x_t._pitch)) if x_t is not None else (_NONE, (0, 0))
     if weight_t is not None:
         dx = torch.empty((M, K), dtype=dx_dtype, device=dy.device)
     if x_t is not None and dw is None:
