@@ -807,8 +807,9 @@ __device__ __forceinline__ void matmul_tile(const MatmulArgs& g, int block) {
     }
 }
 
+// (two waves per SIMD: left alone, the 128 x 128 tile with fp32 scales per row takes 300 registers and one)
 template <int BM, int BN, int WM, int WN, int NST, int FA, int SC, bool NATIVE>
-__global__ __launch_bounds__(WM* WN * 64) void fp8_matmul_kernel(MatmulArgs g) {
+__global__ __launch_bounds__(WM* WN * 64, 2) void fp8_matmul_kernel(MatmulArgs g) {
     matmul_tile<BM, BN, WM, WN, NST, FA, SC, NATIVE>(g, blockIdx.x);
 }
 
@@ -1056,7 +1057,7 @@ __global__ __launch_bounds__(256) void fp8_matmul_empty_kernel(MatmulArgs g) {
 //                                        256 x 256   256 x 128   128 x 128   64 x 64
 //   8192^3      bf16 result, 2^e scales        413         488         499       921
 //   4096^3      bf16 result, 2^e scales         59          71          70       126
-//   4096^3      f16 result, fp32 scales        317         123         133       201   (256 x 256 spills)
+//   4096^3      f16 result, fp32 scales        317         121         133       201   (256 x 256 spills)
 //   2048^3      bf16 result, 2^e scales         33          22          17        18
 //   512 x 4096 x 4096, bf16                     50          31          26        18
 // A 256-row tile takes a CU, two 128 x 128 tiles share one: the large tile is taken where its rounds over the 256 CUs are not
@@ -1145,10 +1146,14 @@ static void launch_matmul(const MatmulArgs& g, int a_fmt, int splits, hipStream_
 
 template <bool NATIVE>
 static void launch_tile(int kind, const MatmulArgs& g, int a_fmt, bool f32s, int splits, hipStream_t s) {
-    if (kind == TILE_256 && !f32s) launch_matmul<256, 256, 2, 4, 2, NATIVE, false>(g, a_fmt, splits, s);
-    else if (kind == TILE_256) launch_matmul<256, 128, 4, 2, 3, NATIVE, true>(g, a_fmt, splits, s);
-    else if (kind == TILE_128 && !f32s) launch_matmul<128, 128, 2, 2, 2, NATIVE, false>(g, a_fmt, splits, s);
-    else if (kind == TILE_128) launch_matmul<128, 128, 2, 2, 2, NATIVE, true>(g, a_fmt, splits, s);
+    // Widened codes with power-of-two scales stay with the smaller tile: two blocks a CU convert and multiply in turn, and 256 x 256
+    // spills (us, 128 x 128 against 256 x 256, fp32 result: 8192 x 8192 x 1024 176 / 206, x 2048 284 / 306, x 4096 534 / 528;
+    // 4096 x 11008 x 4096 343 / 353; 4096 x 4096 x 4096 123 / 121, x 8192 230 / 220).
+    if (kind == TILE_256 && f32s) return launch_matmul<256, 128, 4, 2, 2, NATIVE, true>(g, a_fmt, splits, s);
+    if constexpr (NATIVE)
+        if (kind == TILE_256) return launch_matmul<256, 256, 2, 4, 2, NATIVE, false>(g, a_fmt, splits, s);
+    if (kind != TILE_64 && !f32s) launch_matmul<128, 128, 2, 2, 2, NATIVE, false>(g, a_fmt, splits, s);
+    else if (kind != TILE_64) launch_matmul<128, 128, 2, 2, 2, NATIVE, true>(g, a_fmt, splits, s);
     else if (!f32s) launch_matmul<64, 64, 2, 2, 4, NATIVE, false>(g, a_fmt, splits, s);
     else launch_matmul<64, 64, 2, 2, 4, NATIVE, true>(g, a_fmt, splits, s);
 }
