@@ -8,18 +8,22 @@ scratch) from torch's allocator and synchronises nothing. There is no autograd n
 """
 from __future__ import annotations
 
-from functools import lru_cache
-
 import torch
 
-from . import hip, ops
+from . import ops
+
+try:
+    from .. import _fp8_host
+except ImportError as e:
+    raise ImportError("stylemesh_amd/_fp8_host.so is missing or does not fit this torch: build it with "
+                      "`python -c 'import __graft_entry__ as g; g.build()'` or stylemesh_amd/csrc/build.sh") from e
 
 BLOCK = 128
 FORMATS = {"e4m3": torch.float8_e4m3fn, "e5m2": torch.float8_e5m2}
 _FMT_ID = {torch.float8_e4m3fn: 0, torch.float8_e5m2: 1}                      # SM_FP8_*
 _TYPE_ID = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}           # SM_TYPE_*
 _MAX_DIM = 65535 * 128       # rows / columns of a matrix (the quantiser's grid)
-_NONE = (None, None)
+_NO_MATRIX = (None, None, 0, 0)      # pointers, tiles?, pitch
 
 
 def _blocks(n: int) -> int:
@@ -154,11 +158,11 @@ def pack_scale_bytes(e: torch.Tensor) -> torch.Tensor:
     return e.view(e.shape[0], -1, 4).permute(1, 0, 2).contiguous()
 
 
-def _matrix_arg(x, what):
-    """x: a matrix the kernels read or write; returns its row stride in elements"""
-    if not isinstance(x, torch.Tensor) or x.dtype not in _TYPE_ID or x.dim() != 2:
-        raise ValueError(f"{what} must be a float32 / bfloat16 / float16 matrix, got "
-                         f"{(x.dtype, tuple(x.shape)) if torch.is_tensor(x) else type(x)}")
+def _check_matrix(x, what):
+    """x: a matrix the kernels read or write"""
+    if not isinstance(x, torch.Tensor) or x.dtype not in _TYPE_ID or x.dim() != 2 or x.layout != torch.strided or x.is_neg():
+        raise ValueError(f"{what} must be a strided float32 / bfloat16 / float16 matrix, got "
+                         f"{(x.dtype, tuple(x.shape), x.layout) if isinstance(x, torch.Tensor) else type(x)}")
     (rows, cols), (sr, sc) = x.shape, x.stride()
     # (the stride of a dimension of one element means nothing)
     if (cols > 1 and sc != 1) or (rows > 1 and sr < cols):
@@ -167,39 +171,38 @@ def _matrix_arg(x, what):
     if rows > _MAX_DIM or cols > _MAX_DIM:
         raise ValueError(f"{what}: {tuple(x.shape)} has a dimension above {_MAX_DIM}")
     _check_device(x.get_device())
-    return sr if rows > 1 else max(cols, 1)
+
+
+def _refuse(x, what):
+    """The native call would not take its arguments: says why."""
+    _check_matrix(x, what)
+    raise ValueError(f"{what} cannot be used: {x.dtype} {tuple(x.shape)}, strides {x.stride()} on {x.device}")
 
 
 _new = Fp8Matrix.__new__
 
 
-def _room(rows, cols, dtype, tiles, device):
-    """codes, scales and their pointers of a matrix to be written"""
-    kb = -(-cols // BLOCK)
-    q = torch.empty((rows, kb * BLOCK), dtype=dtype, device=device)
-    s = torch.empty(((kb + 3) // 4, -(-rows // BLOCK) if tiles else rows, 4), dtype=torch.uint8, device=device)
-    return q, s, (q.data_ptr(), s.data_ptr())
-
-
 def _quantize(x, block, fmt, plain, transpose):
-    stride = _matrix_arg(x, "x")
     if fmt not in FORMATS:
         raise ValueError(f"fmt={fmt!r}: 'e4m3' or 'e5m2'")
     if block not in ("rows", "tiles"):
         raise ValueError(f"block={block!r}: 'rows' or 'tiles'")
-    (rows, cols), device, dtype, tiles = x.shape, x.device, FORMATS[fmt], int(block == "tiles")
-    fid, n, t, np, tp = _FMT_ID[dtype], None, None, _NONE, _NONE
+    fid, tiles = _FMT_ID[FORMATS[fmt]], int(block == "tiles")
+    done = None
+    if isinstance(x, torch.Tensor) and x.is_cuda:
+        device = torch.cuda.current_device()
+        done = _fp8_host.quantize(x, fid, tiles, plain, transpose, device, ops.eager_stream())
+    if done is None:
+        _refuse(x, "x")
+    rows, cols, n, t = done
     if plain:
-        q, s, np = _room(rows, cols, dtype, tiles, device)
+        q, s, ptrs = n
         n = _new(Fp8Matrix)
-        n._set(q, s, rows, cols, tiles, fid, 0, np, device.index)
+        n._set(q, s, rows, cols, tiles, fid, 0, ptrs, device)
     if transpose:
-        q, s, tp = _room(cols, rows, dtype, tiles, device)
+        q, s, ptrs = t
         t = _new(Fp8Matrix)
-        t._set(q, s, cols, rows, tiles, fid, 0, tp, device.index)
-    if rows and cols:
-        hip.check(ops.lib.sm_fp8_quantize(x.data_ptr(), _TYPE_ID[x.dtype], rows, cols, stride, fid, tiles, *np, *tp, hip.stream()),
-                  "sm_fp8_quantize")
+        t._set(q, s, cols, rows, tiles, fid, 0, ptrs, device)
     return n, t
 
 
@@ -209,7 +212,7 @@ def fp8_quantize(x: torch.Tensor, block: str = "rows", fmt: str = "e4m3", transp
     finite magnitude into the format's range; x / scale is exact, the code is it rounded to nearest even. NaN stays NaN, an
     infinity becomes NaN (e4m3 has none) or infinity (e5m2); neither touches its neighbours' scale. (A magnitude from
     1.9375 * 2^127 on rounds up to 2^128, which fp32 does not hold: its products are infinite.)"""
-    n, t = _quantize(x, block, fmt, not transpose, transpose)
+    n, t = _quantize(x, block, fmt, not transpose, bool(transpose))
     return t if transpose else n
 
 
@@ -217,21 +220,6 @@ def fp8_quantize_both(x: torch.Tensor, block: str = "rows", fmt: str = "e4m3"):
     """(``fp8_quantize(x)``, ``fp8_quantize(x, transpose=True)``) from one read of ``x``: what a training step needs of its
     activations and output gradients (rows) and of its weights (tiles)."""
     return _quantize(x, block, fmt, True, True)
-
-
-@lru_cache(maxsize=4096)      # (a function of the sizes alone)
-def _matmul_ws(M, N, K):
-    return hip.lib.sm_fp8_matmul_ws_bytes(M, N, K)
-
-
-@lru_cache(maxsize=4096)
-def _linear_ws(M, N, K):
-    return hip.lib.sm_fp8_linear_ws_bytes(M, N, K)
-
-
-@lru_cache(maxsize=4096)
-def _backward_ws(M, N, K, dx, dw):
-    return hip.lib.sm_fp8_linear_backward_ws_bytes(M, N, K, int(dx), int(dw))
 
 
 def matmul_fp8(a: Fp8Matrix, b: Fp8Matrix, out: torch.Tensor | None = None, out_dtype=None, accumulate: bool = False) -> torch.Tensor:
@@ -262,19 +250,14 @@ def matmul_fp8(a: Fp8Matrix, b: Fp8Matrix, out: torch.Tensor | None = None, out_
             out_dtype = torch.bfloat16
         if out_dtype not in _TYPE_ID:
             raise ValueError(f"out_dtype={out_dtype}: float32, bfloat16 or float16")
-        out, stride = torch.empty((M, N), dtype=out_dtype, device=a._data.device), max(N, 1)
+        dtype = _TYPE_ID[out_dtype]
     else:
-        stride = _matrix_arg(out, "out")
+        _check_matrix(out, "out")
         if tuple(out.shape) != (M, N) or (out_dtype is not None and out.dtype != out_dtype):
             raise ValueError(f"out is {out.dtype} {tuple(out.shape)}, the product {out_dtype or out.dtype} {(M, N)}")
-    if M == 0 or N == 0:
-        return out
-    need = _matmul_ws(M, N, K)
-    # (scratch of this call's own: two captured graphs, or two streams, never share slabs)
-    ws = torch.empty(need, dtype=torch.uint8, device=a.device) if need else None
-    hip.check(ops.lib.sm_fp8_matmul(*a._ptrs, a._fmt, a._pitch, *b._ptrs, b._tiles, b._pitch, a._f32, M, N, K,
-                                    out.data_ptr(), _TYPE_ID[out.dtype], stride, int(accumulate), None if ws is None else ws.data_ptr(), need, hip.stream()), "sm_fp8_matmul")
-    return out
+        dtype = 0
+    return _fp8_host.matmul(*a._ptrs, a._fmt, a._pitch, *b._ptrs, b._tiles, b._pitch, a._f32, M, N, K, out, dtype, bool(accumulate),
+                            a._device, ops.eager_stream())
 
 
 def _weight_arg(w, what="weight"):
@@ -288,26 +271,21 @@ def linear_fp8_fwd(x: torch.Tensor, weight: Fp8Matrix, out_dtype=None, keep_tran
     (default: x's). ``keep_transposed``: returns (y, q(x^T)), the second for ``linear_fp8_bwd``'s weight gradient - quantised
     from the same read of x."""
     _weight_arg(weight)
-    stride = _matrix_arg(x, "x")
-    M, K = x.shape
-    if K != weight._cols:
-        raise ValueError(f"x has {K} columns, the weight {weight._cols}")
-    if out_dtype is None:
-        out_dtype = x.dtype
+    if out_dtype is not None and out_dtype not in _TYPE_ID:
+        raise ValueError(f"out_dtype={out_dtype}: float32, bfloat16 or float16")
     if keep_transposed:
         n, t = _quantize(x, "rows", "e4m3", True, True)
-        return matmul_fp8(n, weight, out_dtype=out_dtype), t
-    if out_dtype not in _TYPE_ID:
-        raise ValueError(f"out_dtype={out_dtype}: float32, bfloat16 or float16")
-    _check_device(weight._device)
-    N = weight._rows
-    y = x.new_empty((M, N), dtype=out_dtype)
-    if M and N:
-        need = _linear_ws(M, N, K)
-        ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None      # of this call's own, as matmul_fp8's
-        hip.check(ops.lib.sm_fp8_linear(x.data_ptr(), _TYPE_ID[x.dtype], stride, *weight._ptrs,
-                                    weight._tiles, weight._pitch, M, N, K, y.data_ptr(), _TYPE_ID[out_dtype], N,
-                                    None if ws is None else ws.data_ptr(), need, hip.stream()), "sm_fp8_linear")
+        return matmul_fp8(n, weight, out_dtype=x.dtype if out_dtype is None else out_dtype), t
+    y = None
+    if weight._device >= 0 and weight._device == torch.cuda.current_device():
+        y = _fp8_host.linear(x, *weight._ptrs, weight._tiles, weight._pitch, weight._rows, weight._cols,
+                             -1 if out_dtype is None else _TYPE_ID[out_dtype], weight._device, ops.eager_stream())
+    if y is None:
+        _check_matrix(x, "x")
+        if x.shape[1] != weight._cols:
+            raise ValueError(f"x has {x.shape[1]} columns, the weight {weight._cols}")
+        _check_device(weight._device)
+        _refuse(x, "x")
     return y
 
 
@@ -318,7 +296,7 @@ def linear_fp8_bwd(dy: torch.Tensor, x_t: Fp8Matrix | None, weight_t: Fp8Matrix 
     dw [N, K] = q(dy^T) q(x^T)^T in float32 from ``x_t`` = [K, M] (``keep_transposed``). ``fmt``: format of the gradient's
     codes. ``dw`` / ``accumulate``: write into, or add to, an existing float32 gradient. Either of ``x_t`` / ``weight_t`` may be
     None: that gradient is not computed and None is returned in its place."""
-    stride = _matrix_arg(dy, "dy")
+    _check_matrix(dy, "dy")
     M, N = dy.shape
     if x_t is None and weight_t is None:
         raise ValueError("nothing to compute: both x_t and weight_t are None")
@@ -331,7 +309,7 @@ def linear_fp8_bwd(dy: torch.Tensor, x_t: Fp8Matrix | None, weight_t: Fp8Matrix 
             raise ValueError(f"dy has {N} columns, weight_t {weight_t.cols}")
         if dx_dtype is None:
             dx_dtype = dy.dtype
-        if dx_dtype not in _TYPE_ID:
+        elif dx_dtype not in _TYPE_ID:
             raise ValueError(f"dx_dtype={dx_dtype}: float32, bfloat16 or float16")
     if x_t is not None:
         if _weight_arg(x_t, "x_t").cols != M or x_t.rows != K:
@@ -344,7 +322,8 @@ def linear_fp8_bwd(dy: torch.Tensor, x_t: Fp8Matrix | None, weight_t: Fp8Matrix 
         raise ValueError("dw given, but no x_t to compute it from")
     if K > _MAX_DIM:
         raise ValueError(f"a dimension above {_MAX_DIM}")
-    dw_stride = _matrix_arg(dw, "dw") if dw is not None else max(K, 1)
+    if dw is not None:
+        _check_matrix(dw, "dw")
     _check_device(None if weight_t is None else weight_t._device, None if x_t is None else x_t._device)
     if not (M and N and K):      # a gradient without elements, or a sum without terms
         if weight_t is not None:
@@ -355,16 +334,8 @@ def linear_fp8_bwd(dy: torch.Tensor, x_t: Fp8Matrix | None, weight_t: Fp8Matrix 
             elif not accumulate:
                 dw.zero_()
         return dx, dw
-    wt, wt_args = (weight_t._ptrs, (weight_t._tiles, weight_t._pitch)) if weight_t is not None else (_NONE, (0, 0))
-    xt, xt_args = (x_t._ptrs, (x_t._tiles, x_t._pitch)) if x_t is not None else (_NONE, (0, 0))
-    if weight_t is not None:
-        dx = torch.empty((M, K), dtype=dx_dtype, device=dy.device)
-    if x_t is not None and dw is None:
-        dw = torch.empty((N, K), dtype=torch.float32, device=dy.device)
-    need = _backward_ws(M, N, K, weight_t is not None, x_t is not None)
-    ws = torch.empty(need, dtype=torch.uint8, device=dy.device)      # of this call's own, as matmul_fp8's
-    hip.check(ops.lib.sm_fp8_linear_backward(
-        dy.data_ptr(), _TYPE_ID[dy.dtype], stride, _FMT_ID[FORMATS[fmt]], M, N, K, *wt, *wt_args, *xt, *xt_args,
-        None if dx is None else dx.data_ptr(), 0 if dx is None else _TYPE_ID[dx_dtype], K, None if dw is None else dw.data_ptr(), dw_stride,
-        int(accumulate), ws.data_ptr(), need, hip.stream()), "sm_fp8_linear_backward")
-    return dx, dw
+    wt = (*weight_t._ptrs, weight_t._tiles, weight_t._pitch) if weight_t is not None else _NO_MATRIX
+    xt = (*x_t._ptrs, x_t._tiles, x_t._pitch) if x_t is not None else _NO_MATRIX
+    done = _fp8_host.backward(dy, _FMT_ID[FORMATS[fmt]], K, *wt, *xt, -1 if dx_dtype is None else _TYPE_ID[dx_dtype], dw, bool(accumulate),
+                              dy.get_device(), ops.eager_stream())
+    return done if done is not None else _refuse(dy, "dy")

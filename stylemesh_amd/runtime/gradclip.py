@@ -125,14 +125,14 @@ class GradClip:
         kind = _norm_kind(norm_type)
         out, ws = self._result()
         gp, _, numel, types, _, n = self._args
-        hip.check(ops.lib.sm_grad_norm(gp, numel, types, n, kind, ws.data_ptr(), self._ws_bytes, out.data_ptr(), hip.stream()), "sm_grad_norm")
+        hip.check(ops.lib.sm_grad_norm(gp, numel, types, n, kind, ws.data_ptr(), self._ws_bytes, out.data_ptr(), ops.eager_stream()), "sm_grad_norm")
         return out
 
     def clip(self, max_norm, norm_type=2.0) -> torch.Tensor:
         """Clips, and returns the norm BEFORE clipping (float32 device scalar)."""
         kind, max_norm = _norm_kind(norm_type), _max_norm(max_norm)
         out, ws = self._result()
-        hip.check(ops.lib.sm_grad_clip(*self._args, kind, max_norm, ws.data_ptr(), self._ws_bytes, out.data_ptr(), hip.stream()), "sm_grad_clip")
+        hip.check(ops.lib.sm_grad_clip(*self._args, kind, max_norm, ws.data_ptr(), self._ws_bytes, out.data_ptr(), ops.eager_stream()), "sm_grad_clip")
         return out
 
 
@@ -144,7 +144,7 @@ def grad_norm(grads, norm_type=2.0) -> torch.Tensor:
     ws = torch.empty(ops.lib.sm_grad_norm_ws_bytes(t.n), dtype=torch.uint8, device="cuda")
     out = torch.empty((), dtype=torch.float32, device="cuda")
     hip.check(ops.lib.sm_grad_norm(t.ptrs, t.numel, t.types, t.n, kind, ws.data_ptr(), ws.numel(),
-                                   out.data_ptr(), hip.stream()), "sm_grad_norm")
+                                   out.data_ptr(), ops.eager_stream()), "sm_grad_norm")
     return out
 
 

@@ -47,6 +47,14 @@ class KernelTimer:
 CONV_TIMER: KernelTimer | None = None   # set by bench.py; None = no instrumentation
 
 
+def eager_stream() -> int:
+    """``hip.stream()`` for calls that allocate their own results: a step that is being recorded with one of them in it is not
+    replayed (its pointers would be those of this call)."""
+    if lib is not hip.lib:
+        lib.problem = "a call that allocates its results"
+    return hip.stream()
+
+
 def _hbm_timed(name, nbytes, fn):
     """The step's HBM-bound kernels under the same per-launch events as the convs (tag 'hbm:<name>', work = algorithmic
     bytes): bench.py prices them against the measured copy rate (roofline_hbm)."""

@@ -520,3 +520,43 @@ def test_quantize_large_is_the_definition(rows, cols, dtype, fmt):
     a, b = fp8.fp8_quantize_both(xd, "tiles", fmt)
     _check_matrix(a, x, "tiles", fmt)
     _check_matrix(b, x.t(), "tiles", fmt)
+
+
+def test_a_recorded_step_with_these_calls_is_not_replayed():
+    """They allocate their results: a recording must not come back with this call's pointers."""
+    fp8 = _fp8()
+    from stylemesh_amd.runtime import gradclip, hip, ops, program
+    x = torch.ones(4, 200, device="cuda")
+    w8 = fp8.fp8_quantize(torch.ones(8, 200, device="cuda"), "tiles")
+    q, t = fp8.fp8_quantize_both(x)
+    for call in (lambda: fp8.fp8_quantize(x), lambda: fp8.matmul_fp8(q, w8), lambda: fp8.linear_fp8_fwd(x, w8),
+                 lambda: fp8.linear_fp8_bwd(torch.ones(4, 8, device="cuda"), t, w8.transposed()), lambda: gradclip.clip_grad_norm([x], 1e9),
+                 lambda: gradclip.grad_norm([x])):
+        ops.lib = rec = program.Recorder()
+        try:
+            call()
+        finally:
+            ops.lib = hip.lib
+        assert rec.problem is not None
+
+
+def test_refusals_on_the_device():
+    """What the native calls do not take comes back as a ValueError that names it, and nothing is written."""
+    fp8 = _fp8()
+    x = torch.ones(8, 256, device="cuda")
+    w8 = fp8.fp8_quantize(torch.ones(16, 256, device="cuda"), "tiles")
+    q = fp8.fp8_quantize(x)
+    out = torch.zeros(8, 16, device="cuda")
+    dy, (_, xt), wt = torch.ones(8, 16, device="cuda"), fp8.fp8_quantize_both(x), w8.transposed()
+    for f in (lambda: fp8.fp8_quantize(x.t()), lambda: fp8.fp8_quantize(x[:, ::2]), lambda: fp8.fp8_quantize(x[0]), lambda: fp8.fp8_quantize(x.double()),
+              lambda: fp8.fp8_quantize(x[:1].expand(8, 256)), lambda: fp8.fp8_quantize(x.to_sparse()), lambda: fp8.fp8_quantize_both(x.cpu()),
+              lambda: fp8.linear_fp8_fwd(x.t(), w8), lambda: fp8.linear_fp8_fwd(x[:, :255], w8), lambda: fp8.linear_fp8_fwd(x.cpu(), w8),
+              lambda: fp8.linear_fp8_fwd(x.int(), w8), lambda: fp8.linear_fp8_fwd(x, w8, out_dtype=torch.int32), lambda: fp8.linear_fp8_fwd(None, w8),
+              lambda: fp8.matmul_fp8(q, w8, out=out.t()), lambda: fp8.matmul_fp8(q, w8, out=out[:7]), lambda: fp8.matmul_fp8(q, w8, out=out.cpu()),
+              lambda: fp8.matmul_fp8(q, w8, out=out, out_dtype=torch.float16), lambda: fp8.matmul_fp8(q, w8, out=out[:1].expand(8, 16)),
+              lambda: fp8.linear_fp8_bwd(dy.t(), xt, wt), lambda: fp8.linear_fp8_bwd(dy[:7], xt, wt), lambda: fp8.linear_fp8_bwd(dy, xt, wt, dw=out),
+              lambda: fp8.linear_fp8_bwd(dy, xt, wt, dw=torch.zeros(256, 16, device="cuda").t()), lambda: fp8.linear_fp8_bwd(dy, xt, wt, dx_dtype=torch.int8)):
+        with pytest.raises(ValueError):
+            f()
+    torch.cuda.synchronize()
+    assert not out.any()
