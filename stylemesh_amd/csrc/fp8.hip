@@ -1152,10 +1152,15 @@ static void launch_tile(int kind, const MatmulArgs& g, int a_fmt, bool f32s, int
     if (kind == TILE_256 && f32s) return launch_matmul<256, 128, 4, 2, 2, NATIVE, true>(g, a_fmt, splits, s);
     if constexpr (NATIVE)
         if (kind == TILE_256) return launch_matmul<256, 256, 2, 4, 2, NATIVE, false>(g, a_fmt, splits, s);
+    // A ring of four stages lets two blocks share a CU, one of three stages three: taken where two a CU would leave a second round
+    // (1500 x 1500 x 700 fp32 12.6 -> 10.8 us, 1600 x 1600 x 2000 21.4 -> 18.8; below 512 tiles +-2 %, 128 x 8192 x 4096 12.4 -> 13.6).
+    const bool three = (long long)((g.M + 63) / 64) * ((g.N + 63) / 64) * splits > 512;
     if (kind != TILE_64 && !f32s) launch_matmul<128, 128, 2, 2, 2, NATIVE, false>(g, a_fmt, splits, s);
     else if (kind != TILE_64) launch_matmul<128, 128, 2, 2, 2, NATIVE, true>(g, a_fmt, splits, s);
-    else if (!f32s) launch_matmul<64, 64, 2, 2, 4, NATIVE, false>(g, a_fmt, splits, s);
-    else launch_matmul<64, 64, 2, 2, 4, NATIVE, true>(g, a_fmt, splits, s);
+    else if (!three && !f32s) launch_matmul<64, 64, 2, 2, 4, NATIVE, false>(g, a_fmt, splits, s);
+    else if (!three) launch_matmul<64, 64, 2, 2, 4, NATIVE, true>(g, a_fmt, splits, s);
+    else if (!f32s) launch_matmul<64, 64, 2, 2, 3, NATIVE, false>(g, a_fmt, splits, s);
+    else launch_matmul<64, 64, 2, 2, 3, NATIVE, true>(g, a_fmt, splits, s);
 }
 
 template <int T>
@@ -1368,15 +1373,19 @@ int sm_fp8_linear_backward(const void* dy, int dy_type, size_t dy_stride, int fm
     if (const int e = sm_fp8_quantize(dy, dy_type, M, N, dy_stride, fmt, 0, dx ? w : nullptr, dx ? w + qs : nullptr, dw ? w + t : nullptr,
                                       dw ? w + ts : nullptr, stream))
         return e;
-    // two products of small tiles, neither of which fills the chip: one launch (1029 x 517 x 1283: 8.3 + 8.2 -> 12.8 us)
+    // two products of small tiles, neither of which fills the chip: one launch (1029 x 517 x 1283: 8.3 + 8.2 -> 10.7 us, of which a
+    // ring of three stages - three blocks a CU instead of two - is worth 1.1 and the order below 1)
     if (dx && dw && px.kind == sm::TILE_64 && pw.kind == sm::TILE_64 && px.splits == 1 && pw.splits == 1 && !sm::native_result(dx_type, gx.KB)) {
-        const int b0 = ((gx.M + 63) / 64) * ((gx.N + 63) / 64), b1 = ((gw.M + 63) / 64) * ((gw.N + 63) / 64);
+        // the one with more blocks of K first: its tiles run longest, and the last tiles to start should be short
+        const bool swap = gw.KB > gx.KB;
+        const sm::MatmulArgs &g0 = swap ? gw : gx, &g1 = swap ? gx : gw;
+        const int b0 = ((g0.M + 63) / 64) * ((g0.N + 63) / 64), b1 = ((g1.M + 63) / 64) * ((g1.N + 63) / 64);
         if (fmt == SM_FP8_E4M3)
-            hipLaunchKernelGGL((sm::fp8_matmul_pair_kernel<64, 64, 2, 2, 4, SM_FP8_E4M3, sm::SCALE_POW2, false>), dim3((unsigned)(b0 + b1)), dim3(256),
-                               0, s, gx, gw, b0);
+            hipLaunchKernelGGL((sm::fp8_matmul_pair_kernel<64, 64, 2, 2, 3, SM_FP8_E4M3, sm::SCALE_POW2, false>), dim3((unsigned)(b0 + b1)), dim3(256),
+                               0, s, g0, g1, b0);
         else
-            hipLaunchKernelGGL((sm::fp8_matmul_pair_kernel<64, 64, 2, 2, 4, SM_FP8_E5M2, sm::SCALE_POW2, false>), dim3((unsigned)(b0 + b1)), dim3(256),
-                               0, s, gx, gw, b0);
+            hipLaunchKernelGGL((sm::fp8_matmul_pair_kernel<64, 64, 2, 2, 3, SM_FP8_E5M2, sm::SCALE_POW2, false>), dim3((unsigned)(b0 + b1)), dim3(256),
+                               0, s, g0, g1, b0);
         SM_LAUNCH_CHECK();
         return 0;
     }

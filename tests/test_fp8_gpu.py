@@ -560,3 +560,30 @@ def test_refusals_on_the_device():
             f()
     torch.cuda.synchronize()
     assert not out.any()
+
+
+@pytest.mark.parametrize("M,N,K", [(1500, 1540, 300), (200, 12000, 1300), (1500, 1500, 1)])
+@pytest.mark.parametrize("scale,block", [("e8m0", "rows"), ("f32", "rows"), ("f32", "tiles")])
+def test_matmul_more_small_tiles_than_two_a_cu(M, N, K, scale, block):
+    fp8 = _fp8()
+    a, b, av, bv = _operands(fp8, M, N, K, block, "e4m3", scale, seed=70)
+    ref = av @ bv.t()
+    for dt in (torch.float32, torch.bfloat16):
+        out = fp8.matmul_fp8(a, b, out_dtype=dt)
+        assert ((out.double().cpu() - ref).abs() <= R.matmul_bound(av, bv, dt, ref)).all()
+
+
+@pytest.mark.parametrize("M,N,K", [(1029, 517, 1283), (517, 300, 900), (300, 517, 129)])
+@pytest.mark.parametrize("fmt", ["e4m3", "e5m2"])
+def test_linear_backward_of_both_products_in_one_launch(M, N, K, fmt):
+    """Either product may be the longer one; the result is the two single calls', bit for bit."""
+    fp8 = _fp8()
+    dy, x, w = _rand(M, N, 81, spread=0.5).cuda(), _rand(M, K, 82, spread=0.5).cuda(), _rand(N, K, 83, spread=0.5).cuda()
+    xt, wt = fp8.fp8_quantize(x, transpose=True), fp8.fp8_quantize(w, "tiles", transpose=True)
+    dx, dw = fp8.linear_fp8_bwd(dy, xt, wt, fmt=fmt)
+    q, qt = fp8.fp8_quantize_both(dy, fmt=fmt)
+    assert torch.equal(dx, fp8.matmul_fp8(q, wt, out_dtype=torch.float32)) and torch.equal(dw, fp8.matmul_fp8(qt, xt, out_dtype=torch.float32))
+    base = torch.randn_like(dw)
+    acc = base.clone()
+    fp8.linear_fp8_bwd(dy, xt, wt, fmt=fmt, dw=acc, accumulate=True)
+    assert torch.equal(acc, fp8.matmul_fp8(qt, xt, out=base, accumulate=True))
