@@ -83,6 +83,9 @@ class Fp8Matrix:
         self._data, self._scale, self._rows, self._cols, self._tiles, self._fmt, self._f32 = data, scale, rows, cols, tiles, fmt, f32
         self._ptrs, self._pitch, self._device = ptrs, -(-cols // BLOCK) * BLOCK, device
 
+    def __reduce__(self):      # (a copy's pointers are those of ITS tensors; torch pickles bytes, but no 8-bit floats)
+        return _rebuild, (self._data.view(torch.uint8), self._data.dtype, self._scale, self._cols, self.block)
+
     data = property(lambda self: self._data)
     scale = property(lambda self: self._scale)
     rows = property(lambda self: self._rows)
@@ -150,6 +153,10 @@ class Fp8Matrix:
             e = self.scale.permute(1, 0, 2).reshape(self.scale.shape[1], -1)[:, :_blocks(cols)]
             scale = pack_scale_bytes(e.t())
         return Fp8Matrix(data.view(self.data.dtype), scale, rows, "tiles")
+
+
+def _rebuild(codes, dtype, scale, cols, block):
+    return Fp8Matrix(codes.view(dtype), scale, cols, block)
 
 
 def pack_scale_bytes(e: torch.Tensor) -> torch.Tensor:

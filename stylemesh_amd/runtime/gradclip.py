@@ -113,6 +113,9 @@ class GradClip:
         self._args = (g.ptrs, o.ptrs, g.numel, g.types, o.types, g.n)
         self._ws_bytes = ops.lib.sm_grad_norm_ws_bytes(g.n)
 
+    def __reduce__(self):      # (a copy's tables are those of ITS tensors)
+        return GradClip, (self.grads, None if self.out is self.grads else self.out)
+
     def _result(self):
         """(norm, scratch) of one call: two streams, or two captured graphs, of one plan share nothing"""
         if torch.cuda.current_device() != self.device.index:

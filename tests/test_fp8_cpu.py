@@ -237,3 +237,14 @@ def test_gradient_list_limits():
     clip = lambda out: lib.sm_grad_clip(arr(C.c_void_p, p, p), arr(C.c_void_p, *out), arr(C.c_size_t, 4, 4), ty, ty, 2, 0, 1.0, p, 1 << 14, p, None)
     assert clip((p, 1 << 50)) != 0
     assert lib.sm_grad_norm(arr(C.c_void_p, p, p), arr(C.c_size_t, 4, 4), ty, 2, 0, p + 4, 1 << 14, p, None) != 0
+
+
+def test_copies_have_their_own_pointers():
+    """copy, deepcopy and pickle make a matrix of the new tensors, not one that still points at the old ones."""
+    import copy
+    import pickle
+    for m in (mat(4, 200), mat(300, 200, "tiles"), mat(4, 200, scale="f32")):
+        for c in (copy.copy(m), copy.deepcopy(m), pickle.loads(pickle.dumps(m))):
+            assert c._ptrs == (c.data.data_ptr(), c.scale.data_ptr()) and c.shape == m.shape and c.block == m.block and c._pitch == m._pitch
+            assert torch.equal(c.data.view(torch.uint8), m.data.view(torch.uint8)) and torch.equal(c.scale, m.scale)
+        assert copy.deepcopy(m)._ptrs != m._ptrs

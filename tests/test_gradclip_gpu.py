@@ -241,3 +241,17 @@ def test_one_plan_in_two_graphs():
         eager = plan.norm()
         torch.cuda.synchronize()
         assert torch.equal(eager, want[0]) and all(torch.equal(a, b) for a, b in zip(norms, want))
+
+
+def test_a_copied_plan_works_on_the_copies():
+    import copy
+    gc = _mod()
+    g = [torch.full((5000,), 2.0, device="cuda"), torch.ones(3, device="cuda")]
+    for out in (None, [torch.zeros_like(t) for t in g]):
+        plan = gc.GradClip(g, out)
+        other = copy.deepcopy(plan)
+        other.clip(1.0)
+        assert float(g[0][0]) == 2.0 and (out is None or not out[0].any())
+        assert all(a.data_ptr() != b.data_ptr() for a, b in zip(plan.grads, other.grads))
+        assert float(torch.stack([t.norm() for t in other.out]).norm()) == pytest.approx(1.0, rel=1e-5)
+        assert (other.out is other.grads) == (out is None)
