@@ -51,7 +51,8 @@ class Fp8Matrix:
     ZERO (the product runs over whole blocks; ``from_parts`` pads). ``block``: "rows" - a scale per row and 128 columns - or
     "tiles" - per 128 x 128 tile. ``scale``: uint8 power-of-two scales [ceil(KB / 4), S, 4], byte s = 2^(s - 127), the byte of
     (row, block kb) at [kb / 4, row, kb % 4], KB = ceil(cols / 128), S = rows or ceil(rows / 128) - or float32 scales [KB, S].
-    The tensors are used as they are, no copy is taken."""
+    The tensors are used as they are, no copy is taken - but for codes laid out column by column (quantising ``x.t()`` in plain
+    torch leaves them so), which are copied once, here."""
 
     __slots__ = ("_data", "_scale", "_rows", "_cols", "_tiles", "_fmt", "_f32", "_ptrs", "_pitch", "_device")
 
@@ -60,9 +61,11 @@ class Fp8Matrix:
             raise ValueError(f"block={block!r}: 'rows' or 'tiles'")
         if data.dtype not in _FMT_ID:
             raise ValueError(f"codes of type {data.dtype}: float8_e4m3fn or float8_e5m2")
-        if data.dim() != 2 or not data.is_contiguous() or cols < 0 or data.shape[1] != _blocks(cols) * BLOCK:
-            raise ValueError(f"codes must be contiguous [rows, {_blocks(max(cols, 0)) * BLOCK}] for {cols} columns, got "
-                             f"{tuple(data.shape)}, strides {data.stride()}")
+        if data.dim() != 2 or cols < 0 or data.shape[1] != _blocks(cols) * BLOCK or not (data.is_contiguous() or data.t().is_contiguous()):
+            raise ValueError(f"codes must be dense [rows, {_blocks(max(cols, 0)) * BLOCK}] for {cols} columns, got "
+                             f"{tuple(data.shape)}, strides {data.stride()}; from_parts takes any strides and widths")
+        if not data.is_contiguous():
+            data = data.contiguous()
         if data.data_ptr() % 16:
             raise ValueError("codes must start on a 16-byte boundary")
         kb, s = _blocks(cols), data.shape[0] if block == "rows" else _blocks(data.shape[0])

@@ -248,3 +248,16 @@ def test_copies_have_their_own_pointers():
             assert c._ptrs == (c.data.data_ptr(), c.scale.data_ptr()) and c.shape == m.shape and c.block == m.block and c._pitch == m._pitch
             assert torch.equal(c.data.view(torch.uint8), m.data.view(torch.uint8)) and torch.equal(c.scale, m.scale)
         assert copy.deepcopy(m)._ptrs != m._ptrs
+
+
+def test_codes_laid_out_by_columns_are_copied():
+    """Quantising a transposed matrix in plain torch leaves the codes column by column: the same matrix, rows at the pitch."""
+    g = torch.Generator().manual_seed(4)
+    codes = torch.randint(0, 120, (256, 300), generator=g, dtype=torch.uint8).t()      # [300, 256], strides (1, 300)
+    sc = torch.full((1, 300, 4), 127, dtype=torch.uint8)
+    for dtype in (E4, E5):
+        m = fp8.Fp8Matrix(codes.view(dtype), sc, 256)
+        assert m.data.is_contiguous() and m.data.dtype == dtype and torch.equal(m.data.view(torch.uint8), codes)
+        assert m._ptrs == (m.data.data_ptr(), m.scale.data_ptr()) and m._pitch == 256
+    row = torch.zeros(256, 1, dtype=torch.uint8).t().view(E4)                          # one row: nothing to copy
+    assert fp8.Fp8Matrix(row, torch.full((1, 1, 4), 127, dtype=torch.uint8), 256).data.data_ptr() == row.data_ptr()

@@ -587,3 +587,16 @@ def test_linear_backward_of_both_products_in_one_launch(M, N, K, fmt):
     acc = base.clone()
     fp8.linear_fp8_bwd(dy, xt, wt, fmt=fmt, dw=acc, accumulate=True)
     assert torch.equal(acc, fp8.matmul_fp8(qt, xt, out=base, accumulate=True))
+
+
+@pytest.mark.parametrize("M,N,K", [(256, 130, 300), (128, 70, 257)])
+def test_linear_backward_from_codes_laid_out_by_columns(M, N, K):
+    """Transposed activations quantised in plain torch: with M a multiple of 128 their codes lie column by column."""
+    fp8 = _fp8()
+    x, w, dy = _rand(M, K, 91, spread=0.5).cuda(), _rand(N, K, 92, spread=0.5).cuda(), _rand(M, N, 93, spread=0.5).cuda()
+    want, wt = fp8.fp8_quantize(x, transpose=True), fp8.fp8_quantize(w, "tiles", transpose=True)
+    codes = want.data.view(torch.uint8).t().contiguous().t().view(torch.float8_e4m3fn)
+    assert not codes.is_contiguous()
+    xt = fp8.Fp8Matrix(codes, want.scale, M)
+    for a, b in zip(fp8.linear_fp8_bwd(dy, xt, wt), fp8.linear_fp8_bwd(dy, want, wt)):
+        assert torch.equal(a, b)
