@@ -218,8 +218,7 @@ def prepare(case, seed):
     op = case["op"]
     if op == "backward":
         # the forward pass left the transposed activations in 8 bits; the weight's transpose is made once per update
-        xt8, s["sxt"] = _quantize(s["x"].t(), "rows", "e4m3")
-        s["xt8"] = xt8.contiguous()
+        s["xt8"], s["sxt"] = _quantize(s["x"].t(), "rows", "e4m3")
     if not own:
         return s
     from stylemesh_amd.runtime import fp8, gradclip
