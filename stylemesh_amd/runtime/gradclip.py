@@ -35,9 +35,11 @@ def _dense(t) -> bool:
 
 class _Table:
     """Pointers, element counts and types of a list of tensors as the library reads them (csrc/tensor_list.cpp: one walk in
-    native code)."""
+    native code). Keeps the tensors: the table holds only their addresses, and what a caller made on the way in (an iterator of
+    converted gradients) has no other owner until the launch."""
 
     def __init__(self, tensors, what):
+        self.tensors = tensors
         self.packed, at, odd, device, self.contiguous = _tensor_list.pack(tensors)
         if odd >= 0:
             t = tensors[odd]

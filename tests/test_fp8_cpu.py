@@ -261,3 +261,33 @@ def test_codes_laid_out_by_columns_are_copied():
         assert m._ptrs == (m.data.data_ptr(), m.scale.data_ptr()) and m._pitch == 256
     row = torch.zeros(256, 1, dtype=torch.uint8).t().view(E4)                          # one row: nothing to copy
     assert fp8.Fp8Matrix(row, torch.full((1, 1, 4), 127, dtype=torch.uint8), 256).data.data_ptr() == row.data_ptr()
+
+
+def test_gradients_of_an_iterator_live_until_the_launch(monkeypatch):
+    """A list of temporaries has no owner but the call: their memory must not be handed out again (as this call's scratch, for
+    one) before the launch that reads it."""
+    import weakref
+    from stylemesh_amd.runtime import gradclip, ops
+    refs, alive = [], []
+
+    def temporaries():
+        for _ in range(3):
+            t = torch.ones(4)
+            refs.append(weakref.ref(t))
+            yield t
+            del t
+
+    note = lambda result: alive.append(all(r() is not None for r in refs)) or result
+    real_pack, real_empty = gradclip._tensor_list.pack, torch.empty
+    monkeypatch.setattr(gradclip._tensor_list, "pack", lambda tensors: (*real_pack(tensors)[:3], 0, True))
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch, "empty", lambda *size, dtype, device: note(real_empty(*size, dtype=dtype)))
+    monkeypatch.setattr(ops, "eager_stream", lambda: 0)
+    monkeypatch.setattr(ops, "lib", type("Lib", (), {"sm_grad_norm_ws_bytes": staticmethod(lambda n: 8192),
+                                                     "sm_grad_norm": staticmethod(lambda *a: note(0)),
+                                                     "sm_grad_clip": staticmethod(lambda *a: note(0))}))
+    for call in (lambda: gradclip.grad_norm(temporaries()), lambda: gradclip.clip_grad_norm(temporaries(), 1.0)):
+        refs.clear()
+        alive.clear()
+        call()
+        assert len(alive) == 3 and all(alive)
