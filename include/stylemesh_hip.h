@@ -751,6 +751,7 @@ int sm_tex_sample_mip(const float* const* levels, const int* level_w, const int*
 #define SM_TYPE_F16 2
 #define SM_FP8_E4M3 0
 #define SM_FP8_E5M2 1
+#define SM_FP8_FAST_SUM 16      /* or-ed to SM_TYPE_BF16 as a product's out_type: see sm_fp8_matmul */
 /* x [rows][cols] (x_type, row stride x_stride elements, aligned to its elements) -> q / q_scale: the matrix in 8 bits, and / or
  * qt / qt_scale: its transpose [cols][rows rounded up to 128] with the blocks along the rows (either pair may be NULL); tiles:
  * one scale per 128 x 128 tile instead of per row and block. x is read once. A block's scale is the smallest power of two
@@ -760,9 +761,10 @@ int sm_tex_sample_mip(const float* const* levels, const int* level_w, const int*
 int sm_fp8_quantize(const void* x, int x_type, int rows, int cols, size_t x_stride, int fmt, int tiles, void* q, void* q_scale,
                     void* qt, void* qt_scale, void* stream);
 /* out[M][N] (out_type, row stride out_stride elements) = A B^T, or out += A B^T (accumulate), A [M][K] with scales per row and
- * block, B [N][K] (e4m3) per row and block or per tile (b_tiles); fp32 accumulate, one rounding to out_type. A bf16 result of
- * K > 896 takes the 8-bit matrix instruction, whose sum of eight products keeps 13 bits below the largest of them; every other
- * one widens the codes to bf16, which is exact, and sums in fp32. scale_f32: both scale arrays are floats. a, b: 16-byte
+ * block, B [N][K] (e4m3) per row and block or per tile (b_tiles). The codes are widened to bf16, the sums held in fp32 and rounded
+ * once to out_type. out_type = SM_TYPE_BF16 | SM_FP8_FAST_SUM (no other type takes the flag) permits the 8-bit matrix
+ * instruction, up to twice as fast: its sum of eight products keeps 13 bits below the largest of them, so a result may be off by
+ * 7 * 2^-13 of sum |a||b| (however small the result is). scale_f32: both scale arrays are floats. a, b: 16-byte
  * aligned, scales 4-byte aligned, pitches multiples of 16, at least K rounded up to 128 and at most 0xfffff0; M, N < 2^30.
  * ws: sm_fp8_matmul_ws_bytes(M, N, K) bytes (0: may be NULL) of scratch of this call's own. K = 0: zeros / out as it is. */
 size_t sm_fp8_matmul_ws_bytes(int M, int N, int K);
@@ -771,7 +773,7 @@ int sm_fp8_matmul(const void* a, const void* a_scale, int a_fmt, size_t a_pitch,
                   void* ws, size_t ws_bytes, void* stream);
 
 /* A layer's forward pass: out[M][N] = q(x) W^T, x [M][K] (x_type, row stride x_stride), q = sm_fp8_quantize with row scales in
- * e4m3, W [N][K] e4m3 with power-of-two scales (resident). Up to 16 rows one launch (x is quantised inside the product), above
+ * e4m3, W [N][K] e4m3 with power-of-two scales (resident); out_type as sm_fp8_matmul's. Up to 16 rows one launch (x is quantised inside the product), above
  * sm_fp8_quantize into ws + sm_fp8_matmul. ws: sm_fp8_linear_ws_bytes(M, N, K) bytes (0: may be NULL), 16-byte aligned, of this
  * call's own. */
 size_t sm_fp8_linear_ws_bytes(int M, int N, int K);
@@ -780,7 +782,7 @@ int sm_fp8_linear(const void* x, int x_type, size_t x_stride, const void* w, con
 
 /* Its backward pass (M, N, K > 0): dx[M][K] = q(dy) W from W's transpose wt [K][N], dw[N][K] = q(dy^T) q(x^T)^T (+= with accumulate,
  * fp32) from the transposed activations xt [K][M], both e4m3 with power-of-two scales; dy [M][N] is read once and quantised in
- * fmt. dx or dw may be NULL (not computed; its operand is not looked at). ws: sm_fp8_linear_backward_ws_bytes(M, N, K, dx
+ * fmt; dx_type as sm_fp8_matmul's out_type (dw is always summed in fp32). dx or dw may be NULL (not computed; its operand is not looked at). ws: sm_fp8_linear_backward_ws_bytes(M, N, K, dx
  * wanted, dw wanted) bytes, 16-byte aligned, of this call's own. */
 size_t sm_fp8_linear_backward_ws_bytes(int M, int N, int K, int need_dx, int need_dw);
 int sm_fp8_linear_backward(const void* dy, int dy_type, size_t dy_stride, int fmt, int M, int N, int K, const void* wt, const void* wt_scale,

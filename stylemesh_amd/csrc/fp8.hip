@@ -6,9 +6,9 @@
 //                                        ("rows") or per 128 x 128 tile ("tiles")
 //   product: out[m][n] = sum_kb sa[m][kb] sb[n or n / 128][kb] sum_{k in block kb} a[m][k] b[n][k], fp32 accumulate
 //
-// Power-of-two scales make the quantiser exact up to the one rounding to 8 bits (x 2^-e is exact) and let the matrix
-// cores apply the scales themselves: v_mfma_scale_f32_16x16x128_f8f6f4 takes a block of 128 per instruction and one scale
-// byte per operand row, so a scaled block costs no vector instruction. fp32 scales (any value) take the same kernels with
+// Power-of-two scales make the quantiser exact up to the one rounding to 8 bits (x 2^-e is exact) and cost the product no
+// instruction: they are part of the conversion that widens the codes to bf16, and for sums of fewer bits, where the caller permits
+// them, v_mfma_scale_f32_16x16x128_f8f6f4 takes a block of 128 per instruction and one scale byte per operand row. fp32 scales (any value) take the same kernels with
 // the block's partial sum multiplied in on the vector unit.
 #include <algorithm>
 #include <type_traits>
@@ -1055,25 +1055,26 @@ __global__ __launch_bounds__(256) void fp8_matmul_empty_kernel(MatmulArgs g) {
 
 // Which kernel takes an M x N x 128 KB product, and in how many slices of K. Measured on MI355X (us):
 //                                        256 x 256   256 x 128   128 x 128   64 x 64
-//   8192^3      bf16 result, 2^e scales        413         488         499       921
-//   4096^3      bf16 result, 2^e scales         59          71          70       126
+//   8192^3      fast sums, 2^e scales          413         488         499       921
+//   4096^3      fast sums, 2^e scales           59          71          70       126
 //   4096^3      f16 result, fp32 scales        317         121         133       201   (256 x 256 spills)
-//   2048^3      bf16 result, 2^e scales         33          22          17        18
-//   512 x 4096 x 4096, bf16                     50          31          26        18
+//   2048^3      fast sums, 2^e scales           33          22          17        18
+//   512 x 4096 x 4096, fast sums                50          31          26        18
 // A 256-row tile takes a CU, two 128 x 128 tiles share one: the large tile is taken where its rounds over the 256 CUs are not
 // emptier than the small one's by more than what it gains (1.2 x); below 192 tiles of 128 x 128 the chip is filled with
 // 64 x 64 ones, and where even those are few (a weight gradient of small layers) K is split, at least eight blocks a slice, and
 // the slices are added by a second kernel (128 x 256 x 8192: 27 us in one slice).
-// Up to 32 rows the stream kernel, which needs no LDS and keeps more of B in flight (32 x 4096 x 4096: 9.6 against 12.3 us); above,
-// its rereads of A through the caches cost more (37 x 8200 x 5001: 25 against 20 us).
+// Up to 32 rows the stream kernel, which needs no LDS and keeps more of B in flight (32 x 4096 x 4096, fast sums: 9.6 against 12.3 us);
+// above, its rereads of A through the caches cost more (37 x 8200 x 5001, fast sums: 25 against 20 us).
 enum { TILE_STREAM, TILE_64, TILE_128, TILE_256 };
 struct Plan {
     int kind, splits, kb_per_split;
+    bool fast;      // SM_FP8_FAST_SUM
 };
 static Plan matmul_plan(int M, int N, int KB) {
     const auto tiles = [&](long long bm, long long bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
     const auto fill = [](long long t, long long slots) { return (double)t / (double)((t + slots - 1) / slots * slots); };
-    Plan p{TILE_64, 1, KB};
+    Plan p{TILE_64, 1, KB, false};
     long long t = tiles(64, 64);
     if (M <= 32) {
         p.kind = TILE_STREAM;
@@ -1092,12 +1093,22 @@ static Plan matmul_plan(int M, int N, int KB) {
     return p;
 }
 
-// The 8-bit matrix instruction aligns the products of eight neighbouring k to the largest of them and keeps 13 bits below its
-// leading one (measured; so does the older 16x16x32 form), fp32 beyond that: relative to sum |a||b| an rms error of 2^-19
-// (normal data) to 2^-15 (log-normal, sigma 2) at K = 128, falling with sqrt(K). It is taken where the result is bf16 - half
-// a step is 2^-9 - and K >= 1024, where it stays inside what a plain fp32 sum of K terms may lose (K 2^-23 sum |a||b|).
-// Every other product widens the codes to bf16 (exact, scale included) and sums in fp32 throughout, at half the rate.
-static bool native_result(int out_type, int KB) { return out_type == SM_TYPE_BF16 && KB >= 8; }
+// A result's type, and whether its sums may run on the 8-bit matrix instruction. That instruction (both its forms) aligns the
+// products of eight neighbouring k to the largest of them and keeps 13 bits below its leading one (measured, not documented), fp32
+// beyond that: each of the other seven loses up to 2^-13 of the largest, so a sum is off by up to 7 * 2^-13 of sum |a||b|
+// beside what fp32 loses - of the terms' magnitudes, not of the result, which may be far smaller (rms at K = 128: 2^-19 of it for
+// normal data, 2^-15 for log-normal of sigma 2, falling with sqrt(K)). Those are fewer bits than a sum is owed, so it is taken
+// where the caller asks for it only, and only for bf16 results. Every other product widens the codes to bf16 and sums in fp32: us, fast against
+// that, 8192^3 462 / 844, layer backward 4096^3 208 / 256, 37 x 5001 -> 8200 21.0 / 22.4, 1 x 4096 -> 4096 6.1 / 6.5.
+struct ResultType {
+    int type;
+    bool fast, ok;
+};
+static ResultType result_type(int t) {
+    const int type = t & ~SM_FP8_FAST_SUM;
+    const bool fast = t != type;
+    return {type, fast, type >= 0 && type <= SM_TYPE_F16 && (!fast || type == SM_TYPE_BF16)};
+}
 
 template <int X, int TM, int TB, bool F32S, bool NATIVE, int U>
 static void launch_stream(const StreamArgs& t, int splits, hipStream_t s) {
@@ -1105,9 +1116,9 @@ static void launch_stream(const StreamArgs& t, int splits, hipStream_t s) {
                        dim3(STREAM_WAVES * 64), 0, s, t);
 }
 template <int X>
-static void launch_stream_raw(const StreamArgs& t, int splits, hipStream_t s) {
+static void launch_stream_raw(const StreamArgs& t, bool fast, int splits, hipStream_t s) {
     constexpr int U = X == SM_TYPE_F32 ? 2 : 4;
-    if (native_result(t.g.out_type, t.g.KB)) launch_stream<X, 1, 1, false, true, U>(t, splits, s);
+    if (fast) launch_stream<X, 1, 1, false, true, U>(t, splits, s);
     else launch_stream<X, 1, 1, false, false, U>(t, splits, s);
 }
 template <int X, bool NATIVE>
@@ -1117,9 +1128,9 @@ static void launch_stream_pow2(const StreamArgs& t, int splits, hipStream_t s) {
     else wide ? launch_stream<X, 2, 2, false, NATIVE, 2>(t, splits, s) : launch_stream<X, 2, 1, false, NATIVE, 2>(t, splits, s);
 }
 template <int X>
-static void launch_stream_codes(const StreamArgs& t, bool f32s, int splits, hipStream_t s) {
+static void launch_stream_codes(const StreamArgs& t, bool f32s, bool fast, int splits, hipStream_t s) {
     if (!f32s) {
-        if (native_result(t.g.out_type, t.g.KB)) launch_stream_pow2<X, true>(t, splits, s);
+        if (fast) launch_stream_pow2<X, true>(t, splits, s);
         else launch_stream_pow2<X, false>(t, splits, s);
     } else if (t.g.M <= 16) launch_stream<X, 1, 1, true, false, 4>(t, splits, s);
     else launch_stream<X, 2, 1, true, false, 2>(t, splits, s);
@@ -1225,24 +1236,26 @@ static int prepare_product(sm::MatmulArgs& g, sm::Plan& p, const void* a, const 
                            const void* b_scale, int b_tiles, size_t b_pitch, int M, int N, int K, void* out, int out_type, size_t out_stride,
                            int accumulate, void* ws, size_t ws_bytes) {
     const int KB = (int)(((size_t)K + 127) / 128);
-    if (out_type < 0 || out_type > SM_TYPE_F16 || (a_fmt != SM_FP8_E4M3 && a_fmt != SM_FP8_E5M2) || out == nullptr || out_stride < (size_t)N ||
+    const sm::ResultType rt = sm::result_type(out_type);
+    if (!rt.ok || (a_fmt != SM_FP8_E4M3 && a_fmt != SM_FP8_E5M2) || out == nullptr || out_stride < (size_t)N ||
         a == nullptr || b == nullptr || a_scale == nullptr || b_scale == nullptr || a_pitch < (size_t)KB * 128 || b_pitch < (size_t)KB * 128 ||
         a_pitch % 16 || b_pitch % 16 || (uintptr_t)a % 16 || (uintptr_t)b % 16 || (uintptr_t)a_scale % 4 || (uintptr_t)b_scale % 4 ||
         a_pitch > MAX_PITCH || b_pitch > MAX_PITCH || M > MAX_ROWS || N > MAX_ROWS)
         return (int)hipErrorInvalidValue;
     p = sm::matmul_plan(M, N, KB);
+    p.fast = rt.fast;
     if (p.splits > 1 && (ws == nullptr || ws_bytes < (size_t)p.splits * M * N * sizeof(float))) return (int)hipErrorInvalidValue;
     g = sm::MatmulArgs{(const uint8_t*)a, (const uint8_t*)b, a_scale, b_scale, out, (float*)ws, a_pitch, b_pitch, out_stride, M, N, KB,
-                       b_tiles ? 7 : 0, b_tiles ? (N + 127) / 128 : N, out_type, accumulate, p.kb_per_split};
+                       b_tiles ? 7 : 0, b_tiles ? (N + 127) / 128 : N, rt.type, accumulate, p.kb_per_split};
     return 0;
 }
 
 static int run_product(const sm::MatmulArgs& g, const sm::Plan& p, int a_fmt, bool f32s, int K, hipStream_t s) {
     if (p.kind == sm::TILE_STREAM) {
         const sm::StreamArgs t{g, nullptr, 0, K};
-        if (a_fmt == SM_FP8_E4M3) sm::launch_stream_codes<8 + SM_FP8_E4M3>(t, f32s, p.splits, s);
-        else sm::launch_stream_codes<8 + SM_FP8_E5M2>(t, f32s, p.splits, s);
-    } else if (sm::native_result(g.out_type, g.KB)) {
+        if (a_fmt == SM_FP8_E4M3) sm::launch_stream_codes<8 + SM_FP8_E4M3>(t, f32s, p.fast, p.splits, s);
+        else sm::launch_stream_codes<8 + SM_FP8_E5M2>(t, f32s, p.fast, p.splits, s);
+    } else if (p.fast) {
         sm::launch_tile<true>(p.kind, g, a_fmt, f32s, p.splits, s);
     } else {
         sm::launch_tile<false>(p.kind, g, a_fmt, f32s, p.splits, s);
@@ -1256,8 +1269,8 @@ static int run_product(const sm::MatmulArgs& g, const sm::Plan& p, int a_fmt, bo
 int sm_fp8_matmul(const void* a, const void* a_scale, int a_fmt, size_t a_pitch, const void* b, const void* b_scale, int b_tiles,
                   size_t b_pitch, int scale_f32, int M, int N, int K, void* out, int out_type, size_t out_stride, int accumulate,
                   void* ws, size_t ws_bytes, void* stream) {
-    if (M < 0 || N < 0 || K < 0 || out_type < 0 || out_type > SM_TYPE_F16 || (a_fmt != SM_FP8_E4M3 && a_fmt != SM_FP8_E5M2))
-        return (int)hipErrorInvalidValue;
+    const sm::ResultType rt = sm::result_type(out_type);
+    if (M < 0 || N < 0 || K < 0 || !rt.ok || (a_fmt != SM_FP8_E4M3 && a_fmt != SM_FP8_E5M2)) return (int)hipErrorInvalidValue;
     if (M == 0 || N == 0) return 0;
     hipStream_t s = (hipStream_t)stream;
     sm::MatmulArgs g{};
@@ -1267,7 +1280,7 @@ int sm_fp8_matmul(const void* a, const void* a_scale, int a_fmt, size_t a_pitch,
         g.out_stride = out_stride;
         g.M = M;
         g.N = N;
-        g.out_type = out_type;
+        g.out_type = rt.type;
         const size_t quads = (size_t)(N + 3) / 4 * M;
         if (!accumulate) hipLaunchKernelGGL(sm::fp8_matmul_empty_kernel, dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, s, g);
         SM_LAUNCH_CHECK();
@@ -1293,8 +1306,8 @@ size_t sm_fp8_linear_ws_bytes(int M, int N, int K) {
 
 int sm_fp8_linear(const void* x, int x_type, size_t x_stride, const void* w, const void* w_scale, int w_tiles, size_t w_pitch, int M,
                   int N, int K, void* out, int out_type, size_t out_stride, void* ws, size_t ws_bytes, void* stream) {
-    if (M < 0 || N < 0 || K < 0 || x_type < 0 || x_type > SM_TYPE_F16 || out_type < 0 || out_type > SM_TYPE_F16)
-        return (int)hipErrorInvalidValue;
+    const sm::ResultType rt = sm::result_type(out_type);
+    if (M < 0 || N < 0 || K < 0 || x_type < 0 || x_type > SM_TYPE_F16 || !rt.ok) return (int)hipErrorInvalidValue;
     if (M == 0 || N == 0) return 0;
     if (K > 0 && (x == nullptr || x_stride < (size_t)K || (ws == nullptr && sm_fp8_linear_ws_bytes(M, N, K) > 0) ||
                   ws_bytes < sm_fp8_linear_ws_bytes(M, N, K) || (uintptr_t)ws % 16))
@@ -1315,10 +1328,10 @@ int sm_fp8_linear(const void* x, int x_type, size_t x_stride, const void* w, con
     hipStream_t s = (hipStream_t)stream;
     const sm::Plan p = sm::matmul_plan(M, N, KB);
     sm::StreamArgs t{{nullptr, (const uint8_t*)w, nullptr, w_scale, out, (float*)ws, 0, w_pitch, out_stride, M, N, KB, w_tiles ? 7 : 0,
-                      w_tiles ? (N + 127) / 128 : N, out_type, 0, p.kb_per_split}, x, x_stride, K};
-    if (x_type == SM_TYPE_F32) sm::launch_stream_raw<SM_TYPE_F32>(t, p.splits, s);
-    else if (x_type == SM_TYPE_BF16) sm::launch_stream_raw<SM_TYPE_BF16>(t, p.splits, s);
-    else sm::launch_stream_raw<SM_TYPE_F16>(t, p.splits, s);
+                      w_tiles ? (N + 127) / 128 : N, rt.type, 0, p.kb_per_split}, x, x_stride, K};
+    if (x_type == SM_TYPE_F32) sm::launch_stream_raw<SM_TYPE_F32>(t, rt.fast, p.splits, s);
+    else if (x_type == SM_TYPE_BF16) sm::launch_stream_raw<SM_TYPE_BF16>(t, rt.fast, p.splits, s);
+    else sm::launch_stream_raw<SM_TYPE_F16>(t, rt.fast, p.splits, s);
     SM_LAUNCH_CHECK();
     if (p.splits > 1) sm::launch_reduce(t.g, p.splits, s);
     SM_LAUNCH_CHECK();
@@ -1375,7 +1388,7 @@ int sm_fp8_linear_backward(const void* dy, int dy_type, size_t dy_stride, int fm
         return e;
     // two products of small tiles, neither of which fills the chip: one launch (1029 x 517 x 1283: 8.3 + 8.2 -> 10.7 us, of which a
     // ring of three stages - three blocks a CU instead of two - is worth 1.1 and the order below 1)
-    if (dx && dw && px.kind == sm::TILE_64 && pw.kind == sm::TILE_64 && px.splits == 1 && pw.splits == 1 && !sm::native_result(dx_type, gx.KB)) {
+    if (dx && dw && px.kind == sm::TILE_64 && pw.kind == sm::TILE_64 && px.splits == 1 && pw.splits == 1 && !px.fast) {
         // the one with more blocks of K first: its tiles run longest, and the last tiles to start should be short
         const bool swap = gw.KB > gx.KB;
         const sm::MatmulArgs &g0 = swap ? gw : gx, &g1 = swap ? gx : gw;

@@ -96,11 +96,14 @@ PyObject* quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// matmul(a, a_scale, a_fmt, a_pitch, b, b_scale, b_tiles, b_pitch, f32, M, N, K, out, out_type, accumulate, device, stream) -> out; out: a
-// tensor, or None for a new one of out_type
+// fast: the sums may run on the 8-bit matrix instruction (bfloat16 results)
+int result_type(int type, int fast) { return fast ? type | SM_FP8_FAST_SUM : type; }
+
+// matmul(a, a_scale, a_fmt, a_pitch, b, b_scale, b_tiles, b_pitch, f32, M, N, K, out, out_type, accumulate, fast, device, stream) -> out;
+// out: a tensor, or None for a new one of out_type
 PyObject* matmul(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    if (!expect(n, 17)) return nullptr;
+    if (!expect(n, 18)) return nullptr;
     Args g{a, n};
     void *ap = g.pointer(), *as = g.pointer();
     const int a_fmt = (int)g.integer();
@@ -112,7 +115,7 @@ PyObject* matmul(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const long M = g.integer(), N = g.integer(), K = g.integer();
     PyObject* given = g.object();
     int type = (int)g.integer();
-    const int accumulate = (int)g.integer(), device = (int)g.integer();
+    const int accumulate = (int)g.integer(), fast = (int)g.integer(), device = (int)g.integer();
     void* stream = g.pointer();
     if (PyErr_Occurred()) return nullptr;
     if (M < 0 || N < 0 || K < 0 || M > MAX_DIM || N > MAX_DIM || K > MAX_DIM) Py_RETURN_NONE;
@@ -133,8 +136,8 @@ PyObject* matmul(PyObject*, PyObject* const* a, Py_ssize_t n) {
         at::Tensor ws = need ? room({(int64_t)need}, at::kByte, device) : at::Tensor();
         void *op = out.data_ptr(), *wp = need ? ws.data_ptr() : nullptr;
         if (!launch("sm_fp8_matmul", [&] {
-                return sm_fp8_matmul(ap, as, a_fmt, (size_t)a_pitch, bp, bs, b_tiles, (size_t)b_pitch, f32, (int)M, (int)N, (int)K, op, type,
-                                     (size_t)o.stride, accumulate, wp, need, stream);
+                return sm_fp8_matmul(ap, as, a_fmt, (size_t)a_pitch, bp, bs, b_tiles, (size_t)b_pitch, f32, (int)M, (int)N, (int)K, op,
+                                     result_type(type, fast), (size_t)o.stride, accumulate, wp, need, stream);
             }))
             return nullptr;
     }
@@ -143,17 +146,17 @@ PyObject* matmul(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// linear(x, w, w_scale, w_tiles, w_pitch, N, K, out_type or -1: x's, device, stream) -> y
+// linear(x, w, w_scale, w_tiles, w_pitch, N, K, out_type or -1: x's, fast, device, stream) -> y
 PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    if (!expect(n, 10)) return nullptr;
+    if (!expect(n, 11)) return nullptr;
     Args g{a, n};
     PyObject* x = g.object();
     void *w = g.pointer(), *ws = g.pointer();
     const int tiles = (int)g.integer();
     const long pitch = g.integer(), N = g.integer(), K = g.integer();
     int type = (int)g.integer();
-    const int device = (int)g.integer();
+    const int fast = (int)g.integer(), device = (int)g.integer();
     void* stream = g.pointer();
     if (PyErr_Occurred()) return nullptr;
     Matrix m;
@@ -165,8 +168,8 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
         at::Tensor scratch = need ? room({(int64_t)need}, at::kByte, device) : at::Tensor();      // of this call's own, as matmul's
         void *yp = y.data_ptr(), *sp = need ? scratch.data_ptr() : nullptr;
         if (!launch("sm_fp8_linear", [&] {
-                return sm_fp8_linear(m.p, m.type, (size_t)m.stride, w, ws, tiles, (size_t)pitch, (int)m.rows, (int)N, (int)K, yp, type, (size_t)N, sp,
-                                     need, stream);
+                return sm_fp8_linear(m.p, m.type, (size_t)m.stride, w, ws, tiles, (size_t)pitch, (int)m.rows, (int)N, (int)K, yp,
+                                     result_type(type, fast), (size_t)N, sp, need, stream);
             }))
             return nullptr;
     }
@@ -174,11 +177,11 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// backward(dy, fmt, K, wt, wt_scale, wt_tiles, wt_pitch, xt, xt_scale, xt_tiles, xt_pitch, dx_type or -1: dy's, dw, accumulate, device, stream)
-// -> (dx or None, dw or None), M, N, K > 0; wt / xt None: that gradient is not wanted; dw: a float32 matrix, or None for a new one
+// backward(dy, fmt, K, wt, wt_scale, wt_tiles, wt_pitch, xt, xt_scale, xt_tiles, xt_pitch, dx_type or -1: dy's, dw, accumulate, fast (dx),
+// device, stream) -> (dx or None, dw or None), M, N, K > 0; wt / xt None: that gradient is not wanted; dw: a float32 matrix, or None for a new one
 PyObject* backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    if (!expect(n, 16)) return nullptr;
+    if (!expect(n, 17)) return nullptr;
     Args g{a, n};
     PyObject* dyo = g.object();
     const int fmt = (int)g.integer();
@@ -191,7 +194,7 @@ PyObject* backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const long xt_pitch = g.integer();
     int type = (int)g.integer();
     PyObject* given = g.object();
-    const int accumulate = (int)g.integer(), device = (int)g.integer();
+    const int accumulate = (int)g.integer(), fast = (int)g.integer(), device = (int)g.integer();
     void* stream = g.pointer();
     if (PyErr_Occurred()) return nullptr;
     Matrix dy, w;
@@ -211,7 +214,7 @@ PyObject* backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     void *dxp = wt ? dx.data_ptr() : nullptr, *dwp = xt ? dw.data_ptr() : nullptr, *sp = scratch.data_ptr();
     if (!launch("sm_fp8_linear_backward", [&] {
             return sm_fp8_linear_backward(dy.p, dy.type, (size_t)dy.stride, fmt, (int)dy.rows, (int)dy.cols, (int)K, wt, wts, wt_tiles, (size_t)wt_pitch, xt,
-                                          xts, xt_tiles, (size_t)xt_pitch, dxp, type, (size_t)K, (float*)dwp, (size_t)w.stride, accumulate, sp, need, stream);
+                                          xts, xt_tiles, (size_t)xt_pitch, dxp, result_type(type, fast), (size_t)K, (float*)dwp, (size_t)w.stride, accumulate, sp, need, stream);
         }))
         return nullptr;
     return Py_BuildValue("NN", wt ? THPVariable_Wrap(std::move(dx)) : Py_NewRef(Py_None),

@@ -232,13 +232,20 @@ def fp8_quantize_both(x: torch.Tensor, block: str = "rows", fmt: str = "e4m3"):
     return _quantize(x, block, fmt, True, True)
 
 
-def matmul_fp8(a: Fp8Matrix, b: Fp8Matrix, out: torch.Tensor | None = None, out_dtype=None, accumulate: bool = False) -> torch.Tensor:
+def _check_fast(fast_accum, dtype):
+    if fast_accum and dtype != torch.bfloat16:
+        raise ValueError(f"fast_accum is for bfloat16 results, this one is {dtype}")
+    return bool(fast_accum)
+
+
+def matmul_fp8(a: Fp8Matrix, b: Fp8Matrix, out: torch.Tensor | None = None, out_dtype=None, accumulate: bool = False,
+               fast_accum: bool = False) -> torch.Tensor:
     """[M, N] = A B^T for A [M, K] (``rows`` scales, e4m3 or e5m2) and B [N, K] (e4m3, ``rows`` or ``tiles`` scales), both with
-    power-of-two or both with float32 scales; fp32 accumulate, one rounding to ``out_dtype`` (float32 / bfloat16 / float16;
-    default bfloat16). A bfloat16 result of K > 896 takes the 8-bit matrix instruction, whose sum of eight products keeps 13 bits
-    below the largest of them (far inside the result's half step); every other one widens the codes exactly and sums in fp32.
-    ``out``: result of that type and shape, unit column stride; ``accumulate``: added to it (in fp32, then
-    rounded once)."""
+    power-of-two or both with float32 scales; the codes are widened, the sums held in fp32 and rounded once to ``out_dtype``
+    (float32 / bfloat16 / float16; default bfloat16). ``out``: result of that type and shape, unit column stride; ``accumulate``:
+    added to it (in fp32, then rounded once). ``fast_accum`` (bfloat16 results only) permits the 8-bit matrix instruction, up to twice as
+    fast on large products - its sum of eight products keeps 13 bits below the largest of them, so a result may be off by
+    7 * 2^-13 of sum |a||b|, however small the result itself is (rows with outliers that cancel lose most)."""
     if not isinstance(a, Fp8Matrix) or not isinstance(b, Fp8Matrix):
         raise ValueError("matmul_fp8 takes two Fp8Matrix operands")
     if a._tiles:
@@ -261,13 +268,15 @@ def matmul_fp8(a: Fp8Matrix, b: Fp8Matrix, out: torch.Tensor | None = None, out_
         if out_dtype not in _TYPE_ID:
             raise ValueError(f"out_dtype={out_dtype}: float32, bfloat16 or float16")
         dtype = _TYPE_ID[out_dtype]
+        fast = _check_fast(fast_accum, out_dtype)
     else:
         _check_matrix(out, "out")
         if tuple(out.shape) != (M, N) or (out_dtype is not None and out.dtype != out_dtype):
             raise ValueError(f"out is {out.dtype} {tuple(out.shape)}, the product {out_dtype or out.dtype} {(M, N)}")
         dtype = 0
+        fast = _check_fast(fast_accum, out.dtype)
     return _fp8_host.matmul(*a._ptrs, a._fmt, a._pitch, *b._ptrs, b._tiles, b._pitch, a._f32, M, N, K, out, dtype, bool(accumulate),
-                            a._device, ops.eager_stream())
+                            fast, a._device, ops.eager_stream())
 
 
 def _weight_arg(w, what="weight"):
@@ -276,20 +285,23 @@ def _weight_arg(w, what="weight"):
     return w
 
 
-def linear_fp8_fwd(x: torch.Tensor, weight: Fp8Matrix, out_dtype=None, keep_transposed: bool = False):
+def linear_fp8_fwd(x: torch.Tensor, weight: Fp8Matrix, out_dtype=None, keep_transposed: bool = False, fast_accum: bool = False):
     """y [M, N] = q(x) weight^T for x [M, K] and a resident weight [N, K] (``fp8_quantize(w, block="tiles")``), in ``out_dtype``
     (default: x's). ``keep_transposed``: returns (y, q(x^T)), the second for ``linear_fp8_bwd``'s weight gradient - quantised
-    from the same read of x."""
+    from the same read of x. ``fast_accum``: as ``matmul_fp8``'s."""
     _weight_arg(weight)
     if out_dtype is not None and out_dtype not in _TYPE_ID:
         raise ValueError(f"out_dtype={out_dtype}: float32, bfloat16 or float16")
     if keep_transposed:
         n, t = _quantize(x, "rows", "e4m3", True, True)
-        return matmul_fp8(n, weight, out_dtype=x.dtype if out_dtype is None else out_dtype), t
+        return matmul_fp8(n, weight, out_dtype=x.dtype if out_dtype is None else out_dtype, fast_accum=fast_accum), t
+    if fast_accum:
+        _check_matrix(x, "x")
+        _check_fast(fast_accum, x.dtype if out_dtype is None else out_dtype)
     y = None
     if weight._device >= 0 and weight._device == torch.cuda.current_device():
         y = _fp8_host.linear(x, *weight._ptrs, weight._tiles, weight._pitch, weight._rows, weight._cols,
-                             -1 if out_dtype is None else _TYPE_ID[out_dtype], weight._device, ops.eager_stream())
+                             -1 if out_dtype is None else _TYPE_ID[out_dtype], bool(fast_accum), weight._device, ops.eager_stream())
     if y is None:
         _check_matrix(x, "x")
         if x.shape[1] != weight._cols:
@@ -300,12 +312,13 @@ def linear_fp8_fwd(x: torch.Tensor, weight: Fp8Matrix, out_dtype=None, keep_tran
 
 
 def linear_fp8_bwd(dy: torch.Tensor, x_t: Fp8Matrix | None, weight_t: Fp8Matrix | None, fmt: str = "e4m3", dx_dtype=None,
-                   dw: torch.Tensor | None = None, accumulate: bool = False):
+                   dw: torch.Tensor | None = None, accumulate: bool = False, fast_accum: bool = False):
     """(dx, dw) of ``linear_fp8_fwd``'s layer: dx [M, K] = q(dy) weight (in ``dx_dtype``, default dy's) from
     ``weight_t`` = the weight's transpose [K, N] (``weight.transposed()`` / ``fp8_quantize_both(w, block="tiles")[1]``), and
     dw [N, K] = q(dy^T) q(x^T)^T in float32 from ``x_t`` = [K, M] (``keep_transposed``). ``fmt``: format of the gradient's
     codes. ``dw`` / ``accumulate``: write into, or add to, an existing float32 gradient. Either of ``x_t`` / ``weight_t`` may be
-    None: that gradient is not computed and None is returned in its place."""
+    None: that gradient is not computed and None is returned in its place. ``fast_accum``: as ``matmul_fp8``'s, for dx; dw is
+    always summed in fp32."""
     _check_matrix(dy, "dy")
     M, N = dy.shape
     if x_t is None and weight_t is None:
@@ -321,6 +334,7 @@ def linear_fp8_bwd(dy: torch.Tensor, x_t: Fp8Matrix | None, weight_t: Fp8Matrix 
             dx_dtype = dy.dtype
         elif dx_dtype not in _TYPE_ID:
             raise ValueError(f"dx_dtype={dx_dtype}: float32, bfloat16 or float16")
+        _check_fast(fast_accum, dx_dtype)
     if x_t is not None:
         if _weight_arg(x_t, "x_t").cols != M or x_t.rows != K:
             raise ValueError(f"dy has {M} rows and the layer {K} inputs, x_t is {x_t.shape}")
@@ -347,5 +361,5 @@ def linear_fp8_bwd(dy: torch.Tensor, x_t: Fp8Matrix | None, weight_t: Fp8Matrix 
     wt = (*weight_t._ptrs, weight_t._tiles, weight_t._pitch) if weight_t is not None else _NO_MATRIX
     xt = (*x_t._ptrs, x_t._tiles, x_t._pitch) if x_t is not None else _NO_MATRIX
     done = _fp8_host.backward(dy, _FMT_ID[FORMATS[fmt]], K, *wt, *xt, -1 if dx_dtype is None else _TYPE_ID[dx_dtype], dw, bool(accumulate),
-                              dy.get_device(), ops.eager_stream())
+                              bool(fast_accum and weight_t is not None), dy.get_device(), ops.eager_stream())
     return done if done is not None else _refuse(dy, "dy")

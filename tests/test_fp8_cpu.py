@@ -291,3 +291,21 @@ def test_gradients_of_an_iterator_live_until_the_launch(monkeypatch):
         alive.clear()
         call()
         assert len(alive) == 3 and all(alive)
+
+
+def test_fast_sums_are_for_bfloat16_results():
+    a, b, x = mat(4, 200), mat(6, 200), torch.zeros(4, 200)
+    for f in (lambda: fp8.matmul_fp8(a, b, out_dtype=torch.float32, fast_accum=True), lambda: fp8.matmul_fp8(a, b, out_dtype=torch.float16, fast_accum=True),
+              lambda: fp8.linear_fp8_fwd(x, b, fast_accum=True), lambda: fp8.linear_fp8_fwd(x, b, torch.float16, fast_accum=True),
+              lambda: fp8.linear_fp8_bwd(torch.zeros(4, 6), None, mat(200, 6, "tiles"), fast_accum=True)):
+        with pytest.raises(ValueError):
+            f()
+    lib = hip.lib
+    buf = torch.zeros(1 << 16, dtype=torch.uint8)
+    p = buf.data_ptr() + (-buf.data_ptr()) % 16
+    ok = [p, p, 0, 256, p, p, 0, 256, 0, 4, 6, 200, p, 0, 6, 0, None, 0, None]
+    m = lambda t, **k: lib.sm_fp8_matmul(*[k.get(f"a{i}", v) if i != 13 else t for i, v in enumerate(ok)])
+    for t in (16, 18, 19, 32, 33, -1, -15):
+        assert m(t) != 0 and m(t, a9=0) != 0, t
+        assert lib.sm_fp8_linear(p, 0, 200, p, p, 0, 256, 0, 6, 200, p, t, 6, p, 1 << 15, None) != 0, t
+    assert m(17, a9=0) == 0 and lib.sm_fp8_linear(p, 0, 200, p, p, 0, 256, 0, 6, 200, p, 17, 6, p, 1 << 15, None) == 0

@@ -1,0 +1,116 @@
+"""How many bits the sums of the 8-bit products keep, and over which scales (runtime/fp8.py), against 64 bits."""
+import pytest
+import torch
+
+import fp8_ref as R
+from gpu_util import require_gpu
+
+pytestmark = pytest.mark.gpu
+E4, E5 = torch.float8_e4m3fn, torch.float8_e5m2
+DT = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+
+
+def _fp8():
+    require_gpu()
+    from stylemesh_amd.runtime import fp8
+    return fp8
+
+
+def _matrix(fp8, values, dtype=E4, block="rows", scale="e8m0"):
+    """values (which the format holds) with scales of 1"""
+    r, c = values.shape
+    kb, s = -(-c // 128), r if block == "rows" else -(-r // 128)
+    data = torch.zeros(r, kb * 128, device="cuda")
+    data[:, :c] = values
+    codes = data.to(dtype)
+    assert torch.equal(codes.float(), data)
+    sc = torch.full((-(-kb // 4), s, 4), 127, dtype=torch.uint8, device="cuda") if scale == "e8m0" else torch.ones(kb, s, device="cuda")
+    return fp8.Fp8Matrix(codes, sc, c, block)
+
+
+def _outliers(M, N, K, fmt, seed):
+    """Integers: every eighth column an outlier v that cancels in pairs, small odd and even numbers between. K / 16 v^2 + 9 K <
+    2^24: every partial sum, in any order, is a whole number that fp32 holds, so a sum of fp32 is exact. An outlier's product
+    is at least 2^11 (v >= 48), 13 bits below which the ones of the small products lie or end."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    fits = [v for v in (48, 64, 96, 128, 160, 176, 192, 224, 256, 320, 384, 448) if (K // 16 + 1) * v * v + 9 * K < 1 << 24]
+    v = max(v for v in fits if fmt == E4 or v in (48, 64, 96, 128, 160, 192, 224, 256, 320, 384, 448))      # (e5m2: three bits)
+    a = torch.randint(-3, 4, (M, K), generator=g, device="cuda").float()
+    b = torch.randint(-3, 4, (N, K), generator=g, device="cuda").float()
+    at = torch.arange(0, K // 16 * 16, 8, device="cuda")
+    a[:, at] = v * (1.0 - 2.0 * (torch.arange(at.numel(), device="cuda") % 2))
+    b[:, at] = float(v)
+    return a, b
+
+
+# one shape or more per form: stream (up to 16 rows, 32, long B, split), 64 x 64 (ring of four, of three, split), 128 x 128, 256-row tiles
+FORMS = [(1, 200, 1024), (16, 130, 900), (20, 70, 1024), (32, 6200, 1000), (4, 100, 8192), (100, 200, 1024), (33, 70, 2304), (40, 100, 4100),
+         (1500, 1540, 1024), (1800, 1930, 1000), (4000, 4000, 1024)]
+
+
+@pytest.mark.parametrize("M,N,K", FORMS)
+@pytest.mark.parametrize("scale,block", [("e8m0", "rows"), ("e8m0", "tiles"), ("f32", "rows"), ("f32", "tiles")])
+def test_sums_keep_what_fp32_keeps(M, N, K, scale, block):
+    """Outlier channels that cancel: the result is the small terms' sum, to the last bit, in every form and for every type."""
+    fp8 = _fp8()
+    for fmt in (E4, E5):
+        a, b = _outliers(M, N, K, fmt, 5)
+        ref = a.double() @ b.double().t()
+        qa, qb = _matrix(fp8, a, fmt, "rows", scale), _matrix(fp8, b, E4, block, scale)
+        for dt in DT.values():
+            assert torch.equal(fp8.matmul_fp8(qa, qb, out_dtype=dt), ref.to(dt)), dt
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 200, 1024), (7, 300, 2000), (16, 70, 8192), (60, 90, 1500), (300, 200, 1024)])
+def test_layer_passes_keep_what_fp32_keeps(M, N, K):
+    """The layer's forward pass and its input gradient in bfloat16, on values that the quantiser leaves as they are."""
+    fp8 = _fp8()
+    a, b = _outliers(M, N, K, E4, 6)
+    ref = (a.double() @ b.double().t()).bfloat16()
+    w8 = fp8.fp8_quantize(b, "tiles")
+    for x in (a, a.bfloat16(), a.half()):
+        assert torch.equal(fp8.linear_fp8_fwd(x, w8, out_dtype=torch.bfloat16), ref)
+        assert torch.equal(fp8.linear_fp8_fwd(x, w8, out_dtype=torch.bfloat16, keep_transposed=True)[0], ref)
+    # dx = dy W with dy = a [M, K] and W^T = b [N, K]
+    assert torch.equal(fp8.linear_fp8_bwd(a.bfloat16(), None, w8)[0], ref)
+    assert torch.equal(fp8.linear_fp8_bwd(a, None, w8, dx_dtype=torch.bfloat16)[0], ref)
+
+
+@pytest.mark.parametrize("M,N,K", FORMS)
+@pytest.mark.parametrize("scale,block", [("e8m0", "rows"), ("f32", "tiles")])
+def test_fast_sums_stay_within_their_bound(M, N, K, scale, block):
+    """fast_accum: seven of eight products lose up to 2^-13 of the largest, fp32 sums lose (K + 8) 2^-23, both of sum |a||b|; one
+    rounding to bfloat16. On the outliers it does lose: the exact sums are another arithmetic."""
+    fp8 = _fp8()
+    for fmt in (E4, E5):
+        a, b = _outliers(M, N, K, fmt, 7)
+        ref = a.double() @ b.double().t()
+        qa, qb = _matrix(fp8, a, fmt, "rows", scale), _matrix(fp8, b, E4, block, scale)
+        out = fp8.matmul_fp8(qa, qb, fast_accum=True)
+        lost = (7 * 2.0 ** -13 + (K + 8) * 2.0 ** -23) * (a.double().abs() @ b.double().abs().t())
+        assert out.dtype == torch.bfloat16
+        assert ((out.double() - ref).abs() <= lost + 2.0 ** -8 * (ref.abs() + lost)).all()
+        if K in (1000, 1024) and (scale == "e8m0" or M > 32):      # (few rows under fp32 scales have no such form)
+            assert not torch.equal(out, ref.bfloat16())
+    # values without outliers: small integers are exact under 13 bits too
+    g = torch.Generator(device="cuda").manual_seed(9)
+    a, b = (torch.randint(-3, 4, (r, K), generator=g, device="cuda").float() for r in (M, N))
+    want = (a.double() @ b.double().t()).bfloat16()
+    assert torch.equal(fp8.matmul_fp8(_matrix(fp8, a, E4, "rows", scale), _matrix(fp8, b, E4, block, scale), fast_accum=True), want)
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 200, 1024), (16, 70, 500), (40, 90, 1500), (300, 200, 1024)])
+def test_fast_sums_of_the_layer_passes(M, N, K):
+    fp8 = _fp8()
+    a, b = _outliers(M, N, K, E4, 8)
+    ref = a.double() @ b.double().t()
+    w8, w8t = fp8.fp8_quantize_both(b, "tiles")
+    lost = (7 * 2.0 ** -13 + (K + 8) * 2.0 ** -23) * (a.double().abs() @ b.double().abs().t())
+    ok = lambda y: y.dtype == torch.bfloat16 and bool(((y.double() - ref).abs() <= lost + 2.0 ** -8 * (ref.abs() + lost)).all())
+    for x in (a, a.bfloat16(), a.half()):
+        assert ok(fp8.linear_fp8_fwd(x, w8, out_dtype=torch.bfloat16, fast_accum=True))
+    assert ok(fp8.linear_fp8_fwd(a.bfloat16(), w8, keep_transposed=True, fast_accum=True)[0])
+    # with both gradients: dw is the exact sum whatever is asked of dx (dw [K, N] = q(a^T) q(x^T)^T of integers)
+    x = torch.randint(-3, 4, (M, N), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").float()
+    dx, dw = fp8.linear_fp8_bwd(a.bfloat16(), fp8.fp8_quantize(x, transpose=True), w8, fast_accum=True)
+    assert ok(dx) and torch.equal(dw.double(), a.double().t() @ x.double())
