@@ -114,3 +114,68 @@ def test_fast_sums_of_the_layer_passes(M, N, K):
     x = torch.randint(-3, 4, (M, N), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").float()
     dx, dw = fp8.linear_fp8_bwd(a.bfloat16(), fp8.fp8_quantize(x, transpose=True), w8, fast_accum=True)
     assert ok(dx) and torch.equal(dw.double(), a.double().t() @ x.double())
+
+
+def _spread(rows, cols, fmt, g):
+    """codes over the whole of a format, the largest and the smallest among them, as values"""
+    codes = torch.arange(256, dtype=torch.uint8, device="cuda").view(fmt).float()
+    codes = codes[torch.isfinite(codes)]
+    return codes[torch.randint(0, codes.numel(), (rows, cols), generator=g, device="cuda")]
+
+
+def _scaled(values, scale, block):
+    """value64 [rows, cols] of codes' values under scales [S, KB] (float64)"""
+    f = scale.repeat_interleave(128, dim=1)[:, :values.shape[1]]
+    if block == "tiles":
+        f = f.repeat_interleave(128, dim=0)[:values.shape[0]]
+    return values.double() * f
+
+
+SCALE_FORMS = [(3, 70, 600), (20, 130, 520), (7, 90, 8300), (100, 200, 640), (40, 70, 2400), (1500, 1540, 300), (1800, 1930, 260), (4000, 4000, 260)]
+
+
+def _check_scaled(out, av, bv, K, fast):
+    """Where the terms' magnitudes stay within fp32: the sum's own loss, roundings of the block's factor, product and addition
+    (three half steps of the block's share), and what lies below the normal range, at most 2^-126 an instruction (four a block).
+    Rows and columns that hold a NaN or an infinity are the caller's to look at."""
+    mag = av.abs() @ bv.abs().t()
+    ref = av @ bv.t()
+    ok = mag < 2.0 ** 127
+    lost = (K + 8) * 2.0 ** -23 * mag + (K / 32 + 4) * 2.0 ** -126
+    if fast:
+        lost = lost + 7 * 2.0 ** -13 * mag
+    half = torch.finfo(out.dtype).eps / 2
+    err = (out.double() - ref).abs()
+    assert bool(((err <= lost + half * (ref.abs() + lost)) | ~ok).all())
+    assert float(ok.float().mean()) > 0.3
+
+
+@pytest.mark.parametrize("M,N,K", SCALE_FORMS)
+@pytest.mark.parametrize("block", ["rows", "tiles"])
+def test_fp32_scales_of_any_size(M, N, K, block):
+    """Scales whose product leaves fp32 although their share of the sum does not: large against small sums, large against zero
+    blocks (which stay zero), tiny pairs, zero scales."""
+    fp8 = _fp8()
+    for fmt in (E4, E5):
+        g = torch.Generator(device="cuda").manual_seed(21)
+        a, b = _spread(M, K, fmt, g), _spread(N, K, E4, g)
+        a[0::5, 128:256] = 0
+        a[1::5] *= 2.0 ** -6 if fmt == E4 else 2.0 ** -10
+        a = a.to(fmt).float()
+        kb, s = -(-K // 128), N if block == "rows" else -(-N // 128)
+        u = lambda *shape: 1 + torch.rand(*shape, generator=g, device="cuda")
+        pick = lambda n, e: torch.tensor(e, device="cuda", dtype=torch.float64)[torch.arange(n, device="cuda") % len(e)]
+        two = torch.tensor(2.0, dtype=torch.float64, device="cuda")
+        sa = (torch.pow(two, pick(M, [0, 66, -100, 100, -70, 40]))[:, None] * u(M, kb)).float()
+        sb = (torch.pow(two, pick(s, [66, 0, -120, 20, 80] if block == "rows" else [66, -60]))[:, None] * u(s, kb)).float()
+        sa[0::5, 1] = 3e38
+        sa[2, 0] = 0
+        qa = fp8.Fp8Matrix(_matrix(fp8, a, fmt).data, sa.t().contiguous(), K, "rows")
+        qb = fp8.Fp8Matrix(_matrix(fp8, b).data, sb.t().contiguous(), K, block)
+        av, bv = _scaled(a, sa.double(), "rows"), _scaled(b, sb.double(), block)
+        _check_scaled(fp8.matmul_fp8(qa, qb, out_dtype=torch.float32), av, bv, K, False)
+        _check_scaled(fp8.matmul_fp8(qa, qb, fast_accum=True), av, bv, K, True)
+        sa[1, 0] = float("nan")
+        qa = fp8.Fp8Matrix(qa.data, sa.t().contiguous(), K, "rows")
+        out = fp8.matmul_fp8(qa, qb, out_dtype=torch.float32)
+        assert bool(torch.isnan(out[1]).all()) and not bool(torch.isnan(out[2]).any())
