@@ -764,8 +764,9 @@ int sm_fp8_quantize(const void* x, int x_type, int rows, int cols, size_t x_stri
  * block, B [N][K] (e4m3) per row and block or per tile (b_tiles). The codes are widened to bf16, the sums held in fp32 and rounded
  * once to out_type. out_type = SM_TYPE_BF16 | SM_FP8_FAST_SUM (no other type takes the flag) permits the 8-bit matrix
  * instruction, up to twice as fast: its sum of eight products keeps 13 bits below the largest of them, so a result may be off by
- * 7 * 2^-13 of sum |a||b| (however small the result is). scale_f32: both scale arrays are floats, of any value: a block's
- * sum leaves fp32 only where sum * sa * sb does. a, b: 16-byte
+ * 7 * 2^-13 of sum |a||b| (however small the result is). scale_f32: both scale arrays are floats. Scales of either kind
+ * may have any value: a block's part leaves fp32 only where its sum * sa * sb does (below 2^-126 it may become 0); scales so far
+ * from 1 that their product alone might, cost a second pass over their share. a, b: 16-byte
  * aligned, scales 4-byte aligned, pitches multiples of 16, at least K rounded up to 128 and at most 0xfffff0; M, N < 2^30.
  * ws: sm_fp8_matmul_ws_bytes(M, N, K) bytes (0: may be NULL) of scratch of this call's own. K = 0: zeros / out as it is. */
 size_t sm_fp8_matmul_ws_bytes(int M, int N, int K);

@@ -568,7 +568,9 @@ __device__ __forceinline__ void meet() {
 }
 
 // An operand's 32 codes of a lane as bf16, scaled by 2^(byte - 127): e4m3 / e5m2 have 4 / 3 significant bits, bf16 has 8 and
-// fp32's exponents, so this is exact. scale: the byte in the exponent field of a float.
+// fp32's exponents, so this is exact where bf16 holds code 2^(byte - 127) as a normal number: bytes 32 ... 223 do for every code (17
+// ... 239 of e5m2, 10 ... 246 of e4m3). Beyond them the scale is applied to the block's sum. scale: the byte in the
+// exponent field of a float.
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 struct Wide {
     bf16x8 p[4];
@@ -618,6 +620,12 @@ struct ScaleRange {
 __device__ __forceinline__ float apart(float c, float sa, float sb) {
     return __builtin_amdgcn_ldexpf(c * (__builtin_amdgcn_frexp_mantf(sa) * __builtin_amdgcn_frexp_mantf(sb)),
                                    __builtin_amdgcn_frexp_expf(sa) + __builtin_amdgcn_frexp_expf(sb));
+}
+// the top bit of every byte of d that is in 32 ... 223 (its three top bits are not alike)
+__device__ __forceinline__ unsigned bytes_near(unsigned d) { return (d ^ (d << 1)) | (d ^ (d << 2)); }
+// c 2^(a - 127) 2^(b - 127), rounded once
+__device__ __forceinline__ float apart(float c, int a, int b) {
+    return a == 255 || b == 255 ? __builtin_bit_cast(float, 0x7fc00000u) : __builtin_amdgcn_ldexpf(c, a + b - 254);
 }
 // c[i] += b[i] a over a block of 128 for N rows of tiles: the four instructions of one result depend on each other, so the
 // tiles take turns
@@ -739,6 +747,7 @@ __device__ __forceinline__ void matmul_tile(const MatmulArgs& g, int block) {
     i32x8 b[TN], a;
     constexpr bool BOTH = SC == SCALE_F32_TILES;
     ScaleRange range;
+    unsigned near = ~0u;
     auto step = [&](auto opc, int k) {
         constexpr int OP = decltype(opc)::value;
         const int buf = NST == 2 || NST == 4 ? OP % NST : cur, nbuf = NST == 2 || NST == 4 ? (OP + 1) % NST : cur + 1 == NST ? 0 : cur + 1;
@@ -751,6 +760,11 @@ __device__ __forceinline__ void matmul_tile(const MatmulArgs& g, int block) {
 #pragma unroll
             for (int j = 0; j < TM; ++j) range.take((unsigned)sa[j]);
             if constexpr (BOTH) range.take((unsigned)sb[0]);
+        } else if constexpr (!NATIVE && OP == 0) {
+#pragma unroll
+            for (int j = 0; j < TM; ++j) near &= bytes_near((unsigned)sa[j]);
+#pragma unroll
+            for (int i = 0; i < TN; ++i) near &= bytes_near((unsigned)sb[i]);
         }
         Wide bw[NATIVE ? 1 : TN];
         if constexpr (!NATIVE) {
@@ -814,37 +828,42 @@ __device__ __forceinline__ void matmul_tile(const MatmulArgs& g, int block) {
         }
         meet<0>();      // no load into this block's LDS may outlive it
     }
-    // Scales beyond the range are rare and known only once they are read: the tile is then summed again, block by block, with them
-    // held apart. (A branch in every step keeps the matrix instructions from overlapping the multiply-adds: 4096^3 123 -> 203 us.)
-    if constexpr (F32S) {
-        if (__syncthreads_or(range.far(BOTH))) {
+    // Scales beyond the range are rare and known only once they are read: a wave that met one sums its share again, block by block
+    // from memory, with the scales held apart. (A branch in every step keeps the matrix instructions from overlapping the
+    // multiply-adds: 4096^3 123 -> 203 us.)
+    if constexpr (F32S || !NATIVE) {
+        if (__any(F32S ? range.far(BOTH) : (near & 0x80808080u) != 0x80808080u)) {
 #pragma unroll
             for (int i = 0; i < TN; ++i)
 #pragma unroll
                 for (int j = 0; j < TM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            const auto codes = [&](const uint8_t* base, size_t pitch, int row, int kb) {
+                const uint8_t* p = base + (size_t)row * pitch + (size_t)kb * 128 + lg * 16;
+                return join(*reinterpret_cast<const u32x4*>(p), *reinterpret_cast<const u32x4*>(p + 64));
+            };
             for (int kb = kb0; kb < kb1; ++kb) {
-                stage(0, kb);
-                load_scales(kb, sa, sb);
-                meet<0>();
+                load_scales(F32S ? kb : kb >> 2, sa, sb);
+                const auto byte = [&](int dword) { return dword >> (8 * (kb & 3)) & 255; };
 #pragma unroll
                 for (int j = 0; j < TM; ++j) {
-                    const i32x8 fa = frag(lds[0], wm * TM + j);
+                    const i32x8 ca = codes(g.a, g.a_pitch, min(m0 + (wm * TM + j) * 16 + lr, g.M - 1), kb);
 #pragma unroll
                     for (int i = 0; i < TN; ++i) {
-                        const i32x8 fb = frag(lds[0] + BM * 128, wn * TN + i);
+                        const i32x8 cb = codes(g.b, g.b_pitch, min(n0 + (wn * TN + i) * 16 + lr, g.N - 1), kb);
                         f32x4 c = {0.f, 0.f, 0.f, 0.f};
                         if constexpr (NATIVE) {
-                            c = mfma_block<0, FA>(fb, fa, c, 0x7f7f7f7f, 0x7f7f7f7f);
+                            c = mfma_block<0, FA>(cb, ca, c, 0x7f7f7f7f, 0x7f7f7f7f);
                         } else {
-                            const Wide w = widen<SM_FP8_E4M3>(fb, 1.f);
-                            mfma_wide<1>(&w, widen<FA>(fa, 1.f), &c);
+                            const Wide w = widen<SM_FP8_E4M3>(cb, 1.f);
+                            mfma_wide<1>(&w, widen<FA>(ca, 1.f), &c);
                         }
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            acc[i][j][e] += apart(c[e], as_float(sa[j]), as_float(sb[SC == SCALE_F32_ROWS ? 4 * i + e : 0]));
+                        for (int e = 0; e < 4; ++e) {
+                            if constexpr (F32S) acc[i][j][e] += apart(c[e], as_float(sa[j]), as_float(sb[SC == SCALE_F32_ROWS ? 4 * i + e : 0]));
+                            else acc[i][j][e] += apart(c[e], byte(sa[j]), byte(__shfl(sb[i], lg * 4 + e, 64)));      // (sb: of operand row lr)
+                        }
                     }
                 }
-                meet<0>();      // (the stage has been read)
             }
         }
     }
@@ -1034,6 +1053,22 @@ __global__ __launch_bounds__(STREAM_WAVES * 64) void fp8_stream_kernel(StreamArg
                 } else {
                     codes = join(av[u][j][0], av[u][j][1]);
                     byte = sa[u][j];
+                }
+                if constexpr (!F32S && !NATIVE) {
+                    bool far = (unsigned)(byte - 32) >= 192;
+#pragma unroll
+                    for (int i = 0; i < TB; ++i) far |= (unsigned)(sb[u][i] - 32) >= 192;
+                    if (__any(far)) {      // (bound by memory: the branch costs nothing here)
+#pragma unroll
+                        for (int i = 0; i < TB; ++i) {
+                            const Wide w = widen<SM_FP8_E4M3>(bc[i], 1.f);
+                            f32x4 c = {0.f, 0.f, 0.f, 0.f};
+                            mfma_wide<1>(&w, widen<FA>(codes, 1.f), &c);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) acc[j][i][e] += apart(c[e], byte, __shfl(sb[u][i], lg * 4 + e, 64));
+                        }
+                        continue;
+                    }
                 }
                 f32x4 c[TB];
 #pragma unroll

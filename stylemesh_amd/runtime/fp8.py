@@ -221,7 +221,7 @@ def fp8_quantize(x: torch.Tensor, block: str = "rows", fmt: str = "e4m3", transp
     transpose - as an ``Fp8Matrix`` with power-of-two scales: per block the smallest power of two that brings the largest
     finite magnitude into the format's range; x / scale is exact, the code is it rounded to nearest even. NaN stays NaN, an
     infinity becomes NaN (e4m3 has none) or infinity (e5m2); neither touches its neighbours' scale. (A magnitude from
-    1.9375 * 2^127 on rounds up to 2^128, which fp32 does not hold: its products are infinite.)"""
+    1.9375 * 2^127 on rounds up to 2^128, which fp32 does not hold: ``dequantize`` shows infinity.)"""
     n, t = _quantize(x, block, fmt, not transpose, bool(transpose))
     return t if transpose else n
 

@@ -179,3 +179,50 @@ def test_fp32_scales_of_any_size(M, N, K, block):
         qa = fp8.Fp8Matrix(qa.data, sa.t().contiguous(), K, "rows")
         out = fp8.matmul_fp8(qa, qb, out_dtype=torch.float32)
         assert bool(torch.isnan(out[1]).all()) and not bool(torch.isnan(out[2]).any())
+
+
+@pytest.mark.parametrize("M,N,K", SCALE_FORMS)
+@pytest.mark.parametrize("block", ["rows", "tiles"])
+def test_scale_bytes_of_any_size(M, N, K, block):
+    """Bytes from 0 (2^-127) to 254 under the largest and the smallest codes: values that bf16 or fp32 could not hold, in sums
+    that fp32 does."""
+    fp8 = _fp8()
+    for fmt in (E4, E5):
+        g = torch.Generator(device="cuda").manual_seed(22)
+        a, b = _spread(M, K, fmt, g), _spread(N, K, E4, g)
+        kb, s = -(-K // 128), N if block == "rows" else -(-N // 128)
+        pick = lambda n, e: torch.tensor(e, device="cuda", dtype=torch.int32)[torch.arange(n, device="cuda") % len(e)]
+        ea = pick(M, [0, 127, 254, 3, 200, 30, 225])[:, None] + torch.randint(0, 2, (M, kb), generator=g, device="cuda", dtype=torch.int32)
+        eb = pick(s, [254, 127, 0, 60, 226] if block == "rows" else [253, 0])[:, None].expand(s, kb).contiguous()
+        ea.clamp_(max=254)
+        qa = fp8.Fp8Matrix.from_parts(_matrix(fp8, a, fmt).data[:, :K], ea, "rows")
+        qb = fp8.Fp8Matrix.from_parts(_matrix(fp8, b).data[:, :K], eb, block)
+        two = torch.tensor(2.0, dtype=torch.float64, device="cuda")
+        av, bv = _scaled(a, torch.pow(two, ea.double() - 127), "rows"), _scaled(b, torch.pow(two, eb.double() - 127), block)
+        _check_scaled(fp8.matmul_fp8(qa, qb, out_dtype=torch.float32), av, bv, K, False)
+        _check_scaled(fp8.matmul_fp8(qa, qb, fast_accum=True), av, bv, K, True)
+        ea[1, 0] = 255
+        out = fp8.matmul_fp8(fp8.Fp8Matrix(qa.data, fp8.pack_scale_bytes(ea), K), qb, out_dtype=torch.float32)
+        assert bool(torch.isnan(out[1]).all()) and not bool(torch.isnan(out[0]).any())
+
+
+@pytest.mark.parametrize("M", [1, 16, 40, 200])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_layer_passes_over_the_whole_range(M, dtype):
+    """Activations and output gradients near both ends of fp32 against weights that bring them back."""
+    fp8 = _fp8()
+    N, K = 70, 300
+    g = torch.Generator(device="cuda").manual_seed(23)
+    for ex, ew in ((-125, 100), (120, -110), (-139, 120)):
+        if ex < -133 and dtype == torch.bfloat16:
+            continue
+        x = (torch.randn(M, K, generator=g, device="cuda", dtype=torch.float64) * 2.0 ** ex).to(dtype)
+        w = (torch.randn(N, K, generator=g, device="cuda", dtype=torch.float64) * 2.0 ** ew).float()
+        w8, w8t = fp8.fp8_quantize_both(w, "tiles")
+        xv, wv = R.requantized(x).cuda(), R.requantized(w, "tiles").cuda()
+        for y in (fp8.linear_fp8_fwd(x, w8, out_dtype=torch.float32), fp8.linear_fp8_fwd(x, w8, out_dtype=torch.float32, keep_transposed=True)[0]):
+            _check_scaled(y, xv, wv, K, False)
+        dy = (torch.randn(M, N, generator=g, device="cuda", dtype=torch.float64) * 2.0 ** ex).to(dtype)
+        dx, dw = fp8.linear_fp8_bwd(dy, fp8.fp8_quantize((x.double() * 2.0 ** (ew - ex)).float(), transpose=True), w8t, dx_dtype=torch.float32)
+        _check_scaled(dx, R.requantized(dy).cuda(), wv.t(), N, False)
+        _check_scaled(dw, R.requantized(dy.t()).cuda(), R.requantized((x.double() * 2.0 ** (ew - ex)).float().t()).cuda(), M, False)
