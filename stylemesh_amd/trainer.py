@@ -71,12 +71,24 @@ class JsonlLogger:
         self._pending.clear()
 
 
+def _clip_gradients(params, max_norm):
+    grads = [q.grad for q in params if q.grad is not None]
+    here = torch.cuda.current_device() if grads and grads[0].is_cuda else None
+    if here is not None and all(g.get_device() == here and g.layout == torch.strided
+                                and g.dtype in (torch.float32, torch.bfloat16, torch.float16) for g in grads):
+        from .runtime.gradclip import clip_grad_norm
+        clip_grad_norm(grads, max_norm)
+    else:
+        torch.nn.utils.clip_grad_norm_(params, max_norm)
+
+
 class MiniTrainer:
     def __init__(self, max_epochs=1, logger=None, device=None, rank=0, world_size=1, limit_train_batches=None,
                  limit_val_batches=None, progress=True, gradient_clip_val=0.0):
         """``gradient_clip_val`` (Lightning's Trainer flag; 0 / None: off): the gradients' global 2-norm is clipped to it between
-        backward and the optimizer step - inside the fused update for the texture pipeline, in place on ``param.grad``
-        (``runtime.gradclip.clip_grad_norm``) for any other module."""
+        backward and the optimizer step - inside the fused update for the texture pipeline, in place on ``param.grad`` for any
+        other module: by ``runtime.gradclip.clip_grad_norm`` where it takes the gradients, by torch where they lie on the host, on
+        another device than the current one or in another type."""
         self.gradient_clip_val = 0.0 if gradient_clip_val is None else float(gradient_clip_val)
         if not self.gradient_clip_val >= 0.0:
             raise ValueError(f"gradient_clip_val={gradient_clip_val}: a number >= 0 (0 = no clipping)")
@@ -227,8 +239,7 @@ class MiniTrainer:
                     out["loss"].backward()
                 t_e = time.perf_counter() if timing else 0.0
                 if self.gradient_clip_val and not fused_clip:
-                    from .runtime.gradclip import clip_grad_norm
-                    clip_grad_norm([q.grad for group in opt.param_groups for q in group["params"]], self.gradient_clip_val)
+                    _clip_gradients([q for group in opt.param_groups for q in group["params"]], self.gradient_clip_val)
                 opt.step()
                 self.global_step += 1
                 if timing:

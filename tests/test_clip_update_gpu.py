@@ -200,3 +200,19 @@ def test_refused_values():
         with pytest.raises(ValueError):
             MiniTrainer(gradient_clip_val=bad, logger=object())
     assert MiniTrainer(gradient_clip_val=None, logger=object()).gradient_clip_val == 0.0
+
+
+def test_trainer_clips_double_gradients_on_the_device():
+    """A type that the device operators refuse."""
+    require_gpu()
+    from stylemesh_amd.trainer import _clip_gradients
+    g = torch.Generator().manual_seed(4)
+    params = [torch.nn.Parameter(torch.zeros(3, 5, dtype=torch.float64, device="cuda")), torch.nn.Parameter(torch.zeros(7, device="cuda")),
+              torch.nn.Parameter(torch.zeros(2, device="cuda"))]
+    for q in params[:2]:
+        q.grad = torch.randn(q.shape, generator=g).to(q) * 10
+    want = [q.grad.double().clone() for q in params[:2]]
+    norm = math.sqrt(sum(float(w.square().sum()) for w in want))
+    _clip_gradients(params, 0.5)
+    for q, w in zip(params, want):
+        assert ((q.grad.double() - w * (0.5 / (norm + 1e-6))).abs() <= 2.0 ** -20 * w.abs()).all()
