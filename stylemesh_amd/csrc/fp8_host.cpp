@@ -63,6 +63,11 @@ bool launch(const char* what, F f) {
     return e == 0;
 }
 
+// a caller's tensor was written behind autograd's back: its version counter rises, as after any in-place operation
+void written(const at::Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();      // (inference tensors have no counter)
+}
+
 // room for a matrix of 8-bit codes: (codes, scales, (pointer, pointer)) for Python, the pointers for the library
 PyObject* coded(int64_t rows, int64_t cols, int fmt, int tiles, int device, void** q, void** s) {
     const int64_t kb = (cols + BLOCK - 1) / BLOCK;
@@ -141,8 +146,9 @@ PyObject* matmul(PyObject*, PyObject* const* a, Py_ssize_t n) {
             }))
             return nullptr;
     }
-    if (given != Py_None) return Py_NewRef(given);
-    return THPVariable_Wrap(std::move(out));
+    if (given == Py_None) return THPVariable_Wrap(std::move(out));
+    written(out);
+    return Py_NewRef(given);
     END_HANDLE_TH_ERRORS
 }
 
@@ -217,6 +223,7 @@ PyObject* backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
                                           xts, xt_tiles, (size_t)xt_pitch, dxp, result_type(type, fast), (size_t)K, (float*)dwp, (size_t)w.stride, accumulate, sp, need, stream);
         }))
         return nullptr;
+    if (xt && given != Py_None) written(dw);
     return Py_BuildValue("NN", wt ? THPVariable_Wrap(std::move(dx)) : Py_NewRef(Py_None),
                          !xt ? Py_NewRef(Py_None) : given != Py_None ? Py_NewRef(given) : THPVariable_Wrap(std::move(dw)));
     END_HANDLE_TH_ERRORS

@@ -118,9 +118,28 @@ PyObject* check_outputs(PyObject*, PyObject* args) {
     return PyLong_FromLong(0);
 }
 
+// written(list): the tensors have been written behind autograd's back; their version counters rise, as after any in-place operation
+PyObject* written(PyObject*, PyObject* arg) {
+    if (!PyList_Check(arg)) {
+        PyErr_SetString(PyExc_TypeError, "a list of tensors");
+        return nullptr;
+    }
+    for (Py_ssize_t i = 0; i < PyList_GET_SIZE(arg); ++i) {
+        PyObject* o = PyList_GET_ITEM(arg, i);
+        if (!THPVariable_Check(o)) {
+            PyErr_Format(PyExc_ValueError, "entry %zd is not a tensor", i);
+            return nullptr;
+        }
+        const at::Tensor& t = THPVariable_Unpack(o);
+        if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();      // (inference tensors have no counter)
+    }
+    Py_RETURN_NONE;
+}
+
 PyMethodDef METHODS[] = {
     {"pack", pack, METH_O, "list of tensors -> (table, address, odd one, device, contiguous)"},
     {"check_outputs", check_outputs, METH_VARARGS, "(inputs, outputs) -> 0, or what is wrong with the outputs"},
+    {"written", written, METH_O, "list of tensors: raises their version counters"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef MODULE = {PyModuleDef_HEAD_INIT, "_tensor_list", "Tensor lists as the library's arrays", -1, METHODS, nullptr, nullptr, nullptr, nullptr};
 

@@ -138,6 +138,7 @@ class GradClip:
         kind, max_norm = _norm_kind(norm_type), _max_norm(max_norm)
         out, ws = self._result()
         hip.check(ops.lib.sm_grad_clip(*self._args, kind, max_norm, ws.data_ptr(), self._ws_bytes, out.data_ptr(), ops.eager_stream()), "sm_grad_clip")
+        _tensor_list.written(self.out)      # (autograd refuses a graph that saved one of them before)
         return out
 
 

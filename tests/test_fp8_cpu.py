@@ -309,3 +309,36 @@ def test_fast_sums_are_for_bfloat16_results():
         assert m(t) != 0 and m(t, a9=0) != 0, t
         assert lib.sm_fp8_linear(p, 0, 200, p, p, 0, 256, 0, 6, 200, p, t, 6, p, 1 << 15, None) != 0, t
     assert m(17, a9=0) == 0 and lib.sm_fp8_linear(p, 0, 200, p, p, 0, 256, 0, 6, 200, p, 17, 6, p, 1 << 15, None) == 0
+
+
+def test_clipped_tensors_versions_rise(monkeypatch):
+    """A graph that saved a tensor before it was clipped must be refused by autograd, as after torch's own in-place operations."""
+    from stylemesh_amd import _tensor_list as tl
+    from stylemesh_amd.runtime import gradclip, ops
+    a, b, v = torch.ones(4), torch.ones(6), torch.ones(9)
+    with torch.inference_mode():
+        i = torch.ones(2)
+    before = [t._version for t in (a, v)]
+    tl.written([a, v[2:5], i])
+    assert [t._version for t in (a, v)] == [n + 1 for n in before] and b._version == 0
+    for bad, kind in (((a,), TypeError), ([a, None], ValueError)):
+        with pytest.raises(kind):
+            tl.written(bad)
+    real_pack, real_empty = tl.pack, torch.empty
+    monkeypatch.setattr(tl, "pack", lambda tensors: (*real_pack(tensors)[:3], 0, True))
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch, "empty", lambda *size, dtype, device: real_empty(*size, dtype=dtype))
+    monkeypatch.setattr(ops, "eager_stream", lambda: 0)
+    monkeypatch.setattr(ops, "lib", type("Lib", (), {"sm_grad_norm_ws_bytes": staticmethod(lambda n: 8192), "sm_grad_norm": staticmethod(lambda *a: 0),
+                                                     "sm_grad_clip": staticmethod(lambda *a: 0)}))
+    w = torch.ones(4, requires_grad=True)
+    y = (w * b[:4]).sum()
+    gradclip.clip_grad_norm([b], 1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    out, n = torch.ones(6), b._version
+    plan = gradclip.GradClip([b], [out])
+    plan.norm()
+    assert (b._version, out._version) == (n, 0)
+    plan.clip(1.0)
+    assert (b._version, out._version) == (n, 1)

@@ -600,3 +600,21 @@ def test_linear_backward_from_codes_laid_out_by_columns(M, N, K):
     xt = fp8.Fp8Matrix(codes, want.scale, M)
     for a, b in zip(fp8.linear_fp8_bwd(dy, xt, wt), fp8.linear_fp8_bwd(dy, want, wt)):
         assert torch.equal(a, b)
+
+
+def test_written_tensors_versions_rise():
+    """out and dw of the caller, and clipped gradients: autograd refuses a graph that saved what has been written since."""
+    fp8 = _fp8()
+    from stylemesh_amd.runtime.gradclip import clip_grad_norm
+    x, w = torch.ones(8, 256, device="cuda"), torch.ones(16, 256, device="cuda")
+    a, b = fp8.fp8_quantize(x), fp8.fp8_quantize(w, "tiles")
+    out, dw, g = torch.zeros(8, 16, device="cuda"), torch.zeros(16, 256, device="cuda"), torch.ones(8, 16, device="cuda")
+    for t, call in ((out, lambda: fp8.matmul_fp8(a, b, out=out)), (dw, lambda: fp8.linear_fp8_bwd(g, fp8.fp8_quantize(x, transpose=True), None, dw=dw)),
+                    (g, lambda: clip_grad_norm([g], 0.5))):
+        leaf = torch.ones(t.shape, device="cuda", requires_grad=True)
+        y = (leaf * t).sum()
+        n = t._version
+        call()
+        assert t._version == n + 1
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
