@@ -5,6 +5,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/object_ptr.h>
+#include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
 
 #include <algorithm>
@@ -26,9 +27,10 @@ struct Matrix {
     const void* p = nullptr;
     int64_t rows = 0, cols = 0, stride = 0;
     int type = -1;
-    bool take(PyObject* o, int device) {
+    bool take(PyObject* o, int device, bool in_graph) {      // in_graph: the result would belong to its autograd graph
         if (!THPVariable_Check(o)) return false;
         const at::Tensor& t = THPVariable_Unpack(o);
+        if (in_graph && t.requires_grad() && at::GradMode::is_enabled()) return false;
         if (!t.is_cuda() || t.layout() != at::kStrided || t.dim() != 2 || t.get_device() != device || t.is_neg()) return false;
         for (int i = 0; i < 3; ++i)
             if (t.scalar_type() == TYPES[i]) type = i;
@@ -88,7 +90,7 @@ PyObject* quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
     void* stream = g.pointer();
     if (PyErr_Occurred()) return nullptr;
     Matrix m;
-    if (fmt < 0 || fmt > 1 || !m.take(x, device)) Py_RETURN_NONE;
+    if (fmt < 0 || fmt > 1 || !m.take(x, device, false)) Py_RETURN_NONE;
     void *q = nullptr, *qs = nullptr, *qt = nullptr, *qts = nullptr;
     THPObjectPtr first(plain ? coded(m.rows, m.cols, fmt, tiles, device, &q, &qs) : Py_NewRef(Py_None));
     THPObjectPtr second(transpose ? coded(m.cols, m.rows, fmt, tiles, device, &qt, &qts) : Py_NewRef(Py_None));
@@ -127,7 +129,7 @@ PyObject* matmul(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Matrix o;
     at::Tensor out;
     if (given != Py_None) {
-        if (!o.take(given, device) || o.rows != M || o.cols != N) Py_RETURN_NONE;
+        if (!o.take(given, device, true) || o.rows != M || o.cols != N) Py_RETURN_NONE;
         out = THPVariable_Unpack(given);
         type = o.type;
     } else {
@@ -166,7 +168,7 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     void* stream = g.pointer();
     if (PyErr_Occurred()) return nullptr;
     Matrix m;
-    if (!m.take(x, device) || m.cols != K || N < 0 || N > MAX_DIM || type > 2) Py_RETURN_NONE;
+    if (!m.take(x, device, true) || m.cols != K || N < 0 || N > MAX_DIM || type > 2) Py_RETURN_NONE;
     if (type < 0) type = m.type;
     at::Tensor y = room({m.rows, N}, TYPES[type], device);
     if (m.rows && N) {
@@ -204,12 +206,12 @@ PyObject* backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     void* stream = g.pointer();
     if (PyErr_Occurred()) return nullptr;
     Matrix dy, w;
-    if (!dy.take(dyo, device) || !dy.rows || !dy.cols || K <= 0 || K > MAX_DIM || fmt < 0 || fmt > 1 || type > 2) Py_RETURN_NONE;
+    if (!dy.take(dyo, device, true) || !dy.rows || !dy.cols || K <= 0 || K > MAX_DIM || fmt < 0 || fmt > 1 || type > 2) Py_RETURN_NONE;
     if (type < 0) type = dy.type;
     at::Tensor dx, dw;
     if (wt) dx = room({dy.rows, K}, TYPES[type], device);
     if (xt && given != Py_None) {
-        if (!w.take(given, device) || w.type != 0 || w.rows != dy.cols || w.cols != K) Py_RETURN_NONE;
+        if (!w.take(given, device, true) || w.type != 0 || w.rows != dy.cols || w.cols != K) Py_RETURN_NONE;
         dw = THPVariable_Unpack(given);
     } else if (xt) {
         dw = room({dy.cols, K}, at::kFloat, device);

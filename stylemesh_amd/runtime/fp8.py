@@ -4,7 +4,9 @@ feature maps against filters, activations against a resident weight, and the gra
 
 Every call is asynchronous on torch's current stream, allocates its results (and, for a product that splits its depth, its
 scratch) from torch's allocator and synchronises nothing. There is no autograd node: ``linear_fp8_fwd`` /
-``linear_fp8_bwd`` are the two halves of a step, as the sampler's and the losses' are (``ops.tex_sample_fwd`` / ``_bwd``).
+``linear_fp8_bwd`` are the two halves of a step, as the sampler's and the losses' are (``ops.tex_sample_fwd`` / ``_bwd``), for a
+``torch.autograd.Function`` or a loop of one's own. Where autograd records, a tensor that requires a gradient is refused by them (and
+as ``out`` / ``dw``): the result would silently have none. A quantised copy never has one, whatever it is made from.
 """
 from __future__ import annotations
 
@@ -183,9 +185,17 @@ def _check_matrix(x, what):
     _check_device(x.get_device())
 
 
-def _refuse(x, what):
+def _check_no_graph(x, what):
+    if x.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what} requires a gradient and there is no autograd node: call under torch.no_grad(), in an autograd.Function, "
+                         "or with .detach()")
+
+
+def _refuse(x, what, in_graph=True):
     """The native call would not take its arguments: says why."""
     _check_matrix(x, what)
+    if in_graph:
+        _check_no_graph(x, what)
     raise ValueError(f"{what} cannot be used: {x.dtype} {tuple(x.shape)}, strides {x.stride()} on {x.device}")
 
 
@@ -203,7 +213,7 @@ def _quantize(x, block, fmt, plain, transpose):
         device = torch.cuda.current_device()
         done = _fp8_host.quantize(x, fid, tiles, plain, transpose, device, ops.eager_stream())
     if done is None:
-        _refuse(x, "x")
+        _refuse(x, "x", in_graph=False)
     rows, cols, n, t = done
     if plain:
         q, s, ptrs = n
@@ -271,6 +281,7 @@ def matmul_fp8(a: Fp8Matrix, b: Fp8Matrix, out: torch.Tensor | None = None, out_
         fast = _check_fast(fast_accum, out_dtype)
     else:
         _check_matrix(out, "out")
+        _check_no_graph(out, "out")
         if tuple(out.shape) != (M, N) or (out_dtype is not None and out.dtype != out_dtype):
             raise ValueError(f"out is {out.dtype} {tuple(out.shape)}, the product {out_dtype or out.dtype} {(M, N)}")
         dtype = 0
@@ -293,6 +304,8 @@ def linear_fp8_fwd(x: torch.Tensor, weight: Fp8Matrix, out_dtype=None, keep_tran
     if out_dtype is not None and out_dtype not in _TYPE_ID:
         raise ValueError(f"out_dtype={out_dtype}: float32, bfloat16 or float16")
     if keep_transposed:
+        if isinstance(x, torch.Tensor):
+            _check_no_graph(x, "x")
         n, t = _quantize(x, "rows", "e4m3", True, True)
         return matmul_fp8(n, weight, out_dtype=x.dtype if out_dtype is None else out_dtype, fast_accum=fast_accum), t
     if fast_accum:
@@ -304,6 +317,7 @@ def linear_fp8_fwd(x: torch.Tensor, weight: Fp8Matrix, out_dtype=None, keep_tran
                              -1 if out_dtype is None else _TYPE_ID[out_dtype], bool(fast_accum), weight._device, ops.eager_stream())
     if y is None:
         _check_matrix(x, "x")
+        _check_no_graph(x, "x")
         if x.shape[1] != weight._cols:
             raise ValueError(f"x has {x.shape[1]} columns, the weight {weight._cols}")
         _check_device(weight._device)
@@ -320,6 +334,7 @@ def linear_fp8_bwd(dy: torch.Tensor, x_t: Fp8Matrix | None, weight_t: Fp8Matrix 
     None: that gradient is not computed and None is returned in its place. ``fast_accum``: as ``matmul_fp8``'s, for dx; dw is
     always summed in fp32."""
     _check_matrix(dy, "dy")
+    _check_no_graph(dy, "dy")
     M, N = dy.shape
     if x_t is None and weight_t is None:
         raise ValueError("nothing to compute: both x_t and weight_t are None")
@@ -348,6 +363,7 @@ def linear_fp8_bwd(dy: torch.Tensor, x_t: Fp8Matrix | None, weight_t: Fp8Matrix 
         raise ValueError(f"a dimension above {_MAX_DIM}")
     if dw is not None:
         _check_matrix(dw, "dw")
+        _check_no_graph(dw, "dw")
     _check_device(None if weight_t is None else weight_t._device, None if x_t is None else x_t._device)
     if not (M and N and K):      # a gradient without elements, or a sum without terms
         if weight_t is not None:

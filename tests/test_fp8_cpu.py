@@ -342,3 +342,13 @@ def test_clipped_tensors_versions_rise(monkeypatch):
     assert (b._version, out._version) == (n, 0)
     plan.clip(1.0)
     assert (b._version, out._version) == (n, 1)
+
+
+def test_tensors_of_a_recording_graph_are_refused_on_the_host_too():
+    b, x = mat(6, 200), torch.zeros(4, 200, requires_grad=True)
+    for f in (lambda: fp8._check_no_graph(x, "x"), lambda: fp8._check_no_graph(x * 2, "x"), lambda: fp8.linear_fp8_fwd(x, b, keep_transposed=True)):
+        with pytest.raises(ValueError, match="requires a gradient"):
+            f()
+    with torch.no_grad():
+        fp8._check_no_graph(x, "x")
+    fp8._check_no_graph(x.detach(), "x")

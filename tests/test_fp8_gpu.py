@@ -618,3 +618,41 @@ def test_written_tensors_versions_rise():
         assert t._version == n + 1
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             y.backward()
+
+
+def test_tensors_of_a_recording_graph_are_refused():
+    """A result without a gradient must not come back silently; quantising a parameter is fine, and so are the two halves inside an
+    autograd.Function, whose gradients are the halves' own."""
+    fp8 = _fp8()
+    w = torch.nn.Parameter(_rand(70, 300, 1, spread=0.3).cuda())
+    w8, w8t = fp8.fp8_quantize_both(w, "tiles")
+    assert not w8.scales().requires_grad
+    for x in (torch.ones(4, 300, device="cuda", requires_grad=True), torch.ones(4, 300, device="cuda", requires_grad=True) * 2):
+        q = fp8.fp8_quantize(x)
+        out = torch.zeros(4, 70, device="cuda", requires_grad=True)
+        dy = torch.ones(4, 70, device="cuda")
+        _, xt = fp8.fp8_quantize_both(x)
+        for f in (lambda: fp8.linear_fp8_fwd(x, w8), lambda: fp8.linear_fp8_fwd(x, w8, keep_transposed=True), lambda: fp8.matmul_fp8(q, w8, out=out),
+                  lambda: fp8.linear_fp8_bwd(dy.clone().requires_grad_(), xt, w8t), lambda: fp8.linear_fp8_bwd(dy, xt, w8t, dw=w)):
+            with pytest.raises(ValueError, match="requires a gradient"):
+                f()
+        with torch.no_grad():
+            y = fp8.linear_fp8_fwd(x, w8)
+        assert torch.equal(y, fp8.linear_fp8_fwd(x.detach(), w8)) and not out.any()
+
+    class Layer(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, w):
+            w8, ctx.wt = fp8.fp8_quantize_both(w, "tiles")
+            y, ctx.xt = fp8.linear_fp8_fwd(x, w8, keep_transposed=True)
+            return y
+
+        @staticmethod
+        def backward(ctx, dy):
+            return fp8.linear_fp8_bwd(dy, ctx.xt, ctx.wt)
+
+    x = torch.nn.Parameter(_rand(40, 300, 2, spread=0.3).cuda())
+    dy = _rand(40, 70, 3, spread=0.3).cuda()
+    Layer.apply(x, w).backward(dy)
+    dx, dw = fp8.linear_fp8_bwd(dy, fp8.fp8_quantize(x, transpose=True), w8t)
+    assert torch.equal(x.grad, dx) and torch.equal(w.grad, dw)
