@@ -42,6 +42,24 @@ struct Matrix {
     }
 };
 
+// A matrix of 8-bit codes as its Fp8Matrix keeps it: its addresses are read at every call. False where its tensors no longer hold
+// what the matrix was made of (memory given up or exchanged since: a weight that was moved away, for one).
+bool holds(const at::Tensor& t, int64_t bytes, int device) {
+    return t.is_cuda() && t.get_device() == device && t.is_contiguous() && (int64_t)t.nbytes() == bytes &&
+           t.storage_offset() * (int64_t)t.itemsize() + bytes <= (int64_t)t.storage().nbytes();
+}
+struct Coded {
+    const void *codes = nullptr, *scale = nullptr;
+    bool take(PyObject* data, PyObject* scales, int64_t rows, int64_t pitch, int tiles, int f32, int device) {
+        if (!THPVariable_Check(data) || !THPVariable_Check(scales)) return false;
+        const at::Tensor &d = THPVariable_Unpack(data), &s = THPVariable_Unpack(scales);
+        const int64_t kb = pitch / BLOCK, sr = tiles ? (rows + BLOCK - 1) / BLOCK : rows;
+        if (!holds(d, rows * pitch, device) || !holds(s, f32 ? kb * sr * 4 : (kb + 3) / 4 * sr * 4, device)) return false;
+        codes = d.const_data_ptr(), scale = s.const_data_ptr();
+        return (uintptr_t)codes % 16 == 0 && (uintptr_t)scale % 4 == 0;
+    }
+};
+
 // The arguments of a call, taken in order. Integers and pointers only; a tensor or None is taken as the object.
 struct Args {
     PyObject* const* a;
@@ -70,14 +88,13 @@ void written(const at::Tensor& t) {
     if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();      // (inference tensors have no counter)
 }
 
-// room for a matrix of 8-bit codes: (codes, scales, (pointer, pointer)) for Python, the pointers for the library
+// room for a matrix of 8-bit codes: (codes, scales) for Python, the pointers for the library
 PyObject* coded(int64_t rows, int64_t cols, int fmt, int tiles, int device, void** q, void** s) {
     const int64_t kb = (cols + BLOCK - 1) / BLOCK;
     at::Tensor codes = room({rows, kb * BLOCK}, FORMATS[fmt], device);
     at::Tensor scale = room({(kb + 3) / 4, tiles ? (rows + BLOCK - 1) / BLOCK : rows, 4}, at::kByte, device);
     *q = codes.data_ptr(), *s = scale.data_ptr();
-    return Py_BuildValue("NN(KK)", THPVariable_Wrap(std::move(codes)), THPVariable_Wrap(std::move(scale)), (unsigned long long)*q,
-                         (unsigned long long)*s);
+    return Py_BuildValue("NN", THPVariable_Wrap(std::move(codes)), THPVariable_Wrap(std::move(scale)));
 }
 
 // quantize(x, fmt, tiles, plain, transpose, device, stream) -> (rows, cols, parts or None, parts or None)
@@ -112,10 +129,10 @@ PyObject* matmul(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     if (!expect(n, 18)) return nullptr;
     Args g{a, n};
-    void *ap = g.pointer(), *as = g.pointer();
+    PyObject *ac = g.object(), *as = g.object();
     const int a_fmt = (int)g.integer();
     const long a_pitch = g.integer();
-    void *bp = g.pointer(), *bs = g.pointer();
+    PyObject *bc = g.object(), *bs = g.object();
     const int b_tiles = (int)g.integer();
     const long b_pitch = g.integer();
     const int f32 = (int)g.integer();
@@ -126,6 +143,8 @@ PyObject* matmul(PyObject*, PyObject* const* a, Py_ssize_t n) {
     void* stream = g.pointer();
     if (PyErr_Occurred()) return nullptr;
     if (M < 0 || N < 0 || K < 0 || M > MAX_DIM || N > MAX_DIM || K > MAX_DIM) Py_RETURN_NONE;
+    Coded ca, cb;
+    if (!ca.take(ac, as, M, a_pitch, 0, f32, device) || !cb.take(bc, bs, N, b_pitch, b_tiles, f32, device)) Py_RETURN_NONE;
     Matrix o;
     at::Tensor out;
     if (given != Py_None) {
@@ -143,7 +162,7 @@ PyObject* matmul(PyObject*, PyObject* const* a, Py_ssize_t n) {
         at::Tensor ws = need ? room({(int64_t)need}, at::kByte, device) : at::Tensor();
         void *op = out.data_ptr(), *wp = need ? ws.data_ptr() : nullptr;
         if (!launch("sm_fp8_matmul", [&] {
-                return sm_fp8_matmul(ap, as, a_fmt, (size_t)a_pitch, bp, bs, b_tiles, (size_t)b_pitch, f32, (int)M, (int)N, (int)K, op,
+                return sm_fp8_matmul(ca.codes, ca.scale, a_fmt, (size_t)a_pitch, cb.codes, cb.scale, b_tiles, (size_t)b_pitch, f32, (int)M, (int)N, (int)K, op,
                                      result_type(type, fast), (size_t)o.stride, accumulate, wp, need, stream);
             }))
             return nullptr;
@@ -160,7 +179,7 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!expect(n, 11)) return nullptr;
     Args g{a, n};
     PyObject* x = g.object();
-    void *w = g.pointer(), *ws = g.pointer();
+    PyObject *wc = g.object(), *ws = g.object();
     const int tiles = (int)g.integer();
     const long pitch = g.integer(), N = g.integer(), K = g.integer();
     int type = (int)g.integer();
@@ -169,6 +188,8 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (PyErr_Occurred()) return nullptr;
     Matrix m;
     if (!m.take(x, device, true) || m.cols != K || N < 0 || N > MAX_DIM || type > 2) Py_RETURN_NONE;
+    Coded w;
+    if (!w.take(wc, ws, N, pitch, tiles, 0, device)) Py_RETURN_NONE;
     if (type < 0) type = m.type;
     at::Tensor y = room({m.rows, N}, TYPES[type], device);
     if (m.rows && N) {
@@ -176,7 +197,7 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
         at::Tensor scratch = need ? room({(int64_t)need}, at::kByte, device) : at::Tensor();      // of this call's own, as matmul's
         void *yp = y.data_ptr(), *sp = need ? scratch.data_ptr() : nullptr;
         if (!launch("sm_fp8_linear", [&] {
-                return sm_fp8_linear(m.p, m.type, (size_t)m.stride, w, ws, tiles, (size_t)pitch, (int)m.rows, (int)N, (int)K, yp,
+                return sm_fp8_linear(m.p, m.type, (size_t)m.stride, w.codes, w.scale, tiles, (size_t)pitch, (int)m.rows, (int)N, (int)K, yp,
                                      result_type(type, fast), (size_t)N, sp, need, stream);
             }))
             return nullptr;
@@ -194,10 +215,10 @@ PyObject* backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     PyObject* dyo = g.object();
     const int fmt = (int)g.integer();
     const long K = g.integer();
-    void *wt = g.pointer(), *wts = g.pointer();
+    PyObject *wtc = g.object(), *wts = g.object();
     const int wt_tiles = (int)g.integer();
     const long wt_pitch = g.integer();
-    void *xt = g.pointer(), *xts = g.pointer();
+    PyObject *xtc = g.object(), *xts = g.object();
     const int xt_tiles = (int)g.integer();
     const long xt_pitch = g.integer();
     int type = (int)g.integer();
@@ -207,6 +228,9 @@ PyObject* backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (PyErr_Occurred()) return nullptr;
     Matrix dy, w;
     if (!dy.take(dyo, device, true) || !dy.rows || !dy.cols || K <= 0 || K > MAX_DIM || fmt < 0 || fmt > 1 || type > 2) Py_RETURN_NONE;
+    const bool wt = wtc != Py_None, xt = xtc != Py_None;      // the gradients wanted
+    Coded cw, cx;
+    if ((wt && !cw.take(wtc, wts, K, wt_pitch, wt_tiles, 0, device)) || (xt && !cx.take(xtc, xts, K, xt_pitch, xt_tiles, 0, device))) Py_RETURN_NONE;
     if (type < 0) type = dy.type;
     at::Tensor dx, dw;
     if (wt) dx = room({dy.rows, K}, TYPES[type], device);
@@ -217,12 +241,12 @@ PyObject* backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
         dw = room({dy.cols, K}, at::kFloat, device);
         w.stride = K;
     }
-    const size_t need = sm_fp8_linear_backward_ws_bytes((int)dy.rows, (int)dy.cols, (int)K, wt != nullptr, xt != nullptr);
+    const size_t need = sm_fp8_linear_backward_ws_bytes((int)dy.rows, (int)dy.cols, (int)K, wt, xt);
     at::Tensor scratch = room({(int64_t)need}, at::kByte, device);
     void *dxp = wt ? dx.data_ptr() : nullptr, *dwp = xt ? dw.data_ptr() : nullptr, *sp = scratch.data_ptr();
     if (!launch("sm_fp8_linear_backward", [&] {
-            return sm_fp8_linear_backward(dy.p, dy.type, (size_t)dy.stride, fmt, (int)dy.rows, (int)dy.cols, (int)K, wt, wts, wt_tiles, (size_t)wt_pitch, xt,
-                                          xts, xt_tiles, (size_t)xt_pitch, dxp, result_type(type, fast), (size_t)K, (float*)dwp, (size_t)w.stride, accumulate, sp, need, stream);
+            return sm_fp8_linear_backward(dy.p, dy.type, (size_t)dy.stride, fmt, (int)dy.rows, (int)dy.cols, (int)K, cw.codes, cw.scale, wt_tiles, (size_t)wt_pitch,
+                                          cx.codes, cx.scale, xt_tiles, (size_t)xt_pitch, dxp, result_type(type, fast), (size_t)K, (float*)dwp, (size_t)w.stride, accumulate, sp, need, stream);
         }))
         return nullptr;
     if (xt && given != Py_None) written(dw);

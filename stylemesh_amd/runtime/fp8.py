@@ -25,7 +25,7 @@ FORMATS = {"e4m3": torch.float8_e4m3fn, "e5m2": torch.float8_e5m2}
 _FMT_ID = {torch.float8_e4m3fn: 0, torch.float8_e5m2: 1}                      # SM_FP8_*
 _TYPE_ID = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}           # SM_TYPE_*
 _MAX_DIM = 65535 * 128       # rows / columns of a matrix (the quantiser's grid)
-_NO_MATRIX = (None, None, 0, 0)      # pointers, tiles?, pitch
+_NO_MATRIX = (None, None, 0, 0)      # codes, scales, tiles?, pitch
 
 
 def _blocks(n: int) -> int:
@@ -56,7 +56,7 @@ class Fp8Matrix:
     The tensors are used as they are, no copy is taken - but for codes laid out column by column (quantising ``x.t()`` in plain
     torch leaves them so), which are copied once, here."""
 
-    __slots__ = ("_data", "_scale", "_rows", "_cols", "_tiles", "_fmt", "_f32", "_ptrs", "_pitch", "_device")
+    __slots__ = ("_data", "_scale", "_rows", "_cols", "_tiles", "_fmt", "_f32", "_pitch", "_device")
 
     def __init__(self, data: torch.Tensor, scale: torch.Tensor, cols: int, block: str = "rows"):
         if block not in ("rows", "tiles"):
@@ -80,19 +80,20 @@ class Fp8Matrix:
         if scale.device != data.device:
             raise ValueError(f"codes on {data.device}, scales on {scale.device}")
         self._set(data, scale, data.shape[0], int(cols), int(block == "tiles"), _FMT_ID[data.dtype], int(scale.dtype == torch.float32),
-                  (data.data_ptr(), scale.data_ptr()), data.get_device())
+                  data.get_device())
 
-    def _set(self, data, scale, rows, cols, tiles, fmt, f32, ptrs, device):
-        # what every call hands to the library, of the tensors this object keeps (and never exchanges: the properties are
-        # read-only); device -1: host
+    def _set(self, data, scale, rows, cols, tiles, fmt, f32, device):
+        # what every call hands on, of the tensors this object keeps (and never exchanges: the properties are read-only);
+        # device -1: host
         self._data, self._scale, self._rows, self._cols, self._tiles, self._fmt, self._f32 = data, scale, rows, cols, tiles, fmt, f32
-        self._ptrs, self._pitch, self._device = ptrs, -(-cols // BLOCK) * BLOCK, device
+        self._pitch, self._device = -(-cols // BLOCK) * BLOCK, device
 
-    def __reduce__(self):      # (a copy's pointers are those of ITS tensors; torch pickles bytes, but no 8-bit floats)
+    def __reduce__(self):      # (torch pickles bytes, but no 8-bit floats)
         return _rebuild, (self._data.view(torch.uint8), self._data.dtype, self._scale, self._cols, self.block)
 
     data = property(lambda self: self._data)
     scale = property(lambda self: self._scale)
+    _ptrs = property(lambda self: (self._data.data_ptr(), self._scale.data_ptr()))
     rows = property(lambda self: self._rows)
     cols = property(lambda self: self._cols)
     block = property(lambda self: "tiles" if self._tiles else "rows")
@@ -199,6 +200,18 @@ def _refuse(x, what, in_graph=True):
     raise ValueError(f"{what} cannot be used: {x.dtype} {tuple(x.shape)}, strides {x.stride()} on {x.device}")
 
 
+def _check_held(*matrices):
+    """The native call would not take its matrices: their tensors no longer hold what they were made of."""
+    for m in matrices:
+        if m is not None:
+            try:
+                Fp8Matrix(m._data, m._scale, m._cols, m.block)
+            except (ValueError, RuntimeError) as e:
+                raise ValueError(f"the tensors of an Fp8Matrix {m.shape} were exchanged since it was made: {e}") from None
+            if m._data.shape[0] != m._rows or any(t.untyped_storage().nbytes() < t.storage_offset() * t.itemsize + t.nbytes for t in (m._data, m._scale)):
+                raise ValueError(f"the tensors of an Fp8Matrix {m.shape} were resized since it was made")
+
+
 _new = Fp8Matrix.__new__
 
 
@@ -216,13 +229,13 @@ def _quantize(x, block, fmt, plain, transpose):
         _refuse(x, "x", in_graph=False)
     rows, cols, n, t = done
     if plain:
-        q, s, ptrs = n
+        q, s = n
         n = _new(Fp8Matrix)
-        n._set(q, s, rows, cols, tiles, fid, 0, ptrs, device)
+        n._set(q, s, rows, cols, tiles, fid, 0, device)
     if transpose:
-        q, s, ptrs = t
+        q, s = t
         t = _new(Fp8Matrix)
-        t._set(q, s, cols, rows, tiles, fid, 0, ptrs, device)
+        t._set(q, s, cols, rows, tiles, fid, 0, device)
     return n, t
 
 
@@ -286,8 +299,12 @@ def matmul_fp8(a: Fp8Matrix, b: Fp8Matrix, out: torch.Tensor | None = None, out_
             raise ValueError(f"out is {out.dtype} {tuple(out.shape)}, the product {out_dtype or out.dtype} {(M, N)}")
         dtype = 0
         fast = _check_fast(fast_accum, out.dtype)
-    return _fp8_host.matmul(*a._ptrs, a._fmt, a._pitch, *b._ptrs, b._tiles, b._pitch, a._f32, M, N, K, out, dtype, bool(accumulate),
-                            fast, a._device, ops.eager_stream())
+    done = _fp8_host.matmul(a._data, a._scale, a._fmt, a._pitch, b._data, b._scale, b._tiles, b._pitch, a._f32, M, N, K, out, dtype,
+                            bool(accumulate), fast, a._device, ops.eager_stream())
+    if done is None:
+        _check_held(a, b)
+        _refuse(out, "out")
+    return done
 
 
 def _weight_arg(w, what="weight"):
@@ -313,7 +330,7 @@ def linear_fp8_fwd(x: torch.Tensor, weight: Fp8Matrix, out_dtype=None, keep_tran
         _check_fast(fast_accum, x.dtype if out_dtype is None else out_dtype)
     y = None
     if weight._device >= 0 and weight._device == torch.cuda.current_device():
-        y = _fp8_host.linear(x, *weight._ptrs, weight._tiles, weight._pitch, weight._rows, weight._cols,
+        y = _fp8_host.linear(x, weight._data, weight._scale, weight._tiles, weight._pitch, weight._rows, weight._cols,
                              -1 if out_dtype is None else _TYPE_ID[out_dtype], bool(fast_accum), weight._device, ops.eager_stream())
     if y is None:
         _check_matrix(x, "x")
@@ -321,6 +338,7 @@ def linear_fp8_fwd(x: torch.Tensor, weight: Fp8Matrix, out_dtype=None, keep_tran
         if x.shape[1] != weight._cols:
             raise ValueError(f"x has {x.shape[1]} columns, the weight {weight._cols}")
         _check_device(weight._device)
+        _check_held(weight)
         _refuse(x, "x")
     return y
 
@@ -374,8 +392,11 @@ def linear_fp8_bwd(dy: torch.Tensor, x_t: Fp8Matrix | None, weight_t: Fp8Matrix 
             elif not accumulate:
                 dw.zero_()
         return dx, dw
-    wt = (*weight_t._ptrs, weight_t._tiles, weight_t._pitch) if weight_t is not None else _NO_MATRIX
-    xt = (*x_t._ptrs, x_t._tiles, x_t._pitch) if x_t is not None else _NO_MATRIX
+    wt = (weight_t._data, weight_t._scale, weight_t._tiles, weight_t._pitch) if weight_t is not None else _NO_MATRIX
+    xt = (x_t._data, x_t._scale, x_t._tiles, x_t._pitch) if x_t is not None else _NO_MATRIX
     done = _fp8_host.backward(dy, _FMT_ID[FORMATS[fmt]], K, *wt, *xt, -1 if dx_dtype is None else _TYPE_ID[dx_dtype], dw, bool(accumulate),
                               bool(fast_accum and weight_t is not None), dy.get_device(), ops.eager_stream())
-    return done if done is not None else _refuse(dy, "dy")
+    if done is None:
+        _check_held(weight_t, x_t)
+        _refuse(dy, "dy")
+    return done

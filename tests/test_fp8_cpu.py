@@ -352,3 +352,19 @@ def test_tensors_of_a_recording_graph_are_refused_on_the_host_too():
     with torch.no_grad():
         fp8._check_no_graph(x, "x")
     fp8._check_no_graph(x.detach(), "x")
+
+
+def test_matrices_whose_tensors_were_exchanged_are_named():
+    make = lambda: mat(4, 200)
+    fp8._check_held(make(), None, mat(300, 200, "tiles"), mat(4, 200, scale="f32"))
+    other = torch.zeros(4, 256, dtype=torch.uint8).view(E4)
+    m = make()
+    m.data.set_(other)                                    # as large as before: its own codes from now on
+    fp8._check_held(m)
+    assert m._ptrs[0] == other.data_ptr()
+    for change in (lambda m: m.data.set_(other[:3]), lambda m: m.data.untyped_storage().resize_(0), lambda m: m.scale.set_(m.scale[:, :2].clone()),
+                   lambda m: m.scale.untyped_storage().resize_(3), lambda m: m.data.set_(other[:, :128])):
+        m = make()
+        change(m)
+        with pytest.raises(ValueError, match="since it was made"):
+            fp8._check_held(m)

@@ -656,3 +656,33 @@ def test_tensors_of_a_recording_graph_are_refused():
     Layer.apply(x, w).backward(dy)
     dx, dw = fp8.linear_fp8_bwd(dy, fp8.fp8_quantize(x, transpose=True), w8t)
     assert torch.equal(x.grad, dx) and torch.equal(w.grad, dw)
+
+
+def test_matrices_whose_tensors_were_exchanged():
+    """Addresses are read at every call: codes exchanged for others are the ones used, memory given up is refused."""
+    fp8 = _fp8()
+    g = torch.Generator().manual_seed(2)
+    ints = lambda *s: torch.randint(-3, 4, s, generator=g).float().cuda()
+    x, w, v, dy = ints(5, 300), ints(70, 300), ints(70, 300), ints(5, 70)
+    q, w8, v8 = fp8.fp8_quantize(x), fp8.fp8_quantize(w, "tiles"), fp8.fp8_quantize(v, "tiles")
+    assert torch.equal(w8.scale, v8.scale)
+    xt, wt = fp8.fp8_quantize(x, transpose=True), w8.transposed()
+    calls = lambda: (lambda: fp8.matmul_fp8(q, w8), lambda: fp8.linear_fp8_fwd(x, w8), lambda: fp8.linear_fp8_fwd(x, w8, keep_transposed=True))
+    w8.data.set_(v8.data)
+    want = x @ v.t()
+    assert torch.equal(fp8.matmul_fp8(q, w8, out_dtype=torch.float32), want) and torch.equal(fp8.linear_fp8_fwd(x, w8), want)
+    w8.data.set_(v8.data[:69])
+    for f in calls():
+        with pytest.raises(ValueError, match="since it was made"):
+            f()
+    w8 = fp8.fp8_quantize(w, "tiles")
+    w8.data.untyped_storage().resize_(0)
+    for f in calls():
+        with pytest.raises(ValueError, match="since it was made"):
+            f()
+    for m in (xt, wt):
+        m.scale.untyped_storage().resize_(0)
+        with pytest.raises(ValueError, match="since it was made"):
+            fp8.linear_fp8_bwd(dy, xt if m is xt else None, wt if m is wt else None)
+    q.data.set_(q.data.cpu().view(torch.uint8).cuda().view(torch.float8_e5m2).view(torch.uint8).view(torch.float8_e4m3fn))
+    assert torch.equal(fp8.matmul_fp8(q, fp8.fp8_quantize(w, "tiles"), out_dtype=torch.float32), x @ w.t())
