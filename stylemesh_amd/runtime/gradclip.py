@@ -57,6 +57,9 @@ class _Table:
                 if not t.is_contiguous() and not _dense(t):
                     raise ValueError(f"{what}: strides {t.stride()} of {tuple(t.shape)} leave gaps or overlap")
 
+    def holds(self) -> bool:
+        return _tensor_list.pack(self.tensors)[0] == self.packed
+
 
 def _norm_kind(norm_type) -> int:
     n = float(norm_type)
@@ -82,7 +85,8 @@ _WRONG = (None, "an output has not as many elements as its gradient", "an output
 
 class GradClip:
     """The call's tables for gradients that stay where they are (an arena's views, ``zero_grad(set_to_none=False)``): checked
-    and laid out once, used every step. Keeps the tensors alive; ``grads`` may hold None (a parameter without a gradient).
+    and laid out once, used every step. Keeps the tensors alive, and refuses them where their memory was exchanged since (``module.to``, ``t.data = ...``); ``grads``
+    may hold None (a parameter without a gradient).
     ``out``: one tensor per gradient that receives the clipped values, of any of the three types (both contiguous with as
     many elements, or the same shape and strides); None: the gradients themselves are scaled in place (where nothing is clipped the second pass ends at once).
     Calls on two streams need the caller's ordering only where both write the same outputs: each has scratch of its own."""
@@ -125,9 +129,17 @@ class GradClip:
         return (torch.empty((), dtype=torch.float32, device=self.device),
                 torch.empty(self._ws_bytes, dtype=torch.uint8, device=self.device))
 
+    def _check(self):
+        """Refuses tensors whose memory was exchanged or given up since the plan was made (``module.to``, ``t.data = ...``,
+        ``storage.resize_``): the tables hold addresses."""
+        for table, what in ((self._g, "gradient"),) if self._o is self._g else ((self._g, "gradient"), (self._o, "output")):
+            if not table.holds():
+                raise ValueError(f"a {what}'s memory was exchanged since the plan was made: make a new GradClip")
+
     def norm(self, norm_type=2.0) -> torch.Tensor:
         """The global norm as a float32 device scalar."""
         kind = _norm_kind(norm_type)
+        self._check()
         out, ws = self._result()
         gp, _, numel, types, _, n = self._args
         hip.check(ops.lib.sm_grad_norm(gp, numel, types, n, kind, ws.data_ptr(), self._ws_bytes, out.data_ptr(), ops.eager_stream()), "sm_grad_norm")
@@ -136,6 +148,10 @@ class GradClip:
     def clip(self, max_norm, norm_type=2.0) -> torch.Tensor:
         """Clips, and returns the norm BEFORE clipping (float32 device scalar)."""
         kind, max_norm = _norm_kind(norm_type), _max_norm(max_norm)
+        self._check()
+        return self._clip(kind, max_norm)
+
+    def _clip(self, kind, max_norm):
         out, ws = self._result()
         hip.check(ops.lib.sm_grad_clip(*self._args, kind, max_norm, ws.data_ptr(), self._ws_bytes, out.data_ptr(), ops.eager_stream()), "sm_grad_clip")
         _tensor_list.written(self.out)      # (autograd refuses a graph that saved one of them before)
@@ -157,5 +173,5 @@ def grad_norm(grads, norm_type=2.0) -> torch.Tensor:
 def clip_grad_norm(grads, max_norm, norm_type=2.0, out=None) -> torch.Tensor:
     """``GradClip(grads, out).clip(max_norm, norm_type)`` for a list that changes from call to call: scales the gradients in
     place (or into ``out``) and returns the norm before clipping."""
-    _norm_kind(norm_type), _max_norm(max_norm)
-    return GradClip(grads, out).clip(max_norm, norm_type)
+    kind, max_norm = _norm_kind(norm_type), _max_norm(max_norm)
+    return GradClip(grads, out)._clip(kind, max_norm)

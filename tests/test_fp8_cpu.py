@@ -368,3 +368,34 @@ def test_matrices_whose_tensors_were_exchanged_are_named():
         change(m)
         with pytest.raises(ValueError, match="since it was made"):
             fp8._check_held(m)
+
+
+def test_a_plan_refuses_tensors_whose_memory_was_exchanged(monkeypatch):
+    from stylemesh_amd import _tensor_list as tl
+    from stylemesh_amd.runtime import gradclip, ops
+    launched = []
+    real_pack, real_empty = tl.pack, torch.empty
+
+    def pack(tensors):      # (host tensors: the addresses that the walk leaves out)
+        packed, at, odd, _, contiguous = real_pack(tensors)
+        return b"".join(t.data_ptr().to_bytes(8, "little") for t in tensors) + packed[8 * len(tensors):], at, odd, 0, contiguous
+    monkeypatch.setattr(tl, "pack", pack)
+    monkeypatch.setattr(tl, "check_outputs", lambda a, b: 0)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch, "empty", lambda *size, dtype, device: real_empty(*size, dtype=dtype))
+    monkeypatch.setattr(ops, "eager_stream", lambda: 0)
+    note = staticmethod(lambda *a: launched.append(1) and 0 or 0)
+    monkeypatch.setattr(ops, "lib", type("Lib", (), {"sm_grad_norm_ws_bytes": staticmethod(lambda n: 8192), "sm_grad_norm": note, "sm_grad_clip": note}))
+    for where in ("grads", "out"):
+        for change in (lambda t: setattr(t, "data", t.data.clone()), lambda t: t.untyped_storage().resize_(0), lambda t: t.set_(t[:3].clone()),
+                       lambda t: setattr(t, "data", t.data.half())):
+            grads, out = [torch.ones(4), torch.ones(6)], [torch.ones(4), torch.ones(6)]
+            plan = gradclip.GradClip(grads, out)
+            plan.clip(1.0), plan.norm()
+            n = len(launched)
+            change(getattr(plan, where)[1])
+            for f in (lambda: plan.clip(1.0), plan.norm):
+                with pytest.raises(ValueError, match="exchanged"):
+                    f()
+            assert len(launched) == n == 2
+            launched.clear()

@@ -255,3 +255,19 @@ def test_a_copied_plan_works_on_the_copies():
         assert all(a.data_ptr() != b.data_ptr() for a, b in zip(plan.grads, other.grads))
         assert float(torch.stack([t.norm() for t in other.out]).norm()) == pytest.approx(1.0, rel=1e-5)
         assert (other.out is other.grads) == (out is None)
+
+
+def test_a_plan_refuses_tensors_whose_memory_was_exchanged():
+    gc = _mod()
+    for change in (lambda t: setattr(t, "data", t.data.clone()), lambda t: t.untyped_storage().resize_(0), lambda t: setattr(t, "data", t.data.half())):
+        g, o = [torch.full((5000,), 2.0, device="cuda"), torch.ones(3, device="cuda")], [torch.zeros(5000, device="cuda"), torch.zeros(3, device="cuda")]
+        for plan, t in ((gc.GradClip(g, o), o[0]), (gc.GradClip(g), g[0])):
+            assert float(plan.clip(1e9)) == pytest.approx(math.sqrt(20003.0), rel=1e-6)
+            keep = t.data
+            change(t)
+            for f in (lambda: plan.clip(1.0), plan.norm):
+                with pytest.raises(ValueError, match="exchanged"):
+                    f()
+            if keep.untyped_storage().nbytes():
+                t.data = keep                              # the plan's own memory again
+                assert float(plan.clip(1e9)) == pytest.approx(math.sqrt(20003.0), rel=1e-6)
