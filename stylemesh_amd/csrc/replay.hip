@@ -57,7 +57,8 @@ struct Entry {
     int n_args;
 };
 #define SM_ENTRY(f) Entry{#f, &Thunk<&f>::call, Thunk<&f>::n_args}
-// every entry point whose last parameter is the stream
+// the entry points that a recorded step may hold: all whose last parameter is the stream but those that take tables of a call's own
+// or scratch allocated for it (8-bit operators, gradient lists), and the clipped update, which no step program holds
 const Entry ENTRIES[] = {
     SM_ENTRY(sm_tex_sample_fwd), SM_ENTRY(sm_tex_sample_fwd_grouped), SM_ENTRY(sm_tex_sample_bwd),
     SM_ENTRY(sm_tex_touch_flags), SM_ENTRY(sm_tex_scatter_planned), SM_ENTRY(sm_adam_fused),
@@ -71,8 +72,6 @@ const Entry ENTRIES[] = {
     SM_ENTRY(sm_gram_masked_split2_grouped), SM_ENTRY(sm_style_loss), SM_ENTRY(sm_gram_backward),
     SM_ENTRY(sm_gram_backward_split), SM_ENTRY(sm_style_loss_grouped), SM_ENTRY(sm_gram_backward_split2_grouped),
     SM_ENTRY(sm_mse_masked), SM_ENTRY(sm_copy_floats), SM_ENTRY(sm_zero_floats),
-    SM_ENTRY(sm_fp8_quantize), SM_ENTRY(sm_fp8_matmul), SM_ENTRY(sm_fp8_linear), SM_ENTRY(sm_fp8_linear_backward), SM_ENTRY(sm_grad_norm), SM_ENTRY(sm_grad_clip),
-    SM_ENTRY(sm_adam_grad_clip), SM_ENTRY(sm_adam_fused_clipped),
 };
 constexpr int N_ENTRIES = (int)(sizeof(ENTRIES) / sizeof(ENTRIES[0]));
 

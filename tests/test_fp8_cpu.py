@@ -399,3 +399,10 @@ def test_a_plan_refuses_tensors_whose_memory_was_exchanged(monkeypatch):
                     f()
             assert len(launched) == n == 2
             launched.clear()
+
+
+def test_calls_that_no_step_program_may_hold_are_not_replayable():
+    for name in ("sm_fp8_quantize", "sm_fp8_matmul", "sm_fp8_linear", "sm_fp8_linear_backward", "sm_grad_norm", "sm_grad_clip", "sm_adam_grad_clip",
+                 "sm_adam_fused_clipped"):
+        assert hip.lib.sm_call_id(name.encode()) < 0, name
+    assert hip.lib.sm_call_id(b"sm_adam_fused") >= 0
