@@ -178,6 +178,7 @@ class StepEngine:
         # gradient clipping (0: off): the update waits for the whole gradient's norm, so the split update and the overlapped
         # exchanges, which update a part of the arena before the rest of the gradient exists, are off with it
         self.gradient_clip_val = float(cfg.gradient_clip_val)
+        self._step_clips = None             # does the step that is under way clip? (None: no step is)
         self.grad_clip = torch.zeros(2, device=device)      # {norm of the last clipped step's total gradient, coefficient}
         self._clip_ws = torch.empty(ops.adam_grad_clip_ws_bytes(), dtype=torch.uint8, device=device)
         self.epoch = 0
@@ -1414,6 +1415,7 @@ class StepEngine:
 
     def optimizer_step(self, world_size: int = 1):
         """Fused regulariser-gradient + Adam + clamp + zero-grad over the whole arena (one launch)."""
+        self._close_step()
         self.step_count += 1
         run, self._prog_run = self._prog_run, None
         if run is not None and world_size == 1:          # the update segment of the program step_compute replayed
@@ -1543,6 +1545,13 @@ class StepEngine:
                        self.lr, self.step_count, grad_scale=1.0 / world_size, sumsq_out=self.sumsq,
                        dev_hyper=dev_hyper, touched=touched, touched_log2=tl2, clip=clip)
 
+    def _close_step(self):
+        """What ``step_compute`` did depends on whether the step clips: a part of the update may have been applied, recorded or
+        left to an overlapped exchange without it."""
+        if self._step_clips not in (None, self.gradient_clip_val != 0.0):
+            raise RuntimeError("gradient_clip_val was switched on or off between step_compute() and the step's update")
+        self._step_clips = None
+
     def _clip_launch(self, world_size, touched, touched_log2):
         """Norm and clip coefficient of the gradient the update is about to apply (None: clipping is off)."""
         if self.gradient_clip_val == 0.0:
@@ -1587,6 +1596,7 @@ class StepEngine:
         split update, or inline), then ``reducer.step``: the previous step's deferred sums, this rank's own single-owner
         chunks, the critical exchange + update of the shared chunks, the deferred exchange in the background."""
         assert reducer.chunk_log2 == self.touched_log2
+        self._close_step()
         self.step_count += 1
         a = self.arena
         if self._adam_early_done is not None:
@@ -1621,6 +1631,7 @@ class StepEngine:
     def exchange_and_update(self, world_size: int, reducer):
         """Multi-GPU tail of the step: gradient exchange overlapped with the fused update (``reducer.pipelined``:
         the update of an arena range is issued as soon as its sums arrived, later pieces still on the links)."""
+        self._close_step()
         self.step_count += 1
         self.sumsq.zero_()
         self._grad_dirty = False   # every range is zeroed by its update
@@ -1679,6 +1690,9 @@ class StepEngine:
             raise RuntimeError("step_compute() was called again before optimizer_step() closed the previous step: the "
                                "split update needs exactly one optimizer_step per step (STYLEMESH_SPLIT_UPDATE=0 "
                                "disables the split)")
+        self._step_clips = self.gradient_clip_val != 0.0
+        if self._step_clips and getattr(reducer, "_pending", None) is not None:
+            self.finish_exchange(self._world_size, reducer)      # (of an unclipped step: clipping has just been switched on)
         self.begin_step(batch, reducer, new_view)
         reqs, self._prepare_request = self._prepare_request, []
         self._steps_on_view = getattr(self, "_steps_on_view", 0) + 1

@@ -216,3 +216,33 @@ def test_trainer_clips_double_gradients_on_the_device():
     _clip_gradients(params, 0.5)
     for q, w in zip(params, want):
         assert ((q.grad.double() - w * (0.5 / (norm + 1e-6))).abs() <= 2.0 ** -20 * w.abs()).all()
+
+
+def test_clipping_is_not_switched_inside_a_step():
+    """Small steps are replayed as a program whose update does not clip: switched on between the two halves of such a step,
+    the gradient would silently be applied unclipped."""
+    eng = make_engine(FLAGSETS["with_angle_and_depth"], None)
+    view = to_cuda(small_views((3,))[0])
+    for _ in range(6):
+        eng.step_compute(view)
+        eng.optimizer_step()
+    for first, then in ((0.0, 0.5), (0.5, 0.0)):
+        eng.gradient_clip_val = first
+        eng.step_compute(view)
+        eng.gradient_clip_val = then
+        count = eng.step_count
+        with pytest.raises(RuntimeError, match="gradient_clip_val"):
+            eng.optimizer_step()
+        assert eng.step_count == count
+        eng.gradient_clip_val = first
+        eng.optimizer_step()
+    # a value may change, and a new step takes whatever holds at its start
+    eng.gradient_clip_val = 0.5
+    eng.step_compute(view)
+    eng.gradient_clip_val = 0.25
+    eng.optimizer_step()
+    norm, coef = eng.grad_clip.tolist()
+    assert norm > 0.5 and abs(coef - 0.25 / (norm + 1e-6)) <= 2.0 ** -20 * coef
+    eng.gradient_clip_val = 0.0
+    eng.step_compute(view)
+    eng.optimizer_step()
