@@ -246,3 +246,28 @@ def test_clipping_is_not_switched_inside_a_step():
     eng.gradient_clip_val = 0.0
     eng.step_compute(view)
     eng.optimizer_step()
+
+
+@pytest.mark.parametrize("exchange", ["plain", "pipelined", "owner_aware"])
+def test_two_ranks_clip_by_the_same_norm(exchange):
+    """Two ranks over gloo on one device (they take turns on it), an epoch of the trainer with ``gradient_clip_val``: the norm
+    is the mean gradient's - data terms of both ranks and regulariser - on both, bit for bit, whatever exchange is asked for, and
+    the textures end identical."""
+    require_gpu()
+    import os
+    from test_round2_gpu import REPO, _launch_ranks
+    env = {"STYLEMESH_TEST_BACKEND": "gloo", "STYLEMESH_TEST_CLIP": "0.25"}
+    env.update({"plain": {}, "pipelined": {"STYLEMESH_PIPELINE_EXCHANGE": "1"}, "owner_aware": {"STYLEMESH_DEFERRED_EXCHANGE": "1"}}[exchange])
+    with tempfile.TemporaryDirectory() as tmp:
+        r = _launch_ranks([os.path.join(REPO, "tests", "two_rank_clip_worker.py"), "trainer", tmp], 2, env, timeout=100)
+        assert r.returncode == 0, r.stdout[-3000:] + r.stderr[-3000:]
+        r0, r1 = (torch.load(os.path.join(tmp, f"rank{k}.pt")) for k in (0, 1))
+        c0, c1 = (torch.load(os.path.join(tmp, f"clip{k}.pt")) for k in (0, 1))
+    assert r0["steps"] == r1["steps"] == 6 and not r0["deferred"] and c0["clip"].shape == (6, 2)
+    assert torch.equal(c0["clip"], c1["clip"])
+    for a, b in zip(r0["layers"], r1["layers"]):
+        assert torch.equal(a, b) and float(a.abs().max()) > 0
+    norm, coef, want, applied = c0["clip"][:, 0].double(), c0["clip"][:, 1].double(), c0["want"], c0["applied"]
+    assert ((norm - want).abs() <= 2.0 ** -22 * want).all() and (want > 0.25).all()
+    assert ((coef - 0.25 / (want + 1e-6)).abs() <= 2.0 ** -20 * coef).all()
+    assert ((applied - 0.25).abs() <= 1e-4).all()
