@@ -845,7 +845,7 @@ size_t sm_adam_grad_clip_ws_bytes(void) { return sm::CLIP_BLOCKS * sizeof(double
 
 int sm_adam_grad_clip(const float* p, const float* g, size_t n, const size_t* seg_end, const float* reg_coef, int n_seg, float grad_scale,
                       const int32_t* touched, int touched_chunk_log2, double max_norm, void* ws, size_t ws_bytes, float* clip_out, void* stream) {
-    if (!(max_norm >= 0.0) || clip_out == nullptr || ws == nullptr || ws_bytes < sm::CLIP_BLOCKS * sizeof(double) || n == 0 ||
+    if (!(max_norm >= 0.0) || clip_out == nullptr || ws == nullptr || (uintptr_t)ws % 8 || ws_bytes < sm::CLIP_BLOCKS * sizeof(double) || n == 0 ||
         (touched != nullptr && (touched_chunk_log2 < 2 || touched_chunk_log2 > 24)))
         return (int)hipErrorInvalidValue;
     sm::Segs s;

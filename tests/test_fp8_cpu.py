@@ -406,3 +406,12 @@ def test_calls_that_no_step_program_may_hold_are_not_replayable():
                  "sm_adam_fused_clipped"):
         assert hip.lib.sm_call_id(name.encode()) < 0, name
     assert hip.lib.sm_call_id(b"sm_adam_fused") >= 0
+
+
+def test_clip_scratch_must_be_aligned():
+    import ctypes as C
+    buf = torch.zeros(1 << 16, dtype=torch.uint8)
+    p = buf.data_ptr() + (-buf.data_ptr()) % 16
+    seg, reg = (C.c_size_t * 1)(64), (C.c_float * 1)(0.0)
+    for off in (1, 2, 4):
+        assert hip.lib.sm_adam_grad_clip(p, p, 64, seg, reg, 1, 1.0, None, 0, 1.0, p + off, 1 << 15, p, None) != 0

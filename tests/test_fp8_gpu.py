@@ -686,3 +686,30 @@ def test_matrices_whose_tensors_were_exchanged():
             fp8.linear_fp8_bwd(dy, xt if m is xt else None, wt if m is wt else None)
     q.data.set_(q.data.cpu().view(torch.uint8).cuda().view(torch.float8_e5m2).view(torch.uint8).view(torch.float8_e4m3fn))
     assert torch.equal(fp8.matmul_fp8(q, fp8.fp8_quantize(w, "tiles"), out_dtype=torch.float32), x @ w.t())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("fmt", ["e4m3", "e5m2"])
+def test_quantize_subnormal_values_under_normal_scales(dtype, fmt):
+    """Blocks whose largest value leaves a normal scale (2^-126 and just above) over values below the type's normal range, which the
+    format holds: they keep their codes, in the rows, tiles, transposed and small forms and inside the layer's forward pass."""
+    fp8 = _fp8()
+    fi = torch.finfo(DT[dtype])
+    low = math.log2(fi.smallest_normal)
+    g = torch.Generator().manual_seed(6)
+    for rows, cols in ((20, 300), (1300, 1500)):
+        steps = torch.randint(-64, 65, (rows, cols), generator=g).double()
+        x = steps * 2.0 ** (low - 6)                       # multiples of 1/64 of the smallest normal value: subnormal, or that value
+        top = 2.0 ** (low + torch.arange(cols) % 12)
+        x[torch.arange(rows) % 3 == 0] = torch.where(torch.arange(cols) % 7 == 0, top, x[torch.arange(rows) % 3 == 0])
+        x = x.to(DT[dtype])
+        xd = x.cuda()
+        for block in ("rows", "tiles")[:1 if rows > 1000 else 2]:
+            n, t = fp8.fp8_quantize_both(xd, block, fmt)
+            _check_matrix(n, x, block, fmt)
+            _check_matrix(t, x.t(), block, fmt)
+            assert torch.equal(fp8.fp8_quantize(xd, block, fmt).data.view(torch.uint8), n.data.view(torch.uint8))
+    if fmt == "e4m3":
+        w = torch.eye(300)[:70] * 2.0 ** 100
+        y = fp8.linear_fp8_fwd(x[:9, :300].cuda(), fp8.fp8_quantize(w.cuda(), "tiles"), out_dtype=torch.float32)
+        assert torch.equal(y.double().cpu(), (R.requantized(x[:9, :300]) * 2.0 ** 100)[:, :70].float().double())
