@@ -365,7 +365,7 @@ def live_schedule_leg(args, wl):
         torch.cuda.synchronize()
         t_scene = time.time() - t0
         cmd = SCH.cli_command(root, os.path.join(root, "logs"), args.workload, args.schedule_epochs, wl["index_repeat"], 4)
-        stdout, stderr, rc, wall = SCH.run_cli(cmd, deadline_s=args.schedule_budget_s)
+        stdout, stderr, rc, wall = SCH.run_cli(cmd, deadline_s=args.schedule_budget_s, echo=sys.stderr)
         epochs, loops, per_epoch = SCH.parse_epochs(stdout)
         if not epochs:
             out["live_error"] = f"no epoch finished (rc {rc}): {(stderr or stdout)[-400:]}"

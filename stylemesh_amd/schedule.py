@@ -86,15 +86,21 @@ def cli_command(root, log_dir, workload, epochs, index_repeat, num_workers):
             "--min_pyramid_depth", "0.25", "--min_pyramid_height", "256", "--default_root_dir", log_dir] + FLAGS[workload]
 
 
-def run_cli(cmd, deadline_s=None):
+def run_cli(cmd, deadline_s=None, echo=None):
     """Run the CLI as a fresh child, collecting its standard output line by line. ``deadline_s``: seconds after which the
-    child (this exact process) is ended; what it printed until then is kept. Returns (stdout, stderr tail, return code or
-    None when the deadline ended it, wall-clock seconds)."""
+    child (this exact process) is ended; what it printed until then is kept. ``echo``: a stream that receives the child's
+    per-epoch lines as they come (the whole schedule takes three minutes: a caller that shows nothing for so long looks
+    hung). Returns (stdout, stderr tail, return code or None when the deadline ended it, wall-clock seconds)."""
     t0 = time.time()
     proc = subprocess.Popen(cmd, cwd=REPO, stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True, bufsize=1)
     lines, err = [], []
-    readers = [threading.Thread(target=lambda: lines.extend(iter(proc.stdout.readline, "")), daemon=True),
-               threading.Thread(target=lambda: err.extend(iter(proc.stderr.readline, "")), daemon=True)]
+    def collect(stream, into, show):
+        for line in iter(stream.readline, ""):
+            into.append(line)
+            if show is not None and line.startswith("epoch "):
+                print(line.rstrip(), file=show, flush=True)
+    readers = [threading.Thread(target=collect, args=(proc.stdout, lines, echo), daemon=True),
+               threading.Thread(target=collect, args=(proc.stderr, err, None), daemon=True)]
     for t in readers:
         t.start()
     timed_out = False
