@@ -8,8 +8,8 @@
 //
 // Power-of-two scales make the quantiser exact up to the one rounding to 8 bits (x 2^-e is exact) and cost the product no
 // instruction: they are part of the conversion that widens the codes to bf16, and for sums of fewer bits, where the caller permits
-// them, v_mfma_scale_f32_16x16x128_f8f6f4 takes a block of 128 per instruction and one scale byte per operand row. fp32 scales (any value) take the same kernels with
-// the block's partial sum multiplied in on the vector unit.
+// them, v_mfma_scale_f32_16x16x128_f8f6f4 takes a block of 128 per instruction and one scale byte per operand row. fp32
+// scales (any value) take the same kernels with the block's partial sum multiplied in on the vector unit.
 #include <algorithm>
 #include <type_traits>
 
@@ -1160,7 +1160,7 @@ __global__ __launch_bounds__(256) void fp8_matmul_empty_kernel(MatmulArgs g) {
 //                                        256 x 256   256 x 128   128 x 128   64 x 64
 //   8192^3      fast sums, 2^e scales          413         488         499       921
 //   4096^3      fast sums, 2^e scales           59          71          70       126
-//   4096^3      f16 result, fp32 scales        317         121         133       201   (256 x 256 spills)
+//   4096^3      f16 result, fp32 scales        317         124         133       201   (256 x 256 spills)
 //   2048^3      fast sums, 2^e scales           33          22          17        18
 //   512 x 4096 x 4096, fast sums                50          31          26        18
 // A 256-row tile takes a CU, two 128 x 128 tiles share one: the large tile is taken where its rounds over the 256 CUs are not
@@ -1201,8 +1201,8 @@ static Plan matmul_plan(int M, int N, int KB) {
 // beyond that: each of the other seven loses up to 2^-13 of the largest, so a sum is off by up to 7 * 2^-13 of sum |a||b|
 // beside what fp32 loses - of the terms' magnitudes, not of the result, which may be far smaller (rms at K = 128: 2^-19 of it for
 // normal data, 2^-15 for log-normal of sigma 2, falling with sqrt(K)). Those are fewer bits than a sum is owed, so it is taken
-// where the caller asks for it only, and only for bf16 results. Every other product widens the codes to bf16 and sums in fp32: us, fast against
-// that, 8192^3 462 / 844, layer backward 4096^3 208 / 256, 37 x 5001 -> 8200 21.0 / 22.4, 1 x 4096 -> 4096 6.1 / 6.5.
+// where the caller asks for it only, and only for bf16 results. Every other product widens the codes to bf16 and sums in
+// fp32: us, fast against that, 8192^3 463 / 876, layer backward 4096^3 208 / 260, 37 x 5001 -> 8200 21.0 / 22.4, 1 x 4096 -> 4096 6.1 / 6.7.
 struct ResultType {
     int type;
     bool fast, ok;
