@@ -208,8 +208,8 @@ def _check_held(*matrices):
                 Fp8Matrix(m._data, m._scale, m._cols, m.block)
             except (ValueError, RuntimeError) as e:
                 raise ValueError(f"the tensors of an Fp8Matrix {m.shape} were exchanged since it was made: {e}") from None
-            if m._data.shape[0] != m._rows or any(t.untyped_storage().nbytes() < t.storage_offset() * t.itemsize + t.nbytes for t in (m._data, m._scale)):
-                raise ValueError(f"the tensors of an Fp8Matrix {m.shape} were resized since it was made")
+            if m._data.shape[0] != m._rows or not m._data.is_contiguous() or any(t.untyped_storage().nbytes() < t.storage_offset() * t.itemsize + t.nbytes for t in (m._data, m._scale)):
+                raise ValueError(f"the tensors of an Fp8Matrix {m.shape} were resized or laid out anew since it was made")
 
 
 _new = Fp8Matrix.__new__

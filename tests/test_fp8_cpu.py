@@ -363,7 +363,8 @@ def test_matrices_whose_tensors_were_exchanged_are_named():
     fp8._check_held(m)
     assert m._ptrs[0] == other.data_ptr()
     for change in (lambda m: m.data.set_(other[:3]), lambda m: m.data.untyped_storage().resize_(0), lambda m: m.scale.set_(m.scale[:, :2].clone()),
-                   lambda m: m.scale.untyped_storage().resize_(3), lambda m: m.data.set_(other[:, :128])):
+                   lambda m: m.scale.untyped_storage().resize_(3), lambda m: m.data.set_(other[:, :128]),
+                   lambda m: m.data.set_(torch.zeros(256, 4, dtype=torch.uint8).view(E4).t())):
         m = make()
         change(m)
         with pytest.raises(ValueError, match="since it was made"):

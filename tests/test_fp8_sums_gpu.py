@@ -226,3 +226,20 @@ def test_layer_passes_over_the_whole_range(M, dtype):
         dx, dw = fp8.linear_fp8_bwd(dy, fp8.fp8_quantize((x.double() * 2.0 ** (ew - ex)).float(), transpose=True), w8t, dx_dtype=torch.float32)
         _check_scaled(dx, R.requantized(dy).cuda(), wv.t(), N, False)
         _check_scaled(dw, R.requantized(dy.t()).cuda(), R.requantized((x.double() * 2.0 ** (ew - ex)).float().t()).cuda(), M, False)
+
+
+def test_fast_sums_into_out_and_without_terms():
+    fp8 = _fp8()
+    g = torch.Generator(device="cuda").manual_seed(31)
+    for M, N, K in ((5, 70, 0), (5, 70, 300), (200, 70, 0), (200, 300, 2000)):
+        a, b = (torch.randint(-3, 4, (r, K), generator=g, device="cuda").float() for r in (M, N))
+        old = torch.randint(-8, 9, (M + 2, N + 5), generator=g, device="cuda").bfloat16()
+        want = a.double() @ b.double().t()
+        qa, qb = _matrix(fp8, a), _matrix(fp8, b, block="tiles")
+        for accumulate in (False, True):
+            big = old.clone()
+            out = big[1:M + 1, 2:N + 2]
+            assert fp8.matmul_fp8(qa, qb, out=out, accumulate=accumulate, fast_accum=True) is out
+            assert torch.equal(out, (want + (old[1:M + 1, 2:N + 2].double() if accumulate else 0)).bfloat16())
+            big[1:M + 1, 2:N + 2] = old[1:M + 1, 2:N + 2]
+            assert torch.equal(big, old)
